@@ -59,12 +59,24 @@ class LayerBuffers(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in NAMES + OPTIONAL]
 
 
+class PagedKvStruct(C.Structure):
+    """Mirror of `ds4b200_paged_kv` (device pointers)."""
+    _fields_ = [("row_format", C.c_int32), ("head_dim", C.c_int32), ("n_rot", C.c_int32), ("page_rows", C.c_int32),
+                ("n_pages", C.c_int64)] + [(n, C.c_void_p) for n in ("codes", "scales", "tail", "raw")]
+
+
+class PageArray(C.Structure):
+    """Mirror of `ds4b200_page_array`."""
+    _fields_ = [("base", C.c_void_p), ("page_bytes", C.c_int64)]
+
+
 STAGE_QKV_A, STAGE_Q_B, STAGE_ATTENTION, STAGE_ATTN_OUT, STAGE_FFN_UP, STAGE_FFN_DOWN = range(6)
 StageHook = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_int, C.c_int64, C.c_void_p)
 ChunkHook = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_int64, C.c_void_p)
 
 TABLE_F16, TABLE_Q8_0 = 0, 1
 FP8_BLOCK64_POW2, FP8_ROW_AMAX = 0, 1
+KV_FP8_BLOCK64, KV_FP8_ROW, KV_F32 = 0, 1, 2
 GLU_PLAIN, GLU_CLAMP_REF, GLU_CLAMP_SYM = 0, 1, 2
 
 _P, _I, _L, _F = C.c_void_p, C.c_int, C.c_int64, C.c_float
@@ -132,6 +144,17 @@ SIGNATURES = {
     "ds4b200_compressor_chunk_f32": (_I, [_I, _P, _P, _P, _P, _I, _I, _I, _L, _I, _P, _P, _P, _P]),
     "ds4b200_compressor_step_f32": (_I, [_I, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, C.POINTER(C.c_int), _P]),
     "ds4b200_div_selfcheck": (_I, [C.c_uint64, C.c_uint64, _P, _P]),
+    # paged key-value cache
+    "ds4b200_attn_workspace_bytes": (_L, [_I, _I]),
+    "ds4b200_attn_decode_paged_bf16": (_I, [_P, C.POINTER(PagedKvStruct), _P, _L, _P, _L, _I, _F, _P, _I, _I, _P, _P, _P, _L, _P]),
+    "ds4b200_attn_window_paged_bf16": (_I, [_P, _L, C.POINTER(PagedKvStruct), _P, _L, _P, _P, _L, _I, _F, _P, _I, _I, _P, _P, _P,
+                                            _L, _P]),
+    "ds4b200_pages_workspace_bytes": (_L, [_L, _L, _L]),
+    "ds4b200_pages_copy": (_I, [C.POINTER(PageArray), _I, _L, _P, _L, _P, _P, _L, _P]),
+    "ds4b200_pages_fork": (_I, [C.POINTER(PageArray), _I, _L, _I] + [_P] * 6 + [_L, _L, _P, _L, _P, _P, _L, _P]),
+    "ds4b200_pages_reserve": (_I, [_L, _I] + [_P] * 7 + [_L, _L, _P, _P, _L, _P]),
+    "ds4b200_pages_free": (_I, [_L, _I] + [_P] * 6 + [_L, _L, _P, _L, _P, _P, _L, _P]),
+    "ds4b200_pages_compact": (_I, [C.POINTER(PageArray), _I, _L, _P, _P, _P, _P, _L, _L, _P, _P, _L, _P]),
     # prefill path object (include/ds4b200_path.h)
     "ds4b200_path_create": (_P, [_P]),
     "ds4b200_path_destroy": (None, [_P]),

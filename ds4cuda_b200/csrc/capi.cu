@@ -615,4 +615,169 @@ int ds4b200_e4m3_selfcheck(uint32_t first_bits, uint64_t count, unsigned long lo
     return launched("e4m3_selfcheck");
 }
 
+int64_t ds4b200_attn_workspace_bytes(int n_heads, int head_dim) {
+    if (n_heads < 1 || n_heads > ds4b200::kMaxAttnHeads || head_dim < 1 || head_dim > 512)
+        return fail(-EINVAL, "attn_workspace_bytes: n_heads must be in [1, 1024] and head_dim in [1, 512]");
+    return ds4b200::attn_workspace_bytes(n_heads, head_dim);
+}
+
+static int check_attn(const char *what, const ds4b200_paged_kv *kv, const void *q, const void *out, const void *page_table,
+                      int64_t table_width, const void *kv_len, int64_t n_seqs, int n_heads, float scale, int window,
+                      int n_first, const void *workspace, int64_t workspace_bytes) {
+    REQUIRE(kv && q && out && page_table && kv_len && workspace, "%s: null pointer", what);
+    REQUIRE(kv->row_format == DS4B200_KV_FP8_BLOCK64 || kv->row_format == DS4B200_KV_FP8_ROW || kv->row_format == DS4B200_KV_F32,
+            "%s: unknown row format", what);
+    REQUIRE(kv->head_dim >= 128 && kv->head_dim <= 512 && kv->head_dim % 128 == 0,
+            "%s: head_dim must be 128, 256, 384 or 512", what);
+    REQUIRE(kv->page_rows >= 1 && kv->n_pages >= 0 && kv->n_pages < ((int64_t)1 << 31) / kv->page_rows,
+            "%s: n_pages * page_rows must be below 2^31", what);
+    if (kv->row_format == DS4B200_KV_F32) {
+        REQUIRE(kv->raw && a16(kv->raw), "%s: raw rows missing or not 16-byte aligned", what);
+    } else {
+        REQUIRE(kv->codes && kv->scales && a16(kv->codes) && a4(kv->scales), "%s: codes or scales missing or not aligned", what);
+        if (kv->row_format == DS4B200_KV_FP8_BLOCK64) {
+            REQUIRE(kv->n_rot >= 0 && kv->n_rot % 4 == 0 && kv->n_rot < kv->head_dim && (kv->head_dim - kv->n_rot) % 64 == 0,
+                    "%s: n_rot must be a multiple of 4 with (head_dim - n_rot) %% 64 == 0", what);
+            REQUIRE(kv->n_rot == 0 || (kv->tail && a16(kv->tail)), "%s: tail missing or not 16-byte aligned", what);
+        }
+    }
+    REQUIRE(a16(q) && a16(out) && a16(workspace), "%s: q, out and workspace need 16-byte alignment", what);
+    REQUIRE(table_width >= 1 && table_width < ((int64_t)1 << 31), "%s: table_width must be in [1, 2^31)", what);
+    REQUIRE(n_seqs <= ds4b200::kMaxWindowSeqs, "%s: at most 4096 sequences per call", what);
+    REQUIRE(n_heads >= 1 && n_heads <= ds4b200::kMaxAttnHeads, "%s: n_heads must be in [1, 1024]", what);
+    REQUIRE(scale > -3.0e38f && scale < 3.0e38f, "%s: scale must be finite", what);
+    REQUIRE(window >= 0 && n_first >= 0, "%s: negative window or n_first", what);
+    REQUIRE(workspace_bytes >= ds4b200::attn_workspace_bytes(n_heads, kv->head_dim), "%s: workspace too small", what);
+    return 0;
+}
+
+int ds4b200_attn_decode_paged_bf16(const uint16_t *q, const ds4b200_paged_kv *host_kv, const int32_t *page_table,
+                                   int64_t table_width, const int32_t *kv_len, int64_t n_seqs, int n_heads,
+                                   float scale, const float *sink, int window, int n_first, uint16_t *out,
+                                   float *lse, void *workspace, int64_t workspace_bytes, void *stream) {
+    REQUIRE(n_seqs >= 0, "attn_decode_paged: n_seqs < 0");
+    if (n_seqs == 0) return 0;
+    const int rc = check_attn("attn_decode_paged", host_kv, q, out, page_table, table_width, kv_len, n_seqs, n_heads, scale,
+                              window, n_first, workspace, workspace_bytes);
+    if (rc) return rc;
+    ds4b200::AttnArgs a{q, *host_kv, page_table, kv_len, nullptr, table_width, n_seqs, (int)n_seqs, n_heads, window, n_first,
+                        scale, sink, out, lse, workspace};
+    ds4b200::attn_paged(a, STREAM(stream));
+    return launched("attn_decode_paged");
+}
+
+int ds4b200_attn_window_paged_bf16(const uint16_t *q, int64_t n_tokens, const ds4b200_paged_kv *host_kv,
+                                   const int32_t *page_table, int64_t table_width, const int32_t *kv_len,
+                                   const int32_t *q_start, int64_t n_seqs, int n_heads, float scale,
+                                   const float *sink, int window, int n_first, uint16_t *out, float *lse,
+                                   void *workspace, int64_t workspace_bytes, void *stream) {
+    REQUIRE(n_seqs >= 0 && n_tokens >= 0, "attn_window_paged: negative size");
+    if (n_seqs == 0 || n_tokens == 0) return 0;
+    const int rc = check_attn("attn_window_paged", host_kv, q, out, page_table, table_width, kv_len, n_seqs, n_heads, scale,
+                              window, n_first, workspace, workspace_bytes);
+    if (rc) return rc;
+    REQUIRE(q_start, "attn_window_paged: null pointer");
+    REQUIRE(n_tokens < ((int64_t)1 << 31) / n_heads, "attn_window_paged: n_tokens * n_heads must be below 2^31");
+    ds4b200::AttnArgs a{q, *host_kv, page_table, kv_len, q_start, table_width, n_tokens, (int)n_seqs, n_heads, window, n_first,
+                        scale, sink, out, lse, workspace};
+    ds4b200::attn_paged(a, STREAM(stream));
+    return launched("attn_window_paged");
+}
+
+int64_t ds4b200_pages_workspace_bytes(int64_t n_pages, int64_t n_seqs, int64_t n_list) {
+    if (n_pages < 0 || n_pages > ds4b200::kMaxPages || n_seqs < 0 || n_list < 0)
+        return fail(-EINVAL, "pages_workspace_bytes: sizes must not be negative, n_pages at most 2^20");
+    return ds4b200::pages_workspace_bytes(n_pages, n_seqs, n_list);
+}
+
+static int check_pages(const char *what, int64_t n_pages, int64_t n_seqs, int64_t n_list, const void *status,
+                       const void *workspace, int64_t workspace_bytes) {
+    REQUIRE(n_pages >= 0 && n_pages <= ds4b200::kMaxPages, "%s: n_pages must be in [0, 2^20]", what);
+    REQUIRE(n_seqs >= 0 && n_list >= 0 && n_seqs < ((int64_t)1 << 31) && n_list < ((int64_t)1 << 31), "%s: bad list or sequence count", what);
+    REQUIRE(status && workspace, "%s: null pointer", what);
+    REQUIRE(a4(status) && a16(workspace), "%s: workspace needs 16-byte alignment", what);
+    REQUIRE(workspace_bytes >= ds4b200::pages_workspace_bytes(n_pages, n_seqs, n_list), "%s: workspace too small", what);
+    return 0;
+}
+static int check_tables(const char *what, const ds4b200::PageTables &t, bool lens) {
+    REQUIRE(t.page_rows >= 1, "%s: page_rows must be at least 1", what);
+    REQUIRE(t.width >= 1 && t.width < ((int64_t)1 << 31) / t.page_rows, "%s: table_width * page_rows must be in [1, 2^31)", what);
+    REQUIRE(t.n_pages == 0 || (t.refs_in && t.refs_out), "%s: null pointer", what);
+    REQUIRE(t.n_seqs == 0 || (t.table_in && t.table_out && (!lens || (t.lens_in && t.lens_out))), "%s: null pointer", what);
+    return 0;
+}
+static int check_arrays(const char *what, const ds4b200_page_array *host_arrays, int n_arrays) {
+    REQUIRE(n_arrays >= 0 && n_arrays <= ds4b200::kMaxPageArrays, "%s: at most 192 arrays", what);
+    REQUIRE(n_arrays == 0 || host_arrays, "%s: null pointer", what);
+    int64_t all = 0;
+    for (int i = 0; i < n_arrays; ++i) {
+        REQUIRE(host_arrays[i].base && a4(host_arrays[i].base), "%s: array %d is null or not 4-byte aligned", what, i);
+        REQUIRE(host_arrays[i].page_bytes > 0 && host_arrays[i].page_bytes % 4 == 0,
+                "%s: array %d: page_bytes must be a positive multiple of 4", what, i);
+        all += host_arrays[i].page_bytes;
+        REQUIRE(all <= ((int64_t)1 << 40), "%s: pages of more than 1 TiB", what);
+    }
+    return 0;
+}
+#define CHECKED(call) do { const int rc_ = (call); if (rc_) return rc_; } while (0)
+
+int ds4b200_pages_copy(const ds4b200_page_array *host_arrays, int n_arrays, int64_t n_pages, const int32_t *moves,
+                       int64_t n_moves, int32_t *status, void *workspace, int64_t workspace_bytes, void *stream) {
+    CHECKED(check_pages("pages_copy", n_pages, 0, n_moves, status, workspace, workspace_bytes));
+    CHECKED(check_arrays("pages_copy", host_arrays, n_arrays));
+    REQUIRE(n_moves == 0 || (moves && (reinterpret_cast<uintptr_t>(moves) & 7u) == 0), "pages_copy: moves missing or not 8-byte aligned");
+    ds4b200::pages_copy(host_arrays, n_arrays, n_pages, moves, n_moves, status, workspace, STREAM(stream));
+    return launched("pages_copy");
+}
+
+int ds4b200_pages_fork(const ds4b200_page_array *host_arrays, int n_arrays, int64_t n_pages, int page_rows,
+                       const int32_t *refs_in, int32_t *refs_out, const int32_t *table_in, int32_t *table_out,
+                       const int32_t *lens_in, int32_t *lens_out, int64_t n_seqs, int64_t table_width,
+                       const int32_t *pairs, int64_t n_pairs, int32_t *status, void *workspace,
+                       int64_t workspace_bytes, void *stream) {
+    const ds4b200::PageTables t{refs_in, refs_out, table_in, table_out, lens_in, lens_out, n_pages, n_seqs, table_width, page_rows};
+    CHECKED(check_pages("pages_fork", n_pages, n_seqs, n_pairs, status, workspace, workspace_bytes));
+    CHECKED(check_tables("pages_fork", t, true));
+    CHECKED(check_arrays("pages_fork", host_arrays, n_arrays));
+    REQUIRE(n_pairs == 0 || (pairs && (reinterpret_cast<uintptr_t>(pairs) & 7u) == 0), "pages_fork: pairs missing or not 8-byte aligned");
+    ds4b200::pages_fork(host_arrays, n_arrays, t, pairs, n_pairs, status, workspace, STREAM(stream));
+    return launched("pages_fork");
+}
+
+int ds4b200_pages_reserve(int64_t n_pages, int page_rows, const int32_t *refs_in, int32_t *refs_out,
+                          const int32_t *table_in, int32_t *table_out, const int32_t *lens_in, int32_t *lens_out,
+                          const int32_t *new_lens, int64_t n_seqs, int64_t table_width, int32_t *status,
+                          void *workspace, int64_t workspace_bytes, void *stream) {
+    const ds4b200::PageTables t{refs_in, refs_out, table_in, table_out, lens_in, lens_out, n_pages, n_seqs, table_width, page_rows};
+    CHECKED(check_pages("pages_reserve", n_pages, n_seqs, 0, status, workspace, workspace_bytes));
+    CHECKED(check_tables("pages_reserve", t, true));
+    REQUIRE(n_seqs == 0 || new_lens, "pages_reserve: null pointer");
+    ds4b200::pages_reserve(t, new_lens, status, workspace, STREAM(stream));
+    return launched("pages_reserve");
+}
+
+int ds4b200_pages_free(int64_t n_pages, int page_rows, const int32_t *refs_in, int32_t *refs_out,
+                       const int32_t *table_in, int32_t *table_out, const int32_t *lens_in, int32_t *lens_out,
+                       int64_t n_seqs, int64_t table_width, const int32_t *seqs, int64_t n_list, int32_t *status,
+                       void *workspace, int64_t workspace_bytes, void *stream) {
+    const ds4b200::PageTables t{refs_in, refs_out, table_in, table_out, lens_in, lens_out, n_pages, n_seqs, table_width, page_rows};
+    CHECKED(check_pages("pages_free", n_pages, n_seqs, n_list, status, workspace, workspace_bytes));
+    CHECKED(check_tables("pages_free", t, true));
+    REQUIRE(n_list == 0 || seqs, "pages_free: null pointer");
+    ds4b200::pages_free(t, seqs, n_list, status, workspace, STREAM(stream));
+    return launched("pages_free");
+}
+
+int ds4b200_pages_compact(const ds4b200_page_array *host_arrays, int n_arrays, int64_t n_pages,
+                          const int32_t *refs_in, int32_t *refs_out, const int32_t *table_in, int32_t *table_out,
+                          int64_t n_seqs, int64_t table_width, int32_t *n_live, void *workspace,
+                          int64_t workspace_bytes, void *stream) {
+    const ds4b200::PageTables t{refs_in, refs_out, table_in, table_out, nullptr, nullptr, n_pages, n_seqs, table_width, 1};
+    CHECKED(check_pages("pages_compact", n_pages, n_seqs, 0, n_live, workspace, workspace_bytes));
+    CHECKED(check_tables("pages_compact", t, false));
+    CHECKED(check_arrays("pages_compact", host_arrays, n_arrays));
+    ds4b200::pages_compact(host_arrays, n_arrays, t, n_live, workspace, STREAM(stream));
+    return launched("pages_compact");
+}
+
 }  // extern "C"

@@ -131,4 +131,41 @@ void e4m3_decode(const uint8_t *codes, float *x, int64_t n, cudaStream_t s);
 void e4m3_selfcheck(uint32_t first_bits, uint64_t count, unsigned long long *mismatches,
                     cudaStream_t s);
 
+// pages.cu: the pages of a cache pool (arguments as in the C ABI)
+constexpr int kMaxPageArrays = 192;
+constexpr int64_t kMaxPages = 1 << 20;
+struct PageTables {
+    const int32_t *refs_in; int32_t *refs_out;
+    const int32_t *table_in; int32_t *table_out;
+    const int32_t *lens_in; int32_t *lens_out;
+    int64_t n_pages, n_seqs, width;
+    int page_rows;
+};
+int64_t pages_workspace_bytes(int64_t n_pages, int64_t n_seqs, int64_t n_list);
+void pages_copy(const ds4b200_page_array *host, int n_arrays, int64_t n_pages, const int32_t *moves, int64_t n_moves,
+                int32_t *status, void *ws, cudaStream_t s);
+void pages_fork(const ds4b200_page_array *host, int n_arrays, const PageTables &p, const int32_t *pairs, int64_t n_pairs,
+                int32_t *status, void *ws, cudaStream_t s);
+void pages_reserve(const PageTables &p, const int32_t *new_lens, int32_t *status, void *ws, cudaStream_t s);
+void pages_free(const PageTables &p, const int32_t *seqs, int64_t n_list, int32_t *status, void *ws, cudaStream_t s);
+void pages_compact(const ds4b200_page_array *host, int n_arrays, const PageTables &p, int32_t *n_live, void *ws, cudaStream_t s);
+
+// Attention over a paged cache (attn_paged.cu).  n_seqs sequences; q_start null: one token per sequence.
+struct AttnArgs {
+    const uint16_t *q;
+    ds4b200_paged_kv kv;
+    const int32_t *page_table, *kv_len, *q_start;
+    int64_t table_width, n_tokens;
+    int n_seqs, n_heads, window, n_first;
+    float scale;
+    const float *sink;
+    uint16_t *out;
+    float *lse;
+    void *ws;
+};
+constexpr int kMaxAttnHeads = 1024;
+constexpr int kMaxWindowSeqs = 4096;
+int64_t attn_workspace_bytes(int n_heads, int head_dim);
+void attn_paged(const AttnArgs &a, cudaStream_t s);
+
 }  // namespace ds4b200

@@ -11,7 +11,7 @@ import ctypes as C
 import torch
 
 from . import _lib
-from ._lib import (FP8_BLOCK64_POW2, FP8_ROW_AMAX, GLU_CLAMP_REF, GLU_CLAMP_SYM, GLU_PLAIN,
+from ._lib import (FP8_BLOCK64_POW2, FP8_ROW_AMAX, GLU_CLAMP_REF, GLU_CLAMP_SYM, GLU_PLAIN, KV_F32, KV_FP8_BLOCK64, KV_FP8_ROW,
                    TABLE_F16, TABLE_Q8_0, RopeParams, check)
 
 __all__ = [
@@ -20,6 +20,8 @@ __all__ = [
     "add", "rms_norm_rows", "rms_norm_q8_0_rows", "quantize_q8_0_rows", "quantize_q8_K_rows", "embed_gather_rows", "rope_rows", "rope_table_rows", "rope_q8_0_rows", "fp8_kv_round_trip_rows",
     "rope_fp8_store_rows", "fp8_cache_load_rows", "kv_rows_to_raw", "swa_window_push_rows", "swiglu_rows", "hc_pre_rows", "hc_pre_norm_rows", "output_hc_head_rows", "hc_post_rows", "hc_sinkhorn_rows", "hc_sinkhorn_mix_rows",
     "e4m3_encode", "e4m3_decode", "e4m3_selfcheck", "div_selfcheck", "device_status", "compressor_step", "compressor_chunk", "swiglu_q8_K_rows",
+    "KV_F32", "KV_FP8_BLOCK64", "KV_FP8_ROW", "PagedKv", "PagePool", "attn_workspace", "attn_decode_paged", "attn_window_paged",
+    "pages_copy", "pages_fork", "pages_reserve", "pages_free", "pages_compact",
 ]
 
 
@@ -383,3 +385,193 @@ def div_selfcheck(first: int, count: int) -> int:
     bad = torch.zeros(1, dtype=torch.int64, device="cuda")
     check(_lib.load().ds4b200_div_selfcheck(first, count, _p(bad), _s()))
     return int(bad.item())
+
+
+# ------------------------------------------------------------------ paged key-value cache
+
+def _t(t, dtype, shape, what, device):
+    """Device pointer of a tensor that has to have this type, shape and device."""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or tuple(t.shape) != tuple(shape):
+        have = f"{t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+        raise ValueError(f"{what}: expected {dtype} {tuple(shape)} on {device}, got {have}")
+    return _p(t)
+
+
+def _opt(t, dtype, shape, what, device):
+    return None if t is None else _t(t, dtype, shape, what, device)
+
+
+class PagedKv:
+    """The pool's rows of one layer, as attention reads them: the tensors the store ops fill, seen as pages of
+    `page_rows` rows.  codes uint8 [n_slots, head_dim] with scales f32 [n_slots, n_scales] (and tail f32
+    [n_slots, n_rot] for KV_FP8_BLOCK64), or raw f32 [n_slots, head_dim]."""
+
+    def __init__(self, row_format, page_rows, n_rot=64, codes=None, scales=None, tail=None, raw=None):
+        rows = raw if row_format == KV_F32 else codes
+        if rows is None or rows.dim() != 2:
+            raise ValueError("PagedKv: codes / raw must be [n_slots, head_dim]")
+        n, dim = rows.shape
+        if page_rows < 1 or n % page_rows:
+            raise ValueError("PagedKv: the rows must make whole pages")
+        dev = rows.device
+        k = self.struct = _lib.PagedKvStruct(row_format, dim, n_rot, page_rows, n // page_rows)
+        if row_format == KV_F32:
+            k.raw = _t(raw, torch.float32, (n, dim), "raw", dev)
+        elif row_format in (KV_FP8_BLOCK64, KV_FP8_ROW):
+            n_scales = (dim - n_rot) // 64 if row_format == KV_FP8_BLOCK64 else 1
+            k.codes = _t(codes, torch.uint8, (n, dim), "codes", dev)
+            k.scales = _t(scales, torch.float32, (n, n_scales), "scales", dev)
+            if row_format == KV_FP8_BLOCK64 and n_rot:
+                k.tail = _t(tail, torch.float32, (n, n_rot), "tail", dev)
+        else:
+            raise ValueError("PagedKv: unknown row format")
+        self.tensors = (codes, scales, tail, raw)     # kept alive
+        self.head_dim, self.page_rows, self.n_pages, self.device = dim, page_rows, n // page_rows, dev
+
+
+def attn_workspace(n_heads, head_dim, device="cuda"):
+    """Workspace of the attention ops below; calls that may overlap need one each."""
+    n = _lib.load().ds4b200_attn_workspace_bytes(n_heads, head_dim)
+    if n < 0:
+        check(n)
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def _attn(q, kv, page_table, kv_len, q_start, window, n_first, scale, sink, workspace, out, want_lse):
+    if q.dim() != 3 or q.shape[2] != kv.head_dim:
+        raise ValueError("attention: q must be [tokens, n_heads, head_dim] with the cache's head_dim")
+    T, H, D = q.shape
+    dev = kv.device
+    n_seqs, width = page_table.shape
+    if q_start is None and n_seqs != T:
+        raise ValueError("attn_decode_paged: one token per sequence")
+    with torch.cuda.device(dev):
+        out = torch.empty_like(q) if out is None else out
+        lse = torch.empty((T, H), dtype=torch.float32, device=dev) if want_lse else None
+        ws = attn_workspace(H, D, dev) if workspace is None else workspace
+        args = (page_table.data_ptr() if n_seqs == 0 else _t(page_table, torch.int32, (n_seqs, width), "page_table", dev), width,
+                _t(kv_len, torch.int32, (n_seqs,), "kv_len", dev))
+        rest = (n_seqs, H, D ** -0.5 if scale is None else scale, _opt(sink, torch.float32, (H,), "sink", dev), window, n_first,
+                _t(out, torch.bfloat16, (T, H, D), "out", dev), _p(lse), _p(ws), ws.numel() * ws.element_size(), _s())
+        qp = _t(q, torch.bfloat16, (T, H, D), "q", dev)
+        if q_start is None:
+            check(_lib.load().ds4b200_attn_decode_paged_bf16(qp, C.byref(kv.struct), *args, *rest))
+        else:
+            check(_lib.load().ds4b200_attn_window_paged_bf16(
+                qp, T, C.byref(kv.struct), *args, _t(q_start, torch.int32, (n_seqs + 1,), "q_start", dev), *rest))
+    return (out, lse) if want_lse else out
+
+
+def attn_decode_paged(q, kv, page_table, kv_len, window=0, n_first=0, scale=None, sink=None, workspace=None, out=None,
+                      want_lse=False):
+    """Attention of one new token per sequence.  q bf16 [n_seqs, n_heads, head_dim], kv a PagedKv, page_table int32
+    [n_seqs, width], kv_len int32 [n_seqs] (rows in the cache, the token's own among them).  The token sees the
+    last `window` rows (0: all) and the `n_first` first ones.  scale: 1/sqrt(head_dim) by default; sink f32
+    [n_heads]: a logit without a row.  Returns out bf16 like q, with want_lse (out, lse f32 [n_seqs, n_heads])."""
+    return _attn(q, kv, page_table, kv_len, None, window, n_first, scale, sink, workspace, out, want_lse)
+
+
+def attn_window_paged(q, kv, page_table, kv_len, q_start, window=0, n_first=0, scale=None, sink=None, workspace=None, out=None,
+                      want_lse=False):
+    """Attention of a chunk: tokens q_start[b] .. q_start[b + 1] - 1 of q bf16 [tokens, n_heads, head_dim] are the last
+    rows of sequence b, and each sees the rows up to its own, as in attn_decode_paged.  Rows of `out` outside
+    [q_start[0], q_start[-1]) are left as they are."""
+    return _attn(q, kv, page_table, kv_len, q_start, window, n_first, scale, sink, workspace, out, want_lse)
+
+
+class PagePool:
+    """The buffers whose pages move together (e.g. codes, scales and tail of every layer; each holds `n_pages` pages,
+    by default its first dimension) and the workspace of the page ops on them."""
+
+    def __init__(self, arrays, page_rows, n_seqs, table_width, n_pages=None, max_list=None):
+        if not arrays and n_pages is None:
+            raise ValueError("PagePool: n_pages is needed without arrays")
+        self.n_pages = arrays[0].shape[0] if n_pages is None else n_pages
+        self.page_rows, self.n_seqs, self.width = page_rows, n_seqs, table_width
+        self.arrays = list(arrays)
+        self.device = arrays[0].device if arrays else torch.device("cuda", torch.cuda.current_device())
+        self.c_arrays = (_lib.PageArray * max(1, len(arrays)))()
+        for i, a in enumerate(arrays):
+            size = a.numel() * a.element_size()
+            if a.device != self.device or size % max(1, self.n_pages):
+                raise ValueError(f"PagePool: array {i} does not hold {self.n_pages} whole pages on {self.device}")
+            self.c_arrays[i] = _lib.PageArray(_p(a), size // max(1, self.n_pages))
+        self.max_list = n_seqs if max_list is None else max_list
+        n = _lib.load().ds4b200_pages_workspace_bytes(self.n_pages, n_seqs, self.max_list)
+        if n < 0:
+            check(n)
+        self.workspace = torch.empty(n, dtype=torch.uint8, device=self.device)
+
+    def _ws(self):
+        return _p(self.workspace), self.workspace.numel()
+
+    def _tables(self, refs, table, lens, refs_out, table_out, lens_out):
+        d, n = self.device, (self.n_seqs,)
+        shape = (self.n_seqs, self.width)
+        out = (refs if refs_out is None else refs_out, table if table_out is None else table_out, lens if lens_out is None else lens_out)
+        ptrs = [_t(refs, torch.int32, (self.n_pages,), "refs", d), _t(out[0], torch.int32, (self.n_pages,), "refs_out", d),
+                _t(table, torch.int32, shape, "table", d), _t(out[1], torch.int32, shape, "table_out", d)]
+        if lens is not None:
+            ptrs += [_t(lens, torch.int32, n, "lens", d), _t(out[2], torch.int32, n, "lens_out", d)]
+        return ptrs, out
+
+    def _status(self, status):
+        return torch.empty(1, dtype=torch.int32, device=self.device) if status is None else status
+
+
+def pages_copy(pool, moves, status=None):
+    """Copies page moves[i, 0] to page moves[i, 1] (int32 [n, 2]) in every array; returns the status tensor."""
+    with torch.cuda.device(pool.device):
+        st = pool._status(status)
+        n = moves.shape[0]
+        check(_lib.load().ds4b200_pages_copy(pool.c_arrays, len(pool.arrays), pool.n_pages,
+                                             _t(moves, torch.int32, (n, 2), "moves", pool.device), n,
+                                             _t(st, torch.int32, (1,), "status", pool.device), *pool._ws(), _s()))
+    return st
+
+
+def pages_fork(pool, refs, table, lens, pairs, refs_out=None, table_out=None, lens_out=None, status=None):
+    """Sequence pairs[i, 1] becomes a fork of sequence pairs[i, 0]: full pages shared, a part-filled last page
+    copied.  In place unless *_out are given.  Returns (refs, table, lens, status): status int32 [1], 0 = done,
+    > 0 = free pages missing, -1 = list not valid (nothing changed then)."""
+    with torch.cuda.device(pool.device):
+        ptrs, out = pool._tables(refs, table, lens, refs_out, table_out, lens_out)
+        st = pool._status(status)
+        n = pairs.shape[0]
+        check(_lib.load().ds4b200_pages_fork(pool.c_arrays, len(pool.arrays), pool.n_pages, pool.page_rows, *ptrs, pool.n_seqs,
+                                             pool.width, _t(pairs, torch.int32, (n, 2), "pairs", pool.device), n,
+                                             _t(st, torch.int32, (1,), "status", pool.device), *pool._ws(), _s()))
+    return (*out, st)
+
+
+def pages_reserve(pool, refs, table, lens, new_lens, refs_out=None, table_out=None, lens_out=None, status=None):
+    """Pages for new_lens[b] rows of every sequence.  Returns (refs, table, lens, status) as pages_fork."""
+    with torch.cuda.device(pool.device):
+        ptrs, out = pool._tables(refs, table, lens, refs_out, table_out, lens_out)
+        st = pool._status(status)
+        check(_lib.load().ds4b200_pages_reserve(pool.n_pages, pool.page_rows, *ptrs,
+                                                _t(new_lens, torch.int32, (pool.n_seqs,), "new_lens", pool.device), pool.n_seqs,
+                                                pool.width, _t(st, torch.int32, (1,), "status", pool.device), *pool._ws(), _s()))
+    return (*out, st)
+
+
+def pages_free(pool, refs, table, lens, seqs, refs_out=None, table_out=None, lens_out=None, status=None):
+    """Takes the pages of the listed sequences (int32 [n]) from them.  Returns (refs, table, lens, status)."""
+    with torch.cuda.device(pool.device):
+        ptrs, out = pool._tables(refs, table, lens, refs_out, table_out, lens_out)
+        st = pool._status(status)
+        n = seqs.shape[0]
+        check(_lib.load().ds4b200_pages_free(pool.n_pages, pool.page_rows, *ptrs, pool.n_seqs, pool.width,
+                                             _t(seqs, torch.int32, (n,), "seqs", pool.device), n,
+                                             _t(st, torch.int32, (1,), "status", pool.device), *pool._ws(), _s()))
+    return (*out, st)
+
+
+def pages_compact(pool, refs, table, refs_out=None, table_out=None, n_live=None):
+    """Packs the pages in use to the pool's lower end.  Returns (refs, table, n_live int32 [1])."""
+    with torch.cuda.device(pool.device):
+        ptrs, out = pool._tables(refs, table, None, refs_out, table_out, None)
+        n = pool._status(n_live)
+        check(_lib.load().ds4b200_pages_compact(pool.c_arrays, len(pool.arrays), pool.n_pages, *ptrs, pool.n_seqs, pool.width,
+                                                _t(n, torch.int32, (1,), "n_live", pool.device), *pool._ws(), _s()))
+    return out[0], out[1], n

@@ -440,6 +440,112 @@ int ds4b200_e4m3_selfcheck(uint32_t first_bits, uint64_t count,
 int ds4b200_div_selfcheck(uint64_t first, uint64_t count, unsigned long long *mismatches,
                           void *stream);
 
+/* ---- 3. paged key-value cache -------------------------------------------------------
+ *
+ * A pool of n_pages pages of page_rows rows each; row r of page p is slot p * page_rows + r of the
+ * arrays the store entry points above fill (their `slots`).  One row serves as key and as value of
+ * every head, as in the reference's cache.  page_table[seq][table_width] (int32) names a sequence's pages in
+ * order: row j of the sequence lies in page page_table[seq][j / page_rows].  Entries behind a sequence's
+ * last row are not read.  An entry outside [0, n_pages) hides the rows it would hold. */
+
+/* Row formats: what ds4b200_rope_fp8_store_rows leaves with DS4B200_FP8_BLOCK64_POW2 (codes, scales,
+ * tail) and with DS4B200_FP8_ROW_AMAX (codes, scales), and the f32 rows of
+ * ds4b200_kv_rows_to_raw_f32 (raw). */
+enum { DS4B200_KV_FP8_BLOCK64 = 0, DS4B200_KV_FP8_ROW = 1, DS4B200_KV_F32 = 2 };
+
+typedef struct ds4b200_paged_kv {
+    int row_format;         /* DS4B200_KV_* */
+    int head_dim;           /* 128, 256, 384 or 512 */
+    int n_rot;              /* width of the f32 tail (FP8_BLOCK64; (head_dim - n_rot) % 64 == 0, n_rot % 4 == 0) */
+    int page_rows;          /* rows per page, at least 1 */
+    int64_t n_pages;        /* n_pages * page_rows < 2^31 */
+    const uint8_t *codes;   /* [n_pages * page_rows][head_dim], 16-byte aligned */
+    const float *scales;    /* [n_pages * page_rows][(head_dim - n_rot) / 64 or 1] */
+    const float *tail;      /* [n_pages * page_rows][n_rot], 16-byte aligned */
+    const float *raw;       /* [n_pages * page_rows][head_dim], 16-byte aligned */
+} ds4b200_paged_kv;
+
+/* Attention of one new token per sequence.  q, out bf16 [n_seqs][n_heads][head_dim] (16-byte aligned); the token
+ * of sequence b stands at row kv_len[b] - 1 (its own row is in the cache already) and sees the rows
+ * j < kv_len[b] with j >= kv_len[b] - window or j < n_first (window 0: every row):
+ *     out[b][h] = sum_j exp(s_j - lse) row_j,   s_j = scale * q[b][h] . row_j,
+ *     lse[b][h] = log(sum_j exp(s_j) + exp(sink[h]))
+ * sink (f32 [n_heads], nullable) is the reference's per-head logit without a row (cuda/flash_attn.cu:148).
+ * lse is nullable.  A token that sees no row gets out = 0 and lse = sink[h] or -inf.  kv_len is clamped to
+ * [0, table_width * page_rows].
+ * The products run in f16 with f32 accumulation: q exactly (each row scaled by a power of two), E4M3 rows
+ * exactly, f32 rows and tails rounded to f16 relative to their largest value, softmax weights rounded to f16.
+ * workspace: ds4b200_attn_workspace_bytes(n_heads, head_dim) bytes of device memory, 16-byte aligned, not shared by calls that may
+ * overlap.  n_heads <= 1024.  Results do not depend on the contents of the workspace. */
+int64_t ds4b200_attn_workspace_bytes(int n_heads, int head_dim);
+int ds4b200_attn_decode_paged_bf16(const uint16_t *q, const ds4b200_paged_kv *host_kv, const int32_t *page_table,
+                                   int64_t table_width, const int32_t *kv_len, int64_t n_seqs, int n_heads,
+                                   float scale, const float *sink, int window, int n_first, uint16_t *out,
+                                   float *lse, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Attention of the tokens of a prompt chunk, several sequences in one call.  q, out bf16
+ * [n_tokens][n_heads][head_dim]; tokens q_start[b] .. q_start[b+1] - 1 (device int32 [n_seqs + 1], ascending from
+ * q_start[0] >= 0) are the last rows of sequence b, so token i of its n stands at row kv_len[b] - n + i and
+ * sees rows up to its own, with window and n_first as above.  Tokens outside [q_start[0], q_start[n_seqs])
+ * keep what out (and lse [n_tokens][n_heads]) held.  n_seqs <= 4096. */
+int ds4b200_attn_window_paged_bf16(const uint16_t *q, int64_t n_tokens, const ds4b200_paged_kv *host_kv,
+                                   const int32_t *page_table, int64_t table_width, const int32_t *kv_len,
+                                   const int32_t *q_start, int64_t n_seqs, int n_heads, float scale,
+                                   const float *sink, int window, int n_first, uint16_t *out, float *lse,
+                                   void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Pages of a pool.  refs[n_pages] counts the sequences that hold a page; 0 = free.  New pages are the free pages
+ * of lowest index, handed out in the order of the list or of the sequences.  Every *_out array may be the
+ * *_in array (in place) or another one that overlaps none of the inputs.  host_arrays (n_arrays <= 192, host memory, read during the
+ * call) lists the buffers whose pages move together, e.g. codes, scales and tail of every layer;
+ * page_bytes a multiple of 4.  *status (device int32): 0 done; > 0 that many free pages were missing; -1 the
+ * list or a table entry it leads to is not valid.  With a status other than 0 the outputs equal the
+ * inputs and no page is copied.  workspace: ds4b200_pages_workspace_bytes(n_pages, n_seqs, n_list) bytes,
+ * 16-byte aligned, not shared by calls that may overlap. */
+typedef struct ds4b200_page_array {
+    void *base;
+    int64_t page_bytes;
+} ds4b200_page_array;
+
+int64_t ds4b200_pages_workspace_bytes(int64_t n_pages, int64_t n_seqs, int64_t n_list);
+
+/* Copies page moves[i][0] to page moves[i][1] in every array.  Both in [0, n_pages); a page that is written may
+ * appear once only in the list (status -1 otherwise); a page may be read any number of times. */
+int ds4b200_pages_copy(const ds4b200_page_array *host_arrays, int n_arrays, int64_t n_pages, const int32_t *moves,
+                       int64_t n_moves, int32_t *status, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Sequence pairs[i][1] becomes a fork of sequence pairs[i][0]: it shares the pages that are full and gets
+ * a copy of the last one where that is filled in part.  A sequence may be forked any number of times in a
+ * call; a fork's target may appear once only, as a target, and what its table row held is dropped
+ * without being freed. */
+int ds4b200_pages_fork(const ds4b200_page_array *host_arrays, int n_arrays, int64_t n_pages, int page_rows,
+                       const int32_t *refs_in, int32_t *refs_out, const int32_t *table_in, int32_t *table_out,
+                       const int32_t *lens_in, int32_t *lens_out, int64_t n_seqs, int64_t table_width,
+                       const int32_t *pairs, int64_t n_pairs, int32_t *status, void *workspace,
+                       int64_t workspace_bytes, void *stream);
+
+/* Gives every sequence the pages for new_lens[b] rows (fewer than it has: nothing changes for it), each with
+ * a count of 1; lens_out[b] = max(lens_in[b], new_lens[b]). */
+int ds4b200_pages_reserve(int64_t n_pages, int page_rows, const int32_t *refs_in, int32_t *refs_out,
+                          const int32_t *table_in, int32_t *table_out, const int32_t *lens_in, int32_t *lens_out,
+                          const int32_t *new_lens, int64_t n_seqs, int64_t table_width, int32_t *status,
+                          void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Takes the pages of the listed sequences from them: counts go down by one, table rows become -1, lengths 0.  A
+ * sequence listed twice is freed once. */
+int ds4b200_pages_free(int64_t n_pages, int page_rows, const int32_t *refs_in, int32_t *refs_out,
+                       const int32_t *table_in, int32_t *table_out, const int32_t *lens_in, int32_t *lens_out,
+                       int64_t n_seqs, int64_t table_width, const int32_t *seqs, int64_t n_list, int32_t *status,
+                       void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Packs the pool: with n pages in use, the i-th page in use at or above n moves to the i-th free page below n
+ * (both in ascending order), in every array and every table entry; refs_out is positive below n and 0 from there
+ * on.  *n_live = n (device int32). */
+int ds4b200_pages_compact(const ds4b200_page_array *host_arrays, int n_arrays, int64_t n_pages,
+                          const int32_t *refs_in, int32_t *refs_out, const int32_t *table_in, int32_t *table_out,
+                          int64_t n_seqs, int64_t table_width, int32_t *n_live, void *workspace,
+                          int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
