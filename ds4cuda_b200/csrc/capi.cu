@@ -636,8 +636,7 @@ static int check_attn(const char *what, const ds4b200_paged_kv *kv, const void *
     } else {
         REQUIRE(kv->codes && kv->scales && a16(kv->codes) && a4(kv->scales), "%s: codes or scales missing or not aligned", what);
         if (kv->row_format == DS4B200_KV_FP8_BLOCK64) {
-            REQUIRE(kv->n_rot >= 0 && kv->n_rot % 4 == 0 && kv->n_rot < kv->head_dim && (kv->head_dim - kv->n_rot) % 64 == 0,
-                    "%s: n_rot must be a multiple of 4 with (head_dim - n_rot) %% 64 == 0", what);
+            REQUIRE(kv->n_rot == 0 || kv->n_rot == 64, "%s: n_rot must be 0 or 64", what);
             REQUIRE(kv->n_rot == 0 || (kv->tail && a16(kv->tail)), "%s: tail missing or not 16-byte aligned", what);
         }
     }

@@ -456,7 +456,7 @@ enum { DS4B200_KV_FP8_BLOCK64 = 0, DS4B200_KV_FP8_ROW = 1, DS4B200_KV_F32 = 2 };
 typedef struct ds4b200_paged_kv {
     int row_format;         /* DS4B200_KV_* */
     int head_dim;           /* 128, 256, 384 or 512 */
-    int n_rot;              /* width of the f32 tail (FP8_BLOCK64; (head_dim - n_rot) % 64 == 0, n_rot % 4 == 0) */
+    int n_rot;              /* width of the f32 tail (FP8_BLOCK64): 0 or 64 */
     int page_rows;          /* rows per page, at least 1 */
     int64_t n_pages;        /* n_pages * page_rows < 2^31 */
     const uint8_t *codes;   /* [n_pages * page_rows][head_dim], 16-byte aligned */
@@ -476,7 +476,8 @@ typedef struct ds4b200_paged_kv {
  * The products run in f16 with f32 accumulation: q exactly (each row scaled by a power of two), E4M3 rows
  * exactly, f32 rows and tails rounded to f16 relative to their largest value, softmax weights rounded to f16.
  * workspace: ds4b200_attn_workspace_bytes(n_heads, head_dim) bytes of device memory, 16-byte aligned, not shared by calls that may
- * overlap.  n_heads <= 1024.  Results do not depend on the contents of the workspace. */
+ * overlap.  n_heads <= 1024.  Results do not depend on the contents of the workspace, and a call repeats its bits; the
+ * lengths of all sequences decide where a long one is split, so the last bits of a sequence's result depend on them. */
 int64_t ds4b200_attn_workspace_bytes(int n_heads, int head_dim);
 int ds4b200_attn_decode_paged_bf16(const uint16_t *q, const ds4b200_paged_kv *host_kv, const int32_t *page_table,
                                    int64_t table_width, const int32_t *kv_len, int64_t n_seqs, int n_heads,
