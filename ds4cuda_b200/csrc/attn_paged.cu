@@ -5,6 +5,7 @@
 // lse_h = log(sum_j exp(s_hj) + exp(sink_h)).  One row is key and value of every head (the reference's
 // cache has one KV head; cuda/flash_attn.cu:148-313).
 #include <mutex>
+#include <type_traits>
 
 #include "device_utils.cuh"
 #include "kernels.cuh"
@@ -40,11 +41,12 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kCtas = 148;
 constexpr int kRows = 64;                   // query rows of an item, cache rows of a tile
 constexpr int kLoadWarp0 = 4, kLoadWarps = 8, kMmaWarp = 12;
-constexpr int kThreads = 13 * 32;
+constexpr int kThreads = 16 * 32;            // warps 14 and 15 only make the MMA warps' register group whole
 constexpr int kSplitItems = 4 * kThreads;   // up to this many items the tiles are cut into equal runs
 constexpr int kMinTiles = 2;                // of a run: below, the join costs more than the run saves
 constexpr float kRescale = 8.0f;            // log2 units
 constexpr int kScaleSets = 4;
+constexpr uint32_t kTmem = 0;               // all 512 columns are allocated, so they begin at column 0
 
 struct Meta { int64_t row0; int rows, parts; };
 
@@ -145,7 +147,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
     constexpr int D = NB * 128, kChunks = NB * 2, kTileBytes = kRows * D * 2;
     extern __shared__ __align__(1024) unsigned char smem[];
     unsigned char *q_s = smem, *k_s = smem + kTileBytes, *p_s = smem + 3 * kTileBytes;
-    __shared__ __align__(8) uint64_t full[2], s_full[2], s_free[2], p_full[2], pv_done[2], q_full, q_free;
+    constexpr int kParts = NB > 1 ? 2 : 1, kPart0 = (NB + 1) / 2;      // a tile is handed over in parts: its first kPart0 * 128 dims, the rest
+    __shared__ __align__(8) uint64_t full[2][kParts], s_full[2], s_free[2], p_full[2], pv_done[2][kParts], q_full, q_free;
     __shared__ uint32_t tmem_s;
     __shared__ int abort_s, start_slot, start_tile;
     __shared__ long long scan_s[kThreads / 32];
@@ -154,15 +157,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
     __shared__ float q_mul[kScaleSets][kRows];
     __shared__ __align__(16) float fac_s[kRows], inv_s[kRows];
     volatile int *abort_flag = &abort_s;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
     if (tid == 0) {
         abort_s = 0;
         start_slot = n_slots;
         start_tile = 0;
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&full[i], kLoadWarps); mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4);
-            mbar_init(&p_full[i], 4); mbar_init(&pv_done[i], 1);
+            mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4); mbar_init(&p_full[i], 4);
+            for (int k = 0; k < kParts; ++k) { mbar_init(&full[i][k], kLoadWarps); mbar_init(&pv_done[i][k], 1); }
         }
         mbar_init(&q_full, kLoadWarps); mbar_init(&q_free, 1);
     }
@@ -194,212 +197,270 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
-    const uint32_t tmem = tmem_s, s_tmem = tmem + NB * 64;
+    constexpr uint32_t tmem = kTmem, s_tmem = kTmem + NB * 64;
     if (split) start = Walk{start_slot, start_tile, 1, min(per, total - per * (long long)blockIdx.x)};
 
     if (warp >= kLoadWarp0 && warp < kLoadWarp0 + kLoadWarps) {
         // ------------------------------------------------------------------------------ loaders
+        // Loads run one unit ahead of the stores: a unit is a tile, or 128 dims of one with f32 rows.
+        tc::set_max_registers_up<152>();
+        constexpr bool kF32 = FMT == DS4B200_KV_F32;
+        constexpr int kUnits = kF32 ? NB : 1;
         const int r = (warp - kLoadWarp0) * 8 + (lane >> 2), part = lane & 3;   // four lanes per row, 16 of 64 dims each
         const uint32_t row_off = (uint32_t)(r * 128), sw = (uint32_t)(r & 7);
         const bool tail = FMT == DS4B200_KV_FP8_BLOCK64 && a.kv.n_rot != 0;
         const int n_scales = FMT == DS4B200_KV_FP8_BLOCK64 ? (D - a.kv.n_rot) / 64 : 1;
+        struct Unit {
+            uint4 v[8];                                  // codes of the row by chunk, or 2 chunks of f32
+            float4 tl[FMT == DS4B200_KV_FP8_BLOCK64 ? 4 : 1];
+            float sc0, sc1;
+        };
         Walk w = start;
         Item it;
-        int t0, t1, n = 0, seg = 0;
-        while (w.next(a, group, head_groups, n_slots, it, t0, t1)) {
-            const int32_t *table = a.page_table + it.b * a.table_width;
-            int at = 0;
-            auto find = [&](int t) -> int64_t {          // slot of this lane's row of tile t, or -1
-                const int i = t * kRows + r;
-                at = i < it.first ? i : it.lo + (i - it.first);
-                if (i >= it.n) return -1;
+        int t = 0, t1 = 0;                               // the tile after the one being loaded
+        int64_t slot = -1;                               // this lane's row of it, or -1
+        int at = 0;
+        bool more = w.next(a, group, head_groups, n_slots, it, t, t1), first = more;
+        auto find = [&]() {
+            const int i = t * kRows + r;
+            at = i < it.first ? i : it.lo + (i - it.first);
+            slot = -1;
+            if (more && i < it.n) {
                 const int pg = at / a.kv.page_rows;
-                const int page = __ldg(table + pg);
-                return page < 0 || page >= a.kv.n_pages ? -1 : (int64_t)page * a.kv.page_rows + (at - pg * a.kv.page_rows);
-            };
-            int64_t slot = find(t0);
-            {   // the item's query rows
-                uint4 v[kChunks][2];
-                uint32_t amax = 0;
-                const uint16_t *src = a.q + (it.row0 + r) * D + part * 16;
-#pragma unroll
-                for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        v[c][u] = r < it.rows ? __ldg(reinterpret_cast<const uint4 *>(src + c * 64 + u * 8)) : make_uint4(0, 0, 0, 0);
-                        const uint32_t x[4] = {v[c][u].x, v[c][u].y, v[c][u].z, v[c][u].w};
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) amax = max(amax, max(x[k] & 0x7fff0000u, (x[k] << 16) & 0x7fff0000u));
-                    }
-                amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                float up, down;
-                pow2_parts(__uint_as_float(amax), up, down);
-                tc::wait(&q_free, (uint32_t)((seg & 1) ^ 1), abort_flag, status);
-#pragma unroll
-                for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const uint32_t x[4] = {v[c][u].x, v[c][u].y, v[c][u].z, v[c][u].w};
-                        uint32_t o[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            o[k] = h2_bits(__floats2half2_rn(__uint_as_float(x[k] << 16) * down, __uint_as_float(x[k] & 0xffff0000u) * down));
-                        *reinterpret_cast<uint4 *>(q_s + c * 8192 + row_off + (((uint32_t)(part * 2 + u) ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-                    }
-                if (part == 0) q_mul[seg & (kScaleSets - 1)][r] = up * a.scale * kLog2e;
-                tc::fence_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&q_full);
+                const int page = __ldg(a.page_table + it.b * a.table_width + pg);
+                if (page >= 0 && page < a.kv.n_pages) slot = (int64_t)page * a.kv.page_rows + (at - pg * a.kv.page_rows);
             }
-            for (int t = t0; t < t1; ++t, ++n) {
-                const int buf = n & 1;
-                unsigned char *dst = k_s + buf * kTileBytes + row_off;
-                const uint32_t use = (uint32_t)(((n >> 1) & 1) ^ 1);
-                const int64_t my = slot;
-                const int my_at = at;
-                float mul = 1.0f;
-                if (FMT == DS4B200_KV_F32) {
-                    constexpr int kHalf = kChunks > 4 ? 4 : kChunks;
-                    const float *src = a.kv.raw + my * D + part * 4;
+        };
+        auto load = [&](Unit &u, int64_t my, int unit) {
+            if (kF32) {
+                const float *src = a.kv.raw + my * D + unit * 128 + part * 4;
 #pragma unroll
-                    for (int h = 0; h < kChunks; h += kHalf) {
-                        float4 v[kHalf][4];
+                for (int j = 0; j < 8; ++j)
+                    u.v[j] = my >= 0 ? __ldg(reinterpret_cast<const uint4 *>(src + (j >> 2) * 64 + (j & 3) * 16)) : make_uint4(0, 0, 0, 0);
+            } else {
+                const uint8_t *src = a.kv.codes + my * D + part * 16;
 #pragma unroll
-                        for (int c = 0; c < kHalf; ++c)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                if (h + c < kChunks)
-                                    v[c][j] = my >= 0 ? __ldg(reinterpret_cast<const float4 *>(src + (h + c) * 64 + j * 16)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (h == 0) {
-                            slot = t + 1 < t1 ? find(t + 1) : -1;
-                            tc::wait(&pv_done[buf], use, abort_flag, status);
-                        }
-#pragma unroll
-                        for (int c = 0; c < kHalf; ++c)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                if (h + c < kChunks)
-                                    *reinterpret_cast<uint2 *>(dst + (h + c) * 8192 + (((uint32_t)(2 * j + (part >> 1)) ^ sw) << 4) + (part & 1) * 8) =
-                                        make_uint2(sat_h2(v[c][j].x, v[c][j].y), sat_h2(v[c][j].z, v[c][j].w));
-                    }
+                for (int c = 0; c < kChunks; ++c)
+                    u.v[c] = my >= 0 && !(tail && c == kChunks - 1) ? __ldg(reinterpret_cast<const uint4 *>(src + c * 64)) : make_uint4(0, 0, 0, 0);
+                u.sc0 = u.sc1 = 0.0f;
+                if (FMT == DS4B200_KV_FP8_ROW) {
+                    u.sc0 = my >= 0 ? __ldg(a.kv.scales + my) : 1.0f;
                 } else {
-                    uint4 v[kChunks];
-                    float4 tl[4];
-                    float sc0 = 0.0f, sc1 = 0.0f;
-                    const uint8_t *src = a.kv.codes + my * D + part * 16;
+                    if (my >= 0 && part < n_scales) u.sc0 = __ldg(a.kv.scales + my * n_scales + part);
+                    if (my >= 0 && part + 4 < n_scales) u.sc1 = __ldg(a.kv.scales + my * n_scales + part + 4);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (FMT == DS4B200_KV_FP8_BLOCK64)
+                            u.tl[j] = my >= 0 && tail ? __ldg(reinterpret_cast<const float4 *>(a.kv.tail + my * 64 + part * 16 + j * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+            }
+        };
+        Unit ua, ub;
+        find();
+        int64_t my = slot;
+        int my_at = at, n = 0, seg = -1, unit = 0;
+        bool have = more;
+        float mul = 1.0f;
+        if (have) load(ua, my, 0);
+        auto step = [&](Unit &cur, Unit &nxt) {
+            const int buf = n & 1;
+            const uint32_t use = (uint32_t)(((n >> 1) & 1) ^ 1);
+            unsigned char *dst = k_s + buf * kTileBytes + row_off;
+            if (unit == 0) {
+                // the tile behind this one, and a segment's query rows ahead of its first tile
+                const bool starts = first;
+                const int64_t row0 = it.row0;
+                const int rows = it.rows;
+                first = false;
+                if (++t == t1) { more = w.next(a, group, head_groups, n_slots, it, t, t1); first = more; }
+                find();
+                if (starts) {
+                    ++seg;
+                    uint4 v[kChunks][2];
+                    uint32_t amax = 0;
+                    const uint16_t *src = a.q + (row0 + r) * D + part * 16;
 #pragma unroll
                     for (int c = 0; c < kChunks; ++c)
-                        v[c] = my >= 0 && !(tail && c == kChunks - 1) ? __ldg(reinterpret_cast<const uint4 *>(src + c * 64)) : make_uint4(0, 0, 0, 0);
-                    if (FMT == DS4B200_KV_FP8_ROW) {
-                        if (my >= 0) mul = __ldg(a.kv.scales + my);
-                    } else {
-                        if (my >= 0 && part < n_scales) sc0 = __ldg(a.kv.scales + my * n_scales + part);
-                        if (my >= 0 && part + 4 < n_scales) sc1 = __ldg(a.kv.scales + my * n_scales + part + 4);
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            tl[j] = my >= 0 && tail ? __ldg(reinterpret_cast<const float4 *>(a.kv.tail + my * 64 + part * 16 + j * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    }
-                    slot = t + 1 < t1 ? find(t + 1) : -1;
-                    float down = 1.0f;
-                    if (FMT == DS4B200_KV_FP8_BLOCK64) {
-                        float top = fmaxf(fmaxf(amax4(tl[0]), amax4(tl[1])), fmaxf(amax4(tl[2]), amax4(tl[3]))) * (1.0f / 256.0f);
-                        top = fmaxf(top, fmaxf(sc0, sc1));
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                        pow2_parts(top, mul, down);
-                        sc0 *= down;
-                        sc1 *= down;
-                    }
-                    tc::wait(&pv_done[buf], use, abort_flag, status);
+                        for (int u = 0; u < 2; ++u) {
+                            v[c][u] = r < rows ? __ldg(reinterpret_cast<const uint4 *>(src + c * 64 + u * 8)) : make_uint4(0, 0, 0, 0);
+                            const uint32_t x[4] = {v[c][u].x, v[c][u].y, v[c][u].z, v[c][u].w};
 #pragma unroll
-                    for (int c = 0; c < kChunks; ++c) {
-                        uint32_t o[8];
-                        const uint32_t x[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            o[2 * k] = h2_bits(e4m3x2(x[k] & 0xffffu));
-                            o[2 * k + 1] = h2_bits(e4m3x2(x[k] >> 16));
+                            for (int k = 0; k < 4; ++k) amax = max(amax, max(x[k] & 0x7fff0000u, (x[k] << 16) & 0x7fff0000u));
                         }
-                        if (FMT == DS4B200_KV_FP8_BLOCK64) {
-                            const __half2 f = __float2half2_rn(__shfl_sync(0xffffffffu, c < 4 ? sc0 : sc1, (lane & ~3) | (c & 3)));
+                    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                    float up, down;
+                    pow2_parts(__uint_as_float(amax), up, down);
+                    tc::wait(&q_free, (uint32_t)((seg & 1) ^ 1), abort_flag, status);
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) o[k] = h2_bits(__hmul2(*reinterpret_cast<__half2 *>(&o[k]), f));
-                            if (tail && c == kChunks - 1) {
+                    for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-                                for (int j = 0; j < 4; ++j) {
-                                    o[2 * j] = h2_bits(__floats2half2_rn(tl[j].x * down, tl[j].y * down));
-                                    o[2 * j + 1] = h2_bits(__floats2half2_rn(tl[j].z * down, tl[j].w * down));
-                                }
-                            }
+                        for (int u = 0; u < 2; ++u) {
+                            const uint32_t x[4] = {v[c][u].x, v[c][u].y, v[c][u].z, v[c][u].w};
+                            uint32_t o[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                o[k] = h2_bits(__floats2half2_rn(__uint_as_float(x[k] << 16) * down, __uint_as_float(x[k] & 0xffff0000u) * down));
+                            *reinterpret_cast<uint4 *>(q_s + c * 8192 + row_off + (((uint32_t)(part * 2 + u) ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
                         }
-                        *reinterpret_cast<uint4 *>(dst + c * 8192 + (((uint32_t)(part * 2) ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-                        *reinterpret_cast<uint4 *>(dst + c * 8192 + (((uint32_t)(part * 2 + 1) ^ sw) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
-                    }
+                    if (part == 0) q_mul[seg & (kScaleSets - 1)][r] = up * a.scale * kLog2e;
+                    tc::fence_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&q_full);
                 }
-                if (part == 0) {
-                    mul = mul == 0.0f ? 1.0e-30f : mul;
-                    if (FMT != DS4B200_KV_F32) { row_mul[buf][r] = mul; row_div[buf][r] = 1.0f / mul; }
-                    row_add[buf][r] = my >= 0 ? (FMT == DS4B200_KV_F32 ? 0.0f : log2f(mul)) : -INFINITY;
-                    row_at[buf][r] = my_at;
-                }
+            }
+            if (kUnits > 1 && unit + 1 < kUnits) load(nxt, my, unit + 1);
+            else load(nxt, slot, 0);
+            auto hand_over = [&](int k) {
                 tc::fence_async();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&full[buf]);
+                if (lane == 0) mbar_arrive(&full[buf][k]);
+            };
+            if (kF32) {
+                if (unit == 0) tc::wait(&pv_done[buf][0], use, abort_flag, status);
+                if (kParts > 1 && unit == kPart0) tc::wait(&pv_done[buf][kParts - 1], use, abort_flag, status);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    *reinterpret_cast<uint2 *>(dst + unit * 16384 + (j >> 2) * 8192 + (((uint32_t)(2 * (j & 3) + (part >> 1)) ^ sw) << 4) + (part & 1) * 8) =
+                        make_uint2(sat_h2(__uint_as_float(cur.v[j].x), __uint_as_float(cur.v[j].y)),
+                                   sat_h2(__uint_as_float(cur.v[j].z), __uint_as_float(cur.v[j].w)));
+                if (kParts > 1 && unit == kPart0 - 1) hand_over(0);
+            } else {
+                float down = 1.0f;
+                if (FMT == DS4B200_KV_FP8_ROW) mul = cur.sc0;
+                if (FMT == DS4B200_KV_FP8_BLOCK64) {
+                    float top = fmaxf(cur.sc0, cur.sc1);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) top = fmaxf(top, amax4(cur.tl[FMT == DS4B200_KV_FP8_BLOCK64 ? j : 0]) * (1.0f / 256.0f));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    pow2_parts(top, mul, down);
+                    cur.sc0 *= down;
+                    cur.sc1 *= down;
+                }
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c) {
+                    if (c == 0) tc::wait(&pv_done[buf][0], use, abort_flag, status);
+                    if (kParts > 1 && c == 2 * kPart0) {
+                        hand_over(0);
+                        tc::wait(&pv_done[buf][kParts - 1], use, abort_flag, status);
+                    }
+                    uint32_t o[8];
+                    const uint32_t x[4] = {cur.v[c].x, cur.v[c].y, cur.v[c].z, cur.v[c].w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        o[2 * k] = h2_bits(e4m3x2(x[k] & 0xffffu));
+                        o[2 * k + 1] = h2_bits(e4m3x2(x[k] >> 16));
+                    }
+                    if (FMT == DS4B200_KV_FP8_BLOCK64) {
+                        const __half2 f = __float2half2_rn(__shfl_sync(0xffffffffu, c < 4 ? cur.sc0 : cur.sc1, (lane & ~3) | (c & 3)));
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) o[k] = h2_bits(__hmul2(*reinterpret_cast<__half2 *>(&o[k]), f));
+                        if (tail && c == kChunks - 1) {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const float4 x4 = cur.tl[FMT == DS4B200_KV_FP8_BLOCK64 ? j : 0];
+                                o[2 * j] = h2_bits(__floats2half2_rn(x4.x * down, x4.y * down));
+                                o[2 * j + 1] = h2_bits(__floats2half2_rn(x4.z * down, x4.w * down));
+                            }
+                        }
+                    }
+                    *reinterpret_cast<uint4 *>(dst + c * 8192 + (((uint32_t)(part * 2) ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+                    *reinterpret_cast<uint4 *>(dst + c * 8192 + (((uint32_t)(part * 2 + 1) ^ sw) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+                }
             }
-            ++seg;
+            if (kUnits == 1 || ++unit == kUnits) {
+                unit = 0;
+                if (part == 0) {
+                    mul = mul == 0.0f ? 1.0e-30f : mul;
+                    if (!kF32) { row_mul[buf][r] = mul; row_div[buf][r] = 1.0f / mul; }
+                    row_add[buf][r] = my >= 0 ? (kF32 ? 0.0f : log2f(mul)) : -INFINITY;
+                    row_at[buf][r] = my_at;
+                }
+                hand_over(kParts - 1);
+                my = slot;
+                my_at = at;
+                have = more;
+                ++n;
+            }
+        };
+        while (have) {                                   // two units' registers take turns, so that no copy waits for a load
+            step(ua, ub);
+            if (!have) break;
+            step(ub, ua);
         }
-    } else if (warp == kMmaWarp) {
-        // ------------------------------------------------------------------------------ MMA issuer
-        if (lane == 0) {
-            const uint64_t q_desc = tc::desc(smem_addr(q_s), 0), k_desc = tc::desc(smem_addr(k_s), 0);
-            const uint64_t v_desc = tc::desc(smem_addr(k_s), 8192), p_desc = tc::desc(smem_addr(p_s), 0);
+    } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
+        // ------------------------------------------------------------------------------ MMA issuers, one per product
+        tc::set_max_registers_down<80>();
+        {
+            const uint32_t one = tc::elect();
+            const uint32_t q_desc = tc::desc_lo(smem_addr(q_s), 0), k_desc = tc::desc_lo(smem_addr(k_s), 0);
+            const uint32_t v_desc = tc::desc_lo(smem_addr(k_s), 8192), p_desc = tc::desc_lo(smem_addr(p_s), 0);
             constexpr uint32_t s_idesc = tc::idesc_f16(64, 64, false);
-            auto weighted = [&](int k, bool fresh, uint32_t o_idesc) {      // O^T (+)= V^T P^T of tile k
-                const int buf = k & 1;
+            constexpr uint32_t o_idesc = tc::idesc_f16(128, 64, true);
+            auto weighted = [&](auto which, int k, uint32_t more) {         // O^T (+)= V^T P^T of tile k
+                constexpr int buf = decltype(which)::value;
+                constexpr uint32_t v0 = (uint32_t)((buf * kTileBytes) >> 4), p0 = (uint32_t)((buf * 8192) >> 4);
                 tc::wait(&p_full[buf], (uint32_t)((k >> 1) & 1), abort_flag, status);
                 tc::fence_after();
 #pragma unroll
-                for (int m = 0; m < NB; ++m)
+                for (int m = 0; m < NB; ++m) {
 #pragma unroll
                     for (int ks = 0; ks < 4; ++ks)
-                        tc::mma_f16(tmem + m * 64, v_desc + (uint64_t)((buf * kTileBytes + m * 16384 + ks * 2048) >> 4),
-                                    p_desc + (uint64_t)((buf * 8192 + ks * 32) >> 4), o_idesc, !(fresh && ks == 0));
-                tc::commit(&pv_done[buf]);
+                        tc::mma_f16(one, kTmem + m * 64, v_desc + v0 + (uint32_t)((m * 16384 + ks * 2048) >> 4), p_desc + p0 + (uint32_t)((ks * 32) >> 4),
+                                    o_idesc, ks > 0 ? 1u : more);
+                    if (kParts > 1 && m == kPart0 - 1) tc::commit(one, &pv_done[buf][0]);
+                }
+                tc::commit(one, &pv_done[buf][kParts - 1]);
             };
+            auto scores = [&](auto which, int k) {                          // S = Q K^T of tile k
+                constexpr int buf = decltype(which)::value;
+                constexpr uint32_t k0 = (uint32_t)((buf * kTileBytes) >> 4);
+                tc::wait(&s_free[buf], (uint32_t)(((k >> 1) & 1) ^ 1), abort_flag, status);
+#pragma unroll
+                for (int c = 0; c < kChunks; ++c) {
+                    if (c == 0 || (kParts > 1 && c == 2 * kPart0)) {
+                        tc::wait(&full[buf][c == 0 ? 0 : kParts - 1], (uint32_t)((k >> 1) & 1), abort_flag, status);
+                        tc::fence_after();
+                    }
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks)
+                        tc::mma_f16(one, kTmem + NB * 64 + buf * 64, q_desc + (uint32_t)((c * 8192 + ks * 32) >> 4),
+                                    k_desc + k0 + (uint32_t)((c * 8192 + ks * 32) >> 4), s_idesc, c > 0 || ks > 0);
+                }
+                tc::commit(one, &s_full[buf]);
+            };
+            using Zero = std::integral_constant<int, 0>;
+            using One = std::integral_constant<int, 1>;
             Walk w = start;
             Item it;
             int t0, t1, n = 0, seg = 0;
-            bool fresh = false;
-            uint32_t o_idesc = 0;
-            while (w.next(a, group, head_groups, n_slots, it, t0, t1)) {
-                tc::wait(&q_full, (uint32_t)(seg & 1), abort_flag, status);
-                for (int t = t0; t < t1; ++t, ++n) {
-                    const int buf = n & 1;
-                    tc::wait(&full[buf], (uint32_t)((n >> 1) & 1), abort_flag, status);
-                    tc::wait(&s_free[buf], (uint32_t)(((n >> 1) & 1) ^ 1), abort_flag, status);
-                    tc::fence_after();
-#pragma unroll
-                    for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-                        for (int ks = 0; ks < 4; ++ks)
-                            tc::mma_f16(s_tmem + buf * 64, q_desc + (uint64_t)((c * 8192 + ks * 32) >> 4),
-                                        k_desc + (uint64_t)((buf * kTileBytes + c * 8192 + ks * 32) >> 4), s_idesc, c > 0 || ks > 0);
-                    tc::commit(&s_full[buf]);
-                    if (t + 1 == t1) tc::commit(&q_free);
-                    if (n > 0) weighted(n - 1, fresh, o_idesc);
-                    fresh = t == t0;
-                    o_idesc = tc::idesc_f16(128, (it.rows + 15) / 16 * 16, true);
+            while (__shfl_sync(0xffffffffu, (int)w.next(a, group, head_groups, n_slots, it, t0, t1), 0)) {
+                t0 = __shfl_sync(0xffffffffu, t0, 0);
+                t1 = __shfl_sync(0xffffffffu, t1, 0);
+                if (warp == kMmaWarp) {
+                    tc::wait(&q_full, (uint32_t)(seg & 1), abort_flag, status);
+                    for (int t = t0; t < t1; ++t, ++n) {
+                        if (n & 1) scores(One(), n);
+                        else scores(Zero(), n);
+                    }
+                    tc::commit(one, &q_free);
+                    ++seg;
+                } else {
+                    for (int t = t0; t < t1; ++t, ++n) {
+                        if (n & 1) weighted(One(), n, t > t0);
+                        else weighted(Zero(), n, t > t0);
+                    }
                 }
-                ++seg;
             }
-            if (n > 0) weighted(n - 1, fresh, o_idesc);
         }
         __syncwarp();
+    } else if (warp > kMmaWarp + 1) {
+        tc::set_max_registers_down<80>();
     } else {
         // ------------------------------------------------------------------------------ softmax and output
-        const int row = warp * 16 + lane;               // lanes 0-15 hold a row of S each
-        const bool mine = lane < 16;
+        const int row = warp * 16 + (lane >> 2);        // four lanes share rows `row` and `row` + 8 of S, 16 columns each
         const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
         const bool several = head_groups == 1 && group > 1;
         Meta last{0, 0, 0};
@@ -408,62 +469,67 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
         int t0, t1, n = 0, seg = 0;
         long long done = 0;
         while (w.next(a, group, head_groups, n_slots, it, t0, t1)) {
-            float qk = 0.0f;
-            const int p = it.p0 + (several ? (row & 63) / a.n_heads : 0);
-            const int from = a.window > 0 ? p - a.window : -1;      // rows above it are in the window
-            float m = -INFINITY, l = 0.0f;
+            float qk[2] = {0.0f, 0.0f}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+            const int p[2] = {it.p0 + (several ? row / a.n_heads : 0), it.p0 + (several ? (row + 8) / a.n_heads : 0)};
             for (int t = t0; t < t1; ++t, ++n) {
                 const int buf = n & 1;
-                tc::wait(&full[buf], (uint32_t)((n >> 1) & 1), abort_flag, status);
+                tc::wait(&full[buf][kParts - 1], (uint32_t)((n >> 1) & 1), abort_flag, status);
                 tc::wait(&s_full[buf], (uint32_t)((n >> 1) & 1), abort_flag, status);
                 tc::fence_after();
                 // written ahead of the segment's first tile by the same warps; q_full itself may be phases ahead of this warp
-                if (t == t0 && mine) qk = q_mul[seg & (kScaleSets - 1)][row];
-                uint32_t x0[32], x1[32];
-                tc::ld32(s_tmem + buf * 64 + lane_base, x0);
-                tc::ld32(s_tmem + buf * 64 + 32 + lane_base, x1);
+                if (t == t0)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) qk[h] = q_mul[seg & (kScaleSets - 1)][row + 8 * h];
+                uint32_t x[32];
+                tc::ld_16x64(s_tmem + buf * 64 + lane_base, x);
                 tc::wait_ld();
                 tc::fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&s_free[buf]);
-                float v[64];
-                float top = -INFINITY;
+                float v[2][16], top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int j = 0; j < 64; j += 4) {
-                    const float4 add = *reinterpret_cast<const float4 *>(&row_add[buf][j]);
-                    const float ad[4] = {add.x, add.y, add.z, add.w};
-                    float mu[4] = {1.f, 1.f, 1.f, 1.f};
-                    if (FMT != DS4B200_KV_F32) {
-                        const float4 f = *reinterpret_cast<const float4 *>(&row_mul[buf][j]);
-                        mu[0] = f.x; mu[1] = f.y; mu[2] = f.z; mu[3] = f.w;
-                    }
+                for (int i = 0; i < 8; ++i) {
+                    const int c = 8 * i + 2 * (lane & 3);
+                    const float2 add = *reinterpret_cast<const float2 *>(&row_add[buf][c]);
+                    float2 mu = make_float2(1.0f, 1.0f);
+                    if (FMT != DS4B200_KV_F32) mu = *reinterpret_cast<const float2 *>(&row_mul[buf][c]);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float s = __uint_as_float(j + k < 32 ? x0[(j + k) & 31] : x1[(j + k) & 31]) * qk;
-                        v[j + k] = fmaf(s, mu[k], ad[k]);
+                    for (int h = 0; h < 2; ++h) {
+                        v[h][2 * i] = fmaf(__uint_as_float(x[4 * i + 2 * h]) * qk[h], mu.x, add.x);
+                        v[h][2 * i + 1] = fmaf(__uint_as_float(x[4 * i + 2 * h + 1]) * qk[h], mu.y, add.y);
                     }
                     if (several) {
-                        const int4 at4 = *reinterpret_cast<const int4 *>(&row_at[buf][j]);
-                        const int at[4] = {at4.x, at4.y, at4.z, at4.w};
+                        const int2 at = *reinterpret_cast<const int2 *>(&row_at[buf][c]);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            if (at[k] > p || (at[k] <= from && at[k] >= a.n_first)) v[j + k] = -INFINITY;
+                        for (int h = 0; h < 2; ++h) {
+                            const int from = a.window > 0 ? p[h] - a.window : -1;       // rows above it are in the window
+                            if (at.x > p[h] || (at.x <= from && at.x >= a.n_first)) v[h][2 * i] = -INFINITY;
+                            if (at.y > p[h] || (at.y <= from && at.y >= a.n_first)) v[h][2 * i + 1] = -INFINITY;
+                        }
                     }
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) top = fmaxf(top, v[j + k]);
+                    for (int h = 0; h < 2; ++h) top[h] = fmaxf(top[h], fmaxf(v[h][2 * i], v[h][2 * i + 1]));
                 }
-                const bool grown = mine && m > -INFINITY && top > m + kRescale;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+                    top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+                }
+                const bool grown[2] = {m[0] > -INFINITY && top[0] > m[0] + kRescale, m[1] > -INFINITY && top[1] > m[1] + kRescale};
                 uint32_t any;
                 asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-                             : "=r"(any) : "r"((uint32_t)grown) : "memory");
+                             : "=r"(any) : "r"((uint32_t)(grown[0] || grown[1])) : "memory");
                 if (any) {
                     // every row's accumulators (a column of O^T) follow its maximum; the previous tile's MMAs first
-                    const float f = grown ? exp2f(m - top) : 1.0f;
-                    if (grown) { m = top; l *= f; }
-                    if (mine) fac_s[row] = f;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float f = grown[h] ? tc::exp2_approx(m[h] - top[h]) : 1.0f;
+                        if (grown[h]) { m[h] = top[h]; l[h] *= f; }
+                        if ((lane & 3) == 0) fac_s[row + 8 * h] = f;
+                    }
                     asm volatile("bar.sync 1, 128;" ::: "memory");
                     if (t > t0) {
-                        tc::wait(&pv_done[buf ^ 1], (uint32_t)(((n - 1) >> 1) & 1), abort_flag, status);
+                        tc::wait(&pv_done[buf ^ 1][kParts - 1], (uint32_t)(((n - 1) >> 1) & 1), abort_flag, status);
                         tc::fence_after();
                         for (int col = 0; col < (it.rows + 15) / 16 * 16; col += 16)
 #pragma unroll 1
@@ -478,53 +544,59 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
                         tc::wait_st();
                     }
                 }
-                if (m == -INFINITY) m = top;
-                const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-                for (int j = 0; j < 64; j += 8) {
-                    uint32_t o[4];
+                for (int h = 0; h < 2; ++h) {
+                    if (m[h] == -INFINITY) m[h] = top[h];
+                    const float ref = m[h] == -INFINITY ? 0.0f : m[h];
+                    unsigned char *dst = p_s + buf * 8192 + (row + 8 * h) * 128 + (lane & 3) * 4;
+                    float sum = 0.0f;
 #pragma unroll
-                    for (int k = 0; k < 8; k += 4) {
-                        float e[4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) e[i] = exp2f(v[j + k + i] - ref);
+                    for (int i = 0; i < 8; ++i) {
+                        const float e0 = tc::exp2_approx(v[h][2 * i] - ref), e1 = tc::exp2_approx(v[h][2 * i + 1] - ref);
                         if (FMT == DS4B200_KV_F32) {
-                            l += (e[0] + e[1]) + (e[2] + e[3]);
+                            sum += e0 + e1;
                         } else {
-                            const float4 d = *reinterpret_cast<const float4 *>(&row_div[buf][j + k]);
-                            l += fmaf(e[0], d.x, e[1] * d.y) + fmaf(e[2], d.z, e[3] * d.w);
+                            const float2 d = *reinterpret_cast<const float2 *>(&row_div[buf][8 * i + 2 * (lane & 3)]);
+                            sum = fmaf(e0, d.x, fmaf(e1, d.y, sum));
                         }
-                        o[k / 2] = h2_bits(__floats2half2_rn(e[0], e[1]));
-                        o[k / 2 + 1] = h2_bits(__floats2half2_rn(e[2], e[3]));
+                        *reinterpret_cast<uint32_t *>(dst + (((uint32_t)i ^ (uint32_t)(row & 7)) << 4)) = h2_bits(__floats2half2_rn(e0, e1));
                     }
-                    if (mine)
-                        *reinterpret_cast<uint4 *>(p_s + buf * 8192 + row * 128 + (((uint32_t)(j / 8) ^ (uint32_t)(row & 7)) << 4)) =
-                            make_uint4(o[0], o[1], o[2], o[3]);
+                    l[h] += sum;
                 }
                 tc::fence_async();
                 tc::fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[buf]);
             }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+            }
             // the segment's accumulators
-            tc::wait(&pv_done[(n - 1) & 1], (uint32_t)(((n - 1) >> 1) & 1), abort_flag, status);
+            tc::wait(&pv_done[(n - 1) & 1][kParts - 1], (uint32_t)(((n - 1) >> 1) & 1), abort_flag, status);
             tc::fence_after();
             const bool whole = t0 == 0 && t1 == it.tiles;
-            float inv = 1.0f;
             const int part = 2 * (int)blockIdx.x + (t0 == 0 ? 1 : 0);
-            if (whole) {
-                const float mine2 = l > 0.0f ? m + log2f(l) : (l == l ? -INFINITY : l);
-                float lse2 = mine2;
-                if (a.sink && mine && row < it.rows) {
-                    const float s2 = a.sink[(it.row0 + row) % a.n_heads] * kLog2e, hi = fmaxf(mine2, s2);
-                    lse2 = hi == -INFINITY ? hi : hi + log2f(exp2f(mine2 - hi) + exp2f(s2 - hi));
+            if ((lane & 3) == 0)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int rw = row + 8 * h;
+                    float inv = 1.0f;
+                    if (!whole) {
+                        part_ml[part * kRows + rw] = make_float2(m[h], l[h]);
+                    } else if (rw < it.rows) {
+                        const float own = l[h] > 0.0f ? m[h] + log2f(l[h]) : (l[h] == l[h] ? -INFINITY : l[h]);
+                        float lse2 = own;
+                        if (a.sink) {
+                            const float s2 = a.sink[(it.row0 + rw) % a.n_heads] * kLog2e, hi = fmaxf(own, s2);
+                            lse2 = hi == -INFINITY ? hi : hi + log2f(exp2f(own - hi) + exp2f(s2 - hi));
+                        }
+                        inv = m[h] == -INFINITY ? 0.0f : exp2f(m[h] - lse2);
+                        if (a.lse) a.lse[it.row0 + rw] = lse2 * (1.0f / kLog2e);
+                    }
+                    inv_s[rw] = inv;
                 }
-                inv = m == -INFINITY ? 0.0f : exp2f(m - lse2);
-                if (a.lse && mine && row < it.rows) a.lse[it.row0 + row] = lse2 * (1.0f / kLog2e);
-            } else if (mine) {
-                part_ml[part * kRows + row] = make_float2(m, l);
-            }
-            if (mine) inv_s[row] = inv;
             asm volatile("bar.sync 1, 128;" ::: "memory");
             for (int b = 0; b < NB; ++b)
                 for (int col = 0; col < it.rows; col += 16) {

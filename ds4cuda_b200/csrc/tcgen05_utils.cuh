@@ -15,33 +15,52 @@ __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Shared-memory operand: 128-byte rows, 128-byte swizzle, groups of eight rows 1024 bytes apart; `lbo` is the
-// distance between 64-element column blocks where the operand lies with its long side contiguous.
-__device__ __forceinline__ uint64_t desc(uint32_t saddr, uint32_t lbo) {
-    return ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61) |
-           (uint64_t)((saddr & 0x3FFFFu) >> 4);
-}
+// Shared-memory operands: 128-byte rows, 128-byte swizzle, groups of eight rows 1024 bytes apart.  The low word of the
+// descriptor holds the address and, where the operand lies with its long side contiguous, `lbo`, the distance between
+// blocks of 64 elements of that side; the high word is the same for all.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) { return ((lbo >> 4) << 16) | ((saddr & 0x3FFFFu) >> 4); }
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
 // f16 x f16 -> f32, both operands in shared memory; bit 15: A lies with M contiguous.
 __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool a_m_major) {
     return (1u << 4) | (a_m_major ? 1u << 15 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+// One lane of a converged warp (always the same one).
+__device__ __forceinline__ uint32_t elect() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+    return e;
 }
-// One arrival on `bar` when every MMA this thread has issued so far has finished.
-__device__ __forceinline__ void commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+// Issued by the lane with `one` set, as a predicate of the instruction.  The whole warp runs the loop around it, on values the
+// compiler knows to be uniform (a shuffle from lane 0): the operands then live in uniform registers, and an MMA of M 64, N 64, K 16
+// takes the 32 cycles its 4 KiB of operands need of shared memory.  Issued from a branch that one lane takes, each operand moves
+// to a uniform register for every MMA, and the same MMA took 48 to 150 cycles, depending on the code around it.
+__device__ __forceinline__ void mma_f16(uint32_t one, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\t.reg .b64 x, y;\n\tmov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "setp.ne.b32 q, %6, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHi), "r"(one) : "memory");
 }
-__device__ __forceinline__ void ld32(uint32_t addr, uint32_t (&r)[32]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+// One arrival on `bar` when every MMA the electing lane has issued so far has finished.
+__device__ __forceinline__ void commit(uint32_t one, uint64_t *bar) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+                 ::"r"(smem_addr(bar)), "r"(one) : "memory");
+}
+template <int N> __device__ __forceinline__ void set_max_registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void set_max_registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+// 16 lanes x 64 columns: register 4 i + k of lane t is row t / 4 + 8 (k / 2), column 8 i + 2 (t % 4) + k % 2.
+__device__ __forceinline__ void ld_16x64(uint32_t addr, uint32_t (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
                  "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
                    "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
                    "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
                    "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                  : "r"(addr));
+}
+__device__ __forceinline__ float exp2_approx(float x) {     // ex2.approx.ftz: relative error 2^-22, 0 below 2^-126
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 __device__ __forceinline__ void ld16(uint32_t addr, uint32_t (&r)[16]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -64,13 +83,15 @@ __device__ __forceinline__ bool try_phase(uint64_t *bar, uint32_t parity) {
                  "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(smem_addr(bar)), "r"(parity) : "memory");
     return done != 0;
 }
-static __device__ __noinline__ void wait_slow(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int *status) {
+__device__ __forceinline__ void wait_slow(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int *status) {
     const long long t0 = clock64();
     for (;;) {
         if (*abort_flag) return;
 #pragma unroll 1
-        for (int i = 0; i < 64; ++i)
+        for (int i = 0; i < 64; ++i) {
+            __nanosleep(20);                // a poll is a shared-memory access that competes with the operands of the MMAs
             if (try_phase(bar, parity)) return;
+        }
         if (clock64() - t0 > kWaitCycles) {
             *abort_flag = 1;
             atomicOr(status, kStatusBulkCopyTimeout);
