@@ -41,7 +41,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kCtas = 148;
 constexpr int kRows = 64;                   // query rows of an item, cache rows of a tile
 constexpr int kLoadWarp0 = 4, kLoadWarps = 8, kMmaWarp = 12;
-constexpr int kThreads = 16 * 32;            // warps 14 and 15 only make the MMA warps' register group whole
+constexpr int kThreads = 16 * 32;            // warp 15 only makes a register group whole
 constexpr int kSplitItems = 4 * kThreads;   // up to this many items the tiles are cut into equal runs
 constexpr int kMinTiles = 2;                // of a run: below, the join costs more than the run saves
 constexpr float kRescale = 8.0f;            // log2 units
@@ -104,28 +104,13 @@ __device__ __forceinline__ long long block_scan64(long long v, long long *scratc
     return before + x - v;
 }
 
-// A CTA's run: segments of items.  next() gives the coming segment's item and its tiles [t0, t1).
-struct Walk {
-    int slot, tile, step;
-    long long left;
-    __device__ __forceinline__ bool next(const AttnArgs &a, int group, int head_groups, int n_slots, Item &it, int &t0, int &t1) {
-        while (left > 0 && slot < n_slots) {
-            it = get_item(a, group, head_groups, slot);
-            slot += step;
-            if (it.tiles == 0) continue;
-            t0 = tile;
-            t1 = (int)min((long long)it.tiles, t0 + left);
-            tile = 0;
-            if (step == 1) left -= t1 - t0;
-            return true;
-        }
-        return false;
-    }
-};
-
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
 __device__ __forceinline__ __half2 e4m3x2(uint32_t two) {
     return __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3));
+}
+__device__ __forceinline__ uint32_t h2b(float x, float y) {         // bf16 pair
+    __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<uint32_t *>(&b);
 }
 __device__ __forceinline__ uint32_t sat_h2(float x, float y) {      // finite values beyond f16 become +-65504
     x = fabsf(x) < INFINITY ? fminf(fmaxf(x, -65504.f), 65504.f) : x;
@@ -141,14 +126,58 @@ __device__ __forceinline__ void pow2_parts(float x, float &up, float &down) {
     down = __uint_as_float((uint32_t)(127 - e) << 23);
 }
 
+// What the scheduling warp hands to the others: an item and the tiles [t0, t1) of it that this CTA takes; t1 < 0 ends.
+struct Segment {
+    Item it;
+    int t0, t1;
+};
+constexpr int kSegRing = 4;
+constexpr int kSegReaders = kLoadWarps + 4 + 2;
+
+struct TcArgs {
+    AttnArgs a;
+    int group, head_groups, n_slots, split, page_shift;
+    Meta *meta;
+    float2 *part_ml;
+    float *part_o;
+    int *status;
+};
+
+__device__ __forceinline__ uint4 ld_row16(const void *p) {          // read once per CTA: no place in L1
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+
 template <int NB, int FMT>          // NB: head_dim / 128
-__global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, int group, int head_groups, int n_slots, int split,
-                                                              Meta *meta, float2 *part_ml, float *part_o, int *status) {
+__global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_constant__ TcArgs g) {
     constexpr int D = NB * 128, kChunks = NB * 2, kTileBytes = kRows * D * 2;
+    constexpr int kParts = NB > 1 ? 2 : 1, kPart0 = (NB + 1) / 2;      // a tile is handed over in parts: its first kPart0 * 128 dims, the rest
+    constexpr uint32_t o_tmem = kTmem, s_tmem = kTmem + NB * 64;
+    const AttnArgs &a = g.a;
     extern __shared__ __align__(1024) unsigned char smem[];
     unsigned char *q_s = smem, *k_s = smem + kTileBytes, *p_s = smem + 3 * kTileBytes;
-    constexpr int kParts = NB > 1 ? 2 : 1, kPart0 = (NB + 1) / 2;      // a tile is handed over in parts: its first kPart0 * 128 dims, the rest
     __shared__ __align__(8) uint64_t full[2][kParts], s_full[2], s_free[2], p_full[2], pv_done[2][kParts], q_full, q_free;
+    __shared__ __align__(8) uint64_t seg_full[kSegRing], seg_free[kSegRing];
+    __shared__ Segment seg_s[kSegRing];
     __shared__ uint32_t tmem_s;
     __shared__ int abort_s, start_slot, start_tile;
     __shared__ long long scan_s[kThreads / 32];
@@ -157,187 +186,206 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
     __shared__ float q_mul[kScaleSets][kRows];
     __shared__ __align__(16) float fac_s[kRows], inv_s[kRows];
     volatile int *abort_flag = &abort_s;
+    int *status = g.status;
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
     if (tid == 0) {
         abort_s = 0;
-        start_slot = n_slots;
+        start_slot = g.n_slots;
         start_tile = 0;
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4); mbar_init(&p_full[i], 4);
             for (int k = 0; k < kParts; ++k) { mbar_init(&full[i][k], kLoadWarps); mbar_init(&pv_done[i][k], 1); }
         }
         mbar_init(&q_full, kLoadWarps); mbar_init(&q_free, 1);
+        for (int i = 0; i < kSegRing; ++i) { mbar_init(&seg_full[i], 1); mbar_init(&seg_free[i], kSegReaders); }
     }
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_s)));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    Walk start{(int)blockIdx.x, 0, (int)gridDim.x, 1ll << 62};
-    long long per = 0, total = 0;
-    if (split) {
-        for (int base = 0; base < n_slots; base += kThreads) {
-            const int s = base + tid;
-            long long sum;
-            block_scan64(s < n_slots ? get_item(a, group, head_groups, s).tiles : 0, scan_s, &sum);
-            total += sum;
+    // This CTA's share of the tiles: with `split` a run of the list of all of them, else whole items, every gridDim.x-th.
+    long long per = 1, left = 1ll << 62;
+    if (g.split) {
+        __syncthreads();
+        long long total = 0, seen = 0;
+        for (int pass = 0; pass < 2; ++pass) {
+            const long long from = per * blockIdx.x;
+            for (int base = 0; base < g.n_slots; base += kThreads) {
+                const int s = base + tid;
+                const int tiles = s < g.n_slots ? get_item(a, g.group, g.head_groups, s).tiles : 0;
+                long long sum;
+                const long long before = seen + block_scan64(tiles, scan_s, &sum);
+                if (pass && before <= from && from < before + tiles) { start_slot = s; start_tile = (int)(from - before); }
+                seen += sum;
+            }
+            if (pass == 0) {
+                total = seen;
+                per = max((long long)kMinTiles, (total + kCtas - 1) / kCtas);
+                seen = 0;
+            }
         }
-        per = max((long long)kMinTiles, (total + kCtas - 1) / kCtas);
-        const long long from = per * blockIdx.x;
-        long long seen = 0;
-        for (int base = 0; base < n_slots; base += kThreads) {
-            const int s = base + tid;
-            const int tiles = s < n_slots ? get_item(a, group, head_groups, s).tiles : 0;
-            long long sum;
-            const long long before = seen + block_scan64(tiles, scan_s, &sum);
-            if (before <= from && from < before + tiles) { start_slot = s; start_tile = (int)(from - before); }
-            seen += sum;
-        }
+        left = min(per, total - per * (long long)blockIdx.x);
     }
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
-    constexpr uint32_t tmem = kTmem, s_tmem = kTmem + NB * 64;
-    if (split) start = Walk{start_slot, start_tile, 1, min(per, total - per * (long long)blockIdx.x)};
+
+    // A role takes the segments in order from the ring; every warp of it calls this.
+    int seg = 0;
+    auto next_segment = [&](Segment &sg) -> bool {
+        const int i = seg & (kSegRing - 1);
+        tc::wait(&seg_full[i], (uint32_t)((seg / kSegRing) & 1), abort_flag, status);
+        sg = seg_s[i];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&seg_free[i]);
+        ++seg;
+        return sg.t1 >= 0 && !*abort_flag;
+    };
 
     if (warp >= kLoadWarp0 && warp < kLoadWarp0 + kLoadWarps) {
         // ------------------------------------------------------------------------------ loaders
-        // Loads run one unit ahead of the stores: a unit is a tile, or 128 dims of one with f32 rows.
+        // Four lanes per row, 16 of every 64 dims each.  A register is loaded again, with the next unit's bytes, as soon as
+        // its value is converted, so loads run a tile ahead of the stores.  A unit is a tile, or 128 or 256 dims of one in f32.
         tc::set_max_registers_up<152>();
-        constexpr bool kF32 = FMT == DS4B200_KV_F32;
-        constexpr int kUnits = kF32 ? NB : 1;
-        const int r = (warp - kLoadWarp0) * 8 + (lane >> 2), part = lane & 3;   // four lanes per row, 16 of 64 dims each
+        constexpr bool kF32 = FMT == DS4B200_KV_F32, kBlock = FMT == DS4B200_KV_FP8_BLOCK64;
+        constexpr int kUnitChunks = !kF32 ? kChunks : (NB % 2 ? 2 : 4), kUnits = kChunks / kUnitChunks;
+        constexpr int kRegs = kF32 ? kUnitChunks * 4 : kChunks;
+        const int r = (warp - kLoadWarp0) * 8 + (lane >> 2), part = lane & 3;
         const uint32_t row_off = (uint32_t)(r * 128), sw = (uint32_t)(r & 7);
-        const bool tail = FMT == DS4B200_KV_FP8_BLOCK64 && a.kv.n_rot != 0;
-        const int n_scales = FMT == DS4B200_KV_FP8_BLOCK64 ? (D - a.kv.n_rot) / 64 : 1;
-        struct Unit {
-            uint4 v[8];                                  // codes of the row by chunk, or 2 chunks of f32
-            float4 tl[FMT == DS4B200_KV_FP8_BLOCK64 ? 4 : 1];
-            float sc0, sc1;
-        };
-        Walk w = start;
-        Item it;
-        int t = 0, t1 = 0;                               // the tile after the one being loaded
+        const bool tail = kBlock && a.kv.n_rot != 0;
+        const int n_scales = kBlock ? (D - a.kv.n_rot) / 64 : 1;
+        uint4 v[kRegs];
+        float4 tl[kBlock ? 4 : 1];
+        float sc0 = 0.0f, sc1 = 0.0f;
+        Segment sg;
+        bool more = next_segment(sg), first = more;
+        int t = more ? sg.t0 : 0;                        // the tile that is being loaded
         int64_t slot = -1;                               // this lane's row of it, or -1
         int at = 0;
-        bool more = w.next(a, group, head_groups, n_slots, it, t, t1), first = more;
         auto find = [&]() {
             const int i = t * kRows + r;
-            at = i < it.first ? i : it.lo + (i - it.first);
+            at = i < sg.it.first ? i : sg.it.lo + (i - sg.it.first);
             slot = -1;
-            if (more && i < it.n) {
-                const int pg = at / a.kv.page_rows;
-                const int page = __ldg(a.page_table + it.b * a.table_width + pg);
+            if (more && i < sg.it.n) {
+                const int pg = g.page_shift >= 0 ? at >> g.page_shift : at / a.kv.page_rows;
+                const int page = __ldg(a.page_table + sg.it.b * a.table_width + pg);
                 if (page >= 0 && page < a.kv.n_pages) slot = (int64_t)page * a.kv.page_rows + (at - pg * a.kv.page_rows);
             }
         };
-        auto load = [&](Unit &u, int64_t my, int unit) {
-            if (kF32) {
-                const float *src = a.kv.raw + my * D + unit * 128 + part * 4;
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    u.v[j] = my >= 0 ? __ldg(reinterpret_cast<const uint4 *>(src + (j >> 2) * 64 + (j & 3) * 16)) : make_uint4(0, 0, 0, 0);
-            } else {
-                const uint8_t *src = a.kv.codes + my * D + part * 16;
-#pragma unroll
-                for (int c = 0; c < kChunks; ++c)
-                    u.v[c] = my >= 0 && !(tail && c == kChunks - 1) ? __ldg(reinterpret_cast<const uint4 *>(src + c * 64)) : make_uint4(0, 0, 0, 0);
-                u.sc0 = u.sc1 = 0.0f;
-                if (FMT == DS4B200_KV_FP8_ROW) {
-                    u.sc0 = my >= 0 ? __ldg(a.kv.scales + my) : 1.0f;
-                } else {
-                    if (my >= 0 && part < n_scales) u.sc0 = __ldg(a.kv.scales + my * n_scales + part);
-                    if (my >= 0 && part + 4 < n_scales) u.sc1 = __ldg(a.kv.scales + my * n_scales + part + 4);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if (FMT == DS4B200_KV_FP8_BLOCK64)
-                            u.tl[j] = my >= 0 && tail ? __ldg(reinterpret_cast<const float4 *>(a.kv.tail + my * 64 + part * 16 + j * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
-                }
+        auto load = [&](int64_t my, int unit, int k) {   // register k of a unit
+            v[k] = make_uint4(0, 0, 0, 0);
+            if (my < 0) return;
+            if (kF32) v[k] = ld_row16(a.kv.raw + my * D + unit * (kUnitChunks * 64) + (k >> 2) * 64 + (k & 3) * 16 + part * 4);
+            else if (!(tail && k == kChunks - 1)) v[k] = ld_row16(a.kv.codes + my * D + k * 64 + part * 16);
+        };
+        auto load_scales = [&](int64_t my) {
+            if (FMT == DS4B200_KV_FP8_ROW) sc0 = my >= 0 ? __ldg(a.kv.scales + my) : 1.0f;
+            if (kBlock) {
+                sc0 = my >= 0 && part < n_scales ? __ldg(a.kv.scales + my * n_scales + part) : 0.0f;
+                sc1 = my >= 0 && part + 4 < n_scales ? __ldg(a.kv.scales + my * n_scales + part + 4) : 0.0f;
             }
         };
-        Unit ua, ub;
+        auto load_tail = [&](int64_t my) {
+            if (kBlock)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint4 x = my >= 0 && tail ? ld_row16(a.kv.tail + my * 64 + part * 16 + j * 4) : make_uint4(0, 0, 0, 0);
+                    tl[kBlock ? j : 0] = make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w));
+                }
+        };
         find();
         int64_t my = slot;
-        int my_at = at, n = 0, seg = -1, unit = 0;
+        int my_at = at;
         bool have = more;
-        float mul = 1.0f;
-        if (have) load(ua, my, 0);
-        auto step = [&](Unit &cur, Unit &nxt) {
+#pragma unroll
+        for (int k = 0; k < kRegs; ++k) load(my, 0, k);
+        load_scales(my);
+        load_tail(my);
+        for (int n = 0, nq = 0; have; ++n) {
             const int buf = n & 1;
             const uint32_t use = (uint32_t)(((n >> 1) & 1) ^ 1);
             unsigned char *dst = k_s + buf * kTileBytes + row_off;
-            if (unit == 0) {
-                // the tile behind this one, and a segment's query rows ahead of its first tile
-                const bool starts = first;
-                const int64_t row0 = it.row0;
-                const int rows = it.rows;
-                first = false;
-                if (++t == t1) { more = w.next(a, group, head_groups, n_slots, it, t, t1); first = more; }
-                find();
-                if (starts) {
-                    ++seg;
-                    uint4 v[kChunks][2];
-                    uint32_t amax = 0;
-                    const uint16_t *src = a.q + (row0 + r) * D + part * 16;
+            if (first) {                                 // a segment's query rows come ahead of its first tile
+                uint4 x[kChunks][2];
+                uint32_t amax = 0;
+                const uint16_t *src = a.q + (sg.it.row0 + r) * D + part * 16;
 #pragma unroll
-                    for (int c = 0; c < kChunks; ++c)
+                for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            v[c][u] = r < rows ? __ldg(reinterpret_cast<const uint4 *>(src + c * 64 + u * 8)) : make_uint4(0, 0, 0, 0);
-                            const uint32_t x[4] = {v[c][u].x, v[c][u].y, v[c][u].z, v[c][u].w};
+                    for (int u = 0; u < 2; ++u) x[c][u] = r < sg.it.rows ? ld_row16(src + c * 64 + u * 8) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) amax = max(amax, max(x[k] & 0x7fff0000u, (x[k] << 16) & 0x7fff0000u));
-                        }
-                    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                    float up, down;
-                    pow2_parts(__uint_as_float(amax), up, down);
-                    tc::wait(&q_free, (uint32_t)((seg & 1) ^ 1), abort_flag, status);
+                for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-                    for (int c = 0; c < kChunks; ++c)
+                    for (int u = 0; u < 2; ++u) {
+                        const uint32_t y[4] = {x[c][u].x, x[c][u].y, x[c][u].z, x[c][u].w};
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            const uint32_t x[4] = {v[c][u].x, v[c][u].y, v[c][u].z, v[c][u].w};
-                            uint32_t o[4];
+                        for (int k = 0; k < 4; ++k) amax = max(amax, max(y[k] & 0x7fff0000u, (y[k] << 16) & 0x7fff0000u));
+                    }
+                amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                float up, down;
+                pow2_parts(__uint_as_float(amax), up, down);
+                tc::wait(&q_free, (uint32_t)((nq & 1) ^ 1), abort_flag, status);
 #pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                o[k] = h2_bits(__floats2half2_rn(__uint_as_float(x[k] << 16) * down, __uint_as_float(x[k] & 0xffff0000u) * down));
-                            *reinterpret_cast<uint4 *>(q_s + c * 8192 + row_off + (((uint32_t)(part * 2 + u) ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-                        }
-                    if (part == 0) q_mul[seg & (kScaleSets - 1)][r] = up * a.scale * kLog2e;
-                    tc::fence_async();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&q_full);
-                }
+                for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const uint32_t y[4] = {x[c][u].x, x[c][u].y, x[c][u].z, x[c][u].w};
+                        uint32_t o[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            o[k] = h2_bits(__floats2half2_rn(__uint_as_float(y[k] << 16) * down, __uint_as_float(y[k] & 0xffff0000u) * down));
+                        *reinterpret_cast<uint4 *>(q_s + c * 8192 + row_off + (((uint32_t)(part * 2 + u) ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+                    }
+                if (part == 0) q_mul[nq & (kScaleSets - 1)][r] = up * a.scale * kLog2e;
+                tc::fence_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&q_full);
+                ++nq;
             }
-            if (kUnits > 1 && unit + 1 < kUnits) load(nxt, my, unit + 1);
-            else load(nxt, slot, 0);
+            // the tile behind this one
+            first = false;
+            if (++t == sg.t1) {
+                more = next_segment(sg);
+                first = more;
+                t = sg.t0;
+            }
+            find();
             auto hand_over = [&](int k) {
                 tc::fence_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[buf][k]);
             };
+            float mul = 1.0f;
             if (kF32) {
-                if (unit == 0) tc::wait(&pv_done[buf][0], use, abort_flag, status);
-                if (kParts > 1 && unit == kPart0) tc::wait(&pv_done[buf][kParts - 1], use, abort_flag, status);
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    *reinterpret_cast<uint2 *>(dst + unit * 16384 + (j >> 2) * 8192 + (((uint32_t)(2 * (j & 3) + (part >> 1)) ^ sw) << 4) + (part & 1) * 8) =
-                        make_uint2(sat_h2(__uint_as_float(cur.v[j].x), __uint_as_float(cur.v[j].y)),
-                                   sat_h2(__uint_as_float(cur.v[j].z), __uint_as_float(cur.v[j].w)));
-                if (kParts > 1 && unit == kPart0 - 1) hand_over(0);
+                for (int unit = 0; unit < kUnits; ++unit)
+#pragma unroll
+                    for (int k = 0; k < kRegs; ++k) {
+                        const int c = unit * kUnitChunks + (k >> 2);        // chunk of the row
+                        if (c == 0 && (k & 3) == 0) tc::wait(&pv_done[buf][0], use, abort_flag, status);
+                        if (kParts > 1 && c == 2 * kPart0 && (k & 3) == 0) {
+                            hand_over(0);
+                            tc::wait(&pv_done[buf][kParts - 1], use, abort_flag, status);
+                        }
+                        *reinterpret_cast<uint2 *>(dst + c * 8192 + (((uint32_t)(2 * (k & 3) + (part >> 1)) ^ sw) << 4) + (part & 1) * 8) =
+                            make_uint2(sat_h2(__uint_as_float(v[k].x), __uint_as_float(v[k].y)), sat_h2(__uint_as_float(v[k].z), __uint_as_float(v[k].w)));
+                        if (unit + 1 < kUnits) load(my, unit + 1, k);
+                        else load(slot, 0, k);
+                    }
             } else {
                 float down = 1.0f;
-                if (FMT == DS4B200_KV_FP8_ROW) mul = cur.sc0;
-                if (FMT == DS4B200_KV_FP8_BLOCK64) {
-                    float top = fmaxf(cur.sc0, cur.sc1);
+                if (FMT == DS4B200_KV_FP8_ROW) mul = sc0;
+                if (kBlock) {
+                    float top = fmaxf(sc0, sc1);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) top = fmaxf(top, amax4(cur.tl[FMT == DS4B200_KV_FP8_BLOCK64 ? j : 0]) * (1.0f / 256.0f));
+                    for (int j = 0; j < 4; ++j) top = fmaxf(top, amax4(tl[kBlock ? j : 0]) * (1.0f / 256.0f));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                     pow2_parts(top, mul, down);
-                    cur.sc0 *= down;
-                    cur.sc1 *= down;
+                    sc0 *= down;
+                    sc1 *= down;
                 }
 #pragma unroll
                 for (int c = 0; c < kChunks; ++c) {
@@ -347,146 +395,165 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
                         tc::wait(&pv_done[buf][kParts - 1], use, abort_flag, status);
                     }
                     uint32_t o[8];
-                    const uint32_t x[4] = {cur.v[c].x, cur.v[c].y, cur.v[c].z, cur.v[c].w};
+                    const uint32_t x[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         o[2 * k] = h2_bits(e4m3x2(x[k] & 0xffffu));
                         o[2 * k + 1] = h2_bits(e4m3x2(x[k] >> 16));
                     }
-                    if (FMT == DS4B200_KV_FP8_BLOCK64) {
-                        const __half2 f = __float2half2_rn(__shfl_sync(0xffffffffu, c < 4 ? cur.sc0 : cur.sc1, (lane & ~3) | (c & 3)));
+                    if (kBlock) {
+                        const __half2 f = __float2half2_rn(__shfl_sync(0xffffffffu, c < 4 ? sc0 : sc1, (lane & ~3) | (c & 3)));
 #pragma unroll
                         for (int k = 0; k < 8; ++k) o[k] = h2_bits(__hmul2(*reinterpret_cast<__half2 *>(&o[k]), f));
                         if (tail && c == kChunks - 1) {
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
-                                const float4 x4 = cur.tl[FMT == DS4B200_KV_FP8_BLOCK64 ? j : 0];
-                                o[2 * j] = h2_bits(__floats2half2_rn(x4.x * down, x4.y * down));
-                                o[2 * j + 1] = h2_bits(__floats2half2_rn(x4.z * down, x4.w * down));
+                                const float4 y = tl[kBlock ? j : 0];
+                                o[2 * j] = h2_bits(__floats2half2_rn(y.x * down, y.y * down));
+                                o[2 * j + 1] = h2_bits(__floats2half2_rn(y.z * down, y.w * down));
                             }
                         }
                     }
                     *reinterpret_cast<uint4 *>(dst + c * 8192 + (((uint32_t)(part * 2) ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
                     *reinterpret_cast<uint4 *>(dst + c * 8192 + (((uint32_t)(part * 2 + 1) ^ sw) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+                    load(slot, 0, c);
                 }
+                load_scales(slot);
+                load_tail(slot);
             }
-            if (kUnits == 1 || ++unit == kUnits) {
-                unit = 0;
-                if (part == 0) {
-                    mul = mul == 0.0f ? 1.0e-30f : mul;
-                    if (!kF32) { row_mul[buf][r] = mul; row_div[buf][r] = 1.0f / mul; }
-                    row_add[buf][r] = my >= 0 ? (kF32 ? 0.0f : log2f(mul)) : -INFINITY;
-                    row_at[buf][r] = my_at;
-                }
-                hand_over(kParts - 1);
-                my = slot;
-                my_at = at;
-                have = more;
-                ++n;
+            if (part == 0) {
+                mul = mul == 0.0f ? 1.0e-30f : mul;
+                if (!kF32) { row_mul[buf][r] = mul; row_div[buf][r] = 1.0f / mul; }
+                row_add[buf][r] = my >= 0 ? (kF32 ? 0.0f : log2f(mul)) : -INFINITY;
+                row_at[buf][r] = my_at;
             }
-        };
-        while (have) {                                   // two units' registers take turns, so that no copy waits for a load
-            step(ua, ub);
-            if (!have) break;
-            step(ub, ua);
+            hand_over(kParts - 1);
+            my = slot;
+            my_at = at;
+            have = more;
         }
-    } else if (warp == kMmaWarp || warp == kMmaWarp + 1) {
-        // ------------------------------------------------------------------------------ MMA issuers, one per product
+    } else if (warp >= kMmaWarp) {
         tc::set_max_registers_down<80>();
-        {
-            const uint32_t one = tc::elect();
-            const uint32_t q_desc = tc::desc_lo(smem_addr(q_s), 0), k_desc = tc::desc_lo(smem_addr(k_s), 0);
-            const uint32_t v_desc = tc::desc_lo(smem_addr(k_s), 8192), p_desc = tc::desc_lo(smem_addr(p_s), 0);
-            constexpr uint32_t s_idesc = tc::idesc_f16(64, 64, false);
-            constexpr uint32_t o_idesc = tc::idesc_f16(128, 64, true);
-            auto weighted = [&](auto which, int k, uint32_t more) {         // O^T (+)= V^T P^T of tile k
-                constexpr int buf = decltype(which)::value;
-                constexpr uint32_t v0 = (uint32_t)((buf * kTileBytes) >> 4), p0 = (uint32_t)((buf * 8192) >> 4);
-                tc::wait(&p_full[buf], (uint32_t)((k >> 1) & 1), abort_flag, status);
-                tc::fence_after();
+        const uint32_t one = tc::elect();
+        const uint32_t k_desc = tc::desc_lo(smem_addr(k_s), 0);
+        if (warp == kMmaWarp) {
+            // -------------------------------------------------------------------------- S = Q K^T
+            const uint32_t q_desc = tc::desc_lo(smem_addr(q_s), 0);
+            Segment sg;
+            int n = 0;
+            for (int nq = 0; next_segment(sg); ++nq) {
+                const int t0 = __shfl_sync(0xffffffffu, sg.t0, 0), t1 = __shfl_sync(0xffffffffu, sg.t1, 0);
+                const int rows = __shfl_sync(0xffffffffu, sg.it.n, 0);
+                tc::wait(&q_full, (uint32_t)(nq & 1), abort_flag, status);
+                for (int t = t0; t < t1; ++t, ++n) {
+                    const int buf = n & 1;
+                    const uint32_t phase = (uint32_t)((n >> 1) & 1), k0 = k_desc + (uint32_t)(buf * (kTileBytes >> 4));
+                    const int groups = min(max((rows - t * kRows + 15) >> 4, 1), 4);      // of 16 cache rows
+                    const uint32_t idesc = tc::idesc_f16(64, 0, false) | (uint32_t)groups << 18;
+                    tc::wait(&s_free[buf], phase ^ 1, abort_flag, status);
 #pragma unroll
-                for (int m = 0; m < NB; ++m) {
-#pragma unroll
-                    for (int ks = 0; ks < 4; ++ks)
-                        tc::mma_f16(one, kTmem + m * 64, v_desc + v0 + (uint32_t)((m * 16384 + ks * 2048) >> 4), p_desc + p0 + (uint32_t)((ks * 32) >> 4),
-                                    o_idesc, ks > 0 ? 1u : more);
-                    if (kParts > 1 && m == kPart0 - 1) tc::commit(one, &pv_done[buf][0]);
-                }
-                tc::commit(one, &pv_done[buf][kParts - 1]);
-            };
-            auto scores = [&](auto which, int k) {                          // S = Q K^T of tile k
-                constexpr int buf = decltype(which)::value;
-                constexpr uint32_t k0 = (uint32_t)((buf * kTileBytes) >> 4);
-                tc::wait(&s_free[buf], (uint32_t)(((k >> 1) & 1) ^ 1), abort_flag, status);
-#pragma unroll
-                for (int c = 0; c < kChunks; ++c) {
-                    if (c == 0 || (kParts > 1 && c == 2 * kPart0)) {
-                        tc::wait(&full[buf][c == 0 ? 0 : kParts - 1], (uint32_t)((k >> 1) & 1), abort_flag, status);
+                    for (int part = 0; part < kParts; ++part) {
+                        tc::wait(&full[buf][part], phase, abort_flag, status);
                         tc::fence_after();
-                    }
+#pragma unroll 1
+                        for (int c = part * 2 * kPart0; c < (part + 1 == kParts ? kChunks : 2 * kPart0); ++c)
 #pragma unroll
-                    for (int ks = 0; ks < 4; ++ks)
-                        tc::mma_f16(one, kTmem + NB * 64 + buf * 64, q_desc + (uint32_t)((c * 8192 + ks * 32) >> 4),
-                                    k_desc + k0 + (uint32_t)((c * 8192 + ks * 32) >> 4), s_idesc, c > 0 || ks > 0);
+                            for (int ks = 0; ks < 4; ++ks)
+                                tc::mma_f16(one, s_tmem + buf * 64, q_desc + (uint32_t)(c * 512 + ks * 2), k0 + (uint32_t)(c * 512 + ks * 2), idesc,
+                                            c > 0 || ks > 0);
+                    }
+                    tc::commit(one, &s_full[buf]);
                 }
-                tc::commit(one, &s_full[buf]);
-            };
-            using Zero = std::integral_constant<int, 0>;
-            using One = std::integral_constant<int, 1>;
-            Walk w = start;
-            Item it;
-            int t0, t1, n = 0, seg = 0;
-            while (__shfl_sync(0xffffffffu, (int)w.next(a, group, head_groups, n_slots, it, t0, t1), 0)) {
-                t0 = __shfl_sync(0xffffffffu, t0, 0);
-                t1 = __shfl_sync(0xffffffffu, t1, 0);
-                if (warp == kMmaWarp) {
-                    tc::wait(&q_full, (uint32_t)(seg & 1), abort_flag, status);
-                    for (int t = t0; t < t1; ++t, ++n) {
-                        if (n & 1) scores(One(), n);
-                        else scores(Zero(), n);
+                tc::commit(one, &q_free);
+            }
+        } else if (warp == kMmaWarp + 1) {
+            // -------------------------------------------------------------------------- O^T += V^T P^T
+            const uint32_t v_desc = tc::desc_lo(smem_addr(k_s), 8192), p_desc = tc::desc_lo(smem_addr(p_s), 0);
+            constexpr uint32_t idesc = tc::idesc_f16(128, 64, true);
+            Segment sg;
+            int n = 0;
+            while (next_segment(sg)) {
+                const int t0 = __shfl_sync(0xffffffffu, sg.t0, 0), t1 = __shfl_sync(0xffffffffu, sg.t1, 0);
+                const int rows = __shfl_sync(0xffffffffu, sg.it.n, 0);
+                for (int t = t0; t < t1; ++t, ++n) {
+                    const int buf = n & 1;
+                    const uint32_t v0 = v_desc + (uint32_t)(buf * (kTileBytes >> 4)), p0 = p_desc + (uint32_t)(buf * 512);
+                    const int groups = min(max((rows - t * kRows + 15) >> 4, 1), 4);
+                    tc::wait(&p_full[buf], (uint32_t)((n >> 1) & 1), abort_flag, status);
+                    tc::fence_after();
+#pragma unroll 1
+                    for (int m = 0; m < NB; ++m) {
+#pragma unroll
+                        for (int ks = 0; ks < 4; ++ks)
+                            if (ks < groups)
+                                tc::mma_f16(one, o_tmem + m * 64, v0 + (uint32_t)(m * 1024 + ks * 128), p0 + (uint32_t)(ks * 2), idesc, t > t0 || ks > 0);
+                        if (kParts > 1 && m == kPart0 - 1) tc::commit(one, &pv_done[buf][0]);
                     }
-                    tc::commit(one, &q_free);
-                    ++seg;
-                } else {
-                    for (int t = t0; t < t1; ++t, ++n) {
-                        if (n & 1) weighted(One(), n, t > t0);
-                        else weighted(Zero(), n, t > t0);
-                    }
+                    tc::commit(one, &pv_done[buf][kParts - 1]);
                 }
             }
+        } else if (warp == kMmaWarp + 2) {
+            // -------------------------------------------------------------------------- schedule
+            int slot = g.split ? start_slot : (int)blockIdx.x, tile = g.split ? start_tile : 0;
+            const int step = g.split ? 1 : (int)gridDim.x;
+            for (bool end = false; !end; ++seg) {
+                Segment sg;
+                sg.t0 = 0;
+                sg.t1 = -1;
+                end = true;
+                while (left > 0 && slot < g.n_slots) {
+                    sg.it = get_item(a, g.group, g.head_groups, slot);
+                    slot += step;
+                    if (sg.it.tiles == 0) continue;
+                    sg.t0 = tile;
+                    sg.t1 = (int)min((long long)sg.it.tiles, tile + left);
+                    tile = 0;
+                    if (g.split) left -= sg.t1 - sg.t0;
+                    end = false;
+                    break;
+                }
+                const int i = seg & (kSegRing - 1);
+                tc::wait(&seg_free[i], (uint32_t)(((seg / kSegRing) & 1) ^ 1), abort_flag, status);
+                if (lane == 0) {
+                    seg_s[i] = sg;
+                    mbar_arrive(&seg_full[i]);
+                }
+                __syncwarp();
+                if (*abort_flag) break;
+            }
         }
-        __syncwarp();
-    } else if (warp > kMmaWarp + 1) {
-        tc::set_max_registers_down<80>();
     } else {
         // ------------------------------------------------------------------------------ softmax and output
         const int row = warp * 16 + (lane >> 2);        // four lanes share rows `row` and `row` + 8 of S, 16 columns each
         const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
-        const bool several = head_groups == 1 && group > 1;
+        const bool several = g.head_groups == 1 && g.group > 1;
         Meta last{0, 0, 0};
-        Walk w = start;
-        Item it;
-        int t0, t1, n = 0, seg = 0;
+        Segment sg;
+        int n = 0;
         long long done = 0;
-        while (w.next(a, group, head_groups, n_slots, it, t0, t1)) {
-            float qk[2] = {0.0f, 0.0f}, m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+        for (int nq = 0; next_segment(sg); ++nq) {
+            const Item &it = sg.it;
+            float qk[2] = {0.0f, 0.0f}, m[2] = {-INFINITY, -INFINITY};
+            float2 l[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
             const int p[2] = {it.p0 + (several ? row / a.n_heads : 0), it.p0 + (several ? (row + 8) / a.n_heads : 0)};
-            for (int t = t0; t < t1; ++t, ++n) {
+            for (int t = sg.t0; t < sg.t1; ++t, ++n) {
                 const int buf = n & 1;
-                tc::wait(&full[buf][kParts - 1], (uint32_t)((n >> 1) & 1), abort_flag, status);
-                tc::wait(&s_full[buf], (uint32_t)((n >> 1) & 1), abort_flag, status);
+                const uint32_t phase = (uint32_t)((n >> 1) & 1);
+                tc::wait(&full[buf][kParts - 1], phase, abort_flag, status);
+                tc::wait(&s_full[buf], phase, abort_flag, status);
                 tc::fence_after();
                 // written ahead of the segment's first tile by the same warps; q_full itself may be phases ahead of this warp
-                if (t == t0)
+                if (t == sg.t0)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) qk[h] = q_mul[seg & (kScaleSets - 1)][row + 8 * h];
+                    for (int h = 0; h < 2; ++h) qk[h] = q_mul[nq & (kScaleSets - 1)][row + 8 * h];
                 uint32_t x[32];
                 tc::ld_16x64(s_tmem + buf * 64 + lane_base, x);
                 tc::wait_ld();
                 tc::fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&s_free[buf]);
-                float v[2][16], top[2] = {-INFINITY, -INFINITY};
+                float2 v[2][8];
+                float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const int c = 8 * i + 2 * (lane & 3);
@@ -495,98 +562,109 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
                     if (FMT != DS4B200_KV_F32) mu = *reinterpret_cast<const float2 *>(&row_mul[buf][c]);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        v[h][2 * i] = fmaf(__uint_as_float(x[4 * i + 2 * h]) * qk[h], mu.x, add.x);
-                        v[h][2 * i + 1] = fmaf(__uint_as_float(x[4 * i + 2 * h + 1]) * qk[h], mu.y, add.y);
+                        const float2 s = make_float2(__uint_as_float(x[4 * i + 2 * h]), __uint_as_float(x[4 * i + 2 * h + 1]));
+                        const float2 k = make_float2(qk[h], qk[h]);
+                        v[h][i] = FMT == DS4B200_KV_F32 ? fma2(s, k, add) : fma2(mul2(s, k), mu, add);
                     }
-                    if (several) {
-                        const int2 at = *reinterpret_cast<const int2 *>(&row_at[buf][c]);
+                }
+                if ((t + 1) * kRows > it.n) {            // columns past the rows: S was not computed there
+                    const int end = it.n - t * kRows;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if (8 * i + 2 * (lane & 3) >= end) v[h][i].x = -INFINITY;
+                            if (8 * i + 2 * (lane & 3) + 1 >= end) v[h][i].y = -INFINITY;
+                        }
+                }
+                if (several) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int2 at = *reinterpret_cast<const int2 *>(&row_at[buf][8 * i + 2 * (lane & 3)]);
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             const int from = a.window > 0 ? p[h] - a.window : -1;       // rows above it are in the window
-                            if (at.x > p[h] || (at.x <= from && at.x >= a.n_first)) v[h][2 * i] = -INFINITY;
-                            if (at.y > p[h] || (at.y <= from && at.y >= a.n_first)) v[h][2 * i + 1] = -INFINITY;
+                            if (at.x > p[h] || (at.x <= from && at.x >= a.n_first)) v[h][i].x = -INFINITY;
+                            if (at.y > p[h] || (at.y <= from && at.y >= a.n_first)) v[h][i].y = -INFINITY;
                         }
                     }
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) top[h] = fmaxf(top[h], fmaxf(v[h][2 * i], v[h][2 * i + 1]));
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) top[h] = fmaxf(top[h], fmaxf(v[h][i].x, v[h][i].y));
                     top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
                     top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
                 }
                 const bool grown[2] = {m[0] > -INFINITY && top[0] > m[0] + kRescale, m[1] > -INFINITY && top[1] > m[1] + kRescale};
-                uint32_t any;
-                asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-                             : "=r"(any) : "r"((uint32_t)(grown[0] || grown[1])) : "memory");
+                uint32_t any = 0;
+                if (t > sg.t0)
+                    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                                 : "=r"(any) : "r"((uint32_t)(grown[0] || grown[1])) : "memory");
                 if (any) {
                     // every row's accumulators (a column of O^T) follow its maximum; the previous tile's MMAs first
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const float f = grown[h] ? tc::exp2_approx(m[h] - top[h]) : 1.0f;
-                        if (grown[h]) { m[h] = top[h]; l[h] *= f; }
+                        if (grown[h]) { m[h] = top[h]; l[h] = mul2(l[h], make_float2(f, f)); }
                         if ((lane & 3) == 0) fac_s[row + 8 * h] = f;
                     }
                     asm volatile("bar.sync 1, 128;" ::: "memory");
-                    if (t > t0) {
-                        tc::wait(&pv_done[buf ^ 1][kParts - 1], (uint32_t)(((n - 1) >> 1) & 1), abort_flag, status);
-                        tc::fence_after();
-                        for (int col = 0; col < (it.rows + 15) / 16 * 16; col += 16)
+                    tc::wait(&pv_done[buf ^ 1][kParts - 1], (uint32_t)(((n - 1) >> 1) & 1), abort_flag, status);
+                    tc::fence_after();
 #pragma unroll 1
-                            for (int b = 0; b < NB; ++b) {
-                                uint32_t o[16];
-                                tc::ld16(tmem + b * 64 + col + lane_base, o);
-                                tc::wait_ld();
+                    for (int u = 0; u < NB * 4; ++u) {
+                        uint32_t o[16];
+                        tc::ld16(o_tmem + u * 16 + lane_base, o);
+                        tc::wait_ld();
 #pragma unroll
-                                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * fac_s[col + k]);
-                                tc::st16(tmem + b * 64 + col + lane_base, o);
-                            }
-                        tc::wait_st();
+                        for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * fac_s[(u & 3) * 16 + k]);
+                        tc::st16(o_tmem + u * 16 + lane_base, o);
                     }
+                    tc::wait_st();
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     if (m[h] == -INFINITY) m[h] = top[h];
-                    const float ref = m[h] == -INFINITY ? 0.0f : m[h];
+                    const float ref = m[h] == -INFINITY ? 0.0f : -m[h];
+                    const float2 ref2 = make_float2(ref, ref);
                     unsigned char *dst = p_s + buf * 8192 + (row + 8 * h) * 128 + (lane & 3) * 4;
-                    float sum = 0.0f;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const float e0 = tc::exp2_approx(v[h][2 * i] - ref), e1 = tc::exp2_approx(v[h][2 * i + 1] - ref);
-                        if (FMT == DS4B200_KV_F32) {
-                            sum += e0 + e1;
-                        } else {
-                            const float2 d = *reinterpret_cast<const float2 *>(&row_div[buf][8 * i + 2 * (lane & 3)]);
-                            sum = fmaf(e0, d.x, fmaf(e1, d.y, sum));
-                        }
-                        *reinterpret_cast<uint32_t *>(dst + (((uint32_t)i ^ (uint32_t)(row & 7)) << 4)) = h2_bits(__floats2half2_rn(e0, e1));
+                        float2 e = add2(v[h][i], ref2);
+                        e.x = tc::exp2_approx(e.x);
+                        e.y = tc::exp2_approx(e.y);
+                        if (FMT == DS4B200_KV_F32) l[h] = add2(l[h], e);
+                        else l[h] = fma2(e, *reinterpret_cast<const float2 *>(&row_div[buf][8 * i + 2 * (lane & 3)]), l[h]);
+                        *reinterpret_cast<uint32_t *>(dst + (((uint32_t)i ^ (uint32_t)(row & 7)) << 4)) = h2_bits(__floats2half2_rn(e.x, e.y));
                     }
-                    l[h] += sum;
                 }
                 tc::fence_async();
                 tc::fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[buf]);
             }
+            float sum[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+                sum[h] = l[h].x + l[h].y;
+                sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
+                sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
             }
-            // the segment's accumulators
+            // the segment's accumulators; behind this wait every warp is through with the last segment's inv_s
             tc::wait(&pv_done[(n - 1) & 1][kParts - 1], (uint32_t)(((n - 1) >> 1) & 1), abort_flag, status);
             tc::fence_after();
-            const bool whole = t0 == 0 && t1 == it.tiles;
-            const int part = 2 * (int)blockIdx.x + (t0 == 0 ? 1 : 0);
+            const bool whole = sg.t0 == 0 && sg.t1 == it.tiles;
+            const int part = 2 * (int)blockIdx.x + (sg.t0 == 0 ? 1 : 0);
             if ((lane & 3) == 0)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int rw = row + 8 * h;
                     float inv = 1.0f;
                     if (!whole) {
-                        part_ml[part * kRows + rw] = make_float2(m[h], l[h]);
+                        g.part_ml[part * kRows + rw] = make_float2(m[h], sum[h]);
                     } else if (rw < it.rows) {
-                        const float own = l[h] > 0.0f ? m[h] + log2f(l[h]) : (l[h] == l[h] ? -INFINITY : l[h]);
+                        const float own = sum[h] > 0.0f ? m[h] + log2f(sum[h]) : (sum[h] == sum[h] ? -INFINITY : sum[h]);
                         float lse2 = own;
                         if (a.sink) {
                             const float s2 = a.sink[(it.row0 + rw) % a.n_heads] * kLog2e, hi = fmaxf(own, s2);
@@ -598,35 +676,48 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs a, 
                     inv_s[rw] = inv;
                 }
             asm volatile("bar.sync 1, 128;" ::: "memory");
+            // lane = dim, column = query row
+#pragma unroll 1
             for (int b = 0; b < NB; ++b)
+#pragma unroll 1
                 for (int col = 0; col < it.rows; col += 16) {
                     uint32_t o[16];
-                    tc::ld16(tmem + b * 64 + col + lane_base, o);
+                    tc::ld16(o_tmem + b * 64 + col + lane_base, o);
                     tc::wait_ld();
                     const int d = b * 128 + warp * 32 + lane;
                     if (whole) {
-                        uint16_t *dst = a.out + (it.row0 + col) * D + d;
+                        // four lanes trade values, so that each holds four dims of every fourth row and stores 8 bytes
+                        uint16_t *dst = a.out + (it.row0 + col + (lane & 3)) * D + (d & ~3);
 #pragma unroll
-                        for (int k = 0; k < 16; ++k)
-                            if (col + k < it.rows) dst[k * D] = bf16_bits(__uint_as_float(o[k]) * inv_s[col + k]);
+                        for (int k = 0; k < 16; k += 4) {
+                            const float4 f = *reinterpret_cast<const float4 *>(&inv_s[col + k]);
+                            const float y[4] = {__uint_as_float(o[k]) * f.x, __uint_as_float(o[k + 1]) * f.y,
+                                                __uint_as_float(o[k + 2]) * f.z, __uint_as_float(o[k + 3]) * f.w};
+                            const bool odd = lane & 1, high = lane & 2;
+                            // rows k, k+1 and k+2, k+3: an even lane keeps the even row and takes its neighbour's dim of it
+                            const float a0 = __shfl_xor_sync(0xffffffffu, odd ? y[0] : y[1], 1), a1 = __shfl_xor_sync(0xffffffffu, odd ? y[2] : y[3], 1);
+                            const uint32_t w0 = h2b(odd ? a0 : y[0], odd ? y[1] : a0), w1 = h2b(odd ? a1 : y[2], odd ? y[3] : a1);
+                            const uint32_t got = __shfl_xor_sync(0xffffffffu, high ? w0 : w1, 2);
+                            const uint2 out = high ? make_uint2(got, w1) : make_uint2(w0, got);
+                            if (col + k + (lane & 3) < it.rows) __stcs(reinterpret_cast<uint2 *>(dst + k * D), out);
+                        }
                     } else {
-                        float *dst = part_o + ((int64_t)part * kRows + col) * D + d;
+                        float *dst = g.part_o + ((int64_t)part * kRows + col) * D + d;
 #pragma unroll
                         for (int k = 0; k < 16; ++k)
                             if (col + k < it.rows) dst[k * D] = __uint_as_float(o[k]);
                     }
                 }
             tc::fence_before();
-            if (t0 == 0 && t1 < it.tiles)
+            if (sg.t0 == 0 && sg.t1 < it.tiles)
                 last = Meta{it.row0, it.rows, (int)((per * (long long)blockIdx.x + done + it.tiles - 1) / per) - (int)blockIdx.x + 1};
-            done += t1 - t0;
-            ++seg;
+            done += sg.t1 - sg.t0;
         }
-        if (split && tid == 0) meta[blockIdx.x] = last;
+        if (g.split && tid == 0) g.meta[blockIdx.x] = last;
     }
     tc::fence_before();
     __syncthreads();
-    if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem_s));
 }
 
 // Joins the parts of the item that CTA blockIdx.x began and did not finish; one query row per CTA.
@@ -697,7 +788,10 @@ void launch_tc(const AttnArgs &a, cudaStream_t s) {
     cudaGetDevice(&dev);
     std::call_once(once[dev & 15], [&] { cudaFuncSetAttribute(attn_tc_kernel<NB, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
     const unsigned grid = (unsigned)(split || slots > kCtas ? kCtas : slots);
-    attn_tc_kernel<NB, FMT><<<grid, kThreads, smem, s>>>(a, group, head_groups, (int)slots, split, meta, ml, po, device_status_word());
+    int shift = -1;
+    for (int k = 0; k < 31; ++k) if (a.kv.page_rows == 1 << k) shift = k;
+    const TcArgs g{a, group, head_groups, (int)slots, split, shift, meta, ml, po, device_status_word()};
+    attn_tc_kernel<NB, FMT><<<grid, kThreads, smem, s>>>(g);
     if (split) attn_join_kernel<<<dim3(kCtas, kRows), 128, 0, s>>>(a, meta, ml, po);
 }
 

@@ -7,7 +7,7 @@
 namespace ds4b200 {
 namespace tc {
 
-constexpr long long kWaitCycles = 1ll << 31;      // about a second
+constexpr int kWaitPolls = 1 << 24;               // at 50 ns and more each: about a second
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -75,7 +75,7 @@ __device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&r)[16]) {
                  : "memory");
 }
 
-// A wait on an mbarrier phase.  It polls for at most kWaitCycles; the first that runs out raises the status bit and a
+// A wait on an mbarrier phase.  It polls at most kWaitPolls times; the first that runs out raises the status bit and a
 // CTA-wide flag with which every later wait returns at once, so the kernel always ends (its results are invalid then).
 __device__ __forceinline__ bool try_phase(uint64_t *bar, uint32_t parity) {
     uint32_t done;
@@ -84,20 +84,13 @@ __device__ __forceinline__ bool try_phase(uint64_t *bar, uint32_t parity) {
     return done != 0;
 }
 __device__ __forceinline__ void wait_slow(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int *status) {
-    const long long t0 = clock64();
-    for (;;) {
-        if (*abort_flag) return;
 #pragma unroll 1
-        for (int i = 0; i < 64; ++i) {
-            __nanosleep(20);                // a poll is a shared-memory access that competes with the operands of the MMAs
-            if (try_phase(bar, parity)) return;
-        }
-        if (clock64() - t0 > kWaitCycles) {
-            *abort_flag = 1;
-            atomicOr(status, kStatusBulkCopyTimeout);
-            return;
-        }
+    for (int i = 0; i < kWaitPolls; ++i) {
+        if (try_phase(bar, parity) || *abort_flag) return;
+        __nanosleep(20);                    // a poll is a shared-memory access that competes with the operands of the MMAs
     }
+    *abort_flag = 1;
+    atomicOr(status, kStatusBulkCopyTimeout);
 }
 __device__ __forceinline__ void wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int *status) {
     if (!try_phase(bar, parity)) wait_slow(bar, parity, abort_flag, status);
