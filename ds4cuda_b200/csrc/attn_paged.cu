@@ -131,7 +131,8 @@ struct Segment {
     Item it;
     int t0, t1;
 };
-constexpr int kSegRing = 4;
+constexpr int kSegRing = 8;
+constexpr int kAhead = 3;                   // tiles
 constexpr int kSegReaders = kLoadWarps + 4 + 2;
 
 struct TcArgs {
@@ -148,6 +149,7 @@ __device__ __forceinline__ uint4 ld_row16(const void *p) {          // read once
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
+__device__ __forceinline__ void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
     float2 r;
     asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
@@ -170,7 +172,7 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 template <int NB, int FMT>          // NB: head_dim / 128
 __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_constant__ TcArgs g) {
     constexpr int D = NB * 128, kChunks = NB * 2, kTileBytes = kRows * D * 2;
-    constexpr int kParts = NB > 1 ? 2 : 1, kPart0 = (NB + 1) / 2;      // a tile is handed over in parts: its first kPart0 * 128 dims, the rest
+    constexpr int kParts = NB > 2 ? 2 : 1, kPart0 = 2;                 // a tile is handed over in parts: its first 256 dims, the rest
     constexpr uint32_t o_tmem = kTmem, s_tmem = kTmem + NB * 64;
     const AttnArgs &a = g.a;
     extern __shared__ __align__(1024) unsigned char smem[];
@@ -245,39 +247,80 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 
     if (warp >= kLoadWarp0 && warp < kLoadWarp0 + kLoadWarps) {
         // ------------------------------------------------------------------------------ loaders
-        // Four lanes per row, 16 of every 64 dims each.  A register is loaded again, with the next unit's bytes, as soon as
+        // A warp has eight rows of the tile.  Its loads cover two rows at a time, 256 contiguous bytes of each (16 lanes): whole lines,
+        // and stores of rows r and r + 1 with their 16-byte units XORed by the row fall on all banks.  Scales, tails and the
+        // query rows go by four lanes per row.  A register is loaded again, with the next unit's bytes, as soon as
         // its value is converted, so loads run a tile ahead of the stores.  A unit is a tile, or 128 or 256 dims of one in f32.
         tc::set_max_registers_up<152>();
         constexpr bool kF32 = FMT == DS4B200_KV_F32, kBlock = FMT == DS4B200_KV_FP8_BLOCK64;
         constexpr int kUnitChunks = !kF32 ? kChunks : (NB % 2 ? 2 : 4), kUnits = kChunks / kUnitChunks;
-        constexpr int kRegs = kF32 ? kUnitChunks * 4 : kChunks;
+        constexpr int kSpan = kF32 ? 1 : 4;              // chunks a load of two rows covers (fewer with fewer dims)
+        constexpr int kSteps = (kUnitChunks + kSpan - 1) / kSpan, kRegs = kSteps * 4;
         const int r = (warp - kLoadWarp0) * 8 + (lane >> 2), part = lane & 3;
         const uint32_t row_off = (uint32_t)(r * 128), sw = (uint32_t)(r & 7);
+        // of a load of two rows: which one, and the lane's 16 bytes of its 256; eight consecutive lanes (16 with the 8-byte stores
+        // of f32 rows) have to fall on all banks
+        const int half = kF32 ? lane >> 4 : (lane >> 2) & 1, l16 = kF32 ? lane & 15 : (lane & 3) | ((lane >> 3) << 2);
         const bool tail = kBlock && a.kv.n_rot != 0;
         const int n_scales = kBlock ? (D - a.kv.n_rot) / 64 : 1;
-        uint4 v[kRegs];
+        uint4 v[kRegs];                                  // [step][row pair]
         float4 tl[kBlock ? 4 : 1];
         float sc0 = 0.0f, sc1 = 0.0f;
+        // Tiles are found kAhead ahead of the one being stored: a page-table entry, and the first touch of a page, take a
+        // few thousand cycles, so their lines are prefetched into L2 before the loads of the registers come.
+        struct Tile { int slot, at, rows; int64_t row0; bool is; };     // slot of row r or -1; rows > 0: a segment's first tile, row0 its query rows
         Segment sg;
         bool more = next_segment(sg), first = more;
-        int t = more ? sg.t0 : 0;                        // the tile that is being loaded
-        int64_t slot = -1;                               // this lane's row of it, or -1
-        int at = 0;
-        auto find = [&]() {
+        int t = more ? sg.t0 : 0;
+        Tile found{-1, 0, 0, 0, false};
+        int page = -1, in_page = 0;
+        auto find = [&]() {                              // the walk's tile: its page-table entry is on the way behind this
             const int i = t * kRows + r;
-            at = i < sg.it.first ? i : sg.it.lo + (i - sg.it.first);
-            slot = -1;
+            found.is = more;
+            found.at = i < sg.it.first ? i : sg.it.lo + (i - sg.it.first);
+            found.rows = first ? sg.it.rows : 0;
+            found.row0 = sg.it.row0;
+            page = -1;
             if (more && i < sg.it.n) {
-                const int pg = g.page_shift >= 0 ? at >> g.page_shift : at / a.kv.page_rows;
-                const int page = __ldg(a.page_table + sg.it.b * a.table_width + pg);
-                if (page >= 0 && page < a.kv.n_pages) slot = (int64_t)page * a.kv.page_rows + (at - pg * a.kv.page_rows);
+                const int pg = g.page_shift >= 0 ? found.at >> g.page_shift : found.at / a.kv.page_rows;
+                in_page = found.at - pg * a.kv.page_rows;
+                page = __ldg(a.page_table + sg.it.b * a.table_width + pg);
+            }
+            if (more) {
+                first = false;
+                if (++t == sg.t1) {
+                    more = next_segment(sg);
+                    first = more;
+                    t = sg.t0;
+                }
             }
         };
-        auto load = [&](int64_t my, int unit, int k) {   // register k of a unit
-            v[k] = make_uint4(0, 0, 0, 0);
+        auto take = [&]() -> Tile {                      // what find() looked up
+            found.slot = page >= 0 && page < a.kv.n_pages ? page * a.kv.page_rows + in_page : -1;      // n_pages * page_rows < 2^31
+            if (found.slot >= 0) {
+                const int64_t sl = found.slot;
+                if (kF32) {
+#pragma unroll
+                    for (int u = 0; u < NB; ++u) prefetch_l2(a.kv.raw + sl * D + (u * 4 + part) * 32);
+                } else {
+                    if (part < NB) prefetch_l2(a.kv.codes + sl * D + part * 128);
+                    if (kBlock && part < 2 && tail) prefetch_l2(a.kv.tail + sl * 64 + part * 32);
+                    if (part == 3) prefetch_l2(a.kv.scales + sl * n_scales);
+                }
+            }
+            return found;
+        };
+        auto pair_slot = [&](int of, int j) { return __shfl_sync(0xffffffffu, of, (2 * j + half) * 4); };
+        auto load = [&](int my, int unit, int step, int j) {        // my: the slot of row 2 j + half
+            uint4 &x = v[step * 4 + j];
+            x = make_uint4(0, 0, 0, 0);
             if (my < 0) return;
-            if (kF32) v[k] = ld_row16(a.kv.raw + my * D + unit * (kUnitChunks * 64) + (k >> 2) * 64 + (k & 3) * 16 + part * 4);
-            else if (!(tail && k == kChunks - 1)) v[k] = ld_row16(a.kv.codes + my * D + k * 64 + part * 16);
+            if (kF32) {
+                x = ld_row16(a.kv.raw + (int64_t)my * D + (unit * kUnitChunks + step) * 64 + l16 * 4);
+            } else {
+                const int c = step * 4 + (l16 >> 2);                // chunk of this lane
+                if (c < kChunks && !(tail && c == kChunks - 1)) x = ld_row16(a.kv.codes + (int64_t)my * D + step * 256 + l16 * 16);
+            }
         };
         auto load_scales = [&](int64_t my) {
             if (FMT == DS4B200_KV_FP8_ROW) sc0 = my >= 0 ? __ldg(a.kv.scales + my) : 1.0f;
@@ -294,26 +337,36 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     tl[kBlock ? j : 0] = make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w));
                 }
         };
-        find();
-        int64_t my = slot;
-        int my_at = at;
-        bool have = more;
+        Tile tile[kAhead + 1];                           // [0] is being stored, [1] loaded
 #pragma unroll
-        for (int k = 0; k < kRegs; ++k) load(my, 0, k);
+        for (int k = 0; k <= kAhead; ++k) {
+            find();
+            tile[k] = take();
+        }
+        int my = tile[0].slot;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int ps = pair_slot(my, j);
+#pragma unroll
+            for (int step = 0; step < kSteps; ++step) load(ps, 0, step, j);
+        }
         load_scales(my);
         load_tail(my);
-        for (int n = 0, nq = 0; have; ++n) {
+        for (int n = 0, nq = 0; tile[0].is; ++n) {
             const int buf = n & 1;
             const uint32_t use = (uint32_t)(((n >> 1) & 1) ^ 1);
-            unsigned char *dst = k_s + buf * kTileBytes + row_off;
-            if (first) {                                 // a segment's query rows come ahead of its first tile
+            unsigned char *dst = k_s + buf * kTileBytes;
+            find();
+            my = tile[0].slot;
+            const int slot = tile[1].slot;
+            if (tile[0].rows) {                          // a segment's query rows come ahead of its first tile
                 uint4 x[kChunks][2];
                 uint32_t amax = 0;
-                const uint16_t *src = a.q + (sg.it.row0 + r) * D + part * 16;
+                const uint16_t *src = a.q + (tile[0].row0 + r) * D + part * 16;
 #pragma unroll
                 for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) x[c][u] = r < sg.it.rows ? ld_row16(src + c * 64 + u * 8) : make_uint4(0, 0, 0, 0);
+                    for (int u = 0; u < 2; ++u) x[c][u] = r < tile[0].rows ? ld_row16(src + c * 64 + u * 8) : make_uint4(0, 0, 0, 0);
 #pragma unroll
                 for (int c = 0; c < kChunks; ++c)
 #pragma unroll
@@ -344,93 +397,96 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 if (lane == 0) mbar_arrive(&q_full);
                 ++nq;
             }
-            // the tile behind this one
-            first = false;
-            if (++t == sg.t1) {
-                more = next_segment(sg);
-                first = more;
-                t = sg.t0;
-            }
-            find();
             auto hand_over = [&](int k) {
                 tc::fence_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[buf][k]);
             };
-            float mul = 1.0f;
-            if (kF32) {
+            float mul = 1.0f, down = 1.0f;
+            if (FMT == DS4B200_KV_FP8_ROW) mul = sc0;
+            if (kBlock) {
+                float top = fmaxf(sc0, sc1);
 #pragma unroll
-                for (int unit = 0; unit < kUnits; ++unit)
+                for (int j = 0; j < 4; ++j) top = fmaxf(top, amax4(tl[kBlock ? j : 0]) * (1.0f / 256.0f));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                pow2_parts(top, mul, down);
+                sc0 *= down;
+                sc1 *= down;
+            }
+            int here[4], next[4];                        // slots of this lane's rows, this tile's and the next one's
 #pragma unroll
-                    for (int k = 0; k < kRegs; ++k) {
-                        const int c = unit * kUnitChunks + (k >> 2);        // chunk of the row
-                        if (c == 0 && (k & 3) == 0) tc::wait(&pv_done[buf][0], use, abort_flag, status);
-                        if (kParts > 1 && c == 2 * kPart0 && (k & 3) == 0) {
-                            hand_over(0);
-                            tc::wait(&pv_done[buf][kParts - 1], use, abort_flag, status);
-                        }
-                        *reinterpret_cast<uint2 *>(dst + c * 8192 + (((uint32_t)(2 * (k & 3) + (part >> 1)) ^ sw) << 4) + (part & 1) * 8) =
-                            make_uint2(sat_h2(__uint_as_float(v[k].x), __uint_as_float(v[k].y)), sat_h2(__uint_as_float(v[k].z), __uint_as_float(v[k].w)));
-                        if (unit + 1 < kUnits) load(my, unit + 1, k);
-                        else load(slot, 0, k);
-                    }
-            } else {
-                float down = 1.0f;
-                if (FMT == DS4B200_KV_FP8_ROW) mul = sc0;
-                if (kBlock) {
-                    float top = fmaxf(sc0, sc1);
+            for (int j = 0; j < 4; ++j) {
+                here[j] = kUnits > 1 ? pair_slot(my, j) : 0;
+                next[j] = pair_slot(slot, j);
+            }
+            const int rw = (warp - kLoadWarp0) * 8 + half;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) top = fmaxf(top, amax4(tl[kBlock ? j : 0]) * (1.0f / 256.0f));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    pow2_parts(top, mul, down);
-                    sc0 *= down;
-                    sc1 *= down;
-                }
+            for (int unit = 0; unit < kUnits; ++unit)
 #pragma unroll
-                for (int c = 0; c < kChunks; ++c) {
-                    if (c == 0) tc::wait(&pv_done[buf][0], use, abort_flag, status);
-                    if (kParts > 1 && c == 2 * kPart0) {
+                for (int step = 0; step < kSteps; ++step) {
+                    const int c0 = unit * kUnitChunks + step * kSpan;       // first chunk of the step
+                    if (c0 == 0) tc::wait(&pv_done[buf][0], use, abort_flag, status);
+                    if (kParts > 1 && c0 == 2 * kPart0) {
                         hand_over(0);
                         tc::wait(&pv_done[buf][kParts - 1], use, abort_flag, status);
                     }
-                    uint32_t o[8];
-                    const uint32_t x[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        o[2 * k] = h2_bits(e4m3x2(x[k] & 0xffffu));
-                        o[2 * k + 1] = h2_bits(e4m3x2(x[k] >> 16));
-                    }
-                    if (kBlock) {
-                        const __half2 f = __float2half2_rn(__shfl_sync(0xffffffffu, c < 4 ? sc0 : sc1, (lane & ~3) | (c & 3)));
+                    for (int j = 0; j < 4; ++j) {
+                        uint4 &x = v[step * 4 + j];
+                        const uint32_t r7 = (uint32_t)(2 * j + half);
+                        if (kF32) {
+                            *reinterpret_cast<uint2 *>(dst + c0 * 8192 + (rw + 2 * j) * 128 + ((((uint32_t)l16 >> 1) ^ r7) << 4) + (l16 & 1) * 8) =
+                                make_uint2(sat_h2(__uint_as_float(x.x), __uint_as_float(x.y)), sat_h2(__uint_as_float(x.z), __uint_as_float(x.w)));
+                        } else {
+                            const int c = c0 + (l16 >> 2);
+                            uint32_t o[8];
+                            const uint32_t y[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) o[k] = h2_bits(__hmul2(*reinterpret_cast<__half2 *>(&o[k]), f));
-                        if (tail && c == kChunks - 1) {
+                            for (int k = 0; k < 4; ++k) {
+                                o[2 * k] = h2_bits(e4m3x2(y[k] & 0xffffu));
+                                o[2 * k + 1] = h2_bits(e4m3x2(y[k] >> 16));
+                            }
+                            if (kBlock) {
+                                const __half2 f = __float2half2_rn(__shfl_sync(0xffffffffu, step == 0 ? sc0 : sc1, (2 * j + half) * 4 + (l16 >> 2)));
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const float4 y = tl[kBlock ? j : 0];
-                                o[2 * j] = h2_bits(__floats2half2_rn(y.x * down, y.y * down));
-                                o[2 * j + 1] = h2_bits(__floats2half2_rn(y.z * down, y.w * down));
+                                for (int k = 0; k < 8; ++k) o[k] = h2_bits(__hmul2(*reinterpret_cast<__half2 *>(&o[k]), f));
+                            }
+                            if (c < kChunks && !(tail && c == kChunks - 1)) {
+                                unsigned char *to = dst + c * 8192 + (rw + 2 * j) * 128;
+                                const uint32_t u = (uint32_t)(l16 & 3) * 2;
+                                *reinterpret_cast<uint4 *>(to + ((u ^ r7) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+                                *reinterpret_cast<uint4 *>(to + (((u + 1) ^ r7) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
                             }
                         }
+                        if (unit + 1 < kUnits) load(here[j], unit + 1, step, j);
+                        else load(next[j], 0, step, j);
                     }
-                    *reinterpret_cast<uint4 *>(dst + c * 8192 + (((uint32_t)(part * 2) ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-                    *reinterpret_cast<uint4 *>(dst + c * 8192 + (((uint32_t)(part * 2 + 1) ^ sw) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
-                    load(slot, 0, c);
                 }
-                load_scales(slot);
-                load_tail(slot);
+            if (kBlock && tail) {
+                uint32_t o[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float4 y = tl[kBlock ? j : 0];
+                    o[2 * j] = h2_bits(__floats2half2_rn(y.x * down, y.y * down));
+                    o[2 * j + 1] = h2_bits(__floats2half2_rn(y.z * down, y.w * down));
+                }
+                unsigned char *to = dst + (kChunks - 1) * 8192 + row_off;
+                *reinterpret_cast<uint4 *>(to + (((uint32_t)(part * 2) ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+                *reinterpret_cast<uint4 *>(to + (((uint32_t)(part * 2 + 1) ^ sw) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
             }
+            load_scales(slot);
+            load_tail(slot);
             if (part == 0) {
                 mul = mul == 0.0f ? 1.0e-30f : mul;
                 if (!kF32) { row_mul[buf][r] = mul; row_div[buf][r] = 1.0f / mul; }
                 row_add[buf][r] = my >= 0 ? (kF32 ? 0.0f : log2f(mul)) : -INFINITY;
-                row_at[buf][r] = my_at;
+                row_at[buf][r] = tile[0].at;
             }
             hand_over(kParts - 1);
-            my = slot;
-            my_at = at;
-            have = more;
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) tile[k] = tile[k + 1];
+            tile[kAhead] = take();
         }
     } else if (warp >= kMmaWarp) {
         tc::set_max_registers_down<80>();
