@@ -105,8 +105,9 @@ __device__ __forceinline__ long long block_scan64(long long v, long long *scratc
 }
 
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
-__device__ __forceinline__ __half2 e4m3x2(uint32_t two) {
-    return __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3));
+__device__ __forceinline__ void e4m3x4(uint32_t four, uint32_t &lo, uint32_t &hi) {      // E4M3 -> f16 is exact
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi) : "r"(four));
 }
 __device__ __forceinline__ uint32_t h2b(float x, float y) {         // bf16 pair
     __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
@@ -186,7 +187,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     __shared__ __align__(16) float row_mul[2][kRows], row_add[2][kRows], row_div[2][kRows];
     __shared__ __align__(16) int row_at[2][kRows];
     __shared__ float q_mul[kScaleSets][kRows];
-    __shared__ __align__(16) float fac_s[kRows], inv_s[kRows];
+    __shared__ __align__(16) float fac_s[2][kRows], inv_s[kRows];
+    __shared__ int grown_s[2];                      // 1 + the last tile with a row that has grown
+    __shared__ __align__(8) uint64_t scaled[2];
     volatile int *abort_flag = &abort_s;
     int *status = g.status;
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -196,6 +199,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         start_slot = g.n_slots;
         start_tile = 0;
         for (int i = 0; i < 2; ++i) {
+            grown_s[i] = 0;
+            mbar_init(&scaled[i], 4);
             mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4); mbar_init(&p_full[i], 4);
             for (int k = 0; k < kParts; ++k) { mbar_init(&full[i][k], kLoadWarps); mbar_init(&pv_done[i][k], 1); }
         }
@@ -392,13 +397,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                         *reinterpret_cast<uint4 *>(q_s + c * 8192 + row_off + (((uint32_t)(part * 2 + u) ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
                     }
                 if (part == 0) q_mul[nq & (kScaleSets - 1)][r] = up * a.scale * kLog2e;
-                tc::fence_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_full);
                 ++nq;
             }
+            // The MMA warp makes the stores visible to the async proxy: a proxy fence here would wait for the loads in flight.
             auto hand_over = [&](int k) {
-                tc::fence_async();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[buf][k]);
             };
@@ -443,10 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                             uint32_t o[8];
                             const uint32_t y[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                o[2 * k] = h2_bits(e4m3x2(y[k] & 0xffffu));
-                                o[2 * k + 1] = h2_bits(e4m3x2(y[k] >> 16));
-                            }
+                            for (int k = 0; k < 4; ++k) e4m3x4(y[k], o[2 * k], o[2 * k + 1]);
                             if (kBlock) {
                                 const __half2 f = __float2half2_rn(__shfl_sync(0xffffffffu, step == 0 ? sc0 : sc1, (2 * j + half) * 4 + (l16 >> 2)));
 #pragma unroll
@@ -479,8 +480,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             load_tail(slot);
             if (part == 0) {
                 mul = mul == 0.0f ? 1.0e-30f : mul;
-                if (!kF32) { row_mul[buf][r] = mul; row_div[buf][r] = 1.0f / mul; }
-                row_add[buf][r] = my >= 0 ? (kF32 ? 0.0f : log2f(mul)) : -INFINITY;
+                if (!kF32) { row_mul[buf][r] = mul; row_div[buf][r] = __fdividef(1.0f, mul); }
+                row_add[buf][r] = my >= 0 ? (kF32 ? 0.0f : __log2f(mul)) : -INFINITY;
                 row_at[buf][r] = tile[0].at;
             }
             hand_over(kParts - 1);
@@ -510,6 +511,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 #pragma unroll
                     for (int part = 0; part < kParts; ++part) {
                         tc::wait(&full[buf][part], phase, abort_flag, status);
+                        tc::fence_async();               // for the loaders' stores, of the query rows too
                         tc::fence_after();
 #pragma unroll 1
                         for (int c = part * 2 * kPart0; c < (part + 1 == kParts ? kChunks : 2 * kPart0); ++c)
@@ -526,6 +528,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             // -------------------------------------------------------------------------- O^T += V^T P^T
             const uint32_t v_desc = tc::desc_lo(smem_addr(k_s), 8192), p_desc = tc::desc_lo(smem_addr(p_s), 0);
             constexpr uint32_t idesc = tc::idesc_f16(128, 64, true);
+            uint32_t scaled_uses[2] = {0, 0};
+            auto scaled_phase = [&](int b) { return scaled_uses[b]++ & 1; };
             Segment sg;
             int n = 0;
             while (next_segment(sg)) {
@@ -536,6 +540,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     const uint32_t v0 = v_desc + (uint32_t)(buf * (kTileBytes >> 4)), p0 = p_desc + (uint32_t)(buf * 512);
                     const int groups = min(max((rows - t * kRows + 15) >> 4, 1), 4);
                     tc::wait(&p_full[buf], (uint32_t)((n >> 1) & 1), abort_flag, status);
+                    if (*(volatile int *)&grown_s[buf] == n + 1) tc::wait(&scaled[buf], scaled_phase(buf), abort_flag, status);
+                    tc::fence_async();
                     tc::fence_after();
 #pragma unroll 1
                     for (int m = 0; m < NB; ++m) {
@@ -592,9 +598,31 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             float qk[2] = {0.0f, 0.0f}, m[2] = {-INFINITY, -INFINITY};
             float2 l[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
             const int p[2] = {it.p0 + (several ? row / a.n_heads : 0), it.p0 + (several ? (row + 8) / a.n_heads : 0)};
+            // Scales the accumulators ahead of tile k's product where a row of that tile asked for it.
+            auto follow = [&](int k) {
+                const int buf = k & 1;
+                tc::wait(&p_full[buf], (uint32_t)((k >> 1) & 1), abort_flag, status);
+                if (*(volatile int *)&grown_s[buf] != k + 1) return;
+                tc::wait(&pv_done[buf ^ 1][kParts - 1], (uint32_t)(((k - 1) >> 1) & 1), abort_flag, status);
+                tc::fence_after();
+#pragma unroll 1
+                for (int u = 0; u < NB * 4; ++u) {
+                    uint32_t o[16];
+                    tc::ld16(o_tmem + u * 16 + lane_base, o);
+                    tc::wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fac_s[buf][(u & 3) * 16 + i]);
+                    tc::st16(o_tmem + u * 16 + lane_base, o);
+                }
+                tc::wait_st();
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&scaled[buf]);
+            };
             for (int t = sg.t0; t < sg.t1; ++t, ++n) {
                 const int buf = n & 1;
                 const uint32_t phase = (uint32_t)((n >> 1) & 1);
+                if (t > sg.t0) follow(n - 1);
                 tc::wait(&full[buf][kParts - 1], phase, abort_flag, status);
                 tc::wait(&s_full[buf], phase, abort_flag, status);
                 tc::fence_after();
@@ -652,33 +680,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
                     top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
                 }
-                const bool grown[2] = {m[0] > -INFINITY && top[0] > m[0] + kRescale, m[1] > -INFINITY && top[1] > m[1] + kRescale};
-                uint32_t any = 0;
-                if (t > sg.t0)
-                    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-                                 : "=r"(any) : "r"((uint32_t)(grown[0] || grown[1])) : "memory");
-                if (any) {
-                    // every row's accumulators (a column of O^T) follow its maximum; the previous tile's MMAs first
+                // A row whose maximum has grown past the threshold takes a new reference, and every row's factor for the
+                // accumulators (a column of O^T) is left for follow(), which the four warps run together, at the next tile.
+                bool grown = false;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float f = grown[h] ? tc::exp2_approx(m[h] - top[h]) : 1.0f;
-                        if (grown[h]) { m[h] = top[h]; l[h] = mul2(l[h], make_float2(f, f)); }
-                        if ((lane & 3) == 0) fac_s[row + 8 * h] = f;
+                for (int h = 0; h < 2; ++h) {
+                    float f = 1.0f;
+                    if (m[h] > -INFINITY && top[h] > m[h] + kRescale) {
+                        f = tc::exp2_approx(m[h] - top[h]);
+                        m[h] = top[h];
+                        l[h] = mul2(l[h], make_float2(f, f));
+                        grown = true;
                     }
-                    asm volatile("bar.sync 1, 128;" ::: "memory");
-                    tc::wait(&pv_done[buf ^ 1][kParts - 1], (uint32_t)(((n - 1) >> 1) & 1), abort_flag, status);
-                    tc::fence_after();
-#pragma unroll 1
-                    for (int u = 0; u < NB * 4; ++u) {
-                        uint32_t o[16];
-                        tc::ld16(o_tmem + u * 16 + lane_base, o);
-                        tc::wait_ld();
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * fac_s[(u & 3) * 16 + k]);
-                        tc::st16(o_tmem + u * 16 + lane_base, o);
-                    }
-                    tc::wait_st();
+                    if ((lane & 3) == 0) fac_s[buf][row + 8 * h] = f;
                 }
+                if (grown) grown_s[buf] = n + 1;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     if (m[h] == -INFINITY) m[h] = top[h];
@@ -700,6 +716,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[buf]);
             }
+            follow(n - 1);
             float sum[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
