@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     __shared__ uint32_t tmem_s;
     __shared__ int abort_s, start_slot, start_tile;
     __shared__ long long scan_s[kThreads / 32];
-    __shared__ __align__(16) float row_mul[2][kRows], row_add[2][kRows], row_div[2][kRows];
+    __shared__ __align__(16) float row_fma[2][2 * kRows], row_div[2][kRows];      // by pairs of rows: factor, factor, addend, addend
     __shared__ __align__(16) int row_at[2][kRows];
     __shared__ float q_mul[kScaleSets][kRows];
     __shared__ __align__(16) float fac_s[2][kRows], inv_s[kRows];
@@ -240,12 +240,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 
     // A role takes the segments in order from the ring; every warp of it calls this.
     int seg = 0;
-    auto next_segment = [&](Segment &sg) -> bool {
+    auto next_segment = [&](Segment &sg, bool done = true) -> bool {
         const int i = seg & (kSegRing - 1);
         tc::wait(&seg_full[i], (uint32_t)((seg / kSegRing) & 1), abort_flag, status);
         sg = seg_s[i];
         __syncwarp();
-        if (lane == 0) mbar_arrive(&seg_free[i]);
+        if (done && lane == 0) mbar_arrive(&seg_free[i]);
         ++seg;
         return sg.t1 >= 0 && !*abort_flag;
     };
@@ -273,18 +273,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         float sc0 = 0.0f, sc1 = 0.0f;
         // Tiles are found kAhead ahead of the one being stored: a page-table entry, and the first touch of a page, take a
         // few thousand cycles, so their lines are prefetched into L2 before the loads of the registers come.
-        struct Tile { int slot, at, rows; int64_t row0; bool is; };     // slot of row r or -1; rows > 0: a segment's first tile, row0 its query rows
+        struct Tile { int slot, at, rows; };             // slot of row r or -1; query rows of the segment in its first tile, else 0; -1 at the end
         Segment sg;
-        bool more = next_segment(sg), first = more;
+        bool more = next_segment(sg, false), first = more;
         int t = more ? sg.t0 : 0;
-        Tile found{-1, 0, 0, 0, false};
+        Tile found{-1, 0, -1};
         int page = -1, in_page = 0;
         auto find = [&]() {                              // the walk's tile: its page-table entry is on the way behind this
             const int i = t * kRows + r;
-            found.is = more;
             found.at = i < sg.it.first ? i : sg.it.lo + (i - sg.it.first);
-            found.rows = first ? sg.it.rows : 0;
-            found.row0 = sg.it.row0;
+            found.rows = !more ? -1 : first ? sg.it.rows : 0;
             page = -1;
             if (more && i < sg.it.n) {
                 const int pg = g.page_shift >= 0 ? found.at >> g.page_shift : found.at / a.kv.page_rows;
@@ -294,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             if (more) {
                 first = false;
                 if (++t == sg.t1) {
-                    more = next_segment(sg);
+                    more = next_segment(sg, false);      // given back with its query rows
                     first = more;
                     t = sg.t0;
                 }
@@ -316,15 +314,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             return found;
         };
         auto pair_slot = [&](int of, int j) { return __shfl_sync(0xffffffffu, of, (2 * j + half) * 4); };
-        auto load = [&](int my, int unit, int step, int j) {        // my: the slot of row 2 j + half
+        auto load = [&](int my, bool all, int unit, int step, int j) {      // my: the slot of row 2 j + half; all: of the warp's rows exist
             uint4 &x = v[step * 4 + j];
-            x = make_uint4(0, 0, 0, 0);
-            if (my < 0) return;
+            if (!all) {
+                x = make_uint4(0, 0, 0, 0);
+                if (my < 0) return;
+            }
             if (kF32) {
                 x = ld_row16(a.kv.raw + (int64_t)my * D + (unit * kUnitChunks + step) * 64 + l16 * 4);
             } else {
                 const int c = step * 4 + (l16 >> 2);                // chunk of this lane
-                if (c < kChunks && !(tail && c == kChunks - 1)) x = ld_row16(a.kv.codes + (int64_t)my * D + step * 256 + l16 * 16);
+                // lanes past the codes load the row's first ones, which nobody stores
+                const bool in = c < kChunks && !(tail && c == kChunks - 1);
+                x = ld_row16(a.kv.codes + (int64_t)my * D + (in ? step * 256 + l16 * 16 : 0));
             }
         };
         auto load_scales = [&](int64_t my) {
@@ -353,11 +355,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         for (int j = 0; j < 4; ++j) {
             const int ps = pair_slot(my, j);
 #pragma unroll
-            for (int step = 0; step < kSteps; ++step) load(ps, 0, step, j);
+            for (int step = 0; step < kSteps; ++step) load(ps, false, 0, step, j);
         }
         load_scales(my);
         load_tail(my);
-        for (int n = 0, nq = 0; tile[0].is; ++n) {
+        for (int n = 0, nq = 0; tile[0].rows >= 0; ++n) {
             const int buf = n & 1;
             const uint32_t use = (uint32_t)(((n >> 1) & 1) ^ 1);
             unsigned char *dst = k_s + buf * kTileBytes;
@@ -367,7 +369,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             if (tile[0].rows) {                          // a segment's query rows come ahead of its first tile
                 uint4 x[kChunks][2];
                 uint32_t amax = 0;
-                const uint16_t *src = a.q + (tile[0].row0 + r) * D + part * 16;
+                const int ring = nq & (kSegRing - 1);
+                const uint16_t *src = a.q + (seg_s[ring].it.row0 + r) * D + part * 16;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&seg_free[ring]);
 #pragma unroll
                 for (int c = 0; c < kChunks; ++c)
 #pragma unroll
@@ -424,6 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 here[j] = kUnits > 1 ? pair_slot(my, j) : 0;
                 next[j] = pair_slot(slot, j);
             }
+            const bool all_here = kUnits > 1 && __all_sync(0xffffffffu, my >= 0), all_next = __all_sync(0xffffffffu, slot >= 0);
             const int rw = (warp - kLoadWarp0) * 8 + half;
 #pragma unroll
             for (int unit = 0; unit < kUnits; ++unit)
@@ -460,8 +466,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                                 *reinterpret_cast<uint4 *>(to + (((u + 1) ^ r7) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
                             }
                         }
-                        if (unit + 1 < kUnits) load(here[j], unit + 1, step, j);
-                        else load(next[j], 0, step, j);
+                        if (unit + 1 < kUnits) load(here[j], all_here, unit + 1, step, j);
+                        else load(next[j], all_next, 0, step, j);
                     }
                 }
             if (kBlock && tail) {
@@ -480,8 +486,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             load_tail(slot);
             if (part == 0) {
                 mul = mul == 0.0f ? 1.0e-30f : mul;
-                if (!kF32) { row_mul[buf][r] = mul; row_div[buf][r] = __fdividef(1.0f, mul); }
-                row_add[buf][r] = my >= 0 ? (kF32 ? 0.0f : __log2f(mul)) : -INFINITY;
+                if (!kF32) { row_fma[buf][2 * (r & ~1) + (r & 1)] = mul; row_div[buf][r] = __fdividef(1.0f, mul); }
+                row_fma[buf][2 * (r & ~1) + 2 + (r & 1)] = my >= 0 ? (kF32 ? 0.0f : __log2f(mul)) : -INFINITY;
                 row_at[buf][r] = tile[0].at;
             }
             hand_over(kParts - 1);
@@ -637,18 +643,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&s_free[buf]);
                 float2 v[2][8];
-                float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const int c = 8 * i + 2 * (lane & 3);
-                    const float2 add = *reinterpret_cast<const float2 *>(&row_add[buf][c]);
-                    float2 mu = make_float2(1.0f, 1.0f);
-                    if (FMT != DS4B200_KV_F32) mu = *reinterpret_cast<const float2 *>(&row_mul[buf][c]);
+                    const float4 f = *reinterpret_cast<const float4 *>(&row_fma[buf][2 * (8 * i + 2 * (lane & 3))]);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const float2 s = make_float2(__uint_as_float(x[4 * i + 2 * h]), __uint_as_float(x[4 * i + 2 * h + 1]));
                         const float2 k = make_float2(qk[h], qk[h]);
-                        v[h][i] = FMT == DS4B200_KV_F32 ? fma2(s, k, add) : fma2(mul2(s, k), mu, add);
+                        v[h][i] = FMT == DS4B200_KV_F32 ? fma2(s, k, make_float2(f.z, f.w)) : fma2(mul2(s, k), make_float2(f.x, f.y), make_float2(f.z, f.w));
                     }
                 }
                 if ((t + 1) * kRows > it.n) {            // columns past the rows: S was not computed there
@@ -673,31 +675,39 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                         }
                     }
                 }
+                float top[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
+                    float w[4];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) top[h] = fmaxf(top[h], fmaxf(v[h][i].x, v[h][i].y));
-                    top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-                    top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+                    for (int i = 0; i < 4; ++i) w[i] = fmaxf(fmaxf(v[h][i].x, v[h][i].y), fmaxf(v[h][i + 4].x, v[h][i + 4].y));
+                    top[h] = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
                 }
-                // A row whose maximum has grown past the threshold takes a new reference, and every row's factor for the
-                // accumulators (a column of O^T) is left for follow(), which the four warps run together, at the next tile.
-                bool grown = false;
+                // A row keeps the reference its maximum had until one of its values lies kRescale above it.  Then it takes a
+                // new one, and every row's factor for the accumulators (a column of O^T) is left for follow(), which the
+                // four warps run together, at the next tile.
+                if (__any_sync(0xffffffffu, !(top[0] <= m[0] + kRescale) || !(top[1] <= m[1] + kRescale))) {
+                    bool grown = false;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float f = 1.0f;
-                    if (m[h] > -INFINITY && top[h] > m[h] + kRescale) {
-                        f = tc::exp2_approx(m[h] - top[h]);
-                        m[h] = top[h];
-                        l[h] = mul2(l[h], make_float2(f, f));
-                        grown = true;
+                    for (int h = 0; h < 2; ++h) {
+                        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+                        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+                        float f = 1.0f;
+                        if (m[h] > -INFINITY && top[h] > m[h] + kRescale) {
+                            f = tc::exp2_approx(m[h] - top[h]);
+                            m[h] = top[h];
+                            l[h] = mul2(l[h], make_float2(f, f));
+                            grown = true;
+                        }
+                        if (m[h] == -INFINITY) m[h] = top[h];
+                        if ((lane & 3) == 0) fac_s[buf][row + 8 * h] = f;
                     }
-                    if ((lane & 3) == 0) fac_s[buf][row + 8 * h] = f;
+                    if (grown) grown_s[buf] = n + 1;
+                } else if ((lane & 3) == 0) {
+                    fac_s[buf][row] = fac_s[buf][row + 8] = 1.0f;
                 }
-                if (grown) grown_s[buf] = n + 1;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    if (m[h] == -INFINITY) m[h] = top[h];
                     const float ref = m[h] == -INFINITY ? 0.0f : -m[h];
                     const float2 ref2 = make_float2(ref, ref);
                     unsigned char *dst = p_s + buf * 8192 + (row + 8 * h) * 128 + (lane & 3) * 4;
@@ -749,38 +759,56 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     inv_s[rw] = inv;
                 }
             asm volatile("bar.sync 1, 128;" ::: "memory");
-            // lane = dim, column = query row
+            // In tensor memory a lane is a dim and a column a query row.
+            if (whole) {
+                // 128 dims at a time through the weights' buffers, which are free here: stmatrix turns 8 x 8 blocks around, rows of
+                // 256 bytes with their 16-byte units XORed by the row, and every lane stores 16 bytes of a row
 #pragma unroll 1
-            for (int b = 0; b < NB; ++b)
-#pragma unroll 1
-                for (int col = 0; col < it.rows; col += 16) {
-                    uint32_t o[16];
-                    tc::ld16(o_tmem + b * 64 + col + lane_base, o);
-                    tc::wait_ld();
-                    const int d = b * 128 + warp * 32 + lane;
-                    if (whole) {
-                        // four lanes trade values, so that each holds four dims of every fourth row and stores 8 bytes
-                        uint16_t *dst = a.out + (it.row0 + col + (lane & 3)) * D + (d & ~3);
+                for (int b = 0; b < NB; ++b) {
 #pragma unroll
-                        for (int k = 0; k < 16; k += 4) {
-                            const float4 f = *reinterpret_cast<const float4 *>(&inv_s[col + k]);
-                            const float y[4] = {__uint_as_float(o[k]) * f.x, __uint_as_float(o[k + 1]) * f.y,
-                                                __uint_as_float(o[k + 2]) * f.z, __uint_as_float(o[k + 3]) * f.w};
-                            const bool odd = lane & 1, high = lane & 2;
-                            // rows k, k+1 and k+2, k+3: an even lane keeps the even row and takes its neighbour's dim of it
-                            const float a0 = __shfl_xor_sync(0xffffffffu, odd ? y[0] : y[1], 1), a1 = __shfl_xor_sync(0xffffffffu, odd ? y[2] : y[3], 1);
-                            const uint32_t w0 = h2b(odd ? a0 : y[0], odd ? y[1] : a0), w1 = h2b(odd ? a1 : y[2], odd ? y[3] : a1);
-                            const uint32_t got = __shfl_xor_sync(0xffffffffu, high ? w0 : w1, 2);
-                            const uint2 out = high ? make_uint2(got, w1) : make_uint2(w0, got);
-                            if (col + k + (lane & 3) < it.rows) __stcs(reinterpret_cast<uint2 *>(dst + k * D), out);
+                    for (int hh = 0; hh < 2; ++hh) {                        // 16 of the warp's 32 dims
+                        uint32_t o[32];
+                        tc::ld_16x64(o_tmem + b * 64 + lane_base + ((uint32_t)(hh * 16) << 16), o);
+                        tc::wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 8; i += 2) {
+                            if (8 * i >= it.rows) break;
+                            uint32_t w[4];
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                const float2 f = *reinterpret_cast<const float2 *>(&inv_s[8 * (i + k) + 2 * (lane & 3)]);
+                                w[2 * k] = h2b(__uint_as_float(o[4 * (i + k)]) * f.x, __uint_as_float(o[4 * (i + k) + 1]) * f.y);
+                                w[2 * k + 1] = h2b(__uint_as_float(o[4 * (i + k) + 2]) * f.x, __uint_as_float(o[4 * (i + k) + 3]) * f.y);
+                            }
+                            const int rw = 8 * (i + (lane >> 4)) + (lane & 7), unit = warp * 4 + hh * 2 + ((lane >> 3) & 1);
+                            asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};"
+                                         ::"r"(smem_addr(p_s) + rw * 256 + ((unit ^ (rw & 7)) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
                         }
-                    } else {
-                        float *dst = g.part_o + ((int64_t)part * kRows + col) * D + d;
+                    }
+                    asm volatile("bar.sync 1, 128;" ::: "memory");
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int rw = i * 8 + (tid >> 4), unit = tid & 15;
+                        if (rw < it.rows)
+                            __stcs(reinterpret_cast<uint4 *>(a.out + (it.row0 + rw) * D + b * 128 + unit * 8),
+                                   *reinterpret_cast<const uint4 *>(p_s + rw * 256 + ((unit ^ (rw & 7)) << 4)));
+                    }
+                    asm volatile("bar.sync 1, 128;" ::: "memory");
+                }
+            } else {
+#pragma unroll 1
+                for (int b = 0; b < NB; ++b)
+#pragma unroll 1
+                    for (int col = 0; col < it.rows; col += 16) {
+                        uint32_t o[16];
+                        tc::ld16(o_tmem + b * 64 + col + lane_base, o);
+                        tc::wait_ld();
+                        float *dst = g.part_o + ((int64_t)part * kRows + col) * D + b * 128 + warp * 32 + lane;
 #pragma unroll
                         for (int k = 0; k < 16; ++k)
                             if (col + k < it.rows) dst[k * D] = __uint_as_float(o[k]);
                     }
-                }
+            }
             tc::fence_before();
             if (sg.t0 == 0 && sg.t1 < it.tiles)
                 last = Meta{it.row0, it.rows, (int)((per * (long long)blockIdx.x + done + it.tiles - 1) / per) - (int)blockIdx.x + 1};

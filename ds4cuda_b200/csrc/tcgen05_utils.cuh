@@ -7,7 +7,7 @@
 namespace ds4b200 {
 namespace tc {
 
-constexpr int kWaitPolls = 1 << 22;               // of some 10 ns to 2 us each: between a tenth of a second and a few
+constexpr int kWaitPolls = 1 << 22;               // of about 0.1 us each: about half a second
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -78,16 +78,18 @@ __device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&r)[16]) {
 // A wait on an mbarrier phase.  It polls at most kWaitPolls times; the first that runs out raises the status bit and a
 // CTA-wide flag with which every later wait returns at once, so the kernel always ends (its results are invalid then).
 __device__ __forceinline__ bool try_phase(uint64_t *bar, uint32_t parity) {
-    uint32_t done;                          // the hint lets the hardware hold the warp for up to 2 us instead of polling
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-                 "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(smem_addr(bar)), "r"(parity), "r"(2000u) : "memory");
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(smem_addr(bar)), "r"(parity) : "memory");
     return done != 0;
 }
 __device__ __forceinline__ void wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int *status) {
     if (try_phase(bar, parity)) return;
 #pragma unroll 1
-    for (int i = 0; i < kWaitPolls; ++i)
+    for (int i = 0; i < kWaitPolls; ++i) {
+        __nanosleep(40);                    // a poll takes shared-memory bandwidth from the operands of the MMAs
         if (try_phase(bar, parity) || *abort_flag) return;
+    }
     *abort_flag = 1;
     atomicOr(status, kStatusBulkCopyTimeout);
 }
