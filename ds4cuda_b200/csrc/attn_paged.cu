@@ -40,19 +40,19 @@ constexpr float kLog2e = 1.4426950408889634f;
 // partial sums (f32 O^T, M and l) that attn_join_kernel adds in order.  With many items each CTA takes whole ones.
 constexpr int kCtas = 148;
 constexpr int kRows = 64;                   // query rows of an item, cache rows of a tile
-constexpr int kLoadWarp0 = 4, kLoadWarps = 8, kMmaWarp = 12;
-constexpr int kThreads = 16 * 32;            // warp 15 only makes a register group whole
-constexpr int kSplitItems = 4 * kThreads;   // up to this many items the tiles are cut into equal runs
+constexpr int kSoftWarps = 8, kLoadWarp0 = 8, kLoadWarps = 8, kMmaWarp = 16;
+constexpr int kThreads = 20 * 32;            // the last warp only makes a register group whole
+constexpr int kSplitItems = 2048;   // up to this many items the tiles are cut into equal runs
 constexpr int kMinTiles = 2;                // of a run: below, the join costs more than the run saves
 constexpr float kRescale = 8.0f;            // log2 units
 constexpr int kScaleSets = 4;
 constexpr uint32_t kTmem = 0;               // all 512 columns are allocated, so they begin at column 0
 
-struct Meta { int64_t row0; int rows, parts; };
+struct Meta { int64_t row0; int rows, h0, parts, pad; };
 
 struct Item {
     int64_t row0;                           // first row of q / out, n_heads rows per token
-    int b, rows, p0, first, lo, n, tiles;
+    int b, rows, h0, p0, first, lo, n, tiles;
 };
 
 __device__ __forceinline__ Item get_item(const AttnArgs &a, int group, int head_groups, int slot) {
@@ -86,6 +86,7 @@ __device__ __forceinline__ Item get_item(const AttnArgs &a, int group, int head_
     it.n = max(0, it.first + last + 1 - it.lo);
     it.tiles = ntok <= 0 ? 0 : max(1, (it.n + kRows - 1) / kRows);
     it.row0 = (int64_t)tok0 * a.n_heads + hg * kRows;
+    it.h0 = hg * kRows;
     it.rows = head_groups > 1 ? min(kRows, a.n_heads - hg * kRows) : ntok * a.n_heads;
     return it;
 }
@@ -134,7 +135,7 @@ struct Segment {
 };
 constexpr int kSegRing = 8;
 constexpr int kAhead = 3;                   // tiles
-constexpr int kSegReaders = kLoadWarps + 4 + 2;
+constexpr int kSegReaders = kLoadWarps + kSoftWarps + 2;
 
 struct TcArgs {
     AttnArgs a;
@@ -200,8 +201,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         start_tile = 0;
         for (int i = 0; i < 2; ++i) {
             grown_s[i] = 0;
-            mbar_init(&scaled[i], 4);
-            mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4); mbar_init(&p_full[i], 4);
+            mbar_init(&scaled[i], kSoftWarps);
+            mbar_init(&s_full[i], 1); mbar_init(&s_free[i], kSoftWarps); mbar_init(&p_full[i], kSoftWarps);
             for (int k = 0; k < kParts; ++k) { mbar_init(&full[i][k], kLoadWarps); mbar_init(&pv_done[i][k], 1); }
         }
         mbar_init(&q_full, kLoadWarps); mbar_init(&q_free, 1);
@@ -255,10 +256,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         // A warp has eight rows of the tile.  Its loads cover two rows at a time, 256 contiguous bytes of each (16 lanes): whole lines,
         // and stores of rows r and r + 1 with their 16-byte units XORed by the row fall on all banks.  Scales, tails and the
         // query rows go by four lanes per row.  A register is loaded again, with the next unit's bytes, as soon as
-        // its value is converted, so loads run a tile ahead of the stores.  A unit is a tile, or 128 or 256 dims of one in f32.
-        tc::set_max_registers_up<152>();
+        // its value is converted, so loads run a tile ahead of the stores.  A unit is a tile, or 128 dims of one in f32.
+        tc::set_max_registers_up<136>();
         constexpr bool kF32 = FMT == DS4B200_KV_F32, kBlock = FMT == DS4B200_KV_FP8_BLOCK64;
-        constexpr int kUnitChunks = !kF32 ? kChunks : (NB % 2 ? 2 : 4), kUnits = kChunks / kUnitChunks;
+        constexpr int kUnitChunks = !kF32 ? kChunks : 2, kUnits = kChunks / kUnitChunks;
         constexpr int kSpan = kF32 ? 1 : 4;              // chunks a load of two rows covers (fewer with fewer dims)
         constexpr int kSteps = (kUnitChunks + kSpan - 1) / kSpan, kRegs = kSteps * 4;
         const int r = (warp - kLoadWarp0) * 8 + (lane >> 2), part = lane & 3;
@@ -367,40 +368,46 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             my = tile[0].slot;
             const int slot = tile[1].slot;
             if (tile[0].rows) {                          // a segment's query rows come ahead of its first tile
-                uint4 x[kChunks][2];
-                uint32_t amax = 0;
                 const int ring = nq & (kSegRing - 1);
                 const uint16_t *src = a.q + (seg_s[ring].it.row0 + r) * D + part * 16;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&seg_free[ring]);
+                // as they are where their largest value is within [2^-4, 2^15], else scaled by a power of two in a second pass
+                float up = 1.0f, down = 1.0f;
+#pragma unroll 1
+                for (int pass = 0; pass < 2; ++pass) {
+                    uint32_t amax = 0;
+#pragma unroll 1
+                    for (int c0 = 0; c0 < kChunks; c0 += 4) {
+                        uint4 x[4][2];
 #pragma unroll
-                for (int c = 0; c < kChunks; ++c)
+                        for (int c = 0; c < 4; ++c)
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) x[c][u] = r < tile[0].rows ? ld_row16(src + c * 64 + u * 8) : make_uint4(0, 0, 0, 0);
+                            for (int u = 0; u < 2; ++u)
+                                x[c][u] = r < tile[0].rows && c0 + c < kChunks ? ld_row16(src + (c0 + c) * 64 + u * 8) : make_uint4(0, 0, 0, 0);
+                        if (pass == 0 && c0 == 0) tc::wait(&q_free, (uint32_t)((nq & 1) ^ 1), abort_flag, status);
 #pragma unroll
-                for (int c = 0; c < kChunks; ++c)
+                        for (int c = 0; c < 4; ++c)
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const uint32_t y[4] = {x[c][u].x, x[c][u].y, x[c][u].z, x[c][u].w};
+                            for (int u = 0; u < 2; ++u) {
+                                const uint32_t y[4] = {x[c][u].x, x[c][u].y, x[c][u].z, x[c][u].w};
+                                uint32_t o[4];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) amax = max(amax, max(y[k] & 0x7fff0000u, (y[k] << 16) & 0x7fff0000u));
+                                for (int k = 0; k < 4; ++k) {
+                                    amax = max(amax, max(y[k] & 0x7fff0000u, (y[k] << 16) & 0x7fff0000u));
+                                    o[k] = h2_bits(__floats2half2_rn(__uint_as_float(y[k] << 16) * down, __uint_as_float(y[k] & 0xffff0000u) * down));
+                                }
+                                if (c0 + c < kChunks)
+                                    *reinterpret_cast<uint4 *>(q_s + (c0 + c) * 8192 + row_off + (((uint32_t)(part * 2 + u) ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+                            }
                     }
-                amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                float up, down;
-                pow2_parts(__uint_as_float(amax), up, down);
-                tc::wait(&q_free, (uint32_t)((nq & 1) ^ 1), abort_flag, status);
-#pragma unroll
-                for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const uint32_t y[4] = {x[c][u].x, x[c][u].y, x[c][u].z, x[c][u].w};
-                        uint32_t o[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            o[k] = h2_bits(__floats2half2_rn(__uint_as_float(y[k] << 16) * down, __uint_as_float(y[k] & 0xffff0000u) * down));
-                        *reinterpret_cast<uint4 *>(q_s + c * 8192 + row_off + (((uint32_t)(part * 2 + u) ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-                    }
+                    if (pass) break;
+                    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                    const bool far = amax != 0 && (amax < 0x3d800000u || amax > 0x47000000u);
+                    if (!__any_sync(0xffffffffu, far)) break;
+                    if (far) pow2_parts(__uint_as_float(amax), up, down);
+                }
                 if (part == 0) q_mul[nq & (kScaleSets - 1)][r] = up * a.scale * kLog2e;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&q_full);
@@ -496,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             tile[kAhead] = take();
         }
     } else if (warp >= kMmaWarp) {
-        tc::set_max_registers_down<80>();
+        tc::set_max_registers_down<56>();
         const uint32_t one = tc::elect();
         const uint32_t k_desc = tc::desc_lo(smem_addr(k_s), 0);
         if (warp == kMmaWarp) {
@@ -592,18 +599,25 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         }
     } else {
         // ------------------------------------------------------------------------------ softmax and output
-        const int row = warp * 16 + (lane >> 2);        // four lanes share rows `row` and `row` + 8 of S, 16 columns each
-        const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
+        // Eight warps, two per quarter of tensor memory's lanes: a quarter holds 16 rows of S (lanes 0-15), of which each warp takes
+        // eight, four lanes and 16 columns each.
+        tc::set_max_registers_down<72>();
+        const int quarter = warp & 3, group = warp >> 2;
+        const int row = quarter * 16 + group * 8 + (lane >> 2);
+        const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
         const bool several = g.head_groups == 1 && g.group > 1;
-        Meta last{0, 0, 0};
+        unsigned char *stage = p_s + group * 8192;      // of this group's output, where its weights' buffers are free
+        auto sync_group = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory"); };
+        Meta last{0, 0, 0, 0, 0};
         Segment sg;
         int n = 0;
         long long done = 0;
         for (int nq = 0; next_segment(sg); ++nq) {
             const Item &it = sg.it;
-            float qk[2] = {0.0f, 0.0f}, m[2] = {-INFINITY, -INFINITY};
-            float2 l[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-            const int p[2] = {it.p0 + (several ? row / a.n_heads : 0), it.p0 + (several ? (row + 8) / a.n_heads : 0)};
+            float qk = 0.0f, m = -INFINITY;
+            float2 l = make_float2(0.0f, 0.0f);
+            const int p = it.p0 + (several ? row / a.n_heads : 0);
+            const int from = a.window > 0 ? p - a.window : -1;              // cache rows above it are in the window
             // Scales the accumulators ahead of tile k's product where a row of that tile asked for it.
             auto follow = [&](int k) {
                 const int buf = k & 1;
@@ -612,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 tc::wait(&pv_done[buf ^ 1][kParts - 1], (uint32_t)(((k - 1) >> 1) & 1), abort_flag, status);
                 tc::fence_after();
 #pragma unroll 1
-                for (int u = 0; u < NB * 4; ++u) {
+                for (int u = group; u < NB * 4; u += 2) {
                     uint32_t o[16];
                     tc::ld16(o_tmem + u * 16 + lane_base, o);
                     tc::wait_ld();
@@ -632,94 +646,68 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 tc::wait(&full[buf][kParts - 1], phase, abort_flag, status);
                 tc::wait(&s_full[buf], phase, abort_flag, status);
                 tc::fence_after();
-                // written ahead of the segment's first tile by the same warps; q_full itself may be phases ahead of this warp
-                if (t == sg.t0)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) qk[h] = q_mul[nq & (kScaleSets - 1)][row + 8 * h];
                 uint32_t x[32];
                 tc::ld_16x64(s_tmem + buf * 64 + lane_base, x);
+                // written ahead of the segment's first tile by the same warps; q_full itself may be phases ahead of this warp
+                if (t == sg.t0) qk = q_mul[nq & (kScaleSets - 1)][row];
                 tc::wait_ld();
                 tc::fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&s_free[buf]);
-                float2 v[2][8];
+                float2 v[8];
+                const float2 k2 = make_float2(qk, qk);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float4 f = *reinterpret_cast<const float4 *>(&row_fma[buf][2 * (8 * i + 2 * (lane & 3))]);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float2 s = make_float2(__uint_as_float(x[4 * i + 2 * h]), __uint_as_float(x[4 * i + 2 * h + 1]));
-                        const float2 k = make_float2(qk[h], qk[h]);
-                        v[h][i] = FMT == DS4B200_KV_F32 ? fma2(s, k, make_float2(f.z, f.w)) : fma2(mul2(s, k), make_float2(f.x, f.y), make_float2(f.z, f.w));
-                    }
+                    const float2 s = make_float2(__uint_as_float(group ? x[4 * i + 2] : x[4 * i]), __uint_as_float(group ? x[4 * i + 3] : x[4 * i + 1]));
+                    v[i] = FMT == DS4B200_KV_F32 ? fma2(s, k2, make_float2(f.z, f.w)) : fma2(mul2(s, k2), make_float2(f.x, f.y), make_float2(f.z, f.w));
                 }
                 if ((t + 1) * kRows > it.n) {            // columns past the rows: S was not computed there
-                    const int end = it.n - t * kRows;
+                    const int end = it.n - t * kRows - 2 * (lane & 3);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            if (8 * i + 2 * (lane & 3) >= end) v[h][i].x = -INFINITY;
-                            if (8 * i + 2 * (lane & 3) + 1 >= end) v[h][i].y = -INFINITY;
-                        }
+                    for (int i = 0; i < 8; ++i) {
+                        if (8 * i >= end) v[i].x = -INFINITY;
+                        if (8 * i + 1 >= end) v[i].y = -INFINITY;
+                    }
                 }
                 if (several) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const int2 at = *reinterpret_cast<const int2 *>(&row_at[buf][8 * i + 2 * (lane & 3)]);
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int from = a.window > 0 ? p[h] - a.window : -1;       // rows above it are in the window
-                            if (at.x > p[h] || (at.x <= from && at.x >= a.n_first)) v[h][i].x = -INFINITY;
-                            if (at.y > p[h] || (at.y <= from && at.y >= a.n_first)) v[h][i].y = -INFINITY;
-                        }
+                        if (at.x > p || (at.x <= from && at.x >= a.n_first)) v[i].x = -INFINITY;
+                        if (at.y > p || (at.y <= from && at.y >= a.n_first)) v[i].y = -INFINITY;
                     }
                 }
-                float top[2];
+                float w[4];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float w[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = fmaxf(fmaxf(v[h][i].x, v[h][i].y), fmaxf(v[h][i + 4].x, v[h][i + 4].y));
-                    top[h] = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
-                }
+                for (int i = 0; i < 4; ++i) w[i] = fmaxf(fmaxf(v[i].x, v[i].y), fmaxf(v[i + 4].x, v[i + 4].y));
+                float top = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])), f = 1.0f;
                 // A row keeps the reference its maximum had until one of its values lies kRescale above it.  Then it takes a
                 // new one, and every row's factor for the accumulators (a column of O^T) is left for follow(), which the
-                // four warps run together, at the next tile.
-                if (__any_sync(0xffffffffu, !(top[0] <= m[0] + kRescale) || !(top[1] <= m[1] + kRescale))) {
-                    bool grown = false;
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-                        top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-                        float f = 1.0f;
-                        if (m[h] > -INFINITY && top[h] > m[h] + kRescale) {
-                            f = tc::exp2_approx(m[h] - top[h]);
-                            m[h] = top[h];
-                            l[h] = mul2(l[h], make_float2(f, f));
-                            grown = true;
-                        }
-                        if (m[h] == -INFINITY) m[h] = top[h];
-                        if ((lane & 3) == 0) fac_s[buf][row + 8 * h] = f;
+                // warps run together, at the next tile.
+                if (__any_sync(0xffffffffu, !(top <= m + kRescale))) {
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    if (m > -INFINITY && top > m + kRescale) {
+                        f = tc::exp2_approx(m - top);
+                        m = top;
+                        l = mul2(l, make_float2(f, f));
+                        grown_s[buf] = n + 1;
                     }
-                    if (grown) grown_s[buf] = n + 1;
-                } else if ((lane & 3) == 0) {
-                    fac_s[buf][row] = fac_s[buf][row + 8] = 1.0f;
+                    if (m == -INFINITY) m = top;
                 }
+                if ((lane & 3) == 0) fac_s[buf][row] = f;
+                const float ref = m == -INFINITY ? 0.0f : -m;
+                const float2 ref2 = make_float2(ref, ref);
+                unsigned char *dst = p_s + buf * 8192 + row * 128 + (lane & 3) * 4;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float ref = m[h] == -INFINITY ? 0.0f : -m[h];
-                    const float2 ref2 = make_float2(ref, ref);
-                    unsigned char *dst = p_s + buf * 8192 + (row + 8 * h) * 128 + (lane & 3) * 4;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        float2 e = add2(v[h][i], ref2);
-                        e.x = tc::exp2_approx(e.x);
-                        e.y = tc::exp2_approx(e.y);
-                        if (FMT == DS4B200_KV_F32) l[h] = add2(l[h], e);
-                        else l[h] = fma2(e, *reinterpret_cast<const float2 *>(&row_div[buf][8 * i + 2 * (lane & 3)]), l[h]);
-                        *reinterpret_cast<uint32_t *>(dst + (((uint32_t)i ^ (uint32_t)(row & 7)) << 4)) = h2_bits(__floats2half2_rn(e.x, e.y));
-                    }
+                for (int i = 0; i < 8; ++i) {
+                    float2 e = add2(v[i], ref2);
+                    e.x = tc::exp2_approx(e.x);
+                    e.y = tc::exp2_approx(e.y);
+                    if (FMT == DS4B200_KV_F32) l = add2(l, e);
+                    else l = fma2(e, *reinterpret_cast<const float2 *>(&row_div[buf][8 * i + 2 * (lane & 3)]), l);
+                    *reinterpret_cast<uint32_t *>(dst + (((uint32_t)i ^ (uint32_t)(row & 7)) << 4)) = h2_bits(__floats2half2_rn(e.x, e.y));
                 }
                 tc::fence_async();
                 tc::fence_before();
@@ -727,91 +715,89 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 if (lane == 0) mbar_arrive(&p_full[buf]);
             }
             follow(n - 1);
-            float sum[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                sum[h] = l[h].x + l[h].y;
-                sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 1);
-                sum[h] += __shfl_xor_sync(0xffffffffu, sum[h], 2);
+            float sum = l.x + l.y;
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            const bool whole = sg.t0 == 0 && sg.t1 == it.tiles;
+            const int part = 2 * (int)blockIdx.x + (sg.t0 == 0 ? 1 : 0);
+            float inv = 1.0f, lse2 = 0.0f;
+            if (whole) {
+                lse2 = sum > 0.0f ? m + __log2f(sum) : (sum == sum ? -INFINITY : sum);
+                if (a.sink && row < it.rows) {
+                    const float own = lse2, s2 = __ldg(a.sink + it.h0 + (several ? row % a.n_heads : row)) * kLog2e, hi = fmaxf(own, s2);
+                    if (hi > -INFINITY) lse2 = hi + __log2f(tc::exp2_approx(own - hi) + tc::exp2_approx(s2 - hi));
+                }
+                inv = m == -INFINITY ? 0.0f : tc::exp2_approx(m - lse2);
             }
             // the segment's accumulators; behind this wait every warp is through with the last segment's inv_s
             tc::wait(&pv_done[(n - 1) & 1][kParts - 1], (uint32_t)(((n - 1) >> 1) & 1), abort_flag, status);
             tc::fence_after();
-            const bool whole = sg.t0 == 0 && sg.t1 == it.tiles;
-            const int part = 2 * (int)blockIdx.x + (sg.t0 == 0 ? 1 : 0);
-            if ((lane & 3) == 0)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int rw = row + 8 * h;
-                    float inv = 1.0f;
-                    if (!whole) {
-                        g.part_ml[part * kRows + rw] = make_float2(m[h], sum[h]);
-                    } else if (rw < it.rows) {
-                        const float own = sum[h] > 0.0f ? m[h] + log2f(sum[h]) : (sum[h] == sum[h] ? -INFINITY : sum[h]);
-                        float lse2 = own;
-                        if (a.sink) {
-                            const float s2 = a.sink[(it.row0 + rw) % a.n_heads] * kLog2e, hi = fmaxf(own, s2);
-                            lse2 = hi == -INFINITY ? hi : hi + log2f(exp2f(own - hi) + exp2f(s2 - hi));
-                        }
-                        inv = m[h] == -INFINITY ? 0.0f : exp2f(m[h] - lse2);
-                        if (a.lse) a.lse[it.row0 + rw] = lse2 * (1.0f / kLog2e);
-                    }
-                    inv_s[rw] = inv;
-                }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if ((lane & 3) == 0) {
+                if (!whole) g.part_ml[part * kRows + row] = make_float2(m, sum);
+                else if (a.lse && row < it.rows) a.lse[it.row0 + row] = lse2 * (1.0f / kLog2e);
+                inv_s[row] = inv;
+            }
+            asm volatile("bar.sync 3, 256;" ::: "memory");
             // In tensor memory a lane is a dim and a column a query row.
             if (whole) {
-                // 128 dims at a time through the weights' buffers, which are free here: stmatrix turns 8 x 8 blocks around, rows of
-                // 256 bytes with their 16-byte units XORed by the row, and every lane stores 16 bytes of a row
+                // 128 dims of 32 rows at a time through the weights' buffers, which are free here: stmatrix turns 8 x 8 blocks around, rows
+                // of 256 bytes with their 16-byte units XORed by the row, and every lane stores 16 bytes of a row
 #pragma unroll 1
-                for (int b = 0; b < NB; ++b) {
+                for (int u = group; u < NB * 2; u += 2) {
+                    const int b = u >> 1, r0 = (u & 1) * 32;
+                    if (r0 >= it.rows) continue;
+                    uint32_t o[2][16];
 #pragma unroll
-                    for (int hh = 0; hh < 2; ++hh) {                        // 16 of the warp's 32 dims
-                        uint32_t o[32];
-                        tc::ld_16x64(o_tmem + b * 64 + lane_base + ((uint32_t)(hh * 16) << 16), o);
-                        tc::wait_ld();
+                    for (int hh = 0; hh < 2; ++hh)                          // 16 of the warp's 32 dims
+                        tc::ld_16x32(o_tmem + b * 64 + r0 + lane_base + ((uint32_t)(hh * 16) << 16), o[hh]);
+                    tc::wait_ld();
 #pragma unroll
-                        for (int i = 0; i < 8; i += 2) {
-                            if (8 * i >= it.rows) break;
+                    for (int i = 0; i < 4; i += 2) {
+                        const float2 f0 = *reinterpret_cast<const float2 *>(&inv_s[r0 + 8 * i + 2 * (lane & 3)]);
+                        const float2 f1 = *reinterpret_cast<const float2 *>(&inv_s[r0 + 8 * i + 8 + 2 * (lane & 3)]);
+                        const int rw = 8 * (i + (lane >> 4)) + (lane & 7);
+#pragma unroll
+                        for (int hh = 0; hh < 2; ++hh) {
+                            const uint32_t *y = &o[hh][4 * i];
                             uint32_t w[4];
-#pragma unroll
-                            for (int k = 0; k < 2; ++k) {
-                                const float2 f = *reinterpret_cast<const float2 *>(&inv_s[8 * (i + k) + 2 * (lane & 3)]);
-                                w[2 * k] = h2b(__uint_as_float(o[4 * (i + k)]) * f.x, __uint_as_float(o[4 * (i + k) + 1]) * f.y);
-                                w[2 * k + 1] = h2b(__uint_as_float(o[4 * (i + k) + 2]) * f.x, __uint_as_float(o[4 * (i + k) + 3]) * f.y);
-                            }
-                            const int rw = 8 * (i + (lane >> 4)) + (lane & 7), unit = warp * 4 + hh * 2 + ((lane >> 3) & 1);
+                            w[0] = h2b(__uint_as_float(y[0]) * f0.x, __uint_as_float(y[1]) * f0.y);
+                            w[1] = h2b(__uint_as_float(y[2]) * f0.x, __uint_as_float(y[3]) * f0.y);
+                            w[2] = h2b(__uint_as_float(y[4]) * f1.x, __uint_as_float(y[5]) * f1.y);
+                            w[3] = h2b(__uint_as_float(y[6]) * f1.x, __uint_as_float(y[7]) * f1.y);
+                            const int unit = quarter * 4 + hh * 2 + ((lane >> 3) & 1);
                             asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};"
-                                         ::"r"(smem_addr(p_s) + rw * 256 + ((unit ^ (rw & 7)) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+                                         ::"r"(smem_addr(stage) + rw * 256 + ((unit ^ (rw & 7)) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
                         }
                     }
-                    asm volatile("bar.sync 1, 128;" ::: "memory");
+                    sync_group();
+                    const int t128 = tid & 127, unit = t128 & 15;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int rw = i * 8 + (tid >> 4), unit = tid & 15;
-                        if (rw < it.rows)
-                            __stcs(reinterpret_cast<uint4 *>(a.out + (it.row0 + rw) * D + b * 128 + unit * 8),
-                                   *reinterpret_cast<const uint4 *>(p_s + rw * 256 + ((unit ^ (rw & 7)) << 4)));
+                    for (int i = 0; i < 4; ++i) {
+                        const int rw = i * 8 + (t128 >> 4);
+                        if (r0 + rw < it.rows)
+                            __stcs(reinterpret_cast<uint4 *>(a.out + (it.row0 + r0 + rw) * D + b * 128 + unit * 8),
+                                   *reinterpret_cast<const uint4 *>(stage + rw * 256 + ((unit ^ (rw & 7)) << 4)));
                     }
-                    asm volatile("bar.sync 1, 128;" ::: "memory");
+                    sync_group();
                 }
+                asm volatile("bar.sync 3, 256;" ::: "memory");             // the next weights go where either group's rows were
             } else {
 #pragma unroll 1
-                for (int b = 0; b < NB; ++b)
-#pragma unroll 1
-                    for (int col = 0; col < it.rows; col += 16) {
-                        uint32_t o[16];
-                        tc::ld16(o_tmem + b * 64 + col + lane_base, o);
-                        tc::wait_ld();
-                        float *dst = g.part_o + ((int64_t)part * kRows + col) * D + b * 128 + warp * 32 + lane;
+                for (int u = group; u < NB * 4; u += 2) {
+                    const int b = u >> 2, col = (u & 3) * 16;
+                    if (col >= it.rows) continue;
+                    uint32_t o[16];
+                    tc::ld16(o_tmem + b * 64 + col + lane_base, o);
+                    tc::wait_ld();
+                    float *to = g.part_o + ((int64_t)part * kRows + col) * D + b * 128 + quarter * 32 + lane;
 #pragma unroll
-                        for (int k = 0; k < 16; ++k)
-                            if (col + k < it.rows) dst[k * D] = __uint_as_float(o[k]);
-                    }
+                    for (int k = 0; k < 16; ++k)
+                        if (col + k < it.rows) to[k * D] = __uint_as_float(o[k]);
+                }
             }
             tc::fence_before();
             if (sg.t0 == 0 && sg.t1 < it.tiles)
-                last = Meta{it.row0, it.rows, (int)((per * (long long)blockIdx.x + done + it.tiles - 1) / per) - (int)blockIdx.x + 1};
+                last = Meta{it.row0, it.rows, it.h0, (int)((per * (long long)blockIdx.x + done + it.tiles - 1) / per) - (int)blockIdx.x + 1, 0};
             done += sg.t1 - sg.t0;
         }
         if (g.split && tid == 0) g.meta[blockIdx.x] = last;
@@ -827,9 +813,9 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a, const 
     __shared__ float red[8];
     const Meta it = meta[blockIdx.x];
     const int row = blockIdx.y, D = a.kv.head_dim, tid = threadIdx.x;
-    if (row >= it.rows || it.parts < 2) return;
+    if (it.parts < 2 || row >= it.rows) return;
     auto part_of = [&](int k) { return k == 0 ? 2 * (int)blockIdx.x + 1 : 2 * ((int)blockIdx.x + k); };
-    const float sink2 = a.sink ? a.sink[(it.row0 + row) % a.n_heads] * kLog2e : -INFINITY;
+    const float sink2 = a.sink ? a.sink[it.h0 + row % a.n_heads] * kLog2e : -INFINITY;
     float hi = sink2;
     for (int k = tid; k < it.parts; k += 128) {
         const float2 ml = part_ml[part_of(k) * kRows + row];
