@@ -4,6 +4,7 @@
 // Mathematics: o_h = sum_j exp(s_hj - lse_h) k_j with s_hj = scale q_h . k_j over the visible rows j and
 // lse_h = log(sum_j exp(s_hj) + exp(sink_h)).  One row is key and value of every head (the reference's
 // cache has one KV head; cuda/flash_attn.cu:148-313).
+#include <algorithm>
 #include <mutex>
 #include <type_traits>
 
@@ -42,7 +43,8 @@ constexpr int kCtas = 148;
 constexpr int kRows = 64;                   // query rows of an item, cache rows of a tile
 constexpr int kSoftWarps = 8, kLoadWarp0 = 8, kLoadWarps = 8, kMmaWarp = 16;
 constexpr int kThreads = 20 * 32;            // the last warp only makes a register group whole
-constexpr int kSplitItems = 2048;   // up to this many items the tiles are cut into equal runs
+constexpr int kSplitItems = 4 * kCtas;
+constexpr int kWholeTiles = 3;              // items of up to so many tiles are not cut
 constexpr int kMinTiles = 2;                // of a run: below, the join costs more than the run saves
 constexpr float kRescale = 8.0f;            // log2 units
 constexpr int kScaleSets = 4;
@@ -193,6 +195,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     __shared__ __align__(8) uint64_t scaled[2];
     volatile int *abort_flag = &abort_s;
     int *status = g.status;
+    launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
     if (tid == 0) {
@@ -216,23 +219,26 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     long long per = 1, left = 1ll << 62;
     if (g.split) {
         __syncthreads();
-        long long total = 0, seen = 0;
-        for (int pass = 0; pass < 2; ++pass) {
-            const long long from = per * blockIdx.x;
-            for (int base = 0; base < g.n_slots; base += kThreads) {
-                const int s = base + tid;
-                const int tiles = s < g.n_slots ? get_item(a, g.group, g.head_groups, s).tiles : 0;
-                long long sum;
-                const long long before = seen + block_scan64(tiles, scan_s, &sum);
-                if (pass && before <= from && from < before + tiles) { start_slot = s; start_tile = (int)(from - before); }
-                seen += sum;
-            }
-            if (pass == 0) {
-                total = seen;
-                per = max((long long)kMinTiles, (total + kCtas - 1) / kCtas);
-                seen = 0;
-            }
+        // every thread has the items tid, tid + kThreads, ..: their tiles are counted once, then the run's first one is found
+        constexpr int kMine = (kSplitItems + kThreads - 1) / kThreads;
+        int tiles[kMine];
+        long long before[kMine], total = 0;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            const int s = i * kThreads + tid;
+            tiles[i] = 0;
+            before[i] = total;
+            if (i * kThreads >= g.n_slots) continue;
+            if (s < g.n_slots) tiles[i] = get_item(a, g.group, g.head_groups, s).tiles;
+            long long sum;
+            before[i] += block_scan64(tiles[i], scan_s, &sum);
+            total += sum;
         }
+        per = max((long long)kMinTiles, (total + kCtas - 1) / kCtas);
+        const long long from = per * blockIdx.x;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i)
+            if (before[i] <= from && from < before[i] + tiles[i]) { start_slot = i * kThreads + tid; start_tile = (int)(from - before[i]); }
         left = min(per, total - per * (long long)blockIdx.x);
     }
     tc::fence_before();
@@ -284,6 +290,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             const int i = t * kRows + r;
             found.at = i < sg.it.first ? i : sg.it.lo + (i - sg.it.first);
             found.rows = !more ? -1 : first ? sg.it.rows : 0;
+            if (found.rows > r) {                        // its query rows are wanted when the tile is stored
+#pragma unroll
+                for (int u = 0; u < NB; ++u) prefetch_l2(a.q + (sg.it.row0 + r) * D + (u * 4 + part) * 32);
+            }
             page = -1;
             if (more && i < sg.it.n) {
                 const int pg = g.page_shift >= 0 ? found.at >> g.page_shift : found.at / a.kv.page_rows;
@@ -346,10 +356,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 }
         };
         Tile tile[kAhead + 1];                           // [0] is being stored, [1] loaded
+        {
+            int pages[kAhead + 1], ins[kAhead + 1];
 #pragma unroll
-        for (int k = 0; k <= kAhead; ++k) {
-            find();
-            tile[k] = take();
+            for (int k = 0; k <= kAhead; ++k) {          // the look-ups of the first tiles travel together
+                find();
+                tile[k] = found;
+                pages[k] = page;
+                ins[k] = in_page;
+            }
+#pragma unroll
+            for (int k = 0; k <= kAhead; ++k) {
+                found = tile[k];
+                page = pages[k];
+                in_page = ins[k];
+                tile[k] = take();
+            }
         }
         int my = tile[0].slot;
 #pragma unroll
@@ -807,50 +829,79 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem_s));
 }
 
-// Joins the parts of the item that CTA blockIdx.x began and did not finish; one query row per CTA.
-__global__ void __launch_bounds__(128) attn_join_kernel(const AttnArgs a, const Meta *meta, const float2 *part_ml, const float *part_o) {
-    __shared__ float weight[kCtas];
-    __shared__ float red[8];
-    const Meta it = meta[blockIdx.x];
-    const int row = blockIdx.y, D = a.kv.head_dim, tid = threadIdx.x;
-    if (it.parts < 2 || row >= it.rows) return;
-    auto part_of = [&](int k) { return k == 0 ? 2 * (int)blockIdx.x + 1 : 2 * ((int)blockIdx.x + k); };
-    const float sink2 = a.sink ? a.sink[it.h0 + row % a.n_heads] * kLog2e : -INFINITY;
-    float hi = sink2;
-    for (int k = tid; k < it.parts; k += 128) {
-        const float2 ml = part_ml[part_of(k) * kRows + row];
-        const float v = ml.y > 0.0f ? ml.x + log2f(ml.y) : (ml.y == ml.y ? -INFINITY : ml.y);
-        weight[k] = v;
-        hi = fmaxf(hi, v);
-    }
-    hi = warp_max(hi);
-    if ((tid & 31) == 0) red[tid >> 5] = hi;
-    __syncthreads();
-    hi = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    float sum = 0.0f;
-    for (int k = tid; k < it.parts; k += 128) sum += hi == -INFINITY ? 0.0f : exp2f(weight[k] - hi);
-    sum = warp_sum(sum);
-    if ((tid & 31) == 0) red[4 + (tid >> 5)] = sum;
-    __syncthreads();
-    sum = (red[4] + red[5]) + (red[6] + red[7]);
-    if (a.sink && hi > -INFINITY) sum += exp2f(sink2 - hi);
-    const float lse2 = hi == -INFINITY ? hi : hi + log2f(sum);
-    __syncthreads();
-    for (int k = tid; k < it.parts; k += 128) {
-        const float m = part_ml[part_of(k) * kRows + row].x;
-        weight[k] = m == -INFINITY ? 0.0f : exp2f(m - lse2);
-    }
-    __syncthreads();
-    if (tid == 0 && a.lse) a.lse[it.row0 + row] = lse2 * (1.0f / kLog2e);
-    if (4 * tid < D) {
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-        for (int k = 0; k < it.parts; ++k) {
-            const float4 v = __ldg(reinterpret_cast<const float4 *>(part_o + ((int64_t)part_of(k) * kRows + row) * D + 4 * tid));
-            const float w = weight[k];
-            o = make_float4(fmaf(w, v.x, o.x), fmaf(w, v.y, o.y), fmaf(w, v.z, o.z), fmaf(w, v.w, o.w));
+// Joins the parts of the items that a CTA began and did not finish, in order.  A unit is one query row and 128 dims of such an item, four
+// dims a lane.  An item of few parts takes a warp per unit; one of many (a session of 131072 rows leaves 148 parts of 128 KiB) a
+// CTA, whose eight warps take every eighth part, since the latency of the loads is what a unit costs.
+constexpr int kJoinCtas = 4 * kCtas, kJoinWarps = 8, kJoinFew = 8;
+
+__global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const AttnArgs a, const Meta *meta, const float2 *part_ml, const float *part_o) {
+    __shared__ int begun[2][kCtas], n_begun[2];          // items of few and of many parts
+    __shared__ float weight[kJoinWarps][kCtas];
+    __shared__ float4 sums[kJoinWarps][32];
+    const int D = a.kv.head_dim, slices = D / 128, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    wait_dependency();
+    if (warp < 2) {
+        int n = 0;
+        for (int base = 0; base < kCtas; base += 32) {
+            const int c = base + lane, parts = c < kCtas ? meta[c].parts : 0;
+            const bool is = parts >= 2 && (parts > kJoinFew) == (warp == 1);
+            const uint32_t all = __ballot_sync(0xffffffffu, is);
+            if (is) begun[warp][n + __popc(all & ((1u << lane) - 1))] = c;
+            n += __popc(all);
         }
-        st_bf16x4(a.out + (it.row0 + row) * D + 4 * tid, o);
+        if (lane == 0) n_begun[warp] = n;
+    }
+    __syncthreads();
+    for (int many = 0; many < 2; ++many) {
+        const int units = n_begun[many] * kRows * slices;
+        const int lead = many ? warp : 0, step = many ? kJoinWarps : 1;     // this warp's first part and its stride
+        for (int u = many ? blockIdx.x : blockIdx.x * kJoinWarps + warp; u < units; u += many ? gridDim.x : gridDim.x * kJoinWarps) {
+            const int c = begun[many][u / (kRows * slices)], row = u / slices % kRows, slice = u % slices;
+            const Meta it = meta[c];
+            if (row >= it.rows) continue;
+            auto part_of = [&](int k) { return k == 0 ? 2 * c + 1 : 2 * (c + k); };
+            const float sink2 = a.sink ? __ldg(a.sink + it.h0 + row % a.n_heads) * kLog2e : -INFINITY;
+            const int d = slice * 128 + lane * 4;
+            float hi = sink2;
+            for (int k = lane; k < it.parts; k += 32) {
+                const float2 ml = part_ml[part_of(k) * kRows + row];
+                hi = fmaxf(hi, ml.y > 0.0f ? ml.x + __log2f(ml.y) : (ml.y == ml.y ? -INFINITY : ml.y));
+            }
+            hi = warp_max(hi);
+            float sum = 0.0f;
+            for (int k = lane; k < it.parts; k += 32) {
+                const float2 ml = part_ml[part_of(k) * kRows + row];
+                const float v = ml.y > 0.0f ? ml.x + __log2f(ml.y) : (ml.y == ml.y ? -INFINITY : ml.y);
+                sum += hi == -INFINITY ? 0.0f : tc::exp2_approx(v - hi);
+                weight[warp][k] = ml.x;
+            }
+            sum = warp_sum(sum);
+            if (a.sink && hi > -INFINITY) sum += tc::exp2_approx(sink2 - hi);
+            const float lse2 = hi == -INFINITY ? hi : hi + __log2f(sum);
+            __syncwarp();
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+            for (int k = lead; k < it.parts; k += step) {
+                const float4 x = __ldg(reinterpret_cast<const float4 *>(part_o + ((int64_t)part_of(k) * kRows + row) * D + d));
+                const float m = weight[warp][k], w = m == -INFINITY ? 0.0f : tc::exp2_approx(m - lse2);
+                o = make_float4(fmaf(w, x.x, o.x), fmaf(w, x.y, o.y), fmaf(w, x.z, o.z), fmaf(w, x.w, o.w));
+            }
+            if (many) {
+                sums[warp][lane] = o;
+                __syncthreads();
+                o = sums[0][lane];
+                for (int k = 1; k < kJoinWarps; ++k) {
+                    const float4 x = sums[k][lane];
+                    o = make_float4(o.x + x.x, o.y + x.y, o.z + x.z, o.w + x.w);
+                }
+                __syncthreads();
+            }
+            if (lead == 0) {
+                st_bf16x4(a.out + (it.row0 + row) * D + d, o);
+                if (lane == 0 && slice == 0 && a.lse) a.lse[it.row0 + row] = lse2 * (1.0f / kLog2e);
+            }
+            __syncwarp();
+        }
     }
 }
 
@@ -862,7 +913,12 @@ void launch_tc(const AttnArgs &a, cudaStream_t s) {
     const int head_groups = (a.n_heads + kRows - 1) / kRows;
     const int group = a.q_start && head_groups == 1 ? kRows / a.n_heads : 1;
     const int64_t slots = (a.q_start ? a.n_tokens / group + a.n_seqs + 1 : a.n_seqs) * head_groups;
-    const int split = slots <= kSplitItems;
+    // Equal runs of tiles pay where items are long and few: a run's two ends cost 128 KiB of partial sums each and the join
+    // another launch.  512 prompt tokens of 3 tiles took 91 us cut into runs and XX us as whole items; one session of 131072 rows
+    // takes one CTA as a whole item.
+    const int64_t all_rows = a.table_width * a.kv.page_rows;
+    const int64_t seen = a.window > 0 ? std::min<int64_t>(all_rows, (int64_t)a.window + a.n_first + group - 1) : all_rows;
+    const int split = seen > kWholeTiles * kRows && slots <= kSplitItems;
     unsigned char *ws = static_cast<unsigned char *>(a.ws);
     Meta *meta = reinterpret_cast<Meta *>(ws);
     float2 *ml = reinterpret_cast<float2 *>(ws + kMetaBytes);
@@ -879,7 +935,7 @@ void launch_tc(const AttnArgs &a, cudaStream_t s) {
     for (int k = 0; k < 31; ++k) if (a.kv.page_rows == 1 << k) shift = k;
     const TcArgs g{a, group, head_groups, (int)slots, split, shift, meta, ml, po, device_status_word()};
     attn_tc_kernel<NB, FMT><<<grid, kThreads, smem, s>>>(g);
-    if (split) attn_join_kernel<<<dim3(kCtas, kRows), 128, 0, s>>>(a, meta, ml, po);
+    if (split) launch_behind(attn_join_kernel, kJoinCtas, kJoinWarps * 32, s, a, (const Meta *)meta, (const float2 *)ml, (const float *)po);
 }
 
 template <int NB>

@@ -95,6 +95,7 @@ __device__ __forceinline__ void copy_refs(const Tables &t) {
 __global__ void __launch_bounds__(kPlanThreads) plan_fork_kernel(Tables t, const int2 *pairs, int n_pairs, Work w, int *status) {
     __shared__ int scratch[33];
     __shared__ int bad;
+    launch_dependents();
     const int tid = threadIdx.x;
     if (tid == 0) bad = 0;
     for (int64_t s = tid; s < t.n_seqs; s += kPlanThreads) w.mark[s] = 0;
@@ -152,6 +153,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_fork_kernel(Tables t, const
 __global__ void __launch_bounds__(kPlanThreads) plan_reserve_kernel(Tables t, const int *new_lens, Work w, int *status) {
     __shared__ int scratch[33];
     __shared__ int bad;
+    launch_dependents();
     const int tid = threadIdx.x;
     if (tid == 0) bad = 0;
     __syncthreads();
@@ -190,6 +192,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_reserve_kernel(Tables t, co
 
 __global__ void __launch_bounds__(kPlanThreads) plan_free_kernel(Tables t, const int *seqs, int n_list, Work w, int *status) {
     __shared__ int bad;
+    launch_dependents();
     const int tid = threadIdx.x;
     if (tid == 0) bad = 0;
     for (int64_t s = tid; s < t.n_seqs; s += kPlanThreads) w.mark[s] = 0;
@@ -226,6 +229,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_free_kernel(Tables t, const
 
 __global__ void __launch_bounds__(kPlanThreads) plan_compact_kernel(Tables t, Work w, int *n_live) {
     __shared__ int scratch[33];
+    launch_dependents();
     const int tid = threadIdx.x;
     int live = 0;
     for (int64_t p = tid; p < t.n_pages; p += kPlanThreads) live += t.refs_in[p] > 0;
@@ -260,6 +264,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_compact_kernel(Tables t, Wo
 
 __global__ void __launch_bounds__(kPlanThreads) plan_copy_kernel(const int2 *moves, int n_moves, int64_t n_pages, Work w, int *status) {
     __shared__ int bad;
+    launch_dependents();
     const int tid = threadIdx.x;
     if (tid == 0) bad = 0;
     for (int64_t p = tid; p < n_pages; p += kPlanThreads) w.map[p] = 0;
@@ -305,6 +310,7 @@ __device__ __forceinline__ void move_unit(const unsigned char *src, unsigned cha
 template <int OP>
 __global__ void __launch_bounds__(kMoveThreads) apply_kernel(Tables t, const int2 *pairs, Work w,
                                                              const __grid_constant__ ArrayList a) {
+    wait_dependency();
     const bool done = w.head->status == 0;
     const int64_t step = (int64_t)gridDim.x * kMoveThreads, me = (int64_t)blockIdx.x * kMoveThreads + threadIdx.x;
     if (OP != kCopy) {
@@ -404,7 +410,7 @@ void pages_copy(const ds4b200_page_array *host, int n_arrays, int64_t n_pages, c
     const ArrayList a = list_arrays(host, n_arrays);
     const int2 *mv = reinterpret_cast<const int2 *>(moves);
     plan_copy_kernel<<<1, kPlanThreads, 0, s>>>(mv, (int)n_moves, n_pages, w, status);
-    apply_kernel<kCopy><<<kMoveCtas, kMoveThreads, 0, s>>>(Tables{}, mv, w, a);
+    launch_behind(apply_kernel<kCopy>, kMoveCtas, kMoveThreads, s, Tables{}, mv, w, a);
 }
 
 void pages_fork(const ds4b200_page_array *host, int n_arrays, const PageTables &p, const int32_t *pairs, int64_t n_pairs,
@@ -414,21 +420,21 @@ void pages_fork(const ds4b200_page_array *host, int n_arrays, const PageTables &
     const ArrayList a = list_arrays(host, n_arrays);
     const int2 *pr = reinterpret_cast<const int2 *>(pairs);
     plan_fork_kernel<<<1, kPlanThreads, 0, s>>>(t, pr, (int)n_pairs, w, status);
-    apply_kernel<kFork><<<kMoveCtas, kMoveThreads, 0, s>>>(t, pr, w, a);
+    launch_behind(apply_kernel<kFork>, kMoveCtas, kMoveThreads, s, t, pr, w, a);
 }
 
 void pages_reserve(const PageTables &p, const int32_t *new_lens, int32_t *status, void *ws, cudaStream_t s) {
     const Tables t{p.refs_in, p.refs_out, p.table_in, p.table_out, p.lens_in, p.lens_out, p.n_pages, p.n_seqs, p.width, p.page_rows};
     const Work w = lay_out(ws, p.n_pages, p.n_seqs, 0);
     plan_reserve_kernel<<<1, kPlanThreads, 0, s>>>(t, new_lens, w, status);
-    apply_kernel<kReserve><<<small_grid(p.n_seqs * p.width), kMoveThreads, 0, s>>>(t, nullptr, w, ArrayList{});
+    launch_behind(apply_kernel<kReserve>, small_grid(p.n_seqs * p.width), kMoveThreads, s, t, (const int2 *)nullptr, w, ArrayList{});
 }
 
 void pages_free(const PageTables &p, const int32_t *seqs, int64_t n_list, int32_t *status, void *ws, cudaStream_t s) {
     const Tables t{p.refs_in, p.refs_out, p.table_in, p.table_out, p.lens_in, p.lens_out, p.n_pages, p.n_seqs, p.width, p.page_rows};
     const Work w = lay_out(ws, p.n_pages, p.n_seqs, n_list);
     plan_free_kernel<<<1, kPlanThreads, 0, s>>>(t, seqs, (int)n_list, w, status);
-    apply_kernel<kFree><<<small_grid(p.n_seqs * p.width), kMoveThreads, 0, s>>>(t, nullptr, w, ArrayList{});
+    launch_behind(apply_kernel<kFree>, small_grid(p.n_seqs * p.width), kMoveThreads, s, t, (const int2 *)nullptr, w, ArrayList{});
 }
 
 void pages_compact(const ds4b200_page_array *host, int n_arrays, const PageTables &p, int32_t *n_live, void *ws, cudaStream_t s) {
@@ -436,7 +442,7 @@ void pages_compact(const ds4b200_page_array *host, int n_arrays, const PageTable
     const Work w = lay_out(ws, p.n_pages, p.n_seqs, 0);
     const ArrayList a = list_arrays(host, n_arrays);
     plan_compact_kernel<<<1, kPlanThreads, 0, s>>>(t, w, n_live);
-    apply_kernel<kCompact><<<kMoveCtas, kMoveThreads, 0, s>>>(t, nullptr, w, a);
+    launch_behind(apply_kernel<kCompact>, kMoveCtas, kMoveThreads, s, t, (const int2 *)nullptr, w, a);
 }
 
 }  // namespace ds4b200
