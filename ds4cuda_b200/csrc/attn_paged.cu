@@ -137,6 +137,7 @@ struct Segment {
 };
 constexpr int kSegRing = 8;
 constexpr int kAhead = 3;                   // tiles
+constexpr int kHole = -2, kPast = -2;       // a row without a page; no look-up
 constexpr int kSegReaders = kLoadWarps + kSoftWarps + 2;
 
 struct TcArgs {
@@ -191,6 +192,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     __shared__ __align__(16) int row_at[2][kRows];
     __shared__ float q_mul[kScaleSets][kRows];
     __shared__ __align__(16) float fac_s[2][kRows], inv_s[kRows];
+    __shared__ int odd_s[2];                        // 1 + the last tile with a row that is not a plain f16 row
     __shared__ int grown_s[2];                      // 1 + the last tile with a row that has grown
     __shared__ __align__(8) uint64_t scaled[2];
     volatile int *abort_flag = &abort_s;
@@ -203,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         start_slot = g.n_slots;
         start_tile = 0;
         for (int i = 0; i < 2; ++i) {
-            grown_s[i] = 0;
+            grown_s[i] = odd_s[i] = 0;
             mbar_init(&scaled[i], kSoftWarps);
             mbar_init(&s_full[i], 1); mbar_init(&s_free[i], kSoftWarps); mbar_init(&p_full[i], kSoftWarps);
             for (int k = 0; k < kParts; ++k) { mbar_init(&full[i][k], kLoadWarps); mbar_init(&pv_done[i][k], 1); }
@@ -280,12 +282,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         float sc0 = 0.0f, sc1 = 0.0f;
         // Tiles are found kAhead ahead of the one being stored: a page-table entry, and the first touch of a page, take a
         // few thousand cycles, so their lines are prefetched into L2 before the loads of the registers come.
-        struct Tile { int slot, at, rows; };             // slot of row r or -1; query rows of the segment in its first tile, else 0; -1 at the end
+        struct Tile { int slot, at, rows; };             // slot of row r, -1 past the rows, kHole without a page; query rows of the segment in its first tile, else 0; -1 at the end
         Segment sg;
         bool more = next_segment(sg, false), first = more;
         int t = more ? sg.t0 : 0;
         Tile found{-1, 0, -1};
-        int page = -1, in_page = 0;
+        int page = kPast, in_page = 0;
         auto find = [&]() {                              // the walk's tile: its page-table entry is on the way behind this
             const int i = t * kRows + r;
             found.at = i < sg.it.first ? i : sg.it.lo + (i - sg.it.first);
@@ -294,11 +296,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 #pragma unroll
                 for (int u = 0; u < NB; ++u) prefetch_l2(a.q + (sg.it.row0 + r) * D + (u * 4 + part) * 32);
             }
-            page = -1;
+            page = kPast;
             if (more && i < sg.it.n) {
                 const int pg = g.page_shift >= 0 ? found.at >> g.page_shift : found.at / a.kv.page_rows;
                 in_page = found.at - pg * a.kv.page_rows;
-                page = __ldg(a.page_table + sg.it.b * a.table_width + pg);
+                page = max(__ldg(a.page_table + sg.it.b * a.table_width + pg), -1);
             }
             if (more) {
                 first = false;
@@ -310,7 +312,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             }
         };
         auto take = [&]() -> Tile {                      // what find() looked up
-            found.slot = page >= 0 && page < a.kv.n_pages ? page * a.kv.page_rows + in_page : -1;      // n_pages * page_rows < 2^31
+            found.slot = page >= 0 && page < a.kv.n_pages ? page * a.kv.page_rows + in_page : page == kPast ? -1 : kHole;      // n_pages * page_rows < 2^31
             if (found.slot >= 0) {
                 const int64_t sl = found.slot;
                 if (kF32) {
@@ -440,18 +442,28 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[buf][k]);
             };
+            // Rows whose largest value lies in [2^-9, 2^14] become f16 as they are (E4M3 codes times a power of two stay exact);
+            // others keep a factor, and a tile that has one of those, or a hole, is marked for the softmax.
             float mul = 1.0f, down = 1.0f;
-            if (FMT == DS4B200_KV_FP8_ROW) mul = sc0;
+            bool plain = my >= 0;
+            if (FMT == DS4B200_KV_FP8_ROW) {
+                if (sc0 < 0x1p-18f || sc0 > 0x1p5f) { mul = sc0; sc0 = 1.0f; plain = false; }
+            }
             if (kBlock) {
                 float top = fmaxf(sc0, sc1);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) top = fmaxf(top, amax4(tl[kBlock ? j : 0]) * (1.0f / 256.0f));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                pow2_parts(top, mul, down);
-                sc0 *= down;
-                sc1 *= down;
+                if (top < 0x1p-17f || top > 0x1p5f) {
+                    pow2_parts(top, mul, down);
+                    sc0 *= down;
+                    sc1 *= down;
+                    plain = false;
+                }
             }
+            if (!__all_sync(0xffffffffu, plain || my < 0) && lane == 0) odd_s[buf] = n + 1;
+            if (my == kHole) odd_s[buf] = n + 1;
             int here[4], next[4];                        // slots of this lane's rows, this tile's and the next one's
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -483,8 +495,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                             const uint32_t y[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                             for (int k = 0; k < 4; ++k) e4m3x4(y[k], o[2 * k], o[2 * k + 1]);
-                            if (kBlock) {
-                                const __half2 f = __float2half2_rn(__shfl_sync(0xffffffffu, step == 0 ? sc0 : sc1, (2 * j + half) * 4 + (l16 >> 2)));
+                            if (!kF32) {
+                                const __half2 f = __float2half2_rn(kBlock ? __shfl_sync(0xffffffffu, step == 0 ? sc0 : sc1, (2 * j + half) * 4 + (l16 >> 2))
+                                                                          : __shfl_sync(0xffffffffu, sc0, (2 * j + half) * 4));
 #pragma unroll
                                 for (int k = 0; k < 8; ++k) o[k] = h2_bits(__hmul2(*reinterpret_cast<__half2 *>(&o[k]), f));
                             }
@@ -515,7 +528,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             load_tail(slot);
             if (part == 0) {
                 mul = mul == 0.0f ? 1.0e-30f : mul;
-                if (!kF32) { row_fma[buf][2 * (r & ~1) + (r & 1)] = mul; row_div[buf][r] = __fdividef(1.0f, mul); }
+                row_fma[buf][2 * (r & ~1) + (r & 1)] = mul;
+                row_div[buf][r] = __fdividef(1.0f, mul);
                 row_fma[buf][2 * (r & ~1) + 2 + (r & 1)] = my >= 0 ? (kF32 ? 0.0f : __log2f(mul)) : -INFINITY;
                 row_at[buf][r] = tile[0].at;
             }
@@ -678,11 +692,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 if (lane == 0) mbar_arrive(&s_free[buf]);
                 float2 v[8];
                 const float2 k2 = make_float2(qk, qk);
+                const bool odd = *(volatile int *)&odd_s[buf] == n + 1;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float4 f = *reinterpret_cast<const float4 *>(&row_fma[buf][2 * (8 * i + 2 * (lane & 3))]);
-                    const float2 s = make_float2(__uint_as_float(group ? x[4 * i + 2] : x[4 * i]), __uint_as_float(group ? x[4 * i + 3] : x[4 * i + 1]));
-                    v[i] = FMT == DS4B200_KV_F32 ? fma2(s, k2, make_float2(f.z, f.w)) : fma2(mul2(s, k2), make_float2(f.x, f.y), make_float2(f.z, f.w));
+                for (int i = 0; i < 8; ++i)
+                    v[i] = mul2(make_float2(__uint_as_float(group ? x[4 * i + 2] : x[4 * i]), __uint_as_float(group ? x[4 * i + 3] : x[4 * i + 1])), k2);
+                if (odd) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float4 f = *reinterpret_cast<const float4 *>(&row_fma[buf][2 * (8 * i + 2 * (lane & 3))]);
+                        v[i] = fma2(v[i], make_float2(f.x, f.y), make_float2(f.z, f.w));
+                    }
                 }
                 if ((t + 1) * kRows > it.n) {            // columns past the rows: S was not computed there
                     const int end = it.n - t * kRows - 2 * (lane & 3);
@@ -724,13 +743,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 unsigned char *dst = p_s + buf * 8192 + row * 128 + (lane & 3) * 4;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    float2 e = add2(v[i], ref2);
-                    e.x = tc::exp2_approx(e.x);
-                    e.y = tc::exp2_approx(e.y);
-                    if (FMT == DS4B200_KV_F32) l = add2(l, e);
-                    else l = fma2(e, *reinterpret_cast<const float2 *>(&row_div[buf][8 * i + 2 * (lane & 3)]), l);
-                    *reinterpret_cast<uint32_t *>(dst + (((uint32_t)i ^ (uint32_t)(row & 7)) << 4)) = h2_bits(__floats2half2_rn(e.x, e.y));
+                    v[i] = add2(v[i], ref2);
+                    v[i].x = tc::exp2_approx(v[i].x);
+                    v[i].y = tc::exp2_approx(v[i].y);
+                    *reinterpret_cast<uint32_t *>(dst + (((uint32_t)i ^ (uint32_t)(row & 7)) << 4)) = h2_bits(__floats2half2_rn(v[i].x, v[i].y));
                 }
+                if (odd) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = mul2(v[i], *reinterpret_cast<const float2 *>(&row_div[buf][8 * i + 2 * (lane & 3)]));
+                }
+                l = add2(l, add2(add2(add2(v[0], v[1]), add2(v[2], v[3])), add2(add2(v[4], v[5]), add2(v[6], v[7]))));
                 tc::fence_async();
                 tc::fence_before();
                 __syncwarp();

@@ -473,8 +473,10 @@ typedef struct ds4b200_paged_kv {
  * sink (f32 [n_heads], nullable) is the reference's per-head logit without a row (cuda/flash_attn.cu:148).
  * lse is nullable.  A token that sees no row gets out = 0 and lse = sink[h] or -inf.  kv_len is clamped to
  * [0, table_width * page_rows].
- * The products run in f16 with f32 accumulation: q exactly (each row scaled by a power of two), E4M3 rows
- * exactly, f32 rows and tails rounded to f16 relative to their largest value, softmax weights rounded to f16.
+ * The products run in f16 with f32 accumulation: q exactly (scaled by a power of two where its range asks for it), cache rows
+ * as f16 numbers, as the reference's attention reads its cache (cuda/flash_attn.cu:113-115): exact for
+ * FP8_BLOCK64 codes and for the f16-rounded rows of ds4b200_kv_rows_to_raw_f32, else rounded (FP8 rows outside
+ * [2^-9, 2^14] keep a factor beside them; F32 values beyond +-65504 become that); softmax weights rounded to f16.
  * workspace: ds4b200_attn_workspace_bytes(n_heads, head_dim) bytes of device memory, 16-byte aligned, not shared by calls that may
  * overlap.  n_heads <= 1024.  Results do not depend on the contents of the workspace, and a call repeats its bits; the
  * lengths of all sequences decide where a long one is split, so the last bits of a sequence's result depend on them. */

@@ -42,24 +42,26 @@ def visible(p, window, n_first):
 
 
 def row_factors(fmt, st, n_rot=N_ROT):
-    """r_j of every row, in 64 bits: the scale of a row; the largest power of two that is at most its largest block
-    scale, or its largest tail value / 256; 1 for f32 rows."""
+    """r_j of every row, in 64 bits: 1 for f32 rows and for rows of ordinary size, which are held as f16 numbers; else the
+    scale of a row, or the largest power of two that is at most its largest block scale, or its largest tail value / 256."""
     if fmt == "f32":
         return torch.ones(st["raw"].shape[0], dtype=torch.float64, device=st["raw"].device)
     if fmt == "row":
-        return st["scales"][:, 0].double()
+        r = st["scales"][:, 0].double()
+        return torch.where((r < 2.0 ** -18) | (r > 2.0 ** 5), r, 1.0)
     top = st["scales"].amax(1)
     if n_rot:
         top = torch.maximum(top, st["tail"].abs().amax(1) / 256)
-    return torch.exp2(torch.floor(torch.log2(top.double())))
+    r = torch.exp2(torch.floor(torch.log2(top.double())))
+    return torch.where((top < 2.0 ** -17) | (top > 2.0 ** 5), r, 1.0)
 
 
-def attention(q, rows, slots_of, positions, window, n_first, scale, sink, tail=0, factors=None):
+def attention(q, rows, slots_of, positions, window, n_first, scale, sink, tail=0, factors=None):     # tail: how many of a row's last values are rounded to f16
     """q [T, H, D] (any type), rows [slots, D] f64, slots_of[t][j] the slot of row j of token t's sequence (None: hidden),
     positions[t].  Returns out, lse and the bounds of their errors (see the comments), all f64.
 
     The bounds count the roundings of an implementation that multiplies in f16 and adds in f32: weights to f16 (half a
-    step: 2^-11 of each), the f32 tail to f16 (2^-11 of each value, in the row as value and, through the score, as
+    step: 2^-11 of each), the f32 tail, or a whole row of codes times a scale that is no power of two, to f16 (2^-11 of each value, in the row as value and, through the score, as
     key: a score off by d moves its weight by e^d - 1 <= 2 d and the normaliser by as much), f32 sums that may
     truncate (n additions are off by at most n 2^-23 of the sum of magnitudes: D for a score, the visible rows for an
     output; exp2 and the exponent's own rounding are below 2^-19 (|score| < 64)), and the output to bf16 (2^-8 of the value).

@@ -21,7 +21,7 @@ class Case:
 
     def __init__(self, ops, fmt, heads, dim, page, lens, toks=None, n_rot=64, seed=0, row_scale=None, q_scale=1.0, width=None):
         g = torch.Generator(device="cuda").manual_seed(seed)
-        self.fmt, self.tail = fmt, n_rot if fmt == "block" else 0
+        self.fmt, self.tail = fmt, {"f32": 0, "row": dim, "block": n_rot}[fmt]
         need = [-(-n // page) for n in lens]
         n_pages = sum(need) + 2
         x = torch.randn((n_pages * page, dim), generator=g, device="cuda")
@@ -49,7 +49,7 @@ class Case:
         else:
             self.st["codes"][lost] = 0x7f
             self.st["scales"][lost] = float("nan")
-            if self.tail:
+            if fmt == "block" and n_rot:
                 self.st["tail"][lost] = float("inf")
         self.kv = ops.PagedKv(kind(ops, fmt), page, n_rot, **self.st)
         self.table, self.kv_len = table.cuda(), torch.tensor(lens, dtype=torch.int32, device="cuda")
