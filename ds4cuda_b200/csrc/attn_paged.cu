@@ -42,7 +42,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kCtas = 148;
 constexpr int kRows = 64;                   // query rows of an item, cache rows of a tile
 constexpr int kSoftWarps = 8, kLoadWarp0 = 8, kLoadWarps = 8, kMmaWarp = 16;
-constexpr int kThreads = 20 * 32;            // the last warp only makes a register group whole
+constexpr int kThreads = 20 * 32;            
 constexpr int kSplitItems = 4 * kCtas;
 constexpr int kWholeTiles = 3;              // items of up to so many tiles are not cut
 constexpr int kMinTiles = 2;                // of a run: below, the join costs more than the run saves
@@ -136,9 +136,9 @@ struct Segment {
     int t0, t1;
 };
 constexpr int kSegRing = 8;
-constexpr int kAhead = 3;                   // tiles
-constexpr int kHole = -2, kPast = -2;       // a row without a page; no look-up
-constexpr int kSegReaders = kLoadWarps + kSoftWarps + 2;
+constexpr int kTileRing = 8;                // tiles the finding warp may be ahead of the loaders
+constexpr int kHole = -2;                   // a row without a page
+constexpr int kSegReaders = kSoftWarps + 3;
 
 struct TcArgs {
     AttnArgs a;
@@ -189,7 +189,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     __shared__ int abort_s, start_slot, start_tile;
     __shared__ long long scan_s[kThreads / 32];
     __shared__ __align__(16) float row_fma[2][2 * kRows], row_div[2][kRows];      // by pairs of rows: factor, factor, addend, addend
-    __shared__ __align__(16) int row_at[2][kRows];
+    __shared__ __align__(16) int row_at[2 * kTileRing][kRows];       // a row's place in its sequence
+    __shared__ __align__(16) int slot_s[kTileRing][kRows];          // a tile's rows in the pool (-1 past the rows, or kHole), see find_index()
+    __shared__ int tile_rows[kTileRing];                            // query rows where a tile is its segment's first, else 0; -1 ends
+    __shared__ int64_t tile_row0[kTileRing];                        // and the first of them
+    __shared__ __align__(8) uint64_t tile_full[kTileRing], tile_free[kTileRing];
     __shared__ float q_mul[kScaleSets][kRows];
     __shared__ __align__(16) float fac_s[2][kRows], inv_s[kRows];
     __shared__ int odd_s[2];                        // 1 + the last tile with a row that is not a plain f16 row
@@ -211,6 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             for (int k = 0; k < kParts; ++k) { mbar_init(&full[i][k], kLoadWarps); mbar_init(&pv_done[i][k], 1); }
         }
         mbar_init(&q_full, kLoadWarps); mbar_init(&q_free, 1);
+        for (int i = 0; i < kTileRing; ++i) { mbar_init(&tile_full[i], 1); mbar_init(&tile_free[i], kLoadWarps); }
         for (int i = 0; i < kSegRing; ++i) { mbar_init(&seg_full[i], 1); mbar_init(&seg_free[i], kSegReaders); }
     }
     if (warp == kMmaWarp) {
@@ -249,12 +254,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 
     // A role takes the segments in order from the ring; every warp of it calls this.
     int seg = 0;
-    auto next_segment = [&](Segment &sg, bool done = true) -> bool {
+    auto next_segment = [&](Segment &sg) -> bool {
         const int i = seg & (kSegRing - 1);
         tc::wait(&seg_full[i], (uint32_t)((seg / kSegRing) & 1), abort_flag, status);
         sg = seg_s[i];
         __syncwarp();
-        if (done && lane == 0) mbar_arrive(&seg_free[i]);
+        if (lane == 0) mbar_arrive(&seg_free[i]);
         ++seg;
         return sg.t1 >= 0 && !*abort_flag;
     };
@@ -262,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     if (warp >= kLoadWarp0 && warp < kLoadWarp0 + kLoadWarps) {
         // ------------------------------------------------------------------------------ loaders
         // A warp has eight rows of the tile.  Its loads cover two rows at a time, 256 contiguous bytes of each (16 lanes): whole lines,
-        // and stores of rows r and r + 1 with their 16-byte units XORed by the row fall on all banks.  Scales, tails and the
+        // and stores of rows r and r + 1 with their 16-byte units XORed by the row fall on all banks.  Tails and the
         // query rows go by four lanes per row.  A register is loaded again, with the next unit's bytes, as soon as
         // its value is converted, so loads run a tile ahead of the stores.  A unit is a tile, or 128 dims of one in f32.
         tc::set_max_registers_up<136>();
@@ -270,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         constexpr int kUnitChunks = !kF32 ? kChunks : 2, kUnits = kChunks / kUnitChunks;
         constexpr int kSpan = kF32 ? 1 : 4;              // chunks a load of two rows covers (fewer with fewer dims)
         constexpr int kSteps = (kUnitChunks + kSpan - 1) / kSpan, kRegs = kSteps * 4;
-        const int r = (warp - kLoadWarp0) * 8 + (lane >> 2), part = lane & 3;
+        const int lw = warp - kLoadWarp0, r = lw * 8 + (lane >> 2), part = lane & 3;
         const uint32_t row_off = (uint32_t)(r * 128), sw = (uint32_t)(r & 7);
         // of a load of two rows: which one, and the lane's 16 bytes of its 256; eight consecutive lanes (16 with the 8-byte stores
         // of f32 rows) have to fall on all banks
@@ -278,124 +283,55 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         const bool tail = kBlock && a.kv.n_rot != 0;
         const int n_scales = kBlock ? (D - a.kv.n_rot) / 64 : 1;
         uint4 v[kRegs];                                  // [step][row pair]
+        float sc[kF32 ? 1 : kRegs];                      // the scale of each
         float4 tl[kBlock ? 4 : 1];
-        float sc0 = 0.0f, sc1 = 0.0f;
-        // Tiles are found kAhead ahead of the one being stored: a page-table entry, and the first touch of a page, take a
-        // few thousand cycles, so their lines are prefetched into L2 before the loads of the registers come.
-        struct Tile { int slot, at, rows; };             // slot of row r, -1 past the rows, kHole without a page; query rows of the segment in its first tile, else 0; -1 at the end
-        Segment sg;
-        bool more = next_segment(sg, false), first = more;
-        int t = more ? sg.t0 : 0;
-        Tile found{-1, 0, -1};
-        int page = kPast, in_page = 0;
-        auto find = [&]() {                              // the walk's tile: its page-table entry is on the way behind this
-            const int i = t * kRows + r;
-            found.at = i < sg.it.first ? i : sg.it.lo + (i - sg.it.first);
-            found.rows = !more ? -1 : first ? sg.it.rows : 0;
-            if (found.rows > r) {                        // its query rows are wanted when the tile is stored
-#pragma unroll
-                for (int u = 0; u < NB; ++u) prefetch_l2(a.q + (sg.it.row0 + r) * D + (u * 4 + part) * 32);
-            }
-            page = kPast;
-            if (more && i < sg.it.n) {
-                const int pg = g.page_shift >= 0 ? found.at >> g.page_shift : found.at / a.kv.page_rows;
-                in_page = found.at - pg * a.kv.page_rows;
-                page = max(__ldg(a.page_table + sg.it.b * a.table_width + pg), -1);
-            }
-            if (more) {
-                first = false;
-                if (++t == sg.t1) {
-                    more = next_segment(sg, false);      // given back with its query rows
-                    first = more;
-                    t = sg.t0;
-                }
-            }
+        struct Slots { int pair[4], own; };              // of rows 2 j + half, and of row r
+        auto slots_of = [&](int n) -> Slots {
+            const int i = n & (kTileRing - 1);
+            tc::wait(&tile_full[i], (uint32_t)((n / kTileRing) & 1), abort_flag, status);
+            const int4 p = *reinterpret_cast<const int4 *>(&slot_s[i][lw * 8 + half * 4]);
+            return Slots{{p.x, p.y, p.z, p.w}, kBlock && tail ? slot_s[i][lw * 8 + ((lane >> 2) & 1) * 4 + (lane >> 3)] : 0};
         };
-        auto take = [&]() -> Tile {                      // what find() looked up
-            found.slot = page >= 0 && page < a.kv.n_pages ? page * a.kv.page_rows + in_page : page == kPast ? -1 : kHole;      // n_pages * page_rows < 2^31
-            if (found.slot >= 0) {
-                const int64_t sl = found.slot;
-                if (kF32) {
-#pragma unroll
-                    for (int u = 0; u < NB; ++u) prefetch_l2(a.kv.raw + sl * D + (u * 4 + part) * 32);
-                } else {
-                    if (part < NB) prefetch_l2(a.kv.codes + sl * D + part * 128);
-                    if (kBlock && part < 2 && tail) prefetch_l2(a.kv.tail + sl * 64 + part * 32);
-                    if (part == 3) prefetch_l2(a.kv.scales + sl * n_scales);
-                }
-            }
-            return found;
-        };
-        auto pair_slot = [&](int of, int j) { return __shfl_sync(0xffffffffu, of, (2 * j + half) * 4); };
-        auto load = [&](int my, bool all, int unit, int step, int j) {      // my: the slot of row 2 j + half; all: of the warp's rows exist
-            uint4 &x = v[step * 4 + j];
+        auto load = [&](int my, bool all, int unit, int step, int j) {      // all: of the warp's rows exist
+            const int k = step * 4 + j;
             if (!all) {
-                x = make_uint4(0, 0, 0, 0);
+                v[k] = make_uint4(0, 0, 0, 0);
+                if (!kF32) sc[kF32 ? 0 : k] = 1.0f;
                 if (my < 0) return;
             }
             if (kF32) {
-                x = ld_row16(a.kv.raw + (int64_t)my * D + (unit * kUnitChunks + step) * 64 + l16 * 4);
+                v[k] = ld_row16(a.kv.raw + (int64_t)my * D + (unit * kUnitChunks + step) * 64 + l16 * 4);
             } else {
                 const int c = step * 4 + (l16 >> 2);                // chunk of this lane
                 // lanes past the codes load the row's first ones, which nobody stores
                 const bool in = c < kChunks && !(tail && c == kChunks - 1);
-                x = ld_row16(a.kv.codes + (int64_t)my * D + (in ? step * 256 + l16 * 16 : 0));
+                v[k] = ld_row16(a.kv.codes + (int64_t)my * D + (in ? step * 256 + l16 * 16 : 0));
+                sc[kF32 ? 0 : k] = __ldg(a.kv.scales + (kBlock ? (int64_t)my * n_scales + (in ? c : 0) : (int64_t)my));
             }
         };
-        auto load_scales = [&](int64_t my) {
-            if (FMT == DS4B200_KV_FP8_ROW) sc0 = my >= 0 ? __ldg(a.kv.scales + my) : 1.0f;
-            if (kBlock) {
-                sc0 = my >= 0 && part < n_scales ? __ldg(a.kv.scales + my * n_scales + part) : 0.0f;
-                sc1 = my >= 0 && part + 4 < n_scales ? __ldg(a.kv.scales + my * n_scales + part + 4) : 0.0f;
-            }
-        };
-        auto load_tail = [&](int64_t my) {
+        auto load_tail = [&](int my) {
             if (kBlock)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const uint4 x = my >= 0 && tail ? ld_row16(a.kv.tail + my * 64 + part * 16 + j * 4) : make_uint4(0, 0, 0, 0);
+                    const uint4 x = my >= 0 && tail ? ld_row16(a.kv.tail + (int64_t)my * 64 + part * 16 + j * 4) : make_uint4(0, 0, 0, 0);
                     tl[kBlock ? j : 0] = make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w));
                 }
         };
-        Tile tile[kAhead + 1];                           // [0] is being stored, [1] loaded
-        {
-            int pages[kAhead + 1], ins[kAhead + 1];
+        Slots here = slots_of(0);
+        int rows = tile_rows[0];
+        if (rows >= 0) {
 #pragma unroll
-            for (int k = 0; k <= kAhead; ++k) {          // the look-ups of the first tiles travel together
-                find();
-                tile[k] = found;
-                pages[k] = page;
-                ins[k] = in_page;
-            }
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int k = 0; k <= kAhead; ++k) {
-                found = tile[k];
-                page = pages[k];
-                in_page = ins[k];
-                tile[k] = take();
-            }
+                for (int step = 0; step < kSteps; ++step) load(here.pair[j], false, 0, step, j);
+            load_tail(here.own);
         }
-        int my = tile[0].slot;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int ps = pair_slot(my, j);
-#pragma unroll
-            for (int step = 0; step < kSteps; ++step) load(ps, false, 0, step, j);
-        }
-        load_scales(my);
-        load_tail(my);
-        for (int n = 0, nq = 0; tile[0].rows >= 0; ++n) {
-            const int buf = n & 1;
+        for (int n = 0, nq = 0; rows >= 0 && !*abort_flag; ++n) {
+            const int buf = n & 1, ring = n & (kTileRing - 1);
             const uint32_t use = (uint32_t)(((n >> 1) & 1) ^ 1);
             unsigned char *dst = k_s + buf * kTileBytes;
-            find();
-            my = tile[0].slot;
-            const int slot = tile[1].slot;
-            if (tile[0].rows) {                          // a segment's query rows come ahead of its first tile
-                const int ring = nq & (kSegRing - 1);
-                const uint16_t *src = a.q + (seg_s[ring].it.row0 + r) * D + part * 16;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&seg_free[ring]);
+            if (rows) {                                  // a segment's query rows come ahead of its first tile
+                const uint16_t *src = a.q + (tile_row0[ring] + r) * D + part * 16;
                 // as they are where their largest value is within [2^-4, 2^15], else scaled by a power of two in a second pass
                 float up = 1.0f, down = 1.0f;
 #pragma unroll 1
@@ -408,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                         for (int c = 0; c < 4; ++c)
 #pragma unroll
                             for (int u = 0; u < 2; ++u)
-                                x[c][u] = r < tile[0].rows && c0 + c < kChunks ? ld_row16(src + (c0 + c) * 64 + u * 8) : make_uint4(0, 0, 0, 0);
+                                x[c][u] = r < rows && c0 + c < kChunks ? ld_row16(src + (c0 + c) * 64 + u * 8) : make_uint4(0, 0, 0, 0);
                         if (pass == 0 && c0 == 0) tc::wait(&q_free, (uint32_t)((nq & 1) ^ 1), abort_flag, status);
 #pragma unroll
                         for (int c = 0; c < 4; ++c)
@@ -437,41 +373,74 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 if (lane == 0) mbar_arrive(&q_full);
                 ++nq;
             }
+            const Slots next = slots_of(n + 1);          // the tile behind this one
+            const int next_rows = tile_rows[(n + 1) & (kTileRing - 1)];
+            const bool all_here = kUnits > 1 && __all_sync(0xffffffffu, (here.pair[0] | here.pair[1] | here.pair[2] | here.pair[3]) >= 0);
+            const bool all_next = __all_sync(0xffffffffu, (next.pair[0] | next.pair[1] | next.pair[2] | next.pair[3]) >= 0);
             // The MMA warp makes the stores visible to the async proxy: a proxy fence here would wait for the loads in flight.
             auto hand_over = [&](int k) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[buf][k]);
             };
-            // Rows whose largest value lies in [2^-9, 2^14] become f16 as they are (E4M3 codes times a power of two stay exact);
-            // others keep a factor, and a tile that has one of those, or a hole, is marked for the softmax.
-            float mul = 1.0f, down = 1.0f;
-            bool plain = my >= 0;
-            if (FMT == DS4B200_KV_FP8_ROW) {
-                if (sc0 < 0x1p-18f || sc0 > 0x1p5f) { mul = sc0; sc0 = 1.0f; plain = false; }
-            }
-            if (kBlock) {
-                float top = fmaxf(sc0, sc1);
+            // Rows of ordinary size become f16 as they are (E4M3 codes times a power of two stay exact).  Where one of the warp's rows has
+            // a scale outside [2^-17, 2^5] or a tail value beyond 2^14, its rows keep a factor, and the tile is marked for the softmax.
+            float down = 1.0f;
+            bool bad = false;
+            if (!kF32) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) top = fmaxf(top, amax4(tl[kBlock ? j : 0]) * (1.0f / 256.0f));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                if (top < 0x1p-17f || top > 0x1p5f) {
-                    pow2_parts(top, mul, down);
-                    sc0 *= down;
-                    sc1 *= down;
-                    plain = false;
+                for (int k = 0; k < kRegs; ++k) bad = bad || !(sc[kF32 ? 0 : k] >= 0x1p-17f && sc[kF32 ? 0 : k] <= 0x1p5f);
+                if (kBlock)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) bad = bad || !(amax4(tl[kBlock ? j : 0]) <= 0x1p14f);
+            }
+            const bool hole = here.pair[0] == kHole || here.pair[1] == kHole || here.pair[2] == kHole || here.pair[3] == kHole;
+            if (__any_sync(0xffffffffu, bad || hole)) {
+                if (lane == 0) odd_s[buf] = n + 1;
+                float mine = 1.0f;                       // the factor of row r
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float mul = 1.0f;
+                    if (!kF32) {
+                        float top = sc[kF32 ? 0 : j];
+                        if (kSteps > 1) top = fmaxf(top, sc[kF32 || kSteps < 2 ? 0 : 4 + j]);
+                        if (kBlock) {                    // over the row's lanes (which differ in bits 0, 1, 3, 4), and its tail
+#pragma unroll
+                            for (int o = 1; o < 32; o <<= 1)
+                                if (o != 4) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                            float t4 = 0.0f;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) t4 = fmaxf(t4, amax4(tl[kBlock ? i : 0]));
+                            t4 = fmaxf(t4, __shfl_xor_sync(0xffffffffu, t4, 1));
+                            t4 = fmaxf(t4, __shfl_xor_sync(0xffffffffu, t4, 2));
+                            top = fmaxf(top, __shfl_sync(0xffffffffu, t4, (2 * j + half) * 4) * (1.0f / 256.0f));
+                        }
+                        mul = top;
+                        float inv = 1.0f;
+                        if (kBlock) pow2_parts(top, mul, inv);
+                        if (mul == 0.0f) mul = 1.0e-30f;
+#pragma unroll
+                        for (int st = 0; st < kSteps; ++st) sc[kF32 ? 0 : st * 4 + j] = kBlock ? sc[kF32 ? 0 : st * 4 + j] * inv : 1.0f;
+                    }
+                    const float got = __shfl_sync(0xffffffffu, mul, kF32 ? (lane & 4) << 2 : lane & 4);   // of a lane whose half is row r's parity
+                    if ((lane >> 3) == j) mine = got;
+                    if (l16 == 0) {
+                        const int rw = lw * 8 + 2 * j + half;
+                        row_fma[buf][2 * (rw & ~1) + (rw & 1)] = mul;
+                        row_fma[buf][2 * (rw & ~1) + 2 + (rw & 1)] = here.pair[j] >= 0 ? __log2f(mul) : -INFINITY;
+                        row_div[buf][rw] = __fdividef(1.0f, mul);
+                    }
+                }
+                if (kBlock) down = 1.0f / mine;
+            } else if (l16 == 0) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int rw = lw * 8 + 2 * j + half;
+                    row_fma[buf][2 * (rw & ~1) + (rw & 1)] = 1.0f;
+                    row_fma[buf][2 * (rw & ~1) + 2 + (rw & 1)] = 0.0f;
+                    row_div[buf][rw] = 1.0f;
                 }
             }
-            if (!__all_sync(0xffffffffu, plain || my < 0) && lane == 0) odd_s[buf] = n + 1;
-            if (my == kHole) odd_s[buf] = n + 1;
-            int here[4], next[4];                        // slots of this lane's rows, this tile's and the next one's
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                here[j] = kUnits > 1 ? pair_slot(my, j) : 0;
-                next[j] = pair_slot(slot, j);
-            }
-            const bool all_here = kUnits > 1 && __all_sync(0xffffffffu, my >= 0), all_next = __all_sync(0xffffffffu, slot >= 0);
-            const int rw = (warp - kLoadWarp0) * 8 + half;
+            const int rw = lw * 8 + half;
 #pragma unroll
             for (int unit = 0; unit < kUnits; ++unit)
 #pragma unroll
@@ -484,23 +453,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     }
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        uint4 &x = v[step * 4 + j];
+                        const uint4 x = v[step * 4 + j];
                         const uint32_t r7 = (uint32_t)(2 * j + half);
                         if (kF32) {
                             *reinterpret_cast<uint2 *>(dst + c0 * 8192 + (rw + 2 * j) * 128 + ((((uint32_t)l16 >> 1) ^ r7) << 4) + (l16 & 1) * 8) =
                                 make_uint2(sat_h2(__uint_as_float(x.x), __uint_as_float(x.y)), sat_h2(__uint_as_float(x.z), __uint_as_float(x.w)));
                         } else {
                             const int c = c0 + (l16 >> 2);
+                            const __half2 f = __float2half2_rn(sc[kF32 ? 0 : step * 4 + j]);
                             uint32_t o[8];
                             const uint32_t y[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                             for (int k = 0; k < 4; ++k) e4m3x4(y[k], o[2 * k], o[2 * k + 1]);
-                            if (!kF32) {
-                                const __half2 f = __float2half2_rn(kBlock ? __shfl_sync(0xffffffffu, step == 0 ? sc0 : sc1, (2 * j + half) * 4 + (l16 >> 2))
-                                                                          : __shfl_sync(0xffffffffu, sc0, (2 * j + half) * 4));
 #pragma unroll
-                                for (int k = 0; k < 8; ++k) o[k] = h2_bits(__hmul2(*reinterpret_cast<__half2 *>(&o[k]), f));
-                            }
+                            for (int k = 0; k < 8; ++k) o[k] = h2_bits(__hmul2(*reinterpret_cast<__half2 *>(&o[k]), f));
                             if (c < kChunks && !(tail && c == kChunks - 1)) {
                                 unsigned char *to = dst + c * 8192 + (rw + 2 * j) * 128;
                                 const uint32_t u = (uint32_t)(l16 & 3) * 2;
@@ -508,8 +474,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                                 *reinterpret_cast<uint4 *>(to + (((u + 1) ^ r7) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
                             }
                         }
-                        if (unit + 1 < kUnits) load(here[j], all_here, unit + 1, step, j);
-                        else load(next[j], all_next, 0, step, j);
+                        if (unit + 1 < kUnits) load(here.pair[j], all_here, unit + 1, step, j);
+                        else if (next_rows >= 0) load(next.pair[j], all_next, 0, step, j);
                     }
                 }
             if (kBlock && tail) {
@@ -523,20 +489,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 unsigned char *to = dst + (kChunks - 1) * 8192 + row_off;
                 *reinterpret_cast<uint4 *>(to + (((uint32_t)(part * 2) ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
                 *reinterpret_cast<uint4 *>(to + (((uint32_t)(part * 2 + 1) ^ sw) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
-            }
-            load_scales(slot);
-            load_tail(slot);
-            if (part == 0) {
-                mul = mul == 0.0f ? 1.0e-30f : mul;
-                row_fma[buf][2 * (r & ~1) + (r & 1)] = mul;
-                row_div[buf][r] = __fdividef(1.0f, mul);
-                row_fma[buf][2 * (r & ~1) + 2 + (r & 1)] = my >= 0 ? (kF32 ? 0.0f : __log2f(mul)) : -INFINITY;
-                row_at[buf][r] = tile[0].at;
+                if (next_rows >= 0) load_tail(next.own);
             }
             hand_over(kParts - 1);
-#pragma unroll
-            for (int k = 0; k < kAhead; ++k) tile[k] = tile[k + 1];
-            tile[kAhead] = take();
+            if (lane == 0) mbar_arrive(&tile_free[ring]);
+            here = next;
+            rows = next_rows;
         }
     } else if (warp >= kMmaWarp) {
         tc::set_max_registers_down<56>();
@@ -632,6 +590,65 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 __syncwarp();
                 if (*abort_flag) break;
             }
+        } else {
+            // -------------------------------------------------------------------------- find
+            // The pool rows of the tiles to come, two per lane, up to kTileRing tiles ahead of the loaders: a page-table entry, and the first
+            // touch of a page, take a few thousand cycles, so the rows' lines are fetched into L2 ahead of the loads.
+            constexpr bool kF32 = FMT == DS4B200_KV_F32, kBlock = FMT == DS4B200_KV_FP8_BLOCK64;
+            const bool tail = kBlock && a.kv.n_rot != 0;
+            const int n_scales = kBlock ? (D - a.kv.n_rot) / 64 : 1;
+            Segment sg;
+            int n = 0;
+            for (bool more = true; more;) {
+                more = next_segment(sg);
+                const int t1 = more ? sg.t1 : sg.t0 + 1;                    // one more entry says that it ends
+                for (int t = sg.t0; t < t1; ++t, ++n) {
+                    const int i = n & (kTileRing - 1);
+                    tc::wait(&tile_free[i], (uint32_t)(((n / kTileRing) & 1) ^ 1), abort_flag, status);
+                    if (lane == 0) {
+                        tile_rows[i] = !more ? -1 : t == sg.t0 ? sg.it.rows : 0;
+                        tile_row0[i] = sg.it.row0;
+                    }
+                    int slot[2] = {-1, -1};
+                    if (more) {
+                        int page[2], in[2];
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int k = t * kRows + lane + 32 * h, at = k < sg.it.first ? k : sg.it.lo + (k - sg.it.first);
+                            const int pg = g.page_shift >= 0 ? at >> g.page_shift : at / a.kv.page_rows;
+                            in[h] = at - pg * a.kv.page_rows;
+                            page[h] = k < sg.it.n ? max(__ldg(a.page_table + sg.it.b * a.table_width + pg), -1) : -2;
+                            row_at[n & (2 * kTileRing - 1)][lane + 32 * h] = at;
+                        }
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+                            slot[h] = page[h] == -2 ? -1 : page[h] >= 0 && page[h] < a.kv.n_pages ? page[h] * a.kv.page_rows + in[h] : kHole;
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int r = lane + 32 * h;                        // loaders read the even or the odd rows of eight
+                        slot_s[i][(r & ~7) + (r & 1) * 4 + ((r & 7) >> 1)] = slot[h];
+                        if (slot[h] >= 0) {
+                            const int64_t sl = slot[h];
+                            if (kF32) {
+#pragma unroll
+                                for (int u = 0; u < NB * 4; ++u) prefetch_l2(a.kv.raw + sl * D + u * 32);
+                            } else {
+#pragma unroll
+                                for (int u = 0; u < NB; ++u) prefetch_l2(a.kv.codes + sl * D + u * 128);
+                                prefetch_l2(a.kv.scales + sl * n_scales);
+                                if (tail) { prefetch_l2(a.kv.tail + sl * 64); prefetch_l2(a.kv.tail + sl * 64 + 32); }
+                            }
+                        }
+                        if (more && t == sg.t0 && r < sg.it.rows)           // the segment's query rows
+#pragma unroll
+                            for (int u = 0; u < NB * 2; ++u) prefetch_l2(a.q + (sg.it.row0 + r) * D + u * 64);
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&tile_full[i]);
+                    if (*abort_flag) more = false;
+                }
+            }
         }
     } else {
         // ------------------------------------------------------------------------------ softmax and output
@@ -714,7 +731,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 if (several) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const int2 at = *reinterpret_cast<const int2 *>(&row_at[buf][8 * i + 2 * (lane & 3)]);
+                        const int2 at = *reinterpret_cast<const int2 *>(&row_at[n & (2 * kTileRing - 1)][8 * i + 2 * (lane & 3)]);
                         if (at.x > p || (at.x <= from && at.x >= a.n_first)) v[i].x = -INFINITY;
                         if (at.y > p || (at.y <= from && at.y >= a.n_first)) v[i].y = -INFINITY;
                     }
