@@ -174,6 +174,11 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return r;
 }
 
+struct Bars {
+    uint64_t full[2][2], s_full[2], s_free[2], p_full[2], pv_done[2][2], scaled[2], q_full, q_free;
+    uint64_t seg_full[kSegRing], seg_free[kSegRing], tile_full[kTileRing], tile_free[kTileRing];
+};
+
 template <int NB, int FMT>          // NB: head_dim / 128
 __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_constant__ TcArgs g) {
     constexpr int D = NB * 128, kChunks = NB * 2, kTileBytes = kRows * D * 2;
@@ -182,8 +187,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     const AttnArgs &a = g.a;
     extern __shared__ __align__(1024) unsigned char smem[];
     unsigned char *q_s = smem, *k_s = smem + kTileBytes, *p_s = smem + 3 * kTileBytes;
-    __shared__ __align__(8) uint64_t full[2][kParts], s_full[2], s_free[2], p_full[2], pv_done[2][kParts], q_full, q_free;
-    __shared__ __align__(8) uint64_t seg_full[kSegRing], seg_free[kSegRing];
+    __shared__ __align__(8) Bars bars_s;
     __shared__ Segment seg_s[kSegRing];
     __shared__ uint32_t tmem_s;
     __shared__ int abort_s, start_slot, start_tile;
@@ -193,13 +197,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     __shared__ __align__(16) int slot_s[kTileRing][kRows];          // a tile's rows in the pool (-1 past the rows, or kHole), see find_index()
     __shared__ int tile_rows[kTileRing];                            // query rows where a tile is its segment's first, else 0; -1 ends
     __shared__ int64_t tile_row0[kTileRing];                        // and the first of them
-    __shared__ __align__(8) uint64_t tile_full[kTileRing], tile_free[kTileRing];
     __shared__ float q_mul[kScaleSets][kRows];
     __shared__ __align__(16) float fac_s[2][kRows], inv_s[kRows];
     __shared__ int odd_s[2];                        // 1 + the last tile with a row that is not a plain f16 row
     __shared__ int grown_s[2];                      // 1 + the last tile with a row that has grown
-    __shared__ __align__(8) uint64_t scaled[2];
     volatile int *abort_flag = &abort_s;
+    const uint32_t bars = tc::held(smem_addr(&bars_s));
+#define DS4B200_BAR(name, i) (bars + (uint32_t)offsetof(Bars, name) + 8u * (uint32_t)(i))
     int *status = g.status;
     launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -210,13 +214,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         start_tile = 0;
         for (int i = 0; i < 2; ++i) {
             grown_s[i] = odd_s[i] = 0;
-            mbar_init(&scaled[i], kSoftWarps);
-            mbar_init(&s_full[i], 1); mbar_init(&s_free[i], kSoftWarps); mbar_init(&p_full[i], kSoftWarps);
-            for (int k = 0; k < kParts; ++k) { mbar_init(&full[i][k], kLoadWarps); mbar_init(&pv_done[i][k], 1); }
+            mbar_init(&bars_s.scaled[i], kSoftWarps);
+            mbar_init(&bars_s.s_full[i], 1); mbar_init(&bars_s.s_free[i], kSoftWarps); mbar_init(&bars_s.p_full[i], kSoftWarps);
+            for (int k = 0; k < kParts; ++k) { mbar_init(&bars_s.full[i][k], kLoadWarps); mbar_init(&bars_s.pv_done[i][k], 1); }
         }
-        mbar_init(&q_full, kLoadWarps); mbar_init(&q_free, 1);
-        for (int i = 0; i < kTileRing; ++i) { mbar_init(&tile_full[i], 1); mbar_init(&tile_free[i], kLoadWarps); }
-        for (int i = 0; i < kSegRing; ++i) { mbar_init(&seg_full[i], 1); mbar_init(&seg_free[i], kSegReaders); }
+        mbar_init(&bars_s.q_full, kLoadWarps); mbar_init(&bars_s.q_free, 1);
+        for (int i = 0; i < kTileRing; ++i) { mbar_init(&bars_s.tile_full[i], 1); mbar_init(&bars_s.tile_free[i], kLoadWarps); }
+        for (int i = 0; i < kSegRing; ++i) { mbar_init(&bars_s.seg_full[i], 1); mbar_init(&bars_s.seg_free[i], kSegReaders); }
     }
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_s)));
@@ -256,10 +260,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     int seg = 0;
     auto next_segment = [&](Segment &sg) -> bool {
         const int i = seg & (kSegRing - 1);
-        tc::wait(&seg_full[i], (uint32_t)((seg / kSegRing) & 1), abort_flag, status);
+        tc::wait(DS4B200_BAR(seg_full, i), (uint32_t)((seg / kSegRing) & 1), abort_flag, status);
         sg = seg_s[i];
         __syncwarp();
-        if (lane == 0) mbar_arrive(&seg_free[i]);
+        if (lane == 0) tc::arrive(DS4B200_BAR(seg_free, i));
         ++seg;
         return sg.t1 >= 0 && !*abort_flag;
     };
@@ -288,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         struct Slots { int pair[4], own; };              // of rows 2 j + half, and of row r
         auto slots_of = [&](int n) -> Slots {
             const int i = n & (kTileRing - 1);
-            tc::wait(&tile_full[i], (uint32_t)((n / kTileRing) & 1), abort_flag, status);
+            tc::wait(DS4B200_BAR(tile_full, i), (uint32_t)((n / kTileRing) & 1), abort_flag, status);
             const int4 p = *reinterpret_cast<const int4 *>(&slot_s[i][lw * 8 + half * 4]);
             return Slots{{p.x, p.y, p.z, p.w}, kBlock && tail ? slot_s[i][lw * 8 + ((lane >> 2) & 1) * 4 + (lane >> 3)] : 0};
         };
@@ -345,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 #pragma unroll
                             for (int u = 0; u < 2; ++u)
                                 x[c][u] = r < rows && c0 + c < kChunks ? ld_row16(src + (c0 + c) * 64 + u * 8) : make_uint4(0, 0, 0, 0);
-                        if (pass == 0 && c0 == 0) tc::wait(&q_free, (uint32_t)((nq & 1) ^ 1), abort_flag, status);
+                        if (pass == 0 && c0 == 0) tc::wait(DS4B200_BAR(q_free, 0), (uint32_t)((nq & 1) ^ 1), abort_flag, status);
 #pragma unroll
                         for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -370,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 }
                 if (part == 0) q_mul[nq & (kScaleSets - 1)][r] = up * a.scale * kLog2e;
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&q_full);
+                if (lane == 0) tc::arrive(DS4B200_BAR(q_full, 0));
                 ++nq;
             }
             const Slots next = slots_of(n + 1);          // the tile behind this one
@@ -380,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             // The MMA warp makes the stores visible to the async proxy: a proxy fence here would wait for the loads in flight.
             auto hand_over = [&](int k) {
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&full[buf][k]);
+                if (lane == 0) tc::arrive(DS4B200_BAR(full, (buf) * 2 + (k)));
             };
             // Rows of ordinary size become f16 as they are (E4M3 codes times a power of two stay exact).  Where one of the warp's rows has
             // a scale outside [2^-17, 2^5] or a tail value beyond 2^14, its rows keep a factor, and the tile is marked for the softmax.
@@ -446,10 +450,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 #pragma unroll
                 for (int step = 0; step < kSteps; ++step) {
                     const int c0 = unit * kUnitChunks + step * kSpan;       // first chunk of the step
-                    if (c0 == 0) tc::wait(&pv_done[buf][0], use, abort_flag, status);
+                    if (c0 == 0) tc::wait(DS4B200_BAR(pv_done, (buf) * 2 + (0)), use, abort_flag, status);
                     if (kParts > 1 && c0 == 2 * kPart0) {
                         hand_over(0);
-                        tc::wait(&pv_done[buf][kParts - 1], use, abort_flag, status);
+                        tc::wait(DS4B200_BAR(pv_done, (buf) * 2 + (kParts - 1)), use, abort_flag, status);
                     }
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -492,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 if (next_rows >= 0) load_tail(next.own);
             }
             hand_over(kParts - 1);
-            if (lane == 0) mbar_arrive(&tile_free[ring]);
+            if (lane == 0) tc::arrive(DS4B200_BAR(tile_free, ring));
             here = next;
             rows = next_rows;
         }
@@ -508,16 +512,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             for (int nq = 0; next_segment(sg); ++nq) {
                 const int t0 = __shfl_sync(0xffffffffu, sg.t0, 0), t1 = __shfl_sync(0xffffffffu, sg.t1, 0);
                 const int rows = __shfl_sync(0xffffffffu, sg.it.n, 0);
-                tc::wait(&q_full, (uint32_t)(nq & 1), abort_flag, status);
+                tc::wait<20>(DS4B200_BAR(q_full, 0), (uint32_t)(nq & 1), abort_flag, status);
                 for (int t = t0; t < t1; ++t, ++n) {
                     const int buf = n & 1;
                     const uint32_t phase = (uint32_t)((n >> 1) & 1), k0 = k_desc + (uint32_t)(buf * (kTileBytes >> 4));
                     const int groups = min(max((rows - t * kRows + 15) >> 4, 1), 4);      // of 16 cache rows
                     const uint32_t idesc = tc::idesc_f16(64, 0, false) | (uint32_t)groups << 18;
-                    tc::wait(&s_free[buf], phase ^ 1, abort_flag, status);
+                    tc::wait<20>(DS4B200_BAR(s_free, buf), phase ^ 1, abort_flag, status);
 #pragma unroll
                     for (int part = 0; part < kParts; ++part) {
-                        tc::wait(&full[buf][part], phase, abort_flag, status);
+                        tc::wait<20>(DS4B200_BAR(full, (buf) * 2 + (part)), phase, abort_flag, status);
                         tc::fence_async();               // for the loaders' stores, of the query rows too
                         tc::fence_after();
 #pragma unroll 1
@@ -527,9 +531,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                                 tc::mma_f16(one, s_tmem + buf * 64, q_desc + (uint32_t)(c * 512 + ks * 2), k0 + (uint32_t)(c * 512 + ks * 2), idesc,
                                             c > 0 || ks > 0);
                     }
-                    tc::commit(one, &s_full[buf]);
+                    tc::commit(one, DS4B200_BAR(s_full, buf));
                 }
-                tc::commit(one, &q_free);
+                tc::commit(one, DS4B200_BAR(q_free, 0));
             }
         } else if (warp == kMmaWarp + 1) {
             // -------------------------------------------------------------------------- O^T += V^T P^T
@@ -546,8 +550,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     const int buf = n & 1;
                     const uint32_t v0 = v_desc + (uint32_t)(buf * (kTileBytes >> 4)), p0 = p_desc + (uint32_t)(buf * 512);
                     const int groups = min(max((rows - t * kRows + 15) >> 4, 1), 4);
-                    tc::wait(&p_full[buf], (uint32_t)((n >> 1) & 1), abort_flag, status);
-                    if (*(volatile int *)&grown_s[buf] == n + 1) tc::wait(&scaled[buf], scaled_phase(buf), abort_flag, status);
+                    tc::wait<20>(DS4B200_BAR(p_full, buf), (uint32_t)((n >> 1) & 1), abort_flag, status);
+                    if (*(volatile int *)&grown_s[buf] == n + 1) tc::wait<20>(DS4B200_BAR(scaled, buf), scaled_phase(buf), abort_flag, status);
                     tc::fence_async();
                     tc::fence_after();
 #pragma unroll 1
@@ -556,9 +560,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                         for (int ks = 0; ks < 4; ++ks)
                             if (ks < groups)
                                 tc::mma_f16(one, o_tmem + m * 64, v0 + (uint32_t)(m * 1024 + ks * 128), p0 + (uint32_t)(ks * 2), idesc, t > t0 || ks > 0);
-                        if (kParts > 1 && m == kPart0 - 1) tc::commit(one, &pv_done[buf][0]);
+                        if (kParts > 1 && m == kPart0 - 1) tc::commit(one, DS4B200_BAR(pv_done, (buf) * 2 + (0)));
                     }
-                    tc::commit(one, &pv_done[buf][kParts - 1]);
+                    tc::commit(one, DS4B200_BAR(pv_done, (buf) * 2 + (kParts - 1)));
                 }
             }
         } else if (warp == kMmaWarp + 2) {
@@ -582,10 +586,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     break;
                 }
                 const int i = seg & (kSegRing - 1);
-                tc::wait(&seg_free[i], (uint32_t)(((seg / kSegRing) & 1) ^ 1), abort_flag, status);
+                tc::wait<300>(DS4B200_BAR(seg_free, i), (uint32_t)(((seg / kSegRing) & 1) ^ 1), abort_flag, status);
                 if (lane == 0) {
                     seg_s[i] = sg;
-                    mbar_arrive(&seg_full[i]);
+                    tc::arrive(DS4B200_BAR(seg_full, i));
                 }
                 __syncwarp();
                 if (*abort_flag) break;
@@ -604,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 const int t1 = more ? sg.t1 : sg.t0 + 1;                    // one more entry says that it ends
                 for (int t = sg.t0; t < t1; ++t, ++n) {
                     const int i = n & (kTileRing - 1);
-                    tc::wait(&tile_free[i], (uint32_t)(((n / kTileRing) & 1) ^ 1), abort_flag, status);
+                    tc::wait<300>(DS4B200_BAR(tile_free, i), (uint32_t)(((n / kTileRing) & 1) ^ 1), abort_flag, status);
                     if (lane == 0) {
                         tile_rows[i] = !more ? -1 : t == sg.t0 ? sg.it.rows : 0;
                         tile_row0[i] = sg.it.row0;
@@ -645,7 +649,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                             for (int u = 0; u < NB * 2; ++u) prefetch_l2(a.q + (sg.it.row0 + r) * D + u * 64);
                     }
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&tile_full[i]);
+                    if (lane == 0) tc::arrive(DS4B200_BAR(tile_full, i));
                     if (*abort_flag) more = false;
                 }
             }
@@ -660,6 +664,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
         const bool several = g.head_groups == 1 && g.group > 1;
         unsigned char *stage = p_s + group * 8192;      // of this group's output, where its weights' buffers are free
+        // One warp polls the barriers of the MMAs, the others wait for it here: the hardware's barrier costs them no issue slots.
+        auto sync_all = [&]() { asm volatile("bar.sync 3, 256;" ::: "memory"); };
         auto sync_group = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + group) : "memory"); };
         Meta last{0, 0, 0, 0, 0};
         Segment sg;
@@ -671,12 +677,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             float2 l = make_float2(0.0f, 0.0f);
             const int p = it.p0 + (several ? row / a.n_heads : 0);
             const int from = a.window > 0 ? p - a.window : -1;              // cache rows above it are in the window
-            // Scales the accumulators ahead of tile k's product where a row of that tile asked for it.
+            // Scales the accumulators ahead of tile k's product where a row of that tile asked for it; behind a sync_all().
             auto follow = [&](int k) {
                 const int buf = k & 1;
-                tc::wait(&p_full[buf], (uint32_t)((k >> 1) & 1), abort_flag, status);
                 if (*(volatile int *)&grown_s[buf] != k + 1) return;
-                tc::wait(&pv_done[buf ^ 1][kParts - 1], (uint32_t)(((k - 1) >> 1) & 1), abort_flag, status);
+                tc::wait(DS4B200_BAR(pv_done, (buf ^ 1) * 2 + (kParts - 1)), (uint32_t)(((k - 1) >> 1) & 1), abort_flag, status);
                 tc::fence_after();
 #pragma unroll 1
                 for (int u = group; u < NB * 4; u += 2) {
@@ -690,14 +695,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 tc::wait_st();
                 tc::fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&scaled[buf]);
+                if (lane == 0) tc::arrive(DS4B200_BAR(scaled, buf));
             };
             for (int t = sg.t0; t < sg.t1; ++t, ++n) {
                 const int buf = n & 1;
                 const uint32_t phase = (uint32_t)((n >> 1) & 1);
+                if (warp == 0) {
+                    tc::wait<20>(DS4B200_BAR(full, (buf) * 2 + (kParts - 1)), phase, abort_flag, status);
+                    tc::wait<20>(DS4B200_BAR(s_full, buf), phase, abort_flag, status);
+                }
+                sync_all();
                 if (t > sg.t0) follow(n - 1);
-                tc::wait(&full[buf][kParts - 1], phase, abort_flag, status);
-                tc::wait(&s_full[buf], phase, abort_flag, status);
                 tc::fence_after();
                 uint32_t x[32];
                 tc::ld_16x64(s_tmem + buf * 64 + lane_base, x);
@@ -706,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 tc::wait_ld();
                 tc::fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&s_free[buf]);
+                if (lane == 0) tc::arrive(DS4B200_BAR(s_free, buf));
                 float2 v[8];
                 const float2 k2 = make_float2(qk, qk);
                 const bool odd = *(volatile int *)&odd_s[buf] == n + 1;
@@ -773,8 +781,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 tc::fence_async();
                 tc::fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[buf]);
+                if (lane == 0) tc::arrive(DS4B200_BAR(p_full, buf));
             }
+            sync_all();
             follow(n - 1);
             float sum = l.x + l.y;
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
@@ -790,15 +799,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 }
                 inv = m == -INFINITY ? 0.0f : tc::exp2_approx(m - lse2);
             }
-            // the segment's accumulators; behind this wait every warp is through with the last segment's inv_s
-            tc::wait(&pv_done[(n - 1) & 1][kParts - 1], (uint32_t)(((n - 1) >> 1) & 1), abort_flag, status);
+            // the segment's accumulators
+            if (warp == 0) tc::wait<20>(DS4B200_BAR(pv_done, ((n - 1) & 1) * 2 + (kParts - 1)), (uint32_t)(((n - 1) >> 1) & 1), abort_flag, status);
             tc::fence_after();
             if ((lane & 3) == 0) {
                 if (!whole) g.part_ml[part * kRows + row] = make_float2(m, sum);
                 else if (a.lse && row < it.rows) a.lse[it.row0 + row] = lse2 * (1.0f / kLog2e);
                 inv_s[row] = inv;
             }
-            asm volatile("bar.sync 3, 256;" ::: "memory");
+            sync_all();
+            tc::fence_after();
             // In tensor memory a lane is a dim and a column a query row.
             if (whole) {
                 // 128 dims of 32 rows at a time through the weights' buffers, which are free here: stmatrix turns 8 x 8 blocks around, rows
@@ -841,7 +851,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     }
                     sync_group();
                 }
-                asm volatile("bar.sync 3, 256;" ::: "memory");             // the next weights go where either group's rows were
+                sync_all();                                                 // the next weights go where either group's rows were
             } else {
 #pragma unroll 1
                 for (int u = group; u < NB * 4; u += 2) {

@@ -39,11 +39,11 @@ __device__ __forceinline__ void mma_f16(uint32_t one, uint32_t d, uint32_t a, ui
                  "setp.ne.b32 q, %6, 0;\n\t@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}"
                  ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "n"(kDescHi), "r"(one) : "memory");
 }
-// One arrival on `bar` when every MMA the electing lane has issued so far has finished.
-__device__ __forceinline__ void commit(uint32_t one, uint64_t *bar) {
+// One arrival on the barrier when every MMA the electing lane has issued so far has finished.
+__device__ __forceinline__ void commit(uint32_t one, uint32_t bar) {
     asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
                  "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
-                 ::"r"(smem_addr(bar)), "r"(one) : "memory");
+                 ::"r"(bar), "r"(one) : "memory");
 }
 template <int N> __device__ __forceinline__ void set_max_registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void set_max_registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -82,20 +82,31 @@ __device__ __forceinline__ void st16(uint32_t addr, const uint32_t (&r)[16]) {
                  : "memory");
 }
 
-// A wait on an mbarrier phase.  It polls at most kWaitPolls times; the first that runs out raises the status bit and a
-// CTA-wide flag with which every later wait returns at once, so the kernel always ends (its results are invalid then).
-__device__ __forceinline__ bool try_phase(uint64_t *bar, uint32_t parity) {
+// Barriers go by their shared-memory address, held in a register: from a pointer the compiler works the address out again, three
+// instructions, at every poll.
+__device__ __forceinline__ uint32_t held(uint32_t x) {
+    asm volatile("mov.u32 %0, %0;" : "+r"(x));
+    return x;
+}
+__device__ __forceinline__ void arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ bool try_phase(uint32_t bar, uint32_t parity) {
     uint32_t done;
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-                 "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(smem_addr(bar)), "r"(parity) : "memory");
+                 "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     return done != 0;
 }
-__device__ __forceinline__ void wait(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int *status) {
+// A wait on an mbarrier phase.  It polls at most kWaitPolls times; the first that runs out raises the status bit and a
+// CTA-wide flag with which every later wait returns soon, so the kernel always ends (its results are invalid then).  A poll takes
+// issue slots and shared-memory bandwidth from the warps that work: with polls every 40 ns the waiting warps issued a third of
+// all instructions.
+template <int NS = 100>
+__device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status) {
     if (try_phase(bar, parity)) return;
 #pragma unroll 1
-    for (int i = 0; i < kWaitPolls; ++i) {
-        __nanosleep(40);                    // a poll takes shared-memory bandwidth from the operands of the MMAs
-        if (try_phase(bar, parity) || *abort_flag) return;
+    for (int i = 1; i <= kWaitPolls; ++i) {
+        __nanosleep(NS);
+        if (try_phase(bar, parity)) return;
+        if ((i & 63) == 0 && *abort_flag) return;
     }
     *abort_flag = 1;
     atomicOr(status, kStatusBulkCopyTimeout);
