@@ -154,7 +154,11 @@ __device__ __forceinline__ uint4 ld_row16(const void *p) {          // read once
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
 }
-__device__ __forceinline__ void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+// A row on its way to L2: one instruction of the copy engine, where a prefetch of every line takes the load pipe a cycle each.  p on 16
+// bytes, n a multiple of 16.
+__device__ __forceinline__ void prefetch_l2(const void *p, int n) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p), "r"(n) : "memory");
+}
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
     float2 r;
     asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}"
@@ -199,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     __shared__ int64_t tile_row0[kTileRing];                        // and the first of them
     __shared__ float q_mul[kScaleSets][kRows];
     __shared__ __align__(16) float fac_s[2][kRows], inv_s[kRows];
-    __shared__ int odd_s[2];                        // 1 + the last tile with a row that is not a plain f16 row
+    __shared__ int odd_s[2], odd_w[2][kLoadWarps];  // 1 + the last tile with a row that is not a plain f16 row: of any loader, of each
     __shared__ int grown_s[2];                      // 1 + the last tile with a row that has grown
     volatile int *abort_flag = &abort_s;
     const uint32_t bars = tc::held(smem_addr(&bars_s));
@@ -214,6 +218,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         start_tile = 0;
         for (int i = 0; i < 2; ++i) {
             grown_s[i] = odd_s[i] = 0;
+            for (int k = 0; k < kLoadWarps; ++k) odd_w[i][k] = 0;
             mbar_init(&bars_s.scaled[i], kSoftWarps);
             mbar_init(&bars_s.s_full[i], 1); mbar_init(&bars_s.s_free[i], kSoftWarps); mbar_init(&bars_s.p_full[i], kSoftWarps);
             for (int k = 0; k < kParts; ++k) { mbar_init(&bars_s.full[i][k], kLoadWarps); mbar_init(&bars_s.pv_done[i][k], 1); }
@@ -273,10 +278,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         // A warp has eight rows of the tile.  Its loads cover two rows at a time, 256 contiguous bytes of each (16 lanes): whole lines,
         // and stores of rows r and r + 1 with their 16-byte units XORed by the row fall on all banks.  Tails and the
         // query rows go by four lanes per row.  A register is loaded again, with the next unit's bytes, as soon as
-        // its value is converted, so loads run a tile ahead of the stores.  A unit is a tile, or 128 dims of one in f32.
+        // its value is converted, so loads run a tile ahead of the stores.  A unit is a tile, or 128 or 256 dims of one in f32.
         tc::set_max_registers_up<136>();
         constexpr bool kF32 = FMT == DS4B200_KV_F32, kBlock = FMT == DS4B200_KV_FP8_BLOCK64;
-        constexpr int kUnitChunks = !kF32 ? kChunks : 2, kUnits = kChunks / kUnitChunks;
+        constexpr int kUnitChunks = !kF32 ? kChunks : (NB % 2 ? 2 : 4), kUnits = kChunks / kUnitChunks;
         constexpr int kSpan = kF32 ? 1 : 4;              // chunks a load of two rows covers (fewer with fewer dims)
         constexpr int kSteps = (kUnitChunks + kSpan - 1) / kSpan, kRegs = kSteps * 4;
         const int lw = warp - kLoadWarp0, r = lw * 8 + (lane >> 2), part = lane & 3;
@@ -399,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             }
             const bool hole = here.pair[0] == kHole || here.pair[1] == kHole || here.pair[2] == kHole || here.pair[3] == kHole;
             if (__any_sync(0xffffffffu, bad || hole)) {
-                if (lane == 0) odd_s[buf] = n + 1;
+                if (lane == 0) odd_s[buf] = odd_w[buf][lw] = n + 1;
                 float mine = 1.0f;                       // the factor of row r
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -435,14 +440,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     }
                 }
                 if (kBlock) down = 1.0f / mine;
-            } else if (l16 == 0) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int rw = lw * 8 + 2 * j + half;
-                    row_fma[buf][2 * (rw & ~1) + (rw & 1)] = 1.0f;
-                    row_fma[buf][2 * (rw & ~1) + 2 + (rw & 1)] = 0.0f;
-                    row_div[buf][rw] = 1.0f;
-                }
             }
             const int rw = lw * 8 + half;
 #pragma unroll
@@ -600,7 +597,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             // touch of a page, take a few thousand cycles, so the rows' lines are fetched into L2 ahead of the loads.
             constexpr bool kF32 = FMT == DS4B200_KV_F32, kBlock = FMT == DS4B200_KV_FP8_BLOCK64;
             const bool tail = kBlock && a.kv.n_rot != 0;
-            const int n_scales = kBlock ? (D - a.kv.n_rot) / 64 : 1;
             Segment sg;
             int n = 0;
             for (bool more = true; more;) {
@@ -632,22 +628,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     for (int h = 0; h < 2; ++h) {
                         const int r = lane + 32 * h;                        // loaders read the even or the odd rows of eight
                         slot_s[i][(r & ~7) + (r & 1) * 4 + ((r & 7) >> 1)] = slot[h];
-                        if (slot[h] >= 0) {
+                        // one prefetch per run of neighbours in the pool: 64 of them a tile kept the copy engine busier than the loaders
+                        const int before = __shfl_up_sync(0xffffffffu, slot[h], 1);
+                        const uint32_t heads = __ballot_sync(0xffffffffu, lane == 0 || slot[h] < 0 || slot[h] != before + 1);
+                        if ((heads >> lane & 1) && slot[h] >= 0) {
+                            const uint32_t behind = lane == 31 ? 0 : heads >> (lane + 1);
+                            const int run = behind ? __ffs(behind) : 32 - lane;
                             const int64_t sl = slot[h];
                             if (kF32) {
-#pragma unroll
-                                for (int u = 0; u < NB * 4; ++u) prefetch_l2(a.kv.raw + sl * D + u * 32);
+                                prefetch_l2(a.kv.raw + sl * D, run * D * 4);
                             } else {
-#pragma unroll
-                                for (int u = 0; u < NB; ++u) prefetch_l2(a.kv.codes + sl * D + u * 128);
-                                prefetch_l2(a.kv.scales + sl * n_scales);
-                                if (tail) { prefetch_l2(a.kv.tail + sl * 64); prefetch_l2(a.kv.tail + sl * 64 + 32); }
+                                prefetch_l2(a.kv.codes + sl * D, run * D);
+                                if (tail) prefetch_l2(a.kv.tail + sl * 64, run * 256);
                             }
                         }
-                        if (more && t == sg.t0 && r < sg.it.rows)           // the segment's query rows
-#pragma unroll
-                            for (int u = 0; u < NB * 2; ++u) prefetch_l2(a.q + (sg.it.row0 + r) * D + u * 64);
                     }
+                    if (more && t == sg.t0 && lane == 0) prefetch_l2(a.q + sg.it.row0 * D, sg.it.rows * D * 2);    // the segment's query rows
                     __syncwarp();
                     if (lane == 0) tc::arrive(DS4B200_BAR(tile_full, i));
                     if (*abort_flag) more = false;
@@ -723,7 +719,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     v[i] = mul2(make_float2(__uint_as_float(group ? x[4 * i + 2] : x[4 * i]), __uint_as_float(group ? x[4 * i + 3] : x[4 * i + 1])), k2);
                 if (odd) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
+                    for (int i = 0; i < 8; ++i) {                          // column block i is loader i's
+                        if (odd_w[buf][i] != n + 1) continue;
                         const float4 f = *reinterpret_cast<const float4 *>(&row_fma[buf][2 * (8 * i + 2 * (lane & 3))]);
                         v[i] = fma2(v[i], make_float2(f.x, f.y), make_float2(f.z, f.w));
                     }
@@ -775,7 +772,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 }
                 if (odd) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = mul2(v[i], *reinterpret_cast<const float2 *>(&row_div[buf][8 * i + 2 * (lane & 3)]));
+                    for (int i = 0; i < 8; ++i)
+                        if (odd_w[buf][i] == n + 1) v[i] = mul2(v[i], *reinterpret_cast<const float2 *>(&row_div[buf][8 * i + 2 * (lane & 3)]));
                 }
                 l = add2(l, add2(add2(add2(v[0], v[1]), add2(v[2], v[3])), add2(add2(v[4], v[5]), add2(v[6], v[7]))));
                 tc::fence_async();
