@@ -4,6 +4,8 @@
 // Mathematics: o_h = sum_j exp(s_hj - lse_h) k_j with s_hj = scale q_h . k_j over the visible rows j and
 // lse_h = log(sum_j exp(s_hj) + exp(sink_h)).  One row is key and value of every head (the reference's
 // cache has one KV head; cuda/flash_attn.cu:148-313).
+#include <cuda.h>
+
 #include <algorithm>
 #include <mutex>
 #include <type_traits>
@@ -45,6 +47,7 @@ constexpr int kSoftWarps = 8, kLoadWarp0 = 8, kLoadWarps = 8, kMmaWarp = 16;
 constexpr int kThreads = 20 * 32;            
 constexpr int kSplitItems = 4 * kCtas;
 constexpr int kWholeTiles = 3;              // items of up to so many tiles are not cut
+constexpr int kPackTokens = 64;             // of a chunk whose rows are packed first
 constexpr int kMinTiles = 2;                // of a run: below, the join costs more than the run saves
 constexpr float kRescale = 8.0f;            // log2 units
 constexpr int kScaleSets = 4;
@@ -52,11 +55,43 @@ constexpr uint32_t kTmem = 0;               // all 512 columns are allocated, so
 
 struct Meta { int64_t row0; int rows, h0, parts, pad; };
 
+constexpr int kPacked = 3;                  // in place of a row format: the call's rows lie packed as f16, see attn_pack_kernel
+
+// Where the rows that sequence b's tokens see lie when packed: its first `first` rows, then rows lo .. len - 1, then 16 rows of zeros.
+struct Packed {
+    int len, lo, first;
+    int64_t off;
+};
+__host__ __device__ constexpr int64_t packed_gap(int window, int n_first, int64_t all_rows) {
+    return window > 0 ? (int64_t)window - 1 + n_first + 16 : all_rows + 16;
+}
+__device__ __forceinline__ Packed get_packed(const AttnArgs &a, int b) {
+    const int64_t most = a.table_width * a.kv.page_rows;
+    Packed k;
+    const int q0 = a.q_start[b], q1 = a.q_start[b + 1];
+    k.len = (int)min((int64_t)max(a.kv_len[b], 0), most);
+    const int p0 = k.len - (q1 - q0);
+    k.lo = a.window > 0 && p0 + 1 > a.window ? p0 + 1 - a.window : 0;
+    k.first = min(a.n_first, k.lo);
+    k.off = b * packed_gap(a.window, a.n_first, most) + (a.window > 0 ? q0 - a.q_start[0] : 0);
+    return k;
+}
+
+// The rows an item sees are a list of two runs, each in tiles of 64: `na` rows, then n - na.  Straight from the cache it is one run: the
+// `first` first rows of the sequence, then row lo on.  Packed, rows lo .. come first and the first rows are a run of their own,
+// so that every tile is one box of neighbouring rows.
 struct Item {
     int64_t row0;                           // first row of q / out, n_heads rows per token
-    int b, rows, h0, p0, first, lo, n, tiles;
+    int b, rows, h0, p0, first, lo, n, na, tiles;
+    int at_a, at_b;                         // packed rows where the runs begin
 };
+__device__ __forceinline__ int first_run_tiles(const Item &it) { return (it.na + 63) >> 6; }
+__device__ __forceinline__ int rows_in_tile(const Item &it, int t) {
+    const int ta = first_run_tiles(it);
+    return min(64, t < ta ? it.na - 64 * t : it.n - it.na - 64 * (t - ta));
+}
 
+template <bool PACKED>
 __device__ __forceinline__ Item get_item(const AttnArgs &a, int group, int head_groups, int slot) {
     Item it;
     const int g = slot / head_groups, hg = slot - g * head_groups;
@@ -86,7 +121,15 @@ __device__ __forceinline__ Item get_item(const AttnArgs &a, int group, int head_
     it.lo = a.window > 0 && it.p0 + 1 > a.window ? it.p0 + 1 - a.window : 0;
     it.first = min(a.n_first, it.lo);
     it.n = max(0, it.first + last + 1 - it.lo);
-    it.tiles = ntok <= 0 ? 0 : max(1, (it.n + kRows - 1) / kRows);
+    it.na = it.n;
+    it.at_a = it.at_b = 0;
+    if (PACKED) {
+        const Packed k = get_packed(a, it.b);
+        it.na = max(0, it.n - it.first);
+        it.at_a = (int)(k.off + k.first + it.lo - k.lo);
+        it.at_b = (int)k.off;
+    }
+    it.tiles = ntok <= 0 ? 0 : max(1, ((it.na + 63) >> 6) + ((it.n - it.na + 63) >> 6));
     it.row0 = (int64_t)tok0 * a.n_heads + hg * kRows;
     it.h0 = hg * kRows;
     it.rows = head_groups > 1 ? min(kRows, a.n_heads - hg * kRows) : ntok * a.n_heads;
@@ -138,9 +181,13 @@ struct Segment {
 constexpr int kSegRing = 8;
 constexpr int kTileRing = 8;                // tiles the finding warp may be ahead of the loaders
 constexpr int kHole = -2;                   // a row without a page
-constexpr int kSegReaders = kSoftWarps + 3;
+constexpr int kSegReaders = kSoftWarps + 3;  // and the loaders with packed rows
+constexpr int kPackCtas = 4 * kCtas, kPackWarps = 8;
 
-struct TcArgs {
+struct alignas(64) TcArgs {
+    CUtensorMap rows;                       // packed f16 rows [packed rows][head_dim], boxes of 64 rows x 64 dims
+    const float *fac;                       // a factor for each (0: a hole, NaN: a value that is not finite)
+    const int *odd;                         // kPackCtas: whether a CTA of the packing has met a factor other than 1
     AttnArgs a;
     int group, head_groups, n_slots, split, page_shift;
     Meta *meta;
@@ -187,6 +234,7 @@ template <int NB, int FMT>          // NB: head_dim / 128
 __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_constant__ TcArgs g) {
     constexpr int D = NB * 128, kChunks = NB * 2, kTileBytes = kRows * D * 2;
     constexpr int kParts = NB > 2 ? 2 : 1, kPart0 = 2;                 // a tile is handed over in parts: its first 256 dims, the rest
+    constexpr bool kPre = FMT == kPacked;
     constexpr uint32_t o_tmem = kTmem, s_tmem = kTmem + NB * 64;
     const AttnArgs &a = g.a;
     extern __shared__ __align__(1024) unsigned char smem[];
@@ -221,11 +269,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             for (int k = 0; k < kLoadWarps; ++k) odd_w[i][k] = 0;
             mbar_init(&bars_s.scaled[i], kSoftWarps);
             mbar_init(&bars_s.s_full[i], 1); mbar_init(&bars_s.s_free[i], kSoftWarps); mbar_init(&bars_s.p_full[i], kSoftWarps);
-            for (int k = 0; k < kParts; ++k) { mbar_init(&bars_s.full[i][k], kLoadWarps); mbar_init(&bars_s.pv_done[i][k], 1); }
+            for (int k = 0; k < kParts; ++k) { mbar_init(&bars_s.full[i][k], kPre ? 1 : kLoadWarps); mbar_init(&bars_s.pv_done[i][k], 1); }
         }
         mbar_init(&bars_s.q_full, kLoadWarps); mbar_init(&bars_s.q_free, 1);
         for (int i = 0; i < kTileRing; ++i) { mbar_init(&bars_s.tile_full[i], 1); mbar_init(&bars_s.tile_free[i], kLoadWarps); }
-        for (int i = 0; i < kSegRing; ++i) { mbar_init(&bars_s.seg_full[i], 1); mbar_init(&bars_s.seg_free[i], kSegReaders); }
+        for (int i = 0; i < kSegRing; ++i) { mbar_init(&bars_s.seg_full[i], 1); mbar_init(&bars_s.seg_free[i], kSegReaders + (kPre ? kLoadWarps : 0)); }
     }
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&tmem_s)));
@@ -245,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             tiles[i] = 0;
             before[i] = total;
             if (i * kThreads >= g.n_slots) continue;
-            if (s < g.n_slots) tiles[i] = get_item(a, g.group, g.head_groups, s).tiles;
+            if (s < g.n_slots) tiles[i] = get_item<kPre>(a, g.group, g.head_groups, s).tiles;
             long long sum;
             before[i] += block_scan64(tiles[i], scan_s, &sum);
             total += sum;
@@ -258,7 +306,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         left = min(per, total - per * (long long)blockIdx.x);
     }
     tc::fence_before();
-    __syncthreads();
+    bool any_factor = false;                             // packed rows: there are factors to look at
+    if (kPre) {
+        wait_dependency();
+        any_factor = __syncthreads_or(tid < kPackCtas && *(volatile const int *)(g.odd + tid) != 0);
+    } else {
+        __syncthreads();
+    }
     tc::fence_after();
 
     // A role takes the segments in order from the ring; every warp of it calls this.
@@ -291,6 +345,52 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         const int half = kF32 ? lane >> 4 : (lane >> 2) & 1, l16 = kF32 ? lane & 15 : (lane & 3) | ((lane >> 3) << 2);
         const bool tail = kBlock && a.kv.n_rot != 0;
         const int n_scales = kBlock ? (D - a.kv.n_rot) / 64 : 1;
+        auto load_query = [&](int64_t row0, int rows, int nq) {
+            const uint16_t *src = a.q + (row0 + r) * D + part * 16;
+            // as they are where their largest value is within [2^-4, 2^15], else scaled by a power of two in a second pass
+            float up = 1.0f, down = 1.0f;
+#pragma unroll 1
+            for (int pass = 0; pass < 2; ++pass) {
+                uint32_t amax = 0;
+#pragma unroll 1
+                for (int c0 = 0; c0 < kChunks; c0 += 4) {
+                    uint4 x[4][2];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+                            x[c][u] = r < rows && c0 + c < kChunks ? ld_row16(src + (c0 + c) * 64 + u * 8) : make_uint4(0, 0, 0, 0);
+                    if (pass == 0 && c0 == 0) tc::wait(DS4B200_BAR(q_free, 0), (uint32_t)((nq & 1) ^ 1), abort_flag, status);
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const uint32_t y[4] = {x[c][u].x, x[c][u].y, x[c][u].z, x[c][u].w};
+                            uint32_t o[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                amax = max(amax, max(y[k] & 0x7fff0000u, (y[k] << 16) & 0x7fff0000u));
+                                o[k] = h2_bits(__floats2half2_rn(__uint_as_float(y[k] << 16) * down, __uint_as_float(y[k] & 0xffff0000u) * down));
+                            }
+                            if (c0 + c < kChunks)
+                                *reinterpret_cast<uint4 *>(q_s + (c0 + c) * 8192 + row_off + (((uint32_t)(part * 2 + u) ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+                        }
+                }
+                if (pass) break;
+                amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                const bool far = amax != 0 && (amax < 0x3d800000u || amax > 0x47000000u);
+                if (!__any_sync(0xffffffffu, far)) break;
+                if (far) pow2_parts(__uint_as_float(amax), up, down);
+            }
+            if (part == 0) q_mul[nq & (kScaleSets - 1)][r] = up * a.scale * kLog2e;
+            __syncwarp();
+            if (lane == 0) tc::arrive(DS4B200_BAR(q_full, 0));
+        };
+        if (kPre) {
+            Segment sg;
+            for (int nq = 0; next_segment(sg); ++nq) load_query(sg.it.row0, sg.it.rows, nq);
+        } else {
         uint4 v[kRegs];                                  // [step][row pair]
         float sc[kF32 ? 1 : kRegs];                      // the scale of each
         float4 tl[kBlock ? 4 : 1];
@@ -339,49 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             const int buf = n & 1, ring = n & (kTileRing - 1);
             const uint32_t use = (uint32_t)(((n >> 1) & 1) ^ 1);
             unsigned char *dst = k_s + buf * kTileBytes;
-            if (rows) {                                  // a segment's query rows come ahead of its first tile
-                const uint16_t *src = a.q + (tile_row0[ring] + r) * D + part * 16;
-                // as they are where their largest value is within [2^-4, 2^15], else scaled by a power of two in a second pass
-                float up = 1.0f, down = 1.0f;
-#pragma unroll 1
-                for (int pass = 0; pass < 2; ++pass) {
-                    uint32_t amax = 0;
-#pragma unroll 1
-                    for (int c0 = 0; c0 < kChunks; c0 += 4) {
-                        uint4 x[4][2];
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
-#pragma unroll
-                            for (int u = 0; u < 2; ++u)
-                                x[c][u] = r < rows && c0 + c < kChunks ? ld_row16(src + (c0 + c) * 64 + u * 8) : make_uint4(0, 0, 0, 0);
-                        if (pass == 0 && c0 == 0) tc::wait(DS4B200_BAR(q_free, 0), (uint32_t)((nq & 1) ^ 1), abort_flag, status);
-#pragma unroll
-                        for (int c = 0; c < 4; ++c)
-#pragma unroll
-                            for (int u = 0; u < 2; ++u) {
-                                const uint32_t y[4] = {x[c][u].x, x[c][u].y, x[c][u].z, x[c][u].w};
-                                uint32_t o[4];
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) {
-                                    amax = max(amax, max(y[k] & 0x7fff0000u, (y[k] << 16) & 0x7fff0000u));
-                                    o[k] = h2_bits(__floats2half2_rn(__uint_as_float(y[k] << 16) * down, __uint_as_float(y[k] & 0xffff0000u) * down));
-                                }
-                                if (c0 + c < kChunks)
-                                    *reinterpret_cast<uint4 *>(q_s + (c0 + c) * 8192 + row_off + (((uint32_t)(part * 2 + u) ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-                            }
-                    }
-                    if (pass) break;
-                    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                    const bool far = amax != 0 && (amax < 0x3d800000u || amax > 0x47000000u);
-                    if (!__any_sync(0xffffffffu, far)) break;
-                    if (far) pow2_parts(__uint_as_float(amax), up, down);
-                }
-                if (part == 0) q_mul[nq & (kScaleSets - 1)][r] = up * a.scale * kLog2e;
-                __syncwarp();
-                if (lane == 0) tc::arrive(DS4B200_BAR(q_full, 0));
-                ++nq;
-            }
+            if (rows) load_query(tile_row0[ring], rows, nq++);              // a segment's query rows come ahead of its first tile
             const Slots next = slots_of(n + 1);          // the tile behind this one
             const int next_rows = tile_rows[(n + 1) & (kTileRing - 1)];
             const bool all_here = kUnits > 1 && __all_sync(0xffffffffu, (here.pair[0] | here.pair[1] | here.pair[2] | here.pair[3]) >= 0);
@@ -497,6 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             here = next;
             rows = next_rows;
         }
+        }
     } else if (warp >= kMmaWarp) {
         tc::set_max_registers_down<56>();
         const uint32_t one = tc::elect();
@@ -508,12 +567,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             int n = 0;
             for (int nq = 0; next_segment(sg); ++nq) {
                 const int t0 = __shfl_sync(0xffffffffu, sg.t0, 0), t1 = __shfl_sync(0xffffffffu, sg.t1, 0);
-                const int rows = __shfl_sync(0xffffffffu, sg.it.n, 0);
+                const int n_rows = __shfl_sync(0xffffffffu, sg.it.n, 0), na = __shfl_sync(0xffffffffu, sg.it.na, 0), ta = (na + 63) >> 6;
                 tc::wait<20>(DS4B200_BAR(q_full, 0), (uint32_t)(nq & 1), abort_flag, status);
                 for (int t = t0; t < t1; ++t, ++n) {
                     const int buf = n & 1;
                     const uint32_t phase = (uint32_t)((n >> 1) & 1), k0 = k_desc + (uint32_t)(buf * (kTileBytes >> 4));
-                    const int groups = min(max((rows - t * kRows + 15) >> 4, 1), 4);      // of 16 cache rows
+                    const int groups = min(max(((t < ta ? na - 64 * t : n_rows - na - 64 * (t - ta)) + 15) >> 4, 1), 4);      // of 16 cache rows
                     const uint32_t idesc = tc::idesc_f16(64, 0, false) | (uint32_t)groups << 18;
                     tc::wait<20>(DS4B200_BAR(s_free, buf), phase ^ 1, abort_flag, status);
 #pragma unroll
@@ -542,11 +601,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             int n = 0;
             while (next_segment(sg)) {
                 const int t0 = __shfl_sync(0xffffffffu, sg.t0, 0), t1 = __shfl_sync(0xffffffffu, sg.t1, 0);
-                const int rows = __shfl_sync(0xffffffffu, sg.it.n, 0);
+                const int n_rows = __shfl_sync(0xffffffffu, sg.it.n, 0), na = __shfl_sync(0xffffffffu, sg.it.na, 0), ta = (na + 63) >> 6;
                 for (int t = t0; t < t1; ++t, ++n) {
                     const int buf = n & 1;
                     const uint32_t v0 = v_desc + (uint32_t)(buf * (kTileBytes >> 4)), p0 = p_desc + (uint32_t)(buf * 512);
-                    const int groups = min(max((rows - t * kRows + 15) >> 4, 1), 4);
+                    const int groups = min(max(((t < ta ? na - 64 * t : n_rows - na - 64 * (t - ta)) + 15) >> 4, 1), 4);
                     tc::wait<20>(DS4B200_BAR(p_full, buf), (uint32_t)((n >> 1) & 1), abort_flag, status);
                     if (*(volatile int *)&grown_s[buf] == n + 1) tc::wait<20>(DS4B200_BAR(scaled, buf), scaled_phase(buf), abort_flag, status);
                     tc::fence_async();
@@ -572,7 +631,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 sg.t1 = -1;
                 end = true;
                 while (left > 0 && slot < g.n_slots) {
-                    sg.it = get_item(a, g.group, g.head_groups, slot);
+                    sg.it = get_item<kPre>(a, g.group, g.head_groups, slot);
                     slot += step;
                     if (sg.it.tiles == 0) continue;
                     sg.t0 = tile;
@@ -590,6 +649,28 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 }
                 __syncwarp();
                 if (*abort_flag) break;
+            }
+        } else if (kPre) {
+            // -------------------------------------------------------------------------- copy packed rows
+            Segment sg;
+            int n = 0;
+            while (next_segment(sg)) {
+                for (int t = sg.t0; t < sg.t1; ++t, ++n) {
+                    const int buf = n & 1, ta = first_run_tiles(sg.it);
+                    const int from = t < ta ? sg.it.at_a + 64 * t : sg.it.at_b + 64 * (t - ta);
+#pragma unroll
+                    for (int part = 0; part < kParts; ++part) {
+                        tc::wait<20>(DS4B200_BAR(pv_done, buf * 2 + part), (uint32_t)(((n >> 1) & 1) ^ 1), abort_flag, status);
+                        if (lane == 0) {
+                            constexpr int kFirst = kParts > 1 ? 2 * kPart0 : kChunks;
+                            const int c0 = part * kFirst, c1 = part ? kChunks : kFirst;
+                            tc::expect(DS4B200_BAR(full, buf * 2 + part), (uint32_t)(c1 - c0) * 8192u);
+                            for (int c = c0; c < c1; ++c)
+                                tc::load_box(smem_addr(k_s) + buf * kTileBytes + c * 8192, &g.rows, c * 64, from, DS4B200_BAR(full, buf * 2 + part));
+                        }
+                        __syncwarp();
+                    }
+                }
             }
         } else {
             // -------------------------------------------------------------------------- find
@@ -713,20 +794,27 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 if (lane == 0) tc::arrive(DS4B200_BAR(s_free, buf));
                 float2 v[8];
                 const float2 k2 = make_float2(qk, qk);
-                const bool odd = *(volatile int *)&odd_s[buf] == n + 1;
+                const bool odd = kPre ? any_factor : *(volatile int *)&odd_s[buf] == n + 1;
+                const float *fac = nullptr;              // of the tile's packed rows
+                if (kPre) fac = g.fac + (t < first_run_tiles(it) ? it.at_a + 64 * t : it.at_b + 64 * (t - first_run_tiles(it)));
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     v[i] = mul2(make_float2(__uint_as_float(group ? x[4 * i + 2] : x[4 * i]), __uint_as_float(group ? x[4 * i + 3] : x[4 * i + 1])), k2);
                 if (odd) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {                          // column block i is loader i's
+                        if (kPre) {
+                            const float f0 = __ldg(fac + 8 * i + 2 * (lane & 3)), f1 = __ldg(fac + 8 * i + 2 * (lane & 3) + 1);
+                            v[i] = fma2(v[i], make_float2(f0, f1), make_float2(__log2f(f0), __log2f(f1)));
+                            continue;
+                        }
                         if (odd_w[buf][i] != n + 1) continue;
                         const float4 f = *reinterpret_cast<const float4 *>(&row_fma[buf][2 * (8 * i + 2 * (lane & 3))]);
                         v[i] = fma2(v[i], make_float2(f.x, f.y), make_float2(f.z, f.w));
                     }
                 }
-                if ((t + 1) * kRows > it.n) {            // columns past the rows: S was not computed there
-                    const int end = it.n - t * kRows - 2 * (lane & 3);
+                if (rows_in_tile(it, t) < kRows) {       // columns past the rows: S was not computed there
+                    const int end = rows_in_tile(it, t) - 2 * (lane & 3);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         if (8 * i >= end) v[i].x = -INFINITY;
@@ -736,7 +824,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 if (several) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const int2 at = *reinterpret_cast<const int2 *>(&row_at[n & (2 * kTileRing - 1)][8 * i + 2 * (lane & 3)]);
+                        int2 at;
+                        if (kPre) {
+                            at.x = (t < first_run_tiles(it) ? it.lo + 64 * t : 64 * (t - first_run_tiles(it))) + 8 * i + 2 * (lane & 3);
+                            at.y = at.x + 1;
+                        } else {
+                            at = *reinterpret_cast<const int2 *>(&row_at[n & (2 * kTileRing - 1)][8 * i + 2 * (lane & 3)]);
+                        }
                         if (at.x > p || (at.x <= from && at.x >= a.n_first)) v[i].x = -INFINITY;
                         if (at.y > p || (at.y <= from && at.y >= a.n_first)) v[i].y = -INFINITY;
                     }
@@ -773,7 +867,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 if (odd) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        if (odd_w[buf][i] == n + 1) v[i] = mul2(v[i], *reinterpret_cast<const float2 *>(&row_div[buf][8 * i + 2 * (lane & 3)]));
+                        if (kPre) {
+                            const float f0 = __ldg(fac + 8 * i + 2 * (lane & 3)), f1 = __ldg(fac + 8 * i + 2 * (lane & 3) + 1);
+                            v[i] = mul2(v[i], make_float2(f0 > 0.0f ? __fdividef(1.0f, f0) : 0.0f, f1 > 0.0f ? __fdividef(1.0f, f1) : 0.0f));
+                        } else if (odd_w[buf][i] == n + 1) v[i] = mul2(v[i], *reinterpret_cast<const float2 *>(&row_div[buf][8 * i + 2 * (lane & 3)]));
                 }
                 l = add2(l, add2(add2(add2(v[0], v[1]), add2(v[2], v[3])), add2(add2(v[4], v[5]), add2(v[6], v[7]))));
                 tc::fence_async();
@@ -952,24 +1049,104 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const AttnAr
     }
 }
 
+// The rows a chunk's tokens see, once each, as packed f16 rows: with a window of 128 rows every row is wanted by 128 tokens, and turning it into
+// f16 for each of them cost more than all the rest (4096 tokens: 294 us straight from the cache).  One warp per row.
+// A row whose largest value is outside [2^-9, 2^15] is scaled by a power of two, its factor; a hole has the factor 0, a row with a value
+// that is not finite NaN, with zeros in place of such values, so that it reaches the tokens that see it and no others.
+template <int V>      // float4s of a row per lane: head_dim / 128
+__global__ void __launch_bounds__(kPackWarps * 32) attn_pack_kernel(const AttnArgs a, int64_t bound, uint16_t *rows, float *fac, int *odd) {
+    const int lane = threadIdx.x & 31, dim = a.kv.head_dim;
+    const int64_t most = a.table_width * a.kv.page_rows, gap = packed_gap(a.window, a.n_first, most);
+    bool met = false;
+    launch_dependents();
+    for (int64_t row = (int64_t)blockIdx.x * kPackWarps + (threadIdx.x >> 5); row < bound; row += (int64_t)kPackCtas * kPackWarps) {
+        int lo = 0, hi = a.n_seqs - 1;                   // the last sequence that begins at or before this row
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (mid * gap + (a.window > 0 ? a.q_start[mid] - a.q_start[0] : 0) <= row) lo = mid; else hi = mid - 1;
+        }
+        const Packed k = get_packed(a, lo);
+        const int64_t local = row - k.off;
+        if (local < 0 || local >= (int64_t)k.first + k.len - k.lo + 16) continue;      // 16 rows of zeros behind each sequence
+        const bool is = local < (int64_t)k.first + k.len - k.lo;
+        int64_t slot = -1;
+        if (is) {
+            const int at = local < k.first ? (int)local : (int)(local - k.first) + k.lo, pg = at / a.kv.page_rows;
+            const int page = __ldg(a.page_table + lo * a.table_width + pg);
+            if (page >= 0 && page < a.kv.n_pages) slot = (int64_t)page * a.kv.page_rows + (at - pg * a.kv.page_rows);
+        }
+        float4 r[V];
+        float top = 0.0f;
+        bool finite = true;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int e = 4 * (lane + 32 * j), nope = dim - a.kv.n_rot;
+            r[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (slot >= 0) {
+                if (a.kv.row_format == DS4B200_KV_F32) {
+                    r[j] = ld_ro4(a.kv.raw + slot * dim + e);
+                } else if (a.kv.row_format == DS4B200_KV_FP8_BLOCK64 && e >= nope) {
+                    r[j] = ld_ro4(a.kv.tail + slot * a.kv.n_rot + (e - nope));
+                } else {
+                    const float sc = __ldg(a.kv.scales + (a.kv.row_format == DS4B200_KV_FP8_ROW ? slot : slot * (nope >> 6) + (e >> 6)));
+                    uint32_t x, y;
+                    e4m3x4(__ldg(reinterpret_cast<const uint32_t *>(a.kv.codes + slot * dim + e)), x, y);
+                    const float2 f = f16x2_bits_to_f32(x), h = f16x2_bits_to_f32(y);
+                    r[j] = make_float4(f.x * sc, f.y * sc, h.x * sc, h.y * sc);
+                }
+            }
+            finite = finite && amax4(r[j]) < INFINITY && r[j].x == r[j].x && r[j].y == r[j].y && r[j].z == r[j].z && r[j].w == r[j].w;
+            top = fmaxf(top, amax4(r[j]));
+        }
+        float f = !is || slot >= 0 ? 1.0f : 0.0f, down = 1.0f;
+        if (!__all_sync(0xffffffffu, finite)) {
+            f = __uint_as_float(0x7fffffffu);
+#pragma unroll
+            for (int j = 0; j < V; ++j) r[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        } else {
+            top = warp_max(top);
+            if (top != 0.0f && (top < 0x1p-9f || top > 0x1p15f)) pow2_parts(top, f, down);
+        }
+        met = met || f != 1.0f;
+        if (lane == 0) fac[row] = f;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const uint2 u = make_uint2(h2_bits(__floats2half2_rn(r[j].x * down, r[j].y * down)), h2_bits(__floats2half2_rn(r[j].z * down, r[j].w * down)));
+            *reinterpret_cast<uint2 *>(rows + row * dim + 4 * (lane + 32 * j)) = u;
+        }
+    }
+    met = __syncthreads_or(met);
+    if (threadIdx.x == 0) odd[blockIdx.x] = met;
+}
+
+bool packed_map(CUtensorMap *map, const uint16_t *rows, int64_t n, int dim) {
+    using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                  const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static EncodeFn encode = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+            encode = reinterpret_cast<EncodeFn>(fn);
+        else
+            cudaGetLastError();
+    });
+    if (!encode) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)dim, (cuuint64_t)n}, strides[1] = {(cuuint64_t)dim * 2};
+    const cuuint32_t box[2] = {64, 64}, elem[2] = {1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<uint16_t *>(rows), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The workspace holds either the parts of cut items or packed rows.
+constexpr int64_t kPackRows = 4 * kCtas * kRows;         // f16 rows in the room of 2 kCtas kRows f32 ones
 constexpr int64_t kMetaBytes = (kCtas * (int64_t)sizeof(Meta) + 127) / 128 * 128;
 constexpr int64_t kMlBytes = 2 * kCtas * kRows * (int64_t)sizeof(float2);
 
 template <int NB, int FMT>
-void launch_tc(const AttnArgs &a, cudaStream_t s) {
-    const int head_groups = (a.n_heads + kRows - 1) / kRows;
-    const int group = a.q_start && head_groups == 1 ? kRows / a.n_heads : 1;
-    const int64_t slots = (a.q_start ? a.n_tokens / group + a.n_seqs + 1 : a.n_seqs) * head_groups;
-    // Equal runs of tiles pay where items are long and few: a run's two ends cost 128 KiB of partial sums each and the join
-    // another launch.  512 prompt tokens of 3 tiles took 91 us cut into runs and XX us as whole items; one session of 131072 rows
-    // takes one CTA as a whole item.
-    const int64_t all_rows = a.table_width * a.kv.page_rows;
-    const int64_t seen = a.window > 0 ? std::min<int64_t>(all_rows, (int64_t)a.window + a.n_first + group - 1) : all_rows;
-    const int split = seen > kWholeTiles * kRows && slots <= kSplitItems;
-    unsigned char *ws = static_cast<unsigned char *>(a.ws);
-    Meta *meta = reinterpret_cast<Meta *>(ws);
-    float2 *ml = reinterpret_cast<float2 *>(ws + kMetaBytes);
-    float *po = reinterpret_cast<float *>(ws + kMetaBytes + kMlBytes);
+void launch_tc(const TcArgs &g, bool behind, cudaStream_t s) {
     constexpr int kSmem = 3 * kRows * NB * 256 + 2 * 8192;
     constexpr int kOneCta = 120 * 1024;               // one CTA per SM: each takes the whole tensor memory
     const int smem = kSmem > kOneCta ? kSmem : kOneCta;
@@ -977,19 +1154,48 @@ void launch_tc(const AttnArgs &a, cudaStream_t s) {
     int dev = 0;
     cudaGetDevice(&dev);
     std::call_once(once[dev & 15], [&] { cudaFuncSetAttribute(attn_tc_kernel<NB, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
-    const unsigned grid = (unsigned)(split || slots > kCtas ? kCtas : slots);
-    int shift = -1;
-    for (int k = 0; k < 31; ++k) if (a.kv.page_rows == 1 << k) shift = k;
-    const TcArgs g{a, group, head_groups, (int)slots, split, shift, meta, ml, po, device_status_word()};
-    attn_tc_kernel<NB, FMT><<<grid, kThreads, smem, s>>>(g);
-    if (split) launch_behind(attn_join_kernel, kJoinCtas, kJoinWarps * 32, s, a, (const Meta *)meta, (const float2 *)ml, (const float *)po);
+    const unsigned grid = (unsigned)(g.split || g.n_slots > kCtas ? kCtas : g.n_slots);
+    if (behind) launch_behind(attn_tc_kernel<NB, FMT>, grid, kThreads, smem, s, g);
+    else attn_tc_kernel<NB, FMT><<<grid, kThreads, smem, s>>>(g);
+    if (g.split) launch_behind(attn_join_kernel, kJoinCtas, kJoinWarps * 32, 0, s, g.a, (const Meta *)g.meta, (const float2 *)g.part_ml, (const float *)g.part_o);
 }
 
 template <int NB>
 void launch_fmt(const AttnArgs &a, cudaStream_t s) {
-    if (a.kv.row_format == DS4B200_KV_F32) launch_tc<NB, DS4B200_KV_F32>(a, s);
-    else if (a.kv.row_format == DS4B200_KV_FP8_ROW) launch_tc<NB, DS4B200_KV_FP8_ROW>(a, s);
-    else launch_tc<NB, DS4B200_KV_FP8_BLOCK64>(a, s);
+    TcArgs g{};
+    g.a = a;
+    g.head_groups = (a.n_heads + kRows - 1) / kRows;
+    g.group = a.q_start && g.head_groups == 1 ? kRows / a.n_heads : 1;
+    const int64_t slots = (a.q_start ? a.n_tokens / g.group + a.n_seqs + 1 : a.n_seqs) * g.head_groups;
+    g.n_slots = (int)slots;
+    // Equal runs of tiles pay where items are long and few: a run's two ends cost 128 KiB of partial sums each and the join
+    // another launch.  512 prompt tokens of 3 tiles took 91 us cut into runs and 49 us as whole items; one session of 131072 rows
+    // takes one CTA as a whole item.
+    const int64_t all_rows = a.table_width * a.kv.page_rows;
+    const int64_t seen = a.window > 0 ? std::min<int64_t>(all_rows, (int64_t)a.window + a.n_first + g.group - 1) : all_rows;
+    g.split = seen > kWholeTiles * kRows && slots <= kSplitItems;
+    g.page_shift = -1;
+    for (int k = 0; k < 31; ++k) if (a.kv.page_rows == 1 << k) g.page_shift = k;
+    unsigned char *ws = static_cast<unsigned char *>(a.ws);
+    g.meta = reinterpret_cast<Meta *>(ws);
+    g.part_ml = reinterpret_cast<float2 *>(ws + kMetaBytes);
+    g.part_o = reinterpret_cast<float *>(ws + kMetaBytes + kMlBytes);
+    g.status = device_status_word();
+    static_assert(kPackCtas * sizeof(int) <= kMetaBytes && kPackRows * sizeof(float) <= kMlBytes && kPackCtas <= kThreads, "room for packed rows");
+    const int64_t bound = (a.window > 0 ? a.n_tokens : 0) + a.n_seqs * packed_gap(a.window, a.n_first, all_rows);
+    uint16_t *rows = reinterpret_cast<uint16_t *>(g.part_o);
+    if (a.q_start && !g.split && a.n_tokens >= kPackTokens && bound <= kPackRows && packed_map(&g.rows, rows, bound, a.kv.head_dim)) {
+        g.fac = reinterpret_cast<const float *>(g.part_ml);
+        g.odd = reinterpret_cast<const int *>(ws);
+        attn_pack_kernel<NB><<<kPackCtas, kPackWarps * 32, 0, s>>>(a, bound, rows, reinterpret_cast<float *>(g.part_ml), reinterpret_cast<int *>(ws));
+        launch_tc<NB, kPacked>(g, true, s);
+    } else if (a.kv.row_format == DS4B200_KV_F32) {
+        launch_tc<NB, DS4B200_KV_F32>(g, false, s);
+    } else if (a.kv.row_format == DS4B200_KV_FP8_ROW) {
+        launch_tc<NB, DS4B200_KV_FP8_ROW>(g, false, s);
+    } else {
+        launch_tc<NB, DS4B200_KV_FP8_BLOCK64>(g, false, s);
+    }
 }
 
 }  // namespace

@@ -410,7 +410,7 @@ void pages_copy(const ds4b200_page_array *host, int n_arrays, int64_t n_pages, c
     const ArrayList a = list_arrays(host, n_arrays);
     const int2 *mv = reinterpret_cast<const int2 *>(moves);
     plan_copy_kernel<<<1, kPlanThreads, 0, s>>>(mv, (int)n_moves, n_pages, w, status);
-    launch_behind(apply_kernel<kCopy>, kMoveCtas, kMoveThreads, s, Tables{}, mv, w, a);
+    launch_behind(apply_kernel<kCopy>, kMoveCtas, kMoveThreads, 0, s, Tables{}, mv, w, a);
 }
 
 void pages_fork(const ds4b200_page_array *host, int n_arrays, const PageTables &p, const int32_t *pairs, int64_t n_pairs,
@@ -420,21 +420,21 @@ void pages_fork(const ds4b200_page_array *host, int n_arrays, const PageTables &
     const ArrayList a = list_arrays(host, n_arrays);
     const int2 *pr = reinterpret_cast<const int2 *>(pairs);
     plan_fork_kernel<<<1, kPlanThreads, 0, s>>>(t, pr, (int)n_pairs, w, status);
-    launch_behind(apply_kernel<kFork>, kMoveCtas, kMoveThreads, s, t, pr, w, a);
+    launch_behind(apply_kernel<kFork>, kMoveCtas, kMoveThreads, 0, s, t, pr, w, a);
 }
 
 void pages_reserve(const PageTables &p, const int32_t *new_lens, int32_t *status, void *ws, cudaStream_t s) {
     const Tables t{p.refs_in, p.refs_out, p.table_in, p.table_out, p.lens_in, p.lens_out, p.n_pages, p.n_seqs, p.width, p.page_rows};
     const Work w = lay_out(ws, p.n_pages, p.n_seqs, 0);
     plan_reserve_kernel<<<1, kPlanThreads, 0, s>>>(t, new_lens, w, status);
-    launch_behind(apply_kernel<kReserve>, small_grid(p.n_seqs * p.width), kMoveThreads, s, t, (const int2 *)nullptr, w, ArrayList{});
+    launch_behind(apply_kernel<kReserve>, small_grid(p.n_seqs * p.width), kMoveThreads, 0, s, t, (const int2 *)nullptr, w, ArrayList{});
 }
 
 void pages_free(const PageTables &p, const int32_t *seqs, int64_t n_list, int32_t *status, void *ws, cudaStream_t s) {
     const Tables t{p.refs_in, p.refs_out, p.table_in, p.table_out, p.lens_in, p.lens_out, p.n_pages, p.n_seqs, p.width, p.page_rows};
     const Work w = lay_out(ws, p.n_pages, p.n_seqs, n_list);
     plan_free_kernel<<<1, kPlanThreads, 0, s>>>(t, seqs, (int)n_list, w, status);
-    launch_behind(apply_kernel<kFree>, small_grid(p.n_seqs * p.width), kMoveThreads, s, t, (const int2 *)nullptr, w, ArrayList{});
+    launch_behind(apply_kernel<kFree>, small_grid(p.n_seqs * p.width), kMoveThreads, 0, s, t, (const int2 *)nullptr, w, ArrayList{});
 }
 
 void pages_compact(const ds4b200_page_array *host, int n_arrays, const PageTables &p, int32_t *n_live, void *ws, cudaStream_t s) {
@@ -442,7 +442,7 @@ void pages_compact(const ds4b200_page_array *host, int n_arrays, const PageTable
     const Work w = lay_out(ws, p.n_pages, p.n_seqs, 0);
     const ArrayList a = list_arrays(host, n_arrays);
     plan_compact_kernel<<<1, kPlanThreads, 0, s>>>(t, w, n_live);
-    launch_behind(apply_kernel<kCompact>, kMoveCtas, kMoveThreads, s, t, (const int2 *)nullptr, w, a);
+    launch_behind(apply_kernel<kCompact>, kMoveCtas, kMoveThreads, 0, s, t, (const int2 *)nullptr, w, a);
 }
 
 }  // namespace ds4b200

@@ -95,6 +95,14 @@ __device__ __forceinline__ bool try_phase(uint32_t bar, uint32_t parity) {
                  "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     return done != 0;
 }
+__device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// A box of a two-dimensional tensor map into this CTA's shared memory.
+__device__ __forceinline__ void load_box(uint32_t dst, const void *map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar) : "memory");
+}
 // A wait on an mbarrier phase.  It polls at most kWaitPolls times; the first that runs out raises the status bit and a
 // CTA-wide flag with which every later wait returns soon, so the kernel always ends (its results are invalid then).  A poll takes
 // issue slots and shared-memory bandwidth from the warps that work: with polls every 40 ns the waiting warps issued a third of

@@ -485,3 +485,58 @@ def test_a_serving_run(ops):
     again = ops.attn_decode_paged(q, kv, table, lens)
     assert torch.equal(again, out) and not again[0].any()
     assert ops.device_status() == 0
+
+
+# ------------------------------------------------------------------------------- chunks whose rows are packed first
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("heads,dim,page,lens,toks,window,first", [
+    (64, 512, 16, [300, 1, 500, 70], [90, 1, 64, 70], 128, 4), (64, 256, 64, [200], [200], 33, 0), (20, 384, 7, [333, 90], [100, 33], 60, 20),
+    (2, 128, 64, [400], [400], 128, 64), (100, 128, 32, [150], [90], 100, 200), (64, 128, 64, [40, 1500], [40, 700], 0, 0)])
+def test_packed_chunks_against_64_bits(ops, fmt, heads, dim, page, lens, toks, window, first):
+    """Rows of every size: plain ones, ones that need a factor, holes, and ends of runs inside a group of 16 rows."""
+    c = Case(ops, fmt, heads, dim, page, lens, toks, seed=dim, row_scale=lambda j: (1.0, 1e-4 if fmt != "f32" else 1.0, 3.0)[j % 3])
+    holes = [(0, 0)] + ([(0, 3)] if lens[0] > 5 * page else [])
+    for b, k in holes:
+        c.table[b, k] = -1
+        for j in range(k * page, min((k + 1) * page, lens[b])):
+            c.slots[b][j] = None
+    ws = ops.attn_workspace(heads, dim)
+    ws.fill_(0xff)                                       # NaN wherever something reads what nobody wrote
+    out, lse = ops.attn_window_paged(c.q, c.kv, c.table, c.kv_len, c.q_start, window=window, n_first=first, sink=c.sink, want_lse=True, workspace=ws)
+    c.factors = pack_factors(c)
+    c.tail = 0 if fmt == "f32" else c.tail
+    c.check(out, lse, window, first, c.sink)
+    assert ops.device_status() == 0
+
+
+def pack_factors(c):
+    """Of packed rows: 1, or the power of two at or below a row's largest value where that is outside [2^-9, 2^15]."""
+    top = c.rows.nan_to_num(0.0).abs().amax(1)
+    r = torch.exp2(torch.floor(torch.log2(top.clamp_min(1e-300))))
+    return torch.where((top > 0) & ((top < 2.0 ** -9) | (top > 2.0 ** 15)), r, torch.ones_like(r))
+
+
+def test_nan_in_packed_rows_reaches_only_the_tokens_that_see_it(ops):
+    c = Case(ops, "f32", 64, 128, 64, [200, 150], [200, 100])
+    clean = ops.attn_window_paged(c.q, c.kv, c.table, c.kv_len, c.q_start, window=32, n_first=2)
+    for slot, value in ((c.slots[0][77], float("nan")), (c.slots[1][60], float("inf"))):
+        c.st["raw"][slot, 5] = value
+    out = ops.attn_window_paged(c.q, c.kv, c.table, c.kv_len, c.q_start, window=32, n_first=2)
+    sees = torch.zeros(300, dtype=torch.bool)
+    sees[77:77 + 32] = True
+    sees[200 + 10:200 + 10 + 32] = True
+    bad = out.isnan().flatten(1).any(1).cpu()
+    assert torch.equal(bad, sees)
+    assert torch.equal(out[~sees.cuda()], clean[~sees.cuda()])
+
+
+def test_packed_and_direct_chunks_agree(ops):
+    """The same tokens in a call long enough to pack its rows and in calls that are not."""
+    c = Case(ops, "block", 64, 512, 64, [400], [128])
+    whole = ops.attn_window_paged(c.q, c.kv, c.table, c.kv_len, c.q_start, window=128, n_first=4)
+    for first in range(0, 128, 32):
+        part = ops.attn_window_paged(c.q[first:first + 32].contiguous(), c.kv, c.table, c.kv_len - (96 - first),
+                                     torch.tensor([0, 32], dtype=torch.int32, device="cuda"), window=128, n_first=4)
+        d = (part.float() - whole[first:first + 32].float()).abs()
+        assert bool((d <= 2.0 ** -7 * whole[first:first + 32].float().abs() + 2.0 ** -9).all())
