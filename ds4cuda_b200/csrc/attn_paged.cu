@@ -226,7 +226,7 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 
 struct Bars {
-    uint64_t full[2][2], s_full[2], s_free[2], p_full[2], pv_done[2][2], scaled[2], q_full, q_free;
+    uint64_t full[2][2], s_full[2], s_free[2], p_full[2], pv_done[2][2], scaled[2], q_full, q_free, o_ready[kScaleSets], o_free;
     uint64_t seg_full[kSegRing], seg_free[kSegRing], tile_full[kTileRing], tile_free[kTileRing];
 };
 
@@ -245,12 +245,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     __shared__ int abort_s, start_slot, start_tile;
     __shared__ long long scan_s[kThreads / 32];
     __shared__ __align__(16) float row_fma[2][2 * kRows], row_div[2][kRows];      // by pairs of rows: factor, factor, addend, addend
-    __shared__ __align__(16) int row_at[2 * kTileRing][kRows];       // a row's place in its sequence
-    __shared__ __align__(16) int slot_s[kTileRing][kRows];          // a tile's rows in the pool (-1 past the rows, or kHole), see find_index()
+    __shared__ __align__(16) int row_at[kPre ? 1 : 2 * kTileRing][kRows];       // a row's place in its sequence
+    __shared__ __align__(16) int slot_s[kPre ? 1 : kTileRing][kRows];          // a tile's rows in the pool (-1 past the rows, or kHole), see find_index()
     __shared__ int tile_rows[kTileRing];                            // query rows where a tile is its segment's first, else 0; -1 ends
     __shared__ int64_t tile_row0[kTileRing];                        // and the first of them
     __shared__ float q_mul[kScaleSets][kRows];
-    __shared__ __align__(16) float fac_s[2][kRows], inv_s[kRows];
+    __shared__ __align__(16) float fac_s[2][kRows], inv_s[kScaleSets][kRows];
     __shared__ int odd_s[2], odd_w[2][kLoadWarps];  // 1 + the last tile with a row that is not a plain f16 row: of any loader, of each
     __shared__ int grown_s[2];                      // 1 + the last tile with a row that has grown
     volatile int *abort_flag = &abort_s;
@@ -272,6 +272,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             for (int k = 0; k < kParts; ++k) { mbar_init(&bars_s.full[i][k], kPre ? 1 : kLoadWarps); mbar_init(&bars_s.pv_done[i][k], 1); }
         }
         mbar_init(&bars_s.q_full, kLoadWarps); mbar_init(&bars_s.q_free, 1);
+        mbar_init(&bars_s.o_free, kLoadWarps);
+        // four items: the softmax may be that far ahead of the drain before a product has to wait for it
+        for (int i = 0; i < kScaleSets; ++i) mbar_init(&bars_s.o_ready[i], kSoftWarps);
         for (int i = 0; i < kTileRing; ++i) { mbar_init(&bars_s.tile_full[i], 1); mbar_init(&bars_s.tile_free[i], kLoadWarps); }
         for (int i = 0; i < kSegRing; ++i) { mbar_init(&bars_s.seg_full[i], 1); mbar_init(&bars_s.seg_free[i], kSegReaders + (kPre ? kLoadWarps : 0)); }
     }
@@ -342,6 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         const uint32_t row_off = (uint32_t)(r * 128), sw = (uint32_t)(r & 7);
         // of a load of two rows: which one, and the lane's 16 bytes of its 256; eight consecutive lanes (16 with the 8-byte stores
         // of f32 rows) have to fall on all banks
+        int drained = 0;                                 // tiles of the items whose accumulators are out (packed rows)
         const int half = kF32 ? lane >> 4 : (lane >> 2) & 1, l16 = kF32 ? lane & 15 : (lane & 3) | ((lane >> 3) << 2);
         const bool tail = kBlock && a.kv.n_rot != 0;
         const int n_scales = kBlock ? (D - a.kv.n_rot) / 64 : 1;
@@ -388,8 +392,107 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             if (lane == 0) tc::arrive(DS4B200_BAR(q_full, 0));
         };
         if (kPre) {
-            Segment sg;
-            for (int nq = 0; next_segment(sg); ++nq) load_query(sg.it.row0, sg.it.rows, nq);
+            // With packed rows these warps fetch the query rows and drain the accumulators, one item apart, while the softmax goes on.
+            const int quarter = lw & 3, which = lw >> 2;                    // 32 lanes of tensor memory, 16 of them
+            const uint32_t lanes = (uint32_t)(quarter * 32 + which * 16) << 16;
+            unsigned char *stage = p_s + 2 * 8192;                          // 32 rows of 128 dims
+            auto sync_all = [&]() { asm volatile("bar.sync 4, 256;" ::: "memory"); };
+            Segment sg, next;
+            bool more = next_segment(next);
+            for (int k = -1;; ++k) {
+                // the query rows of item k + 1: all on their way before the last item's products are through
+                if (more) {
+                    uint4 x[kChunks][2];
+                    const uint16_t *src = a.q + (next.it.row0 + r) * D + part * 16;
+                    uint32_t amax = 0;
+#pragma unroll
+                    for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) x[c][u] = r < next.it.rows ? ld_row16(src + c * 64 + u * 8) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const uint32_t y[4] = {x[c][u].x, x[c][u].y, x[c][u].z, x[c][u].w};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) amax = max(amax, max(y[i] & 0x7fff0000u, (y[i] << 16) & 0x7fff0000u));
+                        }
+                    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                    float up = 1.0f, down = 1.0f;
+                    if (amax != 0 && (amax < 0x3d800000u || amax > 0x47000000u)) pow2_parts(__uint_as_float(amax), up, down);
+                    tc::wait(DS4B200_BAR(q_free, 0), (uint32_t)(((k + 1) & 1) ^ 1), abort_flag, status);
+#pragma unroll
+                    for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const uint32_t y[4] = {x[c][u].x, x[c][u].y, x[c][u].z, x[c][u].w};
+                            uint32_t o[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                o[i] = h2_bits(__floats2half2_rn(__uint_as_float(y[i] << 16) * down, __uint_as_float(y[i] & 0xffff0000u) * down));
+                            *reinterpret_cast<uint4 *>(q_s + c * 8192 + row_off + (((uint32_t)(part * 2 + u) ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+                        }
+                    if (part == 0) q_mul[(k + 1) & (kScaleSets - 1)][r] = up * a.scale * kLog2e;
+                    __syncwarp();
+                    if (lane == 0) tc::arrive(DS4B200_BAR(q_full, 0));
+                }
+                // item k's accumulators
+                if (k >= 0) {
+                    tc::wait(DS4B200_BAR(o_ready, k & (kScaleSets - 1)), (uint32_t)((k / kScaleSets) & 1), abort_flag, status);
+                    const int last = drained + sg.t1 - sg.t0 - 1;           // its last tile
+                    drained = last + 1;
+                    tc::wait(DS4B200_BAR(pv_done, (last & 1) * 2 + kParts - 1), (uint32_t)((last >> 1) & 1), abort_flag, status);
+                    tc::fence_after();
+                    constexpr int kHold = NB > 1 ? 2 : 1;                   // blocks of 128 dims read at a time
+#pragma unroll
+                    for (int b0 = 0; b0 < NB; b0 += kHold) {
+                        uint32_t o[kHold][32];
+#pragma unroll
+                        for (int b = 0; b < kHold; ++b)
+                            if (b0 + b < NB) tc::ld_16x64(o_tmem + (b0 + b) * 64 + lanes, o[b]);
+                        tc::wait_ld();
+                        if (b0 + kHold >= NB) {                             // the next item's products may begin
+                            tc::fence_before();
+                            __syncwarp();
+                            if (lane == 0) tc::arrive(DS4B200_BAR(o_free, 0));
+                        }
+#pragma unroll
+                        for (int b = 0; b < kHold; ++b) {
+                            if (b0 + b >= NB) continue;
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {                   // 32 rows
+                                if (h * 32 >= sg.it.rows) continue;
+                                sync_all();                                 // the stage is free
+#pragma unroll
+                                for (int i = 0; i < 4; i += 2) {
+                                    const float2 f0 = *reinterpret_cast<const float2 *>(&inv_s[k & (kScaleSets - 1)][h * 32 + 8 * i + 2 * (lane & 3)]);
+                                    const float2 f1 = *reinterpret_cast<const float2 *>(&inv_s[k & (kScaleSets - 1)][h * 32 + 8 * i + 8 + 2 * (lane & 3)]);
+                                    const uint32_t *y = &o[b][16 * h + 4 * i];
+                                    const uint32_t w0 = h2b(__uint_as_float(y[0]) * f0.x, __uint_as_float(y[1]) * f0.y);
+                                    const uint32_t w1 = h2b(__uint_as_float(y[2]) * f0.x, __uint_as_float(y[3]) * f0.y);
+                                    const uint32_t w2 = h2b(__uint_as_float(y[4]) * f1.x, __uint_as_float(y[5]) * f1.y);
+                                    const uint32_t w3 = h2b(__uint_as_float(y[6]) * f1.x, __uint_as_float(y[7]) * f1.y);
+                                    const int rw = 8 * (i + (lane >> 4)) + (lane & 7), unit = quarter * 4 + which * 2 + ((lane >> 3) & 1);
+                                    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};"
+                                                 ::"r"(smem_addr(stage) + rw * 256 + ((unit ^ (rw & 7)) << 4)), "r"(w0), "r"(w1), "r"(w2), "r"(w3) : "memory");
+                                }
+                                sync_all();
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) {
+                                    const int rw = i * 16 + lw * 2 + (lane >> 4), unit = lane & 15;
+                                    if (h * 32 + rw < sg.it.rows)
+                                        __stcs(reinterpret_cast<uint4 *>(a.out + (sg.it.row0 + h * 32 + rw) * D + (b0 + b) * 128 + unit * 8),
+                                               *reinterpret_cast<const uint4 *>(stage + rw * 256 + ((unit ^ (rw & 7)) << 4)));
+                                }
+                            }
+                        }
+                    }
+                }
+                if (!more) break;
+                sg = next;
+                more = next_segment(next);
+            }
         } else {
         uint4 v[kRegs];                                  // [step][row pair]
         float sc[kF32 ? 1 : kRegs];                      // the scale of each
@@ -398,8 +501,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         auto slots_of = [&](int n) -> Slots {
             const int i = n & (kTileRing - 1);
             tc::wait(DS4B200_BAR(tile_full, i), (uint32_t)((n / kTileRing) & 1), abort_flag, status);
-            const int4 p = *reinterpret_cast<const int4 *>(&slot_s[i][lw * 8 + half * 4]);
-            return Slots{{p.x, p.y, p.z, p.w}, kBlock && tail ? slot_s[i][lw * 8 + ((lane >> 2) & 1) * 4 + (lane >> 3)] : 0};
+            const int4 p = *reinterpret_cast<const int4 *>(&slot_s[kPre ? 0 : i][lw * 8 + half * 4]);
+            return Slots{{p.x, p.y, p.z, p.w}, kBlock && tail ? slot_s[kPre ? 0 : i][lw * 8 + ((lane >> 2) & 1) * 4 + (lane >> 3)] : 0};
         };
         auto load = [&](int my, bool all, int unit, int step, int j) {      // all: of the warp's rows exist
             const int k = step * 4 + j;
@@ -599,8 +702,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             auto scaled_phase = [&](int b) { return scaled_uses[b]++ & 1; };
             Segment sg;
             int n = 0;
-            while (next_segment(sg)) {
+            for (int k = 0; next_segment(sg); ++k) {
                 const int t0 = __shfl_sync(0xffffffffu, sg.t0, 0), t1 = __shfl_sync(0xffffffffu, sg.t1, 0);
+                if (kPre && k > 0) tc::wait<20>(DS4B200_BAR(o_free, 0), (uint32_t)((k - 1) & 1), abort_flag, status);
                 const int n_rows = __shfl_sync(0xffffffffu, sg.it.n, 0), na = __shfl_sync(0xffffffffu, sg.it.na, 0), ta = (na + 63) >> 6;
                 for (int t = t0; t < t1; ++t, ++n) {
                     const int buf = n & 1;
@@ -699,7 +803,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                             const int pg = g.page_shift >= 0 ? at >> g.page_shift : at / a.kv.page_rows;
                             in[h] = at - pg * a.kv.page_rows;
                             page[h] = k < sg.it.n ? max(__ldg(a.page_table + sg.it.b * a.table_width + pg), -1) : -2;
-                            row_at[n & (2 * kTileRing - 1)][lane + 32 * h] = at;
+                            row_at[kPre ? 0 : n & (2 * kTileRing - 1)][lane + 32 * h] = at;
                         }
 #pragma unroll
                         for (int h = 0; h < 2; ++h)
@@ -708,7 +812,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const int r = lane + 32 * h;                        // loaders read the even or the odd rows of eight
-                        slot_s[i][(r & ~7) + (r & 1) * 4 + ((r & 7) >> 1)] = slot[h];
+                        slot_s[kPre ? 0 : i][(r & ~7) + (r & 1) * 4 + ((r & 7) >> 1)] = slot[h];
                         // one prefetch per run of neighbours in the pool: 64 of them a tile kept the copy engine busier than the loaders
                         const int before = __shfl_up_sync(0xffffffffu, slot[h], 1);
                         const uint32_t heads = __ballot_sync(0xffffffffu, lane == 0 || slot[h] < 0 || slot[h] != before + 1);
@@ -829,7 +933,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                             at.x = (t < first_run_tiles(it) ? it.lo + 64 * t : 64 * (t - first_run_tiles(it))) + 8 * i + 2 * (lane & 3);
                             at.y = at.x + 1;
                         } else {
-                            at = *reinterpret_cast<const int2 *>(&row_at[n & (2 * kTileRing - 1)][8 * i + 2 * (lane & 3)]);
+                            at = *reinterpret_cast<const int2 *>(&row_at[kPre ? 0 : n & (2 * kTileRing - 1)][8 * i + 2 * (lane & 3)]);
                         }
                         if (at.x > p || (at.x <= from && at.x >= a.n_first)) v[i].x = -INFINITY;
                         if (at.y > p || (at.y <= from && at.y >= a.n_first)) v[i].y = -INFINITY;
@@ -894,13 +998,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 }
                 inv = m == -INFINITY ? 0.0f : tc::exp2_approx(m - lse2);
             }
+            if (kPre) {                                  // the loaders drain the accumulators
+                if ((lane & 3) == 0) {
+                    if (a.lse && row < it.rows) a.lse[it.row0 + row] = lse2 * (1.0f / kLog2e);
+                    inv_s[nq & (kScaleSets - 1)][row] = inv;
+                }
+                __syncwarp();
+                if (lane == 0) tc::arrive(DS4B200_BAR(o_ready, nq & (kScaleSets - 1)));
+                continue;
+            }
             // the segment's accumulators
             if (warp == 0) tc::wait<20>(DS4B200_BAR(pv_done, ((n - 1) & 1) * 2 + (kParts - 1)), (uint32_t)(((n - 1) >> 1) & 1), abort_flag, status);
             tc::fence_after();
             if ((lane & 3) == 0) {
                 if (!whole) g.part_ml[part * kRows + row] = make_float2(m, sum);
                 else if (a.lse && row < it.rows) a.lse[it.row0 + row] = lse2 * (1.0f / kLog2e);
-                inv_s[row] = inv;
+                inv_s[0][row] = inv;
             }
             sync_all();
             tc::fence_after();
@@ -919,8 +1032,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     tc::wait_ld();
 #pragma unroll
                     for (int i = 0; i < 4; i += 2) {
-                        const float2 f0 = *reinterpret_cast<const float2 *>(&inv_s[r0 + 8 * i + 2 * (lane & 3)]);
-                        const float2 f1 = *reinterpret_cast<const float2 *>(&inv_s[r0 + 8 * i + 8 + 2 * (lane & 3)]);
+                        const float2 f0 = *reinterpret_cast<const float2 *>(&inv_s[0][r0 + 8 * i + 2 * (lane & 3)]);
+                        const float2 f1 = *reinterpret_cast<const float2 *>(&inv_s[0][r0 + 8 * i + 8 + 2 * (lane & 3)]);
                         const int rw = 8 * (i + (lane >> 4)) + (lane & 7);
 #pragma unroll
                         for (int hh = 0; hh < 2; ++hh) {
@@ -1147,7 +1260,7 @@ constexpr int64_t kMlBytes = 2 * kCtas * kRows * (int64_t)sizeof(float2);
 
 template <int NB, int FMT>
 void launch_tc(const TcArgs &g, bool behind, cudaStream_t s) {
-    constexpr int kSmem = 3 * kRows * NB * 256 + 2 * 8192;
+    constexpr int kSmem = 3 * kRows * NB * 256 + (FMT == kPacked ? 3 : 2) * 8192;
     constexpr int kOneCta = 120 * 1024;               // one CTA per SM: each takes the whole tensor memory
     const int smem = kSmem > kOneCta ? kSmem : kOneCta;
     static std::once_flag once[16];
