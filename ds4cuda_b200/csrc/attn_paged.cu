@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     }
     // This CTA's share of the tiles: with `split` a run of the list of all of them, else whole items, every gridDim.x-th.
     long long per = 1, left = 1ll << 62;
-    if (g.split) {
+    if (!kPre && g.split) {
         __syncthreads();
         // every thread has the items tid, tid + kThreads, ..: their tiles are counted once, then the run's first one is found
         constexpr int kMine = (kSplitItems + kThreads - 1) / kThreads;
@@ -444,47 +444,41 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     drained = last + 1;
                     tc::wait(DS4B200_BAR(pv_done, (last & 1) * 2 + kParts - 1), (uint32_t)((last >> 1) & 1), abort_flag, status);
                     tc::fence_after();
-                    constexpr int kHold = NB > 1 ? 2 : 1;                   // blocks of 128 dims read at a time
-#pragma unroll
-                    for (int b0 = 0; b0 < NB; b0 += kHold) {
-                        uint32_t o[kHold][32];
-#pragma unroll
-                        for (int b = 0; b < kHold; ++b)
-                            if (b0 + b < NB) tc::ld_16x64(o_tmem + (b0 + b) * 64 + lanes, o[b]);
+                    // rolled up: with all blocks unrolled this loop alone was 30 KB, and the instruction fetches of all roles stalled for it
+#pragma unroll 1
+                    for (int b = 0; b < NB; ++b) {
+                        uint32_t o[32];
+                        tc::ld_16x64(o_tmem + b * 64 + lanes, o);
                         tc::wait_ld();
-                        if (b0 + kHold >= NB) {                             // the next item's products may begin
+                        if (b + 1 == NB) {                                  // the next item's products may begin
                             tc::fence_before();
                             __syncwarp();
                             if (lane == 0) tc::arrive(DS4B200_BAR(o_free, 0));
                         }
 #pragma unroll
-                        for (int b = 0; b < kHold; ++b) {
-                            if (b0 + b >= NB) continue;
+                        for (int h = 0; h < 2; ++h) {                       // 32 rows
+                            if (h * 32 >= sg.it.rows) continue;
+                            sync_all();                                     // the stage is free
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {                   // 32 rows
-                                if (h * 32 >= sg.it.rows) continue;
-                                sync_all();                                 // the stage is free
+                            for (int i = 0; i < 4; i += 2) {
+                                const float2 f0 = *reinterpret_cast<const float2 *>(&inv_s[k & (kScaleSets - 1)][h * 32 + 8 * i + 2 * (lane & 3)]);
+                                const float2 f1 = *reinterpret_cast<const float2 *>(&inv_s[k & (kScaleSets - 1)][h * 32 + 8 * i + 8 + 2 * (lane & 3)]);
+                                const uint32_t *y = &o[16 * h + 4 * i];
+                                const uint32_t w0 = h2b(__uint_as_float(y[0]) * f0.x, __uint_as_float(y[1]) * f0.y);
+                                const uint32_t w1 = h2b(__uint_as_float(y[2]) * f0.x, __uint_as_float(y[3]) * f0.y);
+                                const uint32_t w2 = h2b(__uint_as_float(y[4]) * f1.x, __uint_as_float(y[5]) * f1.y);
+                                const uint32_t w3 = h2b(__uint_as_float(y[6]) * f1.x, __uint_as_float(y[7]) * f1.y);
+                                const int rw = 8 * (i + (lane >> 4)) + (lane & 7), unit = quarter * 4 + which * 2 + ((lane >> 3) & 1);
+                                asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};"
+                                             ::"r"(smem_addr(stage) + rw * 256 + ((unit ^ (rw & 7)) << 4)), "r"(w0), "r"(w1), "r"(w2), "r"(w3) : "memory");
+                            }
+                            sync_all();
 #pragma unroll
-                                for (int i = 0; i < 4; i += 2) {
-                                    const float2 f0 = *reinterpret_cast<const float2 *>(&inv_s[k & (kScaleSets - 1)][h * 32 + 8 * i + 2 * (lane & 3)]);
-                                    const float2 f1 = *reinterpret_cast<const float2 *>(&inv_s[k & (kScaleSets - 1)][h * 32 + 8 * i + 8 + 2 * (lane & 3)]);
-                                    const uint32_t *y = &o[b][16 * h + 4 * i];
-                                    const uint32_t w0 = h2b(__uint_as_float(y[0]) * f0.x, __uint_as_float(y[1]) * f0.y);
-                                    const uint32_t w1 = h2b(__uint_as_float(y[2]) * f0.x, __uint_as_float(y[3]) * f0.y);
-                                    const uint32_t w2 = h2b(__uint_as_float(y[4]) * f1.x, __uint_as_float(y[5]) * f1.y);
-                                    const uint32_t w3 = h2b(__uint_as_float(y[6]) * f1.x, __uint_as_float(y[7]) * f1.y);
-                                    const int rw = 8 * (i + (lane >> 4)) + (lane & 7), unit = quarter * 4 + which * 2 + ((lane >> 3) & 1);
-                                    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};"
-                                                 ::"r"(smem_addr(stage) + rw * 256 + ((unit ^ (rw & 7)) << 4)), "r"(w0), "r"(w1), "r"(w2), "r"(w3) : "memory");
-                                }
-                                sync_all();
-#pragma unroll
-                                for (int i = 0; i < 2; ++i) {
-                                    const int rw = i * 16 + lw * 2 + (lane >> 4), unit = lane & 15;
-                                    if (h * 32 + rw < sg.it.rows)
-                                        __stcs(reinterpret_cast<uint4 *>(a.out + (sg.it.row0 + h * 32 + rw) * D + (b0 + b) * 128 + unit * 8),
-                                               *reinterpret_cast<const uint4 *>(stage + rw * 256 + ((unit ^ (rw & 7)) << 4)));
-                                }
+                            for (int i = 0; i < 2; ++i) {
+                                const int rw = i * 16 + lw * 2 + (lane >> 4), unit = lane & 15;
+                                if (h * 32 + rw < sg.it.rows)
+                                    __stcs(reinterpret_cast<uint4 *>(a.out + (sg.it.row0 + h * 32 + rw) * D + b * 128 + unit * 8),
+                                           *reinterpret_cast<const uint4 *>(stage + rw * 256 + ((unit ^ (rw & 7)) << 4)));
                             }
                         }
                     }
