@@ -349,45 +349,58 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         const int half = kF32 ? lane >> 4 : (lane >> 2) & 1, l16 = kF32 ? lane & 15 : (lane & 3) | ((lane >> 3) << 2);
         const bool tail = kBlock && a.kv.n_rot != 0;
         const int n_scales = kBlock ? (D - a.kv.n_rot) / 64 : 1;
+        const int q_row = lw * 8 + ((lane >> 3) & 1), q_lane = (lane & 7) | ((lane >> 4) << 3);     // rows q_row + 2 j, 16 of their bytes
         auto load_query = [&](int64_t row0, int rows, int nq) {
-            const uint16_t *src = a.q + (row0 + r) * D + part * 16;
-            // as they are where their largest value is within [2^-4, 2^15], else scaled by a power of two in a second pass
-            float up = 1.0f, down = 1.0f;
+            // two rows at a time, 256 contiguous bytes of each; as they are where a row's largest value is within [2^-4, 2^15], else
+            // scaled by a power of two in a second pass
+            float up[4] = {1.0f, 1.0f, 1.0f, 1.0f}, down[4] = {1.0f, 1.0f, 1.0f, 1.0f};
 #pragma unroll 1
             for (int pass = 0; pass < 2; ++pass) {
-                uint32_t amax = 0;
+                uint32_t amax[4] = {0, 0, 0, 0};
 #pragma unroll 1
-                for (int c0 = 0; c0 < kChunks; c0 += 4) {
+                for (int b0 = 0; b0 < NB; b0 += 2) {
                     uint4 x[4][2];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                    for (int j = 0; j < 4; ++j)
 #pragma unroll
-                        for (int u = 0; u < 2; ++u)
-                            x[c][u] = r < rows && c0 + c < kChunks ? ld_row16(src + (c0 + c) * 64 + u * 8) : make_uint4(0, 0, 0, 0);
-                    if (pass == 0 && c0 == 0) tc::wait(DS4B200_BAR(q_free, 0), (uint32_t)((nq & 1) ^ 1), abort_flag, status);
+                        for (int b = 0; b < 2; ++b)
+                            x[j][b] = q_row + 2 * j < rows && b0 + b < NB ? ld_row16(a.q + (row0 + q_row + 2 * j) * D + (b0 + b) * 128 + q_lane * 8)
+                                                                          : make_uint4(0, 0, 0, 0);
+                    if (pass == 0 && b0 == 0) tc::wait(DS4B200_BAR(q_free, 0), (uint32_t)((nq & 1) ^ 1), abort_flag, status);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
+                    for (int j = 0; j < 4; ++j)
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            const uint32_t y[4] = {x[c][u].x, x[c][u].y, x[c][u].z, x[c][u].w};
+                        for (int b = 0; b < 2; ++b) {
+                            const int rw = q_row + 2 * j;
+                            const uint32_t y[4] = {x[j][b].x, x[j][b].y, x[j][b].z, x[j][b].w};
                             uint32_t o[4];
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                amax = max(amax, max(y[k] & 0x7fff0000u, (y[k] << 16) & 0x7fff0000u));
-                                o[k] = h2_bits(__floats2half2_rn(__uint_as_float(y[k] << 16) * down, __uint_as_float(y[k] & 0xffff0000u) * down));
+                            for (int i = 0; i < 4; ++i) {
+                                amax[j] = max(amax[j], max(y[i] & 0x7fff0000u, (y[i] << 16) & 0x7fff0000u));
+                                o[i] = h2_bits(__floats2half2_rn(__uint_as_float(y[i] << 16) * down[j], __uint_as_float(y[i] & 0xffff0000u) * down[j]));
                             }
-                            if (c0 + c < kChunks)
-                                *reinterpret_cast<uint4 *>(q_s + (c0 + c) * 8192 + row_off + (((uint32_t)(part * 2 + u) ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+                            if (b0 + b < NB)
+                                *reinterpret_cast<uint4 *>(q_s + (2 * (b0 + b) + (q_lane >> 3)) * 8192 + rw * 128 + (((uint32_t)(q_lane & 7) ^ (uint32_t)(rw & 7)) << 4)) =
+                                    make_uint4(o[0], o[1], o[2], o[3]);
                         }
                 }
                 if (pass) break;
-                amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                const bool far = amax != 0 && (amax < 0x3d800000u || amax > 0x47000000u);
+                bool far = false;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1)
+                        if (o != 8) amax[j] = max(amax[j], __shfl_xor_sync(0xffffffffu, amax[j], o));
+                    if (amax[j] != 0 && (amax[j] < 0x3d800000u || amax[j] > 0x47000000u)) {
+                        pow2_parts(__uint_as_float(amax[j]), up[j], down[j]);
+                        far = true;
+                    }
+                }
                 if (!__any_sync(0xffffffffu, far)) break;
-                if (far) pow2_parts(__uint_as_float(amax), up, down);
             }
-            if (part == 0) q_mul[nq & (kScaleSets - 1)][r] = up * a.scale * kLog2e;
+            if (q_lane == 0)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) q_mul[nq & (kScaleSets - 1)][q_row + 2 * j] = up[j] * a.scale * kLog2e;
             __syncwarp();
             if (lane == 0) tc::arrive(DS4B200_BAR(q_full, 0));
         };
@@ -402,38 +415,48 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             for (int k = -1;; ++k) {
                 // the query rows of item k + 1: all on their way before the last item's products are through
                 if (more) {
-                    uint4 x[kChunks][2];
-                    const uint16_t *src = a.q + (next.it.row0 + r) * D + part * 16;
-                    uint32_t amax = 0;
+                    // two rows at a time, 256 contiguous bytes of each; eight lanes of a row make a 128-byte row of the operand
+                    uint4 x[4][NB];
+                    uint32_t amax[4] = {0, 0, 0, 0};
 #pragma unroll
-                    for (int c = 0; c < kChunks; ++c)
+                    for (int j = 0; j < 4; ++j)
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) x[c][u] = r < next.it.rows ? ld_row16(src + c * 64 + u * 8) : make_uint4(0, 0, 0, 0);
+                        for (int b = 0; b < NB; ++b)
+                            x[j][b] = q_row + 2 * j < next.it.rows ? ld_row16(a.q + (next.it.row0 + q_row + 2 * j) * D + b * 128 + q_lane * 8) : make_uint4(0, 0, 0, 0);
+                    float up[4], down[4];
 #pragma unroll
-                    for (int c = 0; c < kChunks; ++c)
+                    for (int j = 0; j < 4; ++j) {
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            const uint32_t y[4] = {x[c][u].x, x[c][u].y, x[c][u].z, x[c][u].w};
+                        for (int b = 0; b < NB; ++b) {
+                            const uint32_t y[4] = {x[j][b].x, x[j][b].y, x[j][b].z, x[j][b].w};
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) amax = max(amax, max(y[i] & 0x7fff0000u, (y[i] << 16) & 0x7fff0000u));
+                            for (int i = 0; i < 4; ++i) amax[j] = max(amax[j], max(y[i] & 0x7fff0000u, (y[i] << 16) & 0x7fff0000u));
                         }
-                    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-                    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-                    float up = 1.0f, down = 1.0f;
-                    if (amax != 0 && (amax < 0x3d800000u || amax > 0x47000000u)) pow2_parts(__uint_as_float(amax), up, down);
+                        up[j] = down[j] = 1.0f;
+                        const bool far = amax[j] < 0x3d800000u || amax[j] > 0x47000000u;
+                        if (__any_sync(0xffffffffu, far)) {                 // a lane's values are far from one: see the whole row's largest
+#pragma unroll
+                            for (int o = 1; o < 32; o <<= 1)
+                                if (o != 8) amax[j] = max(amax[j], __shfl_xor_sync(0xffffffffu, amax[j], o));
+                            if (amax[j] != 0 && (amax[j] < 0x3d800000u || amax[j] > 0x47000000u)) pow2_parts(__uint_as_float(amax[j]), up[j], down[j]);
+                        }
+                    }
                     tc::wait(DS4B200_BAR(q_free, 0), (uint32_t)(((k + 1) & 1) ^ 1), abort_flag, status);
 #pragma unroll
-                    for (int c = 0; c < kChunks; ++c)
+                    for (int j = 0; j < 4; ++j) {
+                        const int rw = q_row + 2 * j;
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            const uint32_t y[4] = {x[c][u].x, x[c][u].y, x[c][u].z, x[c][u].w};
+                        for (int b = 0; b < NB; ++b) {
+                            const uint32_t y[4] = {x[j][b].x, x[j][b].y, x[j][b].z, x[j][b].w};
                             uint32_t o[4];
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
-                                o[i] = h2_bits(__floats2half2_rn(__uint_as_float(y[i] << 16) * down, __uint_as_float(y[i] & 0xffff0000u) * down));
-                            *reinterpret_cast<uint4 *>(q_s + c * 8192 + row_off + (((uint32_t)(part * 2 + u) ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+                                o[i] = h2_bits(__floats2half2_rn(__uint_as_float(y[i] << 16) * down[j], __uint_as_float(y[i] & 0xffff0000u) * down[j]));
+                            *reinterpret_cast<uint4 *>(q_s + (2 * b + (q_lane >> 3)) * 8192 + rw * 128 + (((uint32_t)(q_lane & 7) ^ (uint32_t)(rw & 7)) << 4)) =
+                                make_uint4(o[0], o[1], o[2], o[3]);
                         }
-                    if (part == 0) q_mul[(k + 1) & (kScaleSets - 1)][r] = up * a.scale * kLog2e;
+                        if (q_lane == 0) q_mul[(k + 1) & (kScaleSets - 1)][rw] = up[j] * a.scale * kLog2e;
+                    }
                     __syncwarp();
                     if (lane == 0) tc::arrive(DS4B200_BAR(q_full, 0));
                 }
@@ -753,6 +776,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             Segment sg;
             int n = 0;
             while (next_segment(sg)) {
+                if (lane == 0) prefetch_l2(a.q + sg.it.row0 * D, sg.it.rows * D * 2);       // long before they are wanted
                 for (int t = sg.t0; t < sg.t1; ++t, ++n) {
                     const int buf = n & 1, ta = first_run_tiles(sg.it);
                     const int from = t < ta ? sg.it.at_a + 64 * t : sg.it.at_b + 64 * (t - ta);
