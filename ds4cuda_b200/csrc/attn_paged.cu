@@ -51,6 +51,7 @@ constexpr int kPackTokens = 64;             // of a chunk whose rows are packed 
 constexpr int kMinTiles = 2;                // of a run: below, the join costs more than the run saves
 constexpr float kRescale = 8.0f;            // log2 units
 constexpr int kScaleSets = 4;
+constexpr float kLeast = 0x1p-100f;         // of a row's factor
 constexpr uint32_t kTmem = 0;               // all 512 columns are allocated, so they begin at column 0
 
 struct Meta { int64_t row0; int rows, h0, parts, pad; };
@@ -65,15 +66,21 @@ struct Packed {
 __host__ __device__ constexpr int64_t packed_gap(int window, int n_first, int64_t all_rows) {
     return window > 0 ? (int64_t)window - 1 + n_first + 16 : all_rows + 16;
 }
+// Tokens [x, y) of sequence b: within [0, n_tokens] whatever q_start holds, so that no index leaves its buffer.
+__device__ __forceinline__ int first_token(const AttnArgs &a, int b) { return min(max(a.q_start[b], 0), (int)a.n_tokens); }
+__device__ __forceinline__ int2 tokens_of(const AttnArgs &a, int b) {
+    const int q0 = first_token(a, b);
+    return make_int2(q0, max(first_token(a, b + 1), q0));
+}
 __device__ __forceinline__ Packed get_packed(const AttnArgs &a, int b) {
     const int64_t most = a.table_width * a.kv.page_rows;
     Packed k;
-    const int q0 = a.q_start[b], q1 = a.q_start[b + 1];
+    const int2 q = tokens_of(a, b);
     k.len = (int)min((int64_t)max(a.kv_len[b], 0), most);
-    const int p0 = k.len - (q1 - q0);
+    const int p0 = k.len - (q.y - q.x);
     k.lo = a.window > 0 && p0 + 1 > a.window ? p0 + 1 - a.window : 0;
     k.first = min(a.n_first, k.lo);
-    k.off = b * packed_gap(a.window, a.n_first, most) + (a.window > 0 ? q0 - a.q_start[0] : 0);
+    k.off = b * packed_gap(a.window, a.n_first, most) + (a.window > 0 ? max(q.x - first_token(a, 0), 0) : 0);
     return k;
 }
 
@@ -99,18 +106,17 @@ __device__ __forceinline__ Item get_item(const AttnArgs &a, int group, int head_
     if (a.q_start) {
         // sequence b's groups take the slots from q_start[b] / group + b on (one slot per sequence may stay empty)
         int lo = 0, hi = a.n_seqs - 1;
-        const int off = a.q_start[0] / group;
+        const int off = first_token(a, 0) / group;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if (a.q_start[mid] / group + mid - off <= g) lo = mid; else hi = mid - 1;
+            if (first_token(a, mid) / group + mid - off <= g) lo = mid; else hi = mid - 1;
         }
         it.b = lo;
-        const int q0 = a.q_start[lo], q1 = a.q_start[lo + 1];
-        const int local = (g - (q0 / group + lo - off)) * group;
-        tok0 = q0 + local;
-        ntok = min(group, (int)min((int64_t)q1, a.n_tokens) - tok0);
-        if (tok0 < 0) ntok = 0;
-        it.p0 = local - (q1 - q0);
+        const int2 q = tokens_of(a, lo);
+        const int local = (g - (q.x / group + lo - off)) * group;
+        tok0 = q.x + local;
+        ntok = local < 0 ? 0 : min(group, q.y - tok0);
+        it.p0 = local - (q.y - q.x);
     } else {
         it.b = tok0 = g;
         it.p0 = -1;
@@ -163,6 +169,18 @@ __device__ __forceinline__ uint32_t sat_h2(float x, float y) {      // finite va
     x = fabsf(x) < INFINITY ? fminf(fmaxf(x, -65504.f), 65504.f) : x;
     y = fabsf(y) < INFINITY ? fminf(fmaxf(y, -65504.f), 65504.f) : y;
     return h2_bits(__floats2half2_rn(x, y));
+}
+// f16 pairs: infinities and NaN become zeros; whether there were any
+template <int N>
+__device__ __forceinline__ bool drop_nonfinite(uint32_t (&o)[N]) {
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const uint32_t bad = __vcmpeq2(o[i] & 0x7c007c00u, 0x7c007c00u);
+        any |= bad;
+        o[i] &= ~bad;
+    }
+    return any != 0;
 }
 // 2^e and 2^-e with e the exponent of x (0 for x = 0), both normal
 __device__ __forceinline__ void pow2_parts(float x, float &up, float &down) {
@@ -226,11 +244,11 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 
 struct Bars {
-    uint64_t full[2][2], s_full[2], s_free[2], p_full[2], pv_done[2][2], scaled[2], q_full, q_free, o_ready[kScaleSets], o_free;
+    uint64_t full[2][2], s_full[2], s_free[2], p_full[2], pv_done[2][2], scaled[2], q_full, q_free, o_ready[kScaleSets], o_free, quiet[2];
     uint64_t seg_full[kSegRing], seg_free[kSegRing], tile_full[kTileRing], tile_free[kTileRing];
 };
 
-template <int NB, int FMT>          // NB: head_dim / 128
+template <int NB, int FMT, bool SHARED>     // NB: head_dim / 128; SHARED: an item may hold several tokens (with packed rows always so)
 __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_constant__ TcArgs g) {
     constexpr int D = NB * 128, kChunks = NB * 2, kTileBytes = kRows * D * 2;
     constexpr int kParts = NB > 2 ? 2 : 1, kPart0 = 2;                 // a tile is handed over in parts: its first 256 dims, the rest
@@ -257,6 +275,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     const uint32_t bars = tc::held(smem_addr(&bars_s));
 #define DS4B200_BAR(name, i) (bars + (uint32_t)offsetof(Bars, name) + 8u * (uint32_t)(i))
     int *status = g.status;
+    const bool several = SHARED && g.group > 1;         // tokens in an item
     launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
@@ -266,6 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         start_tile = 0;
         for (int i = 0; i < 2; ++i) {
             grown_s[i] = odd_s[i] = 0;
+            mbar_init(&bars_s.quiet[i], 1);
             for (int k = 0; k < kLoadWarps; ++k) odd_w[i][k] = 0;
             mbar_init(&bars_s.scaled[i], kSoftWarps);
             mbar_init(&bars_s.s_full[i], 1); mbar_init(&bars_s.s_free[i], kSoftWarps); mbar_init(&bars_s.p_full[i], kSoftWarps);
@@ -581,7 +601,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     for (int j = 0; j < 4; ++j) bad = bad || !(amax4(tl[kBlock ? j : 0]) <= 0x1p14f);
             }
             const bool hole = here.pair[0] == kHole || here.pair[1] == kHole || here.pair[2] == kHole || here.pair[3] == kHole;
-            if (__any_sync(0xffffffffu, bad || hole)) {
+            const bool odd = __any_sync(0xffffffffu, bad || hole);
+            if (odd) {
+                tc::wait(DS4B200_BAR(pv_done, (buf) * 2 + (0)), use, abort_flag, status);       // the softmax has done with this buffer's factors
                 if (lane == 0) odd_s[buf] = odd_w[buf][lw] = n + 1;
                 float mine = 1.0f;                       // the factor of row r
 #pragma unroll
@@ -601,12 +623,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                             t4 = fmaxf(t4, __shfl_xor_sync(0xffffffffu, t4, 2));
                             top = fmaxf(top, __shfl_sync(0xffffffffu, t4, (2 * j + half) * 4) * (1.0f / 256.0f));
                         }
-                        mul = top;
-                        float inv = 1.0f;
-                        if (kBlock) pow2_parts(top, mul, inv);
-                        if (mul == 0.0f) mul = 1.0e-30f;
+                        // not below kLeast: the weight times the factor would leave f32's range while the weight still counts
+                        mul = top < kLeast ? kLeast : top;
+                        float inv = 1.0f / mul;
+                        if (kBlock) pow2_parts(top == 0.0f ? top : mul, mul, inv);
 #pragma unroll
-                        for (int st = 0; st < kSteps; ++st) sc[kF32 ? 0 : st * 4 + j] = kBlock ? sc[kF32 ? 0 : st * 4 + j] * inv : 1.0f;
+                        for (int st = 0; st < kSteps; ++st) sc[kF32 ? 0 : st * 4 + j] = kBlock || top < kLeast ? sc[kF32 ? 0 : st * 4 + j] * inv : 1.0f;
                     }
                     const float got = __shfl_sync(0xffffffffu, mul, kF32 ? (lane & 4) << 2 : lane & 4);   // of a lane whose half is row r's parity
                     if ((lane >> 3) == j) mine = got;
@@ -614,11 +636,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                         const int rw = lw * 8 + 2 * j + half;
                         row_fma[buf][2 * (rw & ~1) + (rw & 1)] = mul;
                         row_fma[buf][2 * (rw & ~1) + 2 + (rw & 1)] = here.pair[j] >= 0 ? __log2f(mul) : -INFINITY;
-                        row_div[buf][rw] = __fdividef(1.0f, mul);
+                        row_div[buf][rw] = mul == mul ? 1.0f / mul : 1.0f;
                     }
                 }
                 if (kBlock) down = 1.0f / mine;
             }
+            uint32_t spoilt = 0;                         // bit j: row 2 j + half has a value that is not finite
             const int rw = lw * 8 + half;
 #pragma unroll
             for (int unit = 0; unit < kUnits; ++unit)
@@ -635,8 +658,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                         const uint4 x = v[step * 4 + j];
                         const uint32_t r7 = (uint32_t)(2 * j + half);
                         if (kF32) {
+                            uint32_t o[2] = {sat_h2(__uint_as_float(x.x), __uint_as_float(x.y)), sat_h2(__uint_as_float(x.z), __uint_as_float(x.w))};
+                            if (SHARED && several) spoilt |= (uint32_t)drop_nonfinite(o) << j;
                             *reinterpret_cast<uint2 *>(dst + c0 * 8192 + (rw + 2 * j) * 128 + ((((uint32_t)l16 >> 1) ^ r7) << 4) + (l16 & 1) * 8) =
-                                make_uint2(sat_h2(__uint_as_float(x.x), __uint_as_float(x.y)), sat_h2(__uint_as_float(x.z), __uint_as_float(x.w)));
+                                make_uint2(o[0], o[1]);
                         } else {
                             const int c = c0 + (l16 >> 2);
                             const __half2 f = __float2half2_rn(sc[kF32 ? 0 : step * 4 + j]);
@@ -647,6 +672,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 #pragma unroll
                             for (int k = 0; k < 8; ++k) o[k] = h2_bits(__hmul2(*reinterpret_cast<__half2 *>(&o[k]), f));
                             if (c < kChunks && !(tail && c == kChunks - 1)) {
+                                if (SHARED && several) spoilt |= (uint32_t)drop_nonfinite(o) << j;
                                 unsigned char *to = dst + c * 8192 + (rw + 2 * j) * 128;
                                 const uint32_t u = (uint32_t)(l16 & 3) * 2;
                                 *reinterpret_cast<uint4 *>(to + ((u ^ r7) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
@@ -665,10 +691,31 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     o[2 * j] = h2_bits(__floats2half2_rn(y.x * down, y.y * down));
                     o[2 * j + 1] = h2_bits(__floats2half2_rn(y.z * down, y.w * down));
                 }
+                if (SHARED && several) {                 // row r's flag goes to the lanes that have it as 2 j + half
+                    const uint32_t rows_bad = __ballot_sync(0xffffffffu, drop_nonfinite(o));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) spoilt |= (rows_bad >> (4 * (2 * j + half)) & 15u ? 1u : 0u) << j;
+                }
                 unsigned char *to = dst + (kChunks - 1) * 8192 + row_off;
                 *reinterpret_cast<uint4 *>(to + (((uint32_t)(part * 2) ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
                 *reinterpret_cast<uint4 *>(to + (((uint32_t)(part * 2 + 1) ^ sw) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
                 if (next_rows >= 0) load_tail(next.own);
+            }
+            // Several tokens share the tile, and 0 * NaN would reach the ones that do not see the row: it has zeros where it is not finite, and
+            // the factor NaN for those that see it.
+            if (SHARED && several && __any_sync(0xffffffffu, spoilt != 0)) {
+                if (lane == 0) odd_s[buf] = odd_w[buf][lw] = n + 1;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t who = __ballot_sync(0xffffffffu, spoilt >> j & 1);
+                    const bool is = (who & (kF32 ? 0xffffu << (16 * half) : 0x0f0f0f0fu << (4 * half))) != 0;
+                    if (l16 == 0 && (is || !odd)) {
+                        const int k = rw + 2 * j;
+                        row_fma[buf][2 * (k & ~1) + (k & 1)] = is ? __uint_as_float(0x7fffffffu) : 1.0f;
+                        if (!odd) row_fma[buf][2 * (k & ~1) + 2 + (k & 1)] = 0.0f;
+                        if (!odd) row_div[buf][k] = 1.0f;
+                    }
+                }
             }
             hand_over(kParts - 1);
             if (lane == 0) tc::arrive(DS4B200_BAR(tile_free, ring));
@@ -711,6 +758,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 }
                 tc::commit(one, DS4B200_BAR(q_free, 0));
             }
+            if (*abort_flag) { tc::commit(one, DS4B200_BAR(quiet, 0)); tc::settle(DS4B200_BAR(quiet, 0), 0); }
         } else if (warp == kMmaWarp + 1) {
             // -------------------------------------------------------------------------- O^T += V^T P^T
             const uint32_t v_desc = tc::desc_lo(smem_addr(k_s), 8192), p_desc = tc::desc_lo(smem_addr(p_s), 0);
@@ -742,10 +790,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     tc::commit(one, DS4B200_BAR(pv_done, (buf) * 2 + (kParts - 1)));
                 }
             }
+            if (*abort_flag) { tc::commit(one, DS4B200_BAR(quiet, 1)); tc::settle(DS4B200_BAR(quiet, 1), 0); }
         } else if (warp == kMmaWarp + 2) {
             // -------------------------------------------------------------------------- schedule
             int slot = g.split ? start_slot : (int)blockIdx.x, tile = g.split ? start_tile : 0;
             const int step = g.split ? 1 : (int)gridDim.x;
+            int longest = 0;                             // it waits for whole items, 16 polls of 0.3 us a tile at most
             for (bool end = false; !end; ++seg) {
                 Segment sg;
                 sg.t0 = 0;
@@ -755,6 +805,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     sg.it = get_item<kPre>(a, g.group, g.head_groups, slot);
                     slot += step;
                     if (sg.it.tiles == 0) continue;
+                    longest = max(longest, sg.it.tiles);
                     sg.t0 = tile;
                     sg.t1 = (int)min((long long)sg.it.tiles, tile + left);
                     tile = 0;
@@ -763,7 +814,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     break;
                 }
                 const int i = seg & (kSegRing - 1);
-                tc::wait<300>(DS4B200_BAR(seg_free, i), (uint32_t)(((seg / kSegRing) & 1) ^ 1), abort_flag, status);
+                tc::wait<300>(DS4B200_BAR(seg_free, i), (uint32_t)(((seg / kSegRing) & 1) ^ 1), abort_flag, status, tc::kWaitPolls + 16 * longest);
                 if (lane == 0) {
                     seg_s[i] = sg;
                     tc::arrive(DS4B200_BAR(seg_full, i));
@@ -794,6 +845,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     }
                 }
             }
+            if (*abort_flag)                             // no copy is in flight when the kernel ends
+                for (int k = max(n - 2, 0); k < n; ++k)
+                    for (int part = 0; part < kParts; ++part) tc::settle(DS4B200_BAR(full, (k & 1) * 2 + part), (uint32_t)((k >> 1) & 1));
         } else {
             // -------------------------------------------------------------------------- find
             // The pool rows of the tiles to come, two per lane, up to kTileRing tiles ahead of the loaders: a page-table entry, and the first
@@ -861,7 +915,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         const int quarter = warp & 3, group = warp >> 2;
         const int row = quarter * 16 + group * 8 + (lane >> 2);
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-        const bool several = g.head_groups == 1 && g.group > 1;
         unsigned char *stage = p_s + group * 8192;      // of this group's output, where its weights' buffers are free
         // One warp polls the barriers of the MMAs, the others wait for it here: the hardware's barrier costs them no issue slots.
         auto sync_all = [&]() { asm volatile("bar.sync 3, 256;" ::: "memory"); };
@@ -1194,7 +1247,7 @@ __global__ void __launch_bounds__(kPackWarps * 32) attn_pack_kernel(const AttnAr
         int lo = 0, hi = a.n_seqs - 1;                   // the last sequence that begins at or before this row
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if (mid * gap + (a.window > 0 ? a.q_start[mid] - a.q_start[0] : 0) <= row) lo = mid; else hi = mid - 1;
+            if (mid * gap + (a.window > 0 ? first_token(a, mid) - first_token(a, 0) : 0) <= row) lo = mid; else hi = mid - 1;
         }
         const Packed k = get_packed(a, lo);
         const int64_t local = row - k.off;
@@ -1236,7 +1289,7 @@ __global__ void __launch_bounds__(kPackWarps * 32) attn_pack_kernel(const AttnAr
             for (int j = 0; j < V; ++j) r[j] = make_float4(0.f, 0.f, 0.f, 0.f);
         } else {
             top = warp_max(top);
-            if (top != 0.0f && (top < 0x1p-9f || top > 0x1p15f)) pow2_parts(top, f, down);
+            if (top != 0.0f && (top < 0x1p-9f || top > 0x1p15f)) pow2_parts(fmaxf(top, kLeast), f, down);
         }
         met = met || f != 1.0f;
         if (lane == 0) fac[row] = f;
@@ -1276,18 +1329,16 @@ constexpr int64_t kPackRows = 4 * kCtas * kRows;         // f16 rows in the room
 constexpr int64_t kMetaBytes = (kCtas * (int64_t)sizeof(Meta) + 127) / 128 * 128;
 constexpr int64_t kMlBytes = 2 * kCtas * kRows * (int64_t)sizeof(float2);
 
-template <int NB, int FMT>
-void launch_tc(const TcArgs &g, bool behind, cudaStream_t s) {
+template <int NB, int FMT, bool SHARED>
+void launch_tc(const TcArgs &g, cudaStream_t s) {
     constexpr int kSmem = 3 * kRows * NB * 256 + (FMT == kPacked ? 3 : 2) * 8192;
     constexpr int kOneCta = 120 * 1024;               // one CTA per SM: each takes the whole tensor memory
     const int smem = kSmem > kOneCta ? kSmem : kOneCta;
-    static std::once_flag once[16];
-    int dev = 0;
-    cudaGetDevice(&dev);
-    std::call_once(once[dev & 15], [&] { cudaFuncSetAttribute(attn_tc_kernel<NB, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem); });
+    const auto kernel = attn_tc_kernel<NB, FMT, SHARED>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return;    // launched() reports it
     const unsigned grid = (unsigned)(g.split || g.n_slots > kCtas ? kCtas : g.n_slots);
-    if (behind) launch_behind(attn_tc_kernel<NB, FMT>, grid, kThreads, smem, s, g);
-    else attn_tc_kernel<NB, FMT><<<grid, kThreads, smem, s>>>(g);
+    if (FMT == kPacked) launch_behind(kernel, grid, kThreads, smem, s, g);
+    else kernel<<<grid, kThreads, smem, s>>>(g);
     if (g.split) launch_behind(attn_join_kernel, kJoinCtas, kJoinWarps * 32, 0, s, g.a, (const Meta *)g.meta, (const float2 *)g.part_ml, (const float *)g.part_o);
 }
 
@@ -1319,13 +1370,13 @@ void launch_fmt(const AttnArgs &a, cudaStream_t s) {
         g.fac = reinterpret_cast<const float *>(g.part_ml);
         g.odd = reinterpret_cast<const int *>(ws);
         attn_pack_kernel<NB><<<kPackCtas, kPackWarps * 32, 0, s>>>(a, bound, rows, reinterpret_cast<float *>(g.part_ml), reinterpret_cast<int *>(ws));
-        launch_tc<NB, kPacked>(g, true, s);
+        launch_tc<NB, kPacked, true>(g, s);
     } else if (a.kv.row_format == DS4B200_KV_F32) {
-        launch_tc<NB, DS4B200_KV_F32>(g, false, s);
+        g.group > 1 ? launch_tc<NB, DS4B200_KV_F32, true>(g, s) : launch_tc<NB, DS4B200_KV_F32, false>(g, s);
     } else if (a.kv.row_format == DS4B200_KV_FP8_ROW) {
-        launch_tc<NB, DS4B200_KV_FP8_ROW>(g, false, s);
+        g.group > 1 ? launch_tc<NB, DS4B200_KV_FP8_ROW, true>(g, s) : launch_tc<NB, DS4B200_KV_FP8_ROW, false>(g, s);
     } else {
-        launch_tc<NB, DS4B200_KV_FP8_BLOCK64>(g, false, s);
+        g.group > 1 ? launch_tc<NB, DS4B200_KV_FP8_BLOCK64, true>(g, s) : launch_tc<NB, DS4B200_KV_FP8_BLOCK64, false>(g, s);
     }
 }
 

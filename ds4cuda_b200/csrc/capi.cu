@@ -641,7 +641,7 @@ static int check_attn(const char *what, const ds4b200_paged_kv *kv, const void *
         }
     }
     REQUIRE(a16(q) && a16(out) && a16(workspace), "%s: q, out and workspace need 16-byte alignment", what);
-    REQUIRE(table_width >= 1 && table_width < ((int64_t)1 << 31), "%s: table_width must be in [1, 2^31)", what);
+    REQUIRE(table_width >= 1 && table_width <= (INT32_MAX - 64) / kv->page_rows, "%s: table_width * page_rows must be in [1, 2^31 - 64)", what);
     REQUIRE(n_seqs <= ds4b200::kMaxWindowSeqs, "%s: at most 4096 sequences per call", what);
     REQUIRE(n_heads >= 1 && n_heads <= ds4b200::kMaxAttnHeads, "%s: n_heads must be in [1, 1024]", what);
     REQUIRE(scale > -3.0e38f && scale < 3.0e38f, "%s: scale must be finite", what);

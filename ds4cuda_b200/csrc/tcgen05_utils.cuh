@@ -108,16 +108,22 @@ __device__ __forceinline__ void load_box(uint32_t dst, const void *map, int x, i
 // issue slots and shared-memory bandwidth from the warps that work: with polls every 40 ns the waiting warps issued a third of
 // all instructions.
 template <int NS = 100>
-__device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status) {
+__device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status, int polls = kWaitPolls) {
     if (try_phase(bar, parity)) return;
 #pragma unroll 1
-    for (int i = 1; i <= kWaitPolls; ++i) {
+    for (int i = 1; i <= polls; ++i) {
         __nanosleep(NS);
         if (try_phase(bar, parity)) return;
         if ((i & 63) == 0 && *abort_flag) return;
     }
     *abort_flag = 1;
     atomicOr(status, kStatusBulkCopyTimeout);
+}
+
+// For what is still in flight when a kernel gives up.
+__device__ __forceinline__ void settle(uint32_t bar, uint32_t parity) {
+#pragma unroll 1
+    for (int i = 0; i < (1 << 16) && !try_phase(bar, parity); ++i) __nanosleep(100);
 }
 
 }  // namespace tc

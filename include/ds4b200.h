@@ -472,7 +472,8 @@ typedef struct ds4b200_paged_kv {
  *     lse[b][h] = log(sum_j exp(s_j) + exp(sink[h]))
  * sink (f32 [n_heads], nullable) is the reference's per-head logit without a row (cuda/flash_attn.cu:148).
  * lse is nullable.  A token that sees no row gets out = 0 and lse = sink[h] or -inf.  kv_len is clamped to
- * [0, table_width * page_rows].
+ * [0, table_width * page_rows], which must be below 2^31 - 64.  A row with a value that is not finite reaches the tokens that
+ * see it, as NaN, and no others.
  * The products run in f16 with f32 accumulation: q exactly (scaled by a power of two where its range asks for it), cache rows
  * as f16 numbers, as the reference's attention reads its cache (cuda/flash_attn.cu:113-115): exact for
  * FP8_BLOCK64 codes and for the f16-rounded rows of ds4b200_kv_rows_to_raw_f32, else rounded (FP8 rows outside
@@ -488,7 +489,7 @@ int ds4b200_attn_decode_paged_bf16(const uint16_t *q, const ds4b200_paged_kv *ho
 
 /* Attention of the tokens of a prompt chunk, several sequences in one call.  q, out bf16
  * [n_tokens][n_heads][head_dim]; tokens q_start[b] .. q_start[b+1] - 1 (device int32 [n_seqs + 1], ascending from
- * q_start[0] >= 0) are the last rows of sequence b, so token i of its n stands at row kv_len[b] - n + i and
+ * q_start[0] >= 0, clamped to [0, n_tokens]) are the last rows of sequence b, so token i of its n stands at row kv_len[b] - n + i and
  * sees rows up to its own, with window and n_first as above.  Tokens outside [q_start[0], q_start[n_seqs])
  * keep what out (and lse [n_tokens][n_heads]) held.  n_seqs <= 4096. */
 int ds4b200_attn_window_paged_bf16(const uint16_t *q, int64_t n_tokens, const ds4b200_paged_kv *host_kv,

@@ -540,3 +540,85 @@ def test_packed_and_direct_chunks_agree(ops):
                                      torch.tensor([0, 32], dtype=torch.int32, device="cuda"), window=128, n_first=4)
         d = (part.float() - whole[first:first + 32].float()).abs()
         assert bool((d <= 2.0 ** -7 * whole[first:first + 32].float().abs() + 2.0 ** -9).all())
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("spoil", ["first", "tail", "scale"])
+def test_rows_that_are_not_finite_reach_only_the_tokens_that_see_them(ops, fmt, spoil):
+    """Four tokens of 16 heads share the tiles of a chunk that is too short to be packed."""
+    c = Case(ops, fmt, 16, 512, 64, [200, 90], [30, 11])
+    call = lambda: ops.attn_window_paged(c.q, c.kv, c.table, c.kv_len, c.q_start, window=20, n_first=2)
+    clean = call()
+    slots = c.slots[0][181], c.slots[1][70]                                 # tokens 11 .. 30 see the first; 30 .. 40 (rows 79 .. 89) the second
+    for slot, value in zip(slots, (float("nan"), float("inf"))):
+        if fmt == "f32":
+            c.st["raw"][slot, {"first": 0, "tail": 511, "scale": 200}[spoil]] = value
+        elif spoil == "scale":
+            c.st["scales"].view(c.st["scales"].shape[0], -1)[slot, 0] = value
+        elif spoil == "tail" and fmt == "block":
+            c.st["tail"][slot, 63] = value
+        else:
+            c.st["codes"][slot, 447 if spoil == "tail" else 0] = 0x7f
+    out = call()
+    sees = torch.zeros(41, dtype=torch.bool)
+    sees[11:30] = True
+    sees[30:41] = True
+    assert torch.equal(out.isnan().flatten(1).any(1).cpu(), sees)
+    assert torch.equal(out[~sees.cuda()], clean[~sees.cuda()])
+    assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("fmt", ["row", "block"])
+def test_every_tile_has_factors_of_its_own(ops, fmt):
+    """Rows that need a factor in every tile, other ones in the next tile of the same buffer."""
+    mags = (1e-6, 3e-6, 3e-5, 1e-5)
+    c = Case(ops, fmt, 64, 512, 64, [6000, 4000, 900], row_scale=lambda j: mags[j // 64 % 4])
+    scale = 1.0 / 3e-5 / 16
+    for n_seqs in (1, 3):
+        out, lse = ops.attn_decode_paged(c.q[:n_seqs], c.kv, c.table[:n_seqs], c.kv_len[:n_seqs], scale=scale, want_lse=True)
+        for _ in range(3):
+            again = ops.attn_decode_paged(c.q[:n_seqs], c.kv, c.table[:n_seqs], c.kv_len[:n_seqs], scale=scale)
+            assert torch.equal(again, out)
+    c.check(out, lse, 0, 0, None, scale=scale)
+
+
+def test_bounds_of_sequences_that_are_not_ascending_stay_in_bounds(ops):
+    """Device data that no host check sees: the call ends, and one whose last bound alone is too large counts as clamped."""
+    c = Case(ops, "f32", 16, 128, 64, [90, 80, 100], [20, 30, 50])
+    for bounds in ([0, 1 << 30, 50, 100], [-7, 90, 50, 100], [0, 20, 50, 1 << 30], [1 << 30, -5, 1 << 30, -5]):
+        q_start = torch.tensor(bounds, dtype=torch.int32, device="cuda")
+        for window in (0, 24):
+            out = torch.zeros_like(c.q)
+            ops.attn_window_paged(c.q, c.kv, c.table, c.kv_len, q_start, window=window, n_first=2, out=out)
+            short = torch.zeros_like(c.q[:60])
+            ops.attn_window_paged(c.q[:60], c.kv, c.table, c.kv_len, q_start, window=window, n_first=2, out=short)
+    torch.cuda.synchronize()
+    assert ops.device_status() == 0
+    good = ops.attn_window_paged(c.q, c.kv, c.table, c.kv_len, torch.tensor([0, 20, 50, 1 << 30], dtype=torch.int32, device="cuda"), window=24)
+    c.check(good, None, 24, 0, None)
+
+
+@pytest.mark.parametrize("fmt", ["row", "block"])
+@pytest.mark.parametrize("toks", [0, 3, 70])
+def test_rows_of_zeros_and_tiny_rows_keep_their_weight(ops, fmt, toks):
+    """Such rows count in the softmax's sum, however small what they add to the output."""
+    lens = [300, 90] if toks else [3000, 90]
+    c = Case(ops, fmt, 16, 512, 64, lens, [toks, toks] if toks else None, row_scale=lambda j: (1.0, 0.0, 1e-34, 1e-20)[j % 4])
+    scales = c.st["scales"].view(c.st["scales"].shape[0], -1)
+    for b in range(2):
+        for j, slot in enumerate(c.slots[b]):
+            if j % 8 == 1:
+                scales[slot] = 0.0                                          # whatever a store leaves for a row of zeros, zero is read as zero
+                c.rows[slot] = 0.0
+                c.factors[slot] = 1.0
+            elif j % 8 == 2 and fmt == "row":
+                scales[slot] = 1e-37
+                c.rows[slot] = model.row_values(fmt, {k: v[slot:slot + 1] for k, v in c.st.items()}, 64)[0]
+                c.factors[slot] = 1e-37
+    if toks:
+        out, lse = ops.attn_window_paged(c.q, c.kv, c.table, c.kv_len, c.q_start, want_lse=True)
+    else:
+        out, lse = ops.attn_decode_paged(c.q, c.kv, c.table, c.kv_len, want_lse=True)
+    if toks == 70:
+        c.factors = pack_factors(c)
+    c.check(out, lse, 0, 0, None)

@@ -45,6 +45,8 @@ def test_attention_refusals(lib):
                 dict(tail=None), dict(row_format=_lib.KV_F32), dict(row_format=_lib.KV_F32, raw=PTR + 4), dict(row_format=_lib.KV_FP8_ROW, codes=None)):
         assert decode(lib, kv(**bad)) == EINVAL, bad
         assert window(lib, kv(**bad)) == EINVAL, bad
+    wide = kv(page_rows=1 << 20, n_pages=4)
+    assert decode(lib, wide, width=1 << 11) == EINVAL                        # positions would not fit 32 bits
     for bad in (dict(q=None), dict(q_start=None), dict(n_tokens=-1), dict(n_tokens=1 << 40), dict(n_seqs=4097), dict(ws_bytes=0)):
         assert window(lib, **bad) == EINVAL, bad
     assert decode(lib, n_seqs=0) == 0 and window(lib, n_tokens=0) == 0       # nothing to do, nothing launched
