@@ -170,6 +170,19 @@ __device__ __forceinline__ uint32_t sat_h2(float x, float y) {      // finite va
     y = fabsf(y) < INFINITY ? fminf(fmaxf(y, -65504.f), 65504.f) : y;
     return h2_bits(__floats2half2_rn(x, y));
 }
+__device__ __forceinline__ uint32_t max_bf16x8(uint4 x, uint32_t m) {      // of the magnitudes, in two halves
+    constexpr uint32_t k = 0x7fff7fffu;
+    return __vimax3_s16x2(x.w & k, __vimax3_s16x2(x.y & k, x.z & k, x.x & k), m);
+}
+__device__ __forceinline__ void scale_bf16x8(uint4 &x, float f) {          // f a power of two: exact
+    const __nv_bfloat162 m = __float2bfloat162_rn(f);
+    uint32_t *y = reinterpret_cast<uint32_t *>(&x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<__nv_bfloat162 *>(&y[i]) = __hmul2(*reinterpret_cast<__nv_bfloat162 *>(&y[i]), m);
+}
+__device__ __forceinline__ uint32_t bf16x2_to_f16x2(uint32_t x) {
+    return h2_bits(__floats2half2_rn(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u)));
+}
 // f16 pairs: infinities and NaN become zeros; whether there were any
 template <int N>
 __device__ __forceinline__ bool drop_nonfinite(uint32_t (&o)[N]) {
@@ -430,60 +443,62 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             const uint32_t lanes = (uint32_t)(quarter * 32 + which * 16) << 16;
             unsigned char *stage = p_s + 2 * 8192;                          // 32 rows of 128 dims
             auto sync_all = [&]() { asm volatile("bar.sync 4, 256;" ::: "memory"); };
-            Segment sg, next;
-            bool more = next_segment(next);
+            struct Rows { int64_t row0; int rows, tiles; };
+            auto take = [&](Rows &it) -> bool {
+                Segment sg;
+                if (!next_segment(sg)) return false;
+                it = Rows{sg.it.row0, sg.it.rows, sg.t1 - sg.t0};
+                return true;
+            };
+            Rows cur{0, 0, 0}, next{0, 0, 0};
+            bool more = take(next);
             for (int k = -1;; ++k) {
-                // the query rows of item k + 1: all on their way before the last item's products are through
+                // the query rows of item k + 1, as they are where a lane's largest value is within [2^-4, 2^15], else scaled by a power of two
                 if (more) {
-                    // two rows at a time, 256 contiguous bytes of each; eight lanes of a row make a 128-byte row of the operand
                     uint4 x[4][NB];
-                    uint32_t amax[4] = {0, 0, 0, 0};
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
 #pragma unroll
                         for (int b = 0; b < NB; ++b)
-                            x[j][b] = q_row + 2 * j < next.it.rows ? ld_row16(a.q + (next.it.row0 + q_row + 2 * j) * D + b * 128 + q_lane * 8) : make_uint4(0, 0, 0, 0);
-                    float up[4], down[4];
+                            x[j][b] = q_row + 2 * j < next.rows ? ld_row16(a.q + (next.row0 + q_row + 2 * j) * D + b * 128 + q_lane * 8) : make_uint4(0, 0, 0, 0);
+                    float up[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+                    uint32_t amax[4];
+                    bool far = false;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
+                        amax[j] = 0;
 #pragma unroll
-                        for (int b = 0; b < NB; ++b) {
-                            const uint32_t y[4] = {x[j][b].x, x[j][b].y, x[j][b].z, x[j][b].w};
+                        for (int b = 0; b < NB; ++b) amax[j] = max_bf16x8(x[j][b], amax[j]);
+                        amax[j] = max(amax[j] & 0xffff0000u, amax[j] << 16);
+                        far = far || amax[j] < 0x3d800000u || amax[j] > 0x47000000u;
+                    }
+                    if (__any_sync(0xffffffffu, far))                       // see the rows' largest
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) amax[j] = max(amax[j], max(y[i] & 0x7fff0000u, (y[i] << 16) & 0x7fff0000u));
-                        }
-                        up[j] = down[j] = 1.0f;
-                        const bool far = amax[j] < 0x3d800000u || amax[j] > 0x47000000u;
-                        if (__any_sync(0xffffffffu, far)) {                 // a lane's values are far from one: see the whole row's largest
+                        for (int j = 0; j < 4; ++j) {
+                            float down = 1.0f;
 #pragma unroll
                             for (int o = 1; o < 32; o <<= 1)
                                 if (o != 8) amax[j] = max(amax[j], __shfl_xor_sync(0xffffffffu, amax[j], o));
-                            if (amax[j] != 0 && (amax[j] < 0x3d800000u || amax[j] > 0x47000000u)) pow2_parts(__uint_as_float(amax[j]), up[j], down[j]);
+                            if (amax[j] != 0 && (amax[j] < 0x3d800000u || amax[j] > 0x47000000u)) pow2_parts(__uint_as_float(amax[j]), up[j], down);
+#pragma unroll
+                            for (int b = 0; b < NB; ++b) scale_bf16x8(x[j][b], down);
                         }
-                    }
                     tc::wait(DS4B200_BAR(q_free, 0), (uint32_t)(((k + 1) & 1) ^ 1), abort_flag, status);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int rw = q_row + 2 * j;
 #pragma unroll
-                        for (int b = 0; b < NB; ++b) {
-                            const uint32_t y[4] = {x[j][b].x, x[j][b].y, x[j][b].z, x[j][b].w};
-                            uint32_t o[4];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                o[i] = h2_bits(__floats2half2_rn(__uint_as_float(y[i] << 16) * down[j], __uint_as_float(y[i] & 0xffff0000u) * down[j]));
+                        for (int b = 0; b < NB; ++b)
                             *reinterpret_cast<uint4 *>(q_s + (2 * b + (q_lane >> 3)) * 8192 + rw * 128 + (((uint32_t)(q_lane & 7) ^ (uint32_t)(rw & 7)) << 4)) =
-                                make_uint4(o[0], o[1], o[2], o[3]);
-                        }
+                                make_uint4(bf16x2_to_f16x2(x[j][b].x), bf16x2_to_f16x2(x[j][b].y), bf16x2_to_f16x2(x[j][b].z), bf16x2_to_f16x2(x[j][b].w));
                         if (q_lane == 0) q_mul[(k + 1) & (kScaleSets - 1)][rw] = up[j] * a.scale * kLog2e;
                     }
                     __syncwarp();
                     if (lane == 0) tc::arrive(DS4B200_BAR(q_full, 0));
                 }
-                // item k's accumulators
-                if (k >= 0) {
+                if (k >= 0) {                                               // item k's accumulators
                     tc::wait(DS4B200_BAR(o_ready, k & (kScaleSets - 1)), (uint32_t)((k / kScaleSets) & 1), abort_flag, status);
-                    const int last = drained + sg.t1 - sg.t0 - 1;           // its last tile
+                    const int last = drained + cur.tiles - 1;               // its last tile
                     drained = last + 1;
                     tc::wait(DS4B200_BAR(pv_done, (last & 1) * 2 + kParts - 1), (uint32_t)((last >> 1) & 1), abort_flag, status);
                     tc::fence_after();
@@ -500,35 +515,38 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                         }
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {                       // 32 rows
-                            if (h * 32 >= sg.it.rows) continue;
+                            if (h * 32 >= cur.rows) continue;
                             sync_all();                                     // the stage is free
 #pragma unroll
                             for (int i = 0; i < 4; i += 2) {
-                                const float2 f0 = *reinterpret_cast<const float2 *>(&inv_s[k & (kScaleSets - 1)][h * 32 + 8 * i + 2 * (lane & 3)]);
-                                const float2 f1 = *reinterpret_cast<const float2 *>(&inv_s[k & (kScaleSets - 1)][h * 32 + 8 * i + 8 + 2 * (lane & 3)]);
-                                const uint32_t *y = &o[16 * h + 4 * i];
-                                const uint32_t w0 = h2b(__uint_as_float(y[0]) * f0.x, __uint_as_float(y[1]) * f0.y);
-                                const uint32_t w1 = h2b(__uint_as_float(y[2]) * f0.x, __uint_as_float(y[3]) * f0.y);
-                                const uint32_t w2 = h2b(__uint_as_float(y[4]) * f1.x, __uint_as_float(y[5]) * f1.y);
-                                const uint32_t w3 = h2b(__uint_as_float(y[6]) * f1.x, __uint_as_float(y[7]) * f1.y);
+                                uint32_t w[4];
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    const float2 f = *reinterpret_cast<const float2 *>(&inv_s[k & (kScaleSets - 1)][h * 32 + 8 * (i + e) + 2 * (lane & 3)]);
+                                    const uint32_t *y = &o[16 * h + 4 * (i + e)];
+                                    const float2 y0 = mul2(make_float2(__uint_as_float(y[0]), __uint_as_float(y[1])), f);
+                                    const float2 y1 = mul2(make_float2(__uint_as_float(y[2]), __uint_as_float(y[3])), f);
+                                    w[2 * e] = h2b(y0.x, y0.y);
+                                    w[2 * e + 1] = h2b(y1.x, y1.y);
+                                }
                                 const int rw = 8 * (i + (lane >> 4)) + (lane & 7), unit = quarter * 4 + which * 2 + ((lane >> 3) & 1);
                                 asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};"
-                                             ::"r"(smem_addr(stage) + rw * 256 + ((unit ^ (rw & 7)) << 4)), "r"(w0), "r"(w1), "r"(w2), "r"(w3) : "memory");
+                                             ::"r"(smem_addr(stage) + rw * 256 + ((unit ^ (rw & 7)) << 4)), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
                             }
                             sync_all();
 #pragma unroll
                             for (int i = 0; i < 2; ++i) {
                                 const int rw = i * 16 + lw * 2 + (lane >> 4), unit = lane & 15;
-                                if (h * 32 + rw < sg.it.rows)
-                                    __stcs(reinterpret_cast<uint4 *>(a.out + (sg.it.row0 + h * 32 + rw) * D + b * 128 + unit * 8),
+                                if (h * 32 + rw < cur.rows)
+                                    __stcs(reinterpret_cast<uint4 *>(a.out + (cur.row0 + h * 32 + rw) * D + b * 128 + unit * 8),
                                            *reinterpret_cast<const uint4 *>(stage + rw * 256 + ((unit ^ (rw & 7)) << 4)));
                             }
                         }
                     }
                 }
                 if (!more) break;
-                sg = next;
-                more = next_segment(next);
+                cur = next;
+                more = take(next);
             }
         } else {
         uint4 v[kRegs];                                  // [step][row pair]
@@ -888,16 +906,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                         // one prefetch per run of neighbours in the pool: 64 of them a tile kept the copy engine busier than the loaders
                         const int before = __shfl_up_sync(0xffffffffu, slot[h], 1);
                         const uint32_t heads = __ballot_sync(0xffffffffu, lane == 0 || slot[h] < 0 || slot[h] != before + 1);
-                        if ((heads >> lane & 1) && slot[h] >= 0) {
+                        if (!kF32 && (heads >> lane & 1) && slot[h] >= 0) {     // f32 rows: 2 KiB of loads in flight a row do better alone (96 sequences 82 us, 68)
                             const uint32_t behind = lane == 31 ? 0 : heads >> (lane + 1);
                             const int run = behind ? __ffs(behind) : 32 - lane;
                             const int64_t sl = slot[h];
-                            if (kF32) {
-                                prefetch_l2(a.kv.raw + sl * D, run * D * 4);
-                            } else {
-                                prefetch_l2(a.kv.codes + sl * D, run * D);
-                                if (tail) prefetch_l2(a.kv.tail + sl * 64, run * 256);
-                            }
+                            prefetch_l2(a.kv.codes + sl * D, run * D);
+                            if (tail) prefetch_l2(a.kv.tail + sl * 64, run * 256);
                         }
                     }
                     if (more && t == sg.t0 && lane == 0) prefetch_l2(a.q + sg.it.row0 * D, sg.it.rows * D * 2);    // the segment's query rows
@@ -973,8 +987,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 const float *fac = nullptr;              // of the tile's packed rows
                 if (kPre) fac = g.fac + (t < first_run_tiles(it) ? it.at_a + 64 * t : it.at_b + 64 * (t - first_run_tiles(it)));
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    v[i] = mul2(make_float2(__uint_as_float(group ? x[4 * i + 2] : x[4 * i]), __uint_as_float(group ? x[4 * i + 3] : x[4 * i + 1])), k2);
+                for (int i = 0; i < 8; ++i) {
+                    if (group) v[i] = mul2(make_float2(__uint_as_float(x[4 * i + 2]), __uint_as_float(x[4 * i + 3])), k2);
+                    else v[i] = mul2(make_float2(__uint_as_float(x[4 * i]), __uint_as_float(x[4 * i + 1])), k2);
+                }
                 if (odd) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {                          // column block i is loader i's
