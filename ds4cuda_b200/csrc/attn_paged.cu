@@ -383,9 +383,42 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         const bool tail = kBlock && a.kv.n_rot != 0;
         const int n_scales = kBlock ? (D - a.kv.n_rot) / 64 : 1;
         const int q_row = lw * 8 + ((lane >> 3) & 1), q_lane = (lane & 7) | ((lane >> 4) << 3);     // rows q_row + 2 j, 16 of their bytes
+        // The query rows: two at a time, 256 contiguous bytes of each, eight lanes of a row making a 128-byte row of the operand.
+        auto query_16 = [&](int64_t row0, int rows, int j, int b) {
+            return q_row + 2 * j < rows ? ld_row16(a.q + (row0 + q_row + 2 * j) * D + b * 128 + q_lane * 8) : make_uint4(0, 0, 0, 0);
+        };
+        auto store_query = [&](const uint4 &x, int j, int b) {
+            const int rw = q_row + 2 * j;
+            *reinterpret_cast<uint4 *>(q_s + (2 * b + (q_lane >> 3)) * 8192 + rw * 128 + (((uint32_t)(q_lane & 7) ^ (uint32_t)(rw & 7)) << 4)) =
+                make_uint4(bf16x2_to_f16x2(x.x), bf16x2_to_f16x2(x.y), bf16x2_to_f16x2(x.z), bf16x2_to_f16x2(x.w));
+        };
+        // Whether a row's largest value (in amax as two halves per lane) is so far from one that it is scaled; then up and down are its scale.
+        auto query_scales = [&](uint32_t (&amax)[4], float (&up)[4], float (&down)[4]) -> bool {
+            bool far = false;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                amax[j] = max(amax[j] & 0xffff0000u, amax[j] << 16);
+                far = far || amax[j] < 0x3d800000u || amax[j] > 0x47000000u;
+            }
+            if (!__any_sync(0xffffffffu, far)) return false;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1)
+                    if (o != 8) amax[j] = max(amax[j], __shfl_xor_sync(0xffffffffu, amax[j], o));
+                if (amax[j] != 0 && (amax[j] < 0x3d800000u || amax[j] > 0x47000000u)) pow2_parts(__uint_as_float(amax[j]), up[j], down[j]);
+            }
+            return true;
+        };
+        auto set_query_scales = [&](const float (&up)[4], int nq) {
+            if (q_lane == 0)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) q_mul[nq & (kScaleSets - 1)][q_row + 2 * j] = up[j] * a.scale * kLog2e;
+            __syncwarp();
+            if (lane == 0) tc::arrive(DS4B200_BAR(q_full, 0));
+        };
         auto load_query = [&](int64_t row0, int rows, int nq) {
-            // two rows at a time, 256 contiguous bytes of each; as they are where a row's largest value is within [2^-4, 2^15], else
-            // scaled by a power of two in a second pass
+            // half a row's dims at a time, as they are where its largest value is within [2^-4, 2^15], else scaled by a power of two in a second pass
             float up[4] = {1.0f, 1.0f, 1.0f, 1.0f}, down[4] = {1.0f, 1.0f, 1.0f, 1.0f};
 #pragma unroll 1
             for (int pass = 0; pass < 2; ++pass) {
@@ -396,46 +429,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
 #pragma unroll
-                        for (int b = 0; b < 2; ++b)
-                            x[j][b] = q_row + 2 * j < rows && b0 + b < NB ? ld_row16(a.q + (row0 + q_row + 2 * j) * D + (b0 + b) * 128 + q_lane * 8)
-                                                                          : make_uint4(0, 0, 0, 0);
+                        for (int b = 0; b < 2; ++b) x[j][b] = b0 + b < NB ? query_16(row0, rows, j, b0 + b) : make_uint4(0, 0, 0, 0);
                     if (pass == 0 && b0 == 0) tc::wait(DS4B200_BAR(q_free, 0), (uint32_t)((nq & 1) ^ 1), abort_flag, status);
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
 #pragma unroll
                         for (int b = 0; b < 2; ++b) {
-                            const int rw = q_row + 2 * j;
-                            const uint32_t y[4] = {x[j][b].x, x[j][b].y, x[j][b].z, x[j][b].w};
-                            uint32_t o[4];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                amax[j] = max(amax[j], max(y[i] & 0x7fff0000u, (y[i] << 16) & 0x7fff0000u));
-                                o[i] = h2_bits(__floats2half2_rn(__uint_as_float(y[i] << 16) * down[j], __uint_as_float(y[i] & 0xffff0000u) * down[j]));
-                            }
-                            if (b0 + b < NB)
-                                *reinterpret_cast<uint4 *>(q_s + (2 * (b0 + b) + (q_lane >> 3)) * 8192 + rw * 128 + (((uint32_t)(q_lane & 7) ^ (uint32_t)(rw & 7)) << 4)) =
-                                    make_uint4(o[0], o[1], o[2], o[3]);
+                            amax[j] = max_bf16x8(x[j][b], amax[j]);
+                            scale_bf16x8(x[j][b], down[j]);
+                            if (b0 + b < NB) store_query(x[j][b], j, b0 + b);
                         }
                 }
-                if (pass) break;
-                bool far = false;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-#pragma unroll
-                    for (int o = 1; o < 32; o <<= 1)
-                        if (o != 8) amax[j] = max(amax[j], __shfl_xor_sync(0xffffffffu, amax[j], o));
-                    if (amax[j] != 0 && (amax[j] < 0x3d800000u || amax[j] > 0x47000000u)) {
-                        pow2_parts(__uint_as_float(amax[j]), up[j], down[j]);
-                        far = true;
-                    }
-                }
-                if (!__any_sync(0xffffffffu, far)) break;
+                if (pass || !query_scales(amax, up, down)) break;
             }
-            if (q_lane == 0)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) q_mul[nq & (kScaleSets - 1)][q_row + 2 * j] = up[j] * a.scale * kLog2e;
-            __syncwarp();
-            if (lane == 0) tc::arrive(DS4B200_BAR(q_full, 0));
+            set_query_scales(up, nq);
         };
         if (kPre) {
             // With packed rows these warps fetch the query rows and drain the accumulators, one item apart, while the softmax goes on.
@@ -456,45 +463,27 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 // the query rows of item k + 1, as they are where a lane's largest value is within [2^-4, 2^15], else scaled by a power of two
                 if (more) {
                     uint4 x[4][NB];
+                    uint32_t amax[4] = {0, 0, 0, 0};
+                    float up[4] = {1.0f, 1.0f, 1.0f, 1.0f}, down[4] = {1.0f, 1.0f, 1.0f, 1.0f};
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
 #pragma unroll
-                        for (int b = 0; b < NB; ++b)
-                            x[j][b] = q_row + 2 * j < next.rows ? ld_row16(a.q + (next.row0 + q_row + 2 * j) * D + b * 128 + q_lane * 8) : make_uint4(0, 0, 0, 0);
-                    float up[4] = {1.0f, 1.0f, 1.0f, 1.0f};
-                    uint32_t amax[4];
-                    bool far = false;
+                        for (int b = 0; b < NB; ++b) x[j][b] = query_16(next.row0, next.rows, j, b);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        amax[j] = 0;
+                    for (int j = 0; j < 4; ++j)
 #pragma unroll
                         for (int b = 0; b < NB; ++b) amax[j] = max_bf16x8(x[j][b], amax[j]);
-                        amax[j] = max(amax[j] & 0xffff0000u, amax[j] << 16);
-                        far = far || amax[j] < 0x3d800000u || amax[j] > 0x47000000u;
-                    }
-                    if (__any_sync(0xffffffffu, far))                       // see the rows' largest
+                    if (query_scales(amax, up, down))
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            float down = 1.0f;
+                        for (int j = 0; j < 4; ++j)
 #pragma unroll
-                            for (int o = 1; o < 32; o <<= 1)
-                                if (o != 8) amax[j] = max(amax[j], __shfl_xor_sync(0xffffffffu, amax[j], o));
-                            if (amax[j] != 0 && (amax[j] < 0x3d800000u || amax[j] > 0x47000000u)) pow2_parts(__uint_as_float(amax[j]), up[j], down);
-#pragma unroll
-                            for (int b = 0; b < NB; ++b) scale_bf16x8(x[j][b], down);
-                        }
+                            for (int b = 0; b < NB; ++b) scale_bf16x8(x[j][b], down[j]);
                     tc::wait(DS4B200_BAR(q_free, 0), (uint32_t)(((k + 1) & 1) ^ 1), abort_flag, status);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int rw = q_row + 2 * j;
+                    for (int j = 0; j < 4; ++j)
 #pragma unroll
-                        for (int b = 0; b < NB; ++b)
-                            *reinterpret_cast<uint4 *>(q_s + (2 * b + (q_lane >> 3)) * 8192 + rw * 128 + (((uint32_t)(q_lane & 7) ^ (uint32_t)(rw & 7)) << 4)) =
-                                make_uint4(bf16x2_to_f16x2(x[j][b].x), bf16x2_to_f16x2(x[j][b].y), bf16x2_to_f16x2(x[j][b].z), bf16x2_to_f16x2(x[j][b].w));
-                        if (q_lane == 0) q_mul[(k + 1) & (kScaleSets - 1)][rw] = up[j] * a.scale * kLog2e;
-                    }
-                    __syncwarp();
-                    if (lane == 0) tc::arrive(DS4B200_BAR(q_full, 0));
+                        for (int b = 0; b < NB; ++b) store_query(x[j][b], j, b);
+                    set_query_scales(up, k + 1);
                 }
                 if (k >= 0) {                                               // item k's accumulators
                     tc::wait(DS4B200_BAR(o_ready, k & (kScaleSets - 1)), (uint32_t)((k / kScaleSets) & 1), abort_flag, status);
