@@ -21,31 +21,42 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // ------------------------------------------------------------------------------------- tensor cores
 //
-// An item is up to 64 query rows that share their cache rows: the heads of one token (of up to 64 / n_heads tokens,
-// when a chunk's heads are few).  A CTA walks over tiles of 64 cache rows:
-//   * eight warps load the tile's rows through the page table, turn them into f16 and store them once, as 128-byte
-//     rows of 64 dims with the 128-byte swizzle.  The same bytes serve both products: as the K-major B operand of
-//     S = Q K^T and as the M-contiguous A operand of O^T += V^T P^T, since a key row is its value row;
-//   * one thread issues the MMAs: S (M 64 query rows, N 64 cache rows, K head_dim) and, per 128 dims of the output,
-//     O^T (M 128 dims, N query rows, K 64 cache rows).  O^T takes 64 tensor-memory columns per 128 dims, so 512 dims and two S
-//     buffers fit; O itself (64 rows in 512 columns) would leave no room for S;
-//   * four warps take S from tensor memory, one query row per lane, keep the running maximum and sum of the softmax in f32,
-//     and leave the weights as f16 (relative error 2^-12) in shared memory.  The accumulators are rescaled only when a
-//     row's maximum has grown by more than 2^8 since its last reference, which later tiles rarely bring.
-// S of tile n + 1 is issued ahead of O^T of tile n, so the tensor cores work while the softmax of a tile runs.
+// An item is up to 64 query rows that share their cache rows: the heads of one token (of up to 64 / n_heads tokens, when a chunk's
+// heads are few).  A CTA walks over tiles of 64 cache rows, with a role for each of its 20 warps:
+//   * eight load the tile's rows, turn them into f16 and store them once, as 128-byte rows of 64 dims with the 128-byte
+//     swizzle.  The same bytes serve both products: as the K-major B operand of S = Q K^T and as the M-contiguous A
+//     operand of O^T += V^T P^T, since a key row is its value row;
+//   * one issues S (M 64 query rows, N 64 cache rows, K head_dim), one, per 128 dims of the output, O^T (M 128 dims, N 64 query rows,
+//     K 64 cache rows).  O^T takes 64 tensor-memory columns per 128 dims, so 512 dims and two S buffers fit; O itself (64
+//     rows, 512 columns) would leave no room for S.  S of tile n + 1 is issued ahead of O^T of tile n, so the tensor
+//     cores work while the softmax of a tile runs;
+//   * eight take S from tensor memory, keep the running maximum and sum of the softmax in f32, and leave the weights as f16 (half a
+//     step: 2^-12 of each) in shared memory.  The accumulators are rescaled only when a row's maximum has grown by more
+//     than 2^8 since its last reference, which later tiles rarely bring;
+//   * one hands out the items, one looks the tiles' rows up in the page table and touches them ahead of the loads.
 //
-// Scales.  A cache row is a row factor times f16 numbers: E4M3 codes themselves with the row's scale; codes times their
-// block's scale relative to the row's largest power of two (exact, the scales are powers of two) with the f32 tail likewise; f32 rows as they are.
-// The factor r_j enters the scores, and as log2 r_j the exponent of the weights, so that P holds r_j exp(s_j - M) <= 1
-// and the sum takes P / r_j back.  A query row is scaled by a power of two, which loses nothing of bf16's 8 bits in f16.
+// Scales.  A cache row is a row factor times f16 numbers.  Rows of ordinary size have the factor 1: codes times a scale that is
+// a power of two are exact in f16, codes times another scale are rounded (2^-11), as f32 rows are.  A row whose
+// scale or tail is far from one keeps a factor r_j, which enters the scores, and as log2 r_j the exponent of the weights,
+// so that P holds r_j exp(s_j - M) <= 1 and the sum takes P / r_j back.  A query row is scaled by a power of two, which
+// loses nothing of bf16's 8 bits in f16.
 //
-// Work.  With few items the list of all tiles is cut into equal runs, one per CTA; an item that several CTAs share leaves
-// partial sums (f32 O^T, M and l) that attn_join_kernel adds in order.  With many items each CTA takes whole ones.
+// Work.  Where items are long and few the list of all tiles is cut into equal runs, one per CTA; an item that several CTAs share
+// leaves partial sums (f32 O^T, M and l) that attn_join_kernel adds in order.  Else each CTA takes whole items.  A chunk of
+// kPackTokens or more has its rows packed as f16 once (attn_pack_kernel); a tile is then eight TMA boxes, and the loaders
+// fetch query rows and drain O^T instead, beside the softmax of the next item.
+//
+// Bound.  Shared memory: a tile of 512 dims is 64 KiB written and, by the MMAs, 224 KiB read at 128 bytes a cycle (1792 cycles; an MMA
+// of M 64, N 64, K 16 reads 4 KiB in 32), which with the loads' own pass through L1, the weights and the query rows makes 2700 to
+// 2900 cycles a tile; from HBM a tile of FP8 rows needs 1400, of f32 rows 5600.  Halves of that traffic would need the codes
+// themselves as operands, and the weights as two or three 8-bit pieces.  Measured (64 heads, 512 dims): one session of 131072
+// rows, codes with a tail, 62 us (77 MB: 1.25 TB/s, 15 us at 6566 GB/s); 64 sequences of 1 to 8192 FP8 rows 94 us (162 MB, 1.7 TB/s);
+// 96 sequences of 16 heads, window 128 + 64 first f32 rows 64 us (75 MB of distinct rows ...).
 constexpr int kCtas = 148;
 constexpr int kRows = 64;                   // query rows of an item, cache rows of a tile
 constexpr int kSoftWarps = 8, kLoadWarp0 = 8, kLoadWarps = 8, kMmaWarp = 16;
-constexpr int kThreads = 20 * 32;            
-constexpr int kSplitItems = 4 * kCtas;
+constexpr int kThreads = 20 * 32;
+constexpr int kSplitItems = 4 * kCtas;      // more of them are not cut
 constexpr int kWholeTiles = 3;              // items of up to so many tiles are not cut
 constexpr int kPackTokens = 64;             // of a chunk whose rows are packed first
 constexpr int kMinTiles = 2;                // of a run: below, the join costs more than the run saves
@@ -216,7 +227,7 @@ constexpr int kSegReaders = kSoftWarps + 3;  // and the loaders with packed rows
 constexpr int kPackCtas = 4 * kCtas, kPackWarps = 8;
 
 struct alignas(64) TcArgs {
-    CUtensorMap rows;                       // packed f16 rows [packed rows][head_dim], boxes of 64 rows x 64 dims
+    CUtensorMap rows, few;                  // packed f16 rows [packed rows][head_dim], boxes of 64 rows x 64 dims, and of 16 rows
     const float *fac;                       // a factor for each (0: a hole, NaN: a value that is not finite)
     const int *odd;                         // kPackCtas: whether a CTA of the packing has met a factor other than 1
     AttnArgs a;
@@ -257,7 +268,7 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 
 struct Bars {
-    uint64_t full[2][2], s_full[2], s_free[2], p_full[2], pv_done[2][2], scaled[2], q_full, q_free, o_ready[kScaleSets], o_free, quiet[2];
+    uint64_t full[2][2], s_full[2], s_free[2], p_full[2], pv_done[2][2], scaled[2], q_full, q_free, o_ready[kScaleSets], o_half, o_free[2], quiet[2];
     uint64_t seg_full[kSegRing], seg_free[kSegRing], tile_full[kTileRing], tile_free[kTileRing];
 };
 
@@ -266,7 +277,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     constexpr int D = NB * 128, kChunks = NB * 2, kTileBytes = kRows * D * 2;
     constexpr int kParts = NB > 2 ? 2 : 1, kPart0 = 2;                 // a tile is handed over in parts: its first 256 dims, the rest
     constexpr bool kPre = FMT == kPacked;
-    constexpr uint32_t o_tmem = kTmem, s_tmem = kTmem + NB * 64;
+    // Tensor memory: six blocks of 64 columns for O^T, two for S.  With packed rows the items go round the six blocks, so that the
+    // products of the next item begin while the last one's accumulators are read: with 512 dims its first two blocks are free
+    // at once, the others when two have been read.
+    constexpr int kOBlocks = 6, kFree = kOBlocks - NB;
+    constexpr uint32_t o_tmem = kTmem, s_tmem = kTmem + kOBlocks * 64;
+    auto o_block = [](int base, int b) -> uint32_t { return o_tmem + (uint32_t)(base + b >= kOBlocks ? base + b - kOBlocks : base + b) * 64; };
+    auto next_base = [](int base) { return !kPre ? 0 : base + NB >= kOBlocks ? base + NB - kOBlocks : base + NB; };
     const AttnArgs &a = g.a;
     extern __shared__ __align__(1024) unsigned char smem[];
     unsigned char *q_s = smem, *k_s = smem + kTileBytes, *p_s = smem + 3 * kTileBytes;
@@ -298,14 +315,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         start_tile = 0;
         for (int i = 0; i < 2; ++i) {
             grown_s[i] = odd_s[i] = 0;
-            mbar_init(&bars_s.quiet[i], 1);
+            mbar_init(&bars_s.quiet[i], 1); mbar_init(&bars_s.o_free[i], kLoadWarps);
             for (int k = 0; k < kLoadWarps; ++k) odd_w[i][k] = 0;
             mbar_init(&bars_s.scaled[i], kSoftWarps);
             mbar_init(&bars_s.s_full[i], 1); mbar_init(&bars_s.s_free[i], kSoftWarps); mbar_init(&bars_s.p_full[i], kSoftWarps);
             for (int k = 0; k < kParts; ++k) { mbar_init(&bars_s.full[i][k], kPre ? 1 : kLoadWarps); mbar_init(&bars_s.pv_done[i][k], 1); }
         }
         mbar_init(&bars_s.q_full, kLoadWarps); mbar_init(&bars_s.q_free, 1);
-        mbar_init(&bars_s.o_free, kLoadWarps);
+        mbar_init(&bars_s.o_half, kLoadWarps);
         // four items: the softmax may be that far ahead of the drain before a product has to wait for it
         for (int i = 0; i < kScaleSets; ++i) mbar_init(&bars_s.o_ready[i], kSoftWarps);
         for (int i = 0; i < kTileRing; ++i) { mbar_init(&bars_s.tile_full[i], 1); mbar_init(&bars_s.tile_free[i], kLoadWarps); }
@@ -458,6 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 return true;
             };
             Rows cur{0, 0, 0}, next{0, 0, 0};
+            int base = 0;
             bool more = take(next);
             for (int k = -1;; ++k) {
                 // the query rows of item k + 1, as they are where a lane's largest value is within [2^-4, 2^15], else scaled by a power of two
@@ -495,12 +513,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 #pragma unroll 1
                     for (int b = 0; b < NB; ++b) {
                         uint32_t o[32];
-                        tc::ld_16x64(o_tmem + b * 64 + lanes, o);
+                        tc::ld_16x64(o_block(base, b) + lanes, o);
                         tc::wait_ld();
-                        if (b + 1 == NB) {                                  // the next item's products may begin
+                        if (b + 1 == NB || b + 1 == NB - kFree) {
                             tc::fence_before();
                             __syncwarp();
-                            if (lane == 0) tc::arrive(DS4B200_BAR(o_free, 0));
+                            if (lane == 0) tc::arrive(b + 1 == NB ? DS4B200_BAR(o_free, k & 1) : DS4B200_BAR(o_half, 0));
                         }
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {                       // 32 rows
@@ -534,6 +552,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     }
                 }
                 if (!more) break;
+                if (k >= 0) base = next_base(base);
                 cur = next;
                 more = take(next);
             }
@@ -774,9 +793,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             auto scaled_phase = [&](int b) { return scaled_uses[b]++ & 1; };
             Segment sg;
             int n = 0;
-            for (int k = 0; next_segment(sg); ++k) {
+            int base = 0;
+            for (int k = 0; next_segment(sg); ++k, base = next_base(base)) {
                 const int t0 = __shfl_sync(0xffffffffu, sg.t0, 0), t1 = __shfl_sync(0xffffffffu, sg.t1, 0);
-                if (kPre && k > 0) tc::wait<20>(DS4B200_BAR(o_free, 0), (uint32_t)((k - 1) & 1), abort_flag, status);
+                if (kPre && k > 1) tc::wait<20>(DS4B200_BAR(o_free, k & 1), (uint32_t)(((k - 2) >> 1) & 1), abort_flag, status);
                 const int n_rows = __shfl_sync(0xffffffffu, sg.it.n, 0), na = __shfl_sync(0xffffffffu, sg.it.na, 0), ta = (na + 63) >> 6;
                 for (int t = t0; t < t1; ++t, ++n) {
                     const int buf = n & 1;
@@ -788,10 +808,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     tc::fence_after();
 #pragma unroll 1
                     for (int m = 0; m < NB; ++m) {
+                        if (kPre && kFree < NB && m == kFree && t == t0 && k > 0) {
+                            tc::wait<20>(DS4B200_BAR(o_half, 0), (uint32_t)((k - 1) & 1), abort_flag, status);
+                            tc::fence_after();
+                        }
+                        const uint32_t o_m = __shfl_sync(0xffffffffu, o_block(base, m), 0);
 #pragma unroll
                         for (int ks = 0; ks < 4; ++ks)
                             if (ks < groups)
-                                tc::mma_f16(one, o_tmem + m * 64, v0 + (uint32_t)(m * 1024 + ks * 128), p0 + (uint32_t)(ks * 2), idesc, t > t0 || ks > 0);
+                                tc::mma_f16(one, o_m, v0 + (uint32_t)(m * 1024 + ks * 128), p0 + (uint32_t)(ks * 2), idesc, t > t0 || ks > 0);
                         if (kParts > 1 && m == kPart0 - 1) tc::commit(one, DS4B200_BAR(pv_done, (buf) * 2 + (0)));
                     }
                     tc::commit(one, DS4B200_BAR(pv_done, (buf) * 2 + (kParts - 1)));
@@ -838,15 +863,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 for (int t = sg.t0; t < sg.t1; ++t, ++n) {
                     const int buf = n & 1, ta = first_run_tiles(sg.it);
                     const int from = t < ta ? sg.it.at_a + 64 * t : sg.it.at_b + 64 * (t - ta);
+                    // up to 16 rows (the MMAs read no more of them either): a window of 128 and 4 first rows ...
+                    const bool few = rows_in_tile(sg.it, t) <= 16;
 #pragma unroll
                     for (int part = 0; part < kParts; ++part) {
                         tc::wait<20>(DS4B200_BAR(pv_done, buf * 2 + part), (uint32_t)(((n >> 1) & 1) ^ 1), abort_flag, status);
                         if (lane == 0) {
                             constexpr int kFirst = kParts > 1 ? 2 * kPart0 : kChunks;
                             const int c0 = part * kFirst, c1 = part ? kChunks : kFirst;
-                            tc::expect(DS4B200_BAR(full, buf * 2 + part), (uint32_t)(c1 - c0) * 8192u);
+                            tc::expect(DS4B200_BAR(full, buf * 2 + part), (uint32_t)(c1 - c0) * (few ? 2048u : 8192u));
                             for (int c = c0; c < c1; ++c)
-                                tc::load_box(smem_addr(k_s) + buf * kTileBytes + c * 8192, &g.rows, c * 64, from, DS4B200_BAR(full, buf * 2 + part));
+                                tc::load_box(smem_addr(k_s) + buf * kTileBytes + c * 8192, few ? &g.few : &g.rows, c * 64, from, DS4B200_BAR(full, buf * 2 + part));
                         }
                         __syncwarp();
                     }
@@ -926,7 +953,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         Segment sg;
         int n = 0;
         long long done = 0;
-        for (int nq = 0; next_segment(sg); ++nq) {
+        int base = 0;
+        for (int nq = 0; next_segment(sg); ++nq, base = next_base(base)) {
             const Item &it = sg.it;
             float qk = 0.0f, m = -INFINITY;
             float2 l = make_float2(0.0f, 0.0f);
@@ -941,11 +969,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 #pragma unroll 1
                 for (int u = group; u < NB * 4; u += 2) {
                     uint32_t o[16];
-                    tc::ld16(o_tmem + u * 16 + lane_base, o);
+                    const uint32_t at = o_block(base, u >> 2) + (u & 3) * 16 + lane_base;
+                    tc::ld16(at, o);
                     tc::wait_ld();
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fac_s[buf][(u & 3) * 16 + i]);
-                    tc::st16(o_tmem + u * 16 + lane_base, o);
+                    tc::st16(at, o);
                 }
                 tc::wait_st();
                 tc::fence_before();
@@ -1308,7 +1337,7 @@ __global__ void __launch_bounds__(kPackWarps * 32) attn_pack_kernel(const AttnAr
     if (threadIdx.x == 0) odd[blockIdx.x] = met;
 }
 
-bool packed_map(CUtensorMap *map, const uint16_t *rows, int64_t n, int dim) {
+bool packed_map(CUtensorMap *map, const uint16_t *rows, int64_t n, int dim, int box_rows) {
     using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                                   const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -1324,7 +1353,7 @@ bool packed_map(CUtensorMap *map, const uint16_t *rows, int64_t n, int dim) {
     });
     if (!encode) return false;
     const cuuint64_t dims[2] = {(cuuint64_t)dim, (cuuint64_t)n}, strides[1] = {(cuuint64_t)dim * 2};
-    const cuuint32_t box[2] = {64, 64}, elem[2] = {1, 1};
+    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows}, elem[2] = {1, 1};
     return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<uint16_t *>(rows), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -1371,7 +1400,8 @@ void launch_fmt(const AttnArgs &a, cudaStream_t s) {
     static_assert(kPackCtas * sizeof(int) <= kMetaBytes && kPackRows * sizeof(float) <= kMlBytes && kPackCtas <= kThreads, "room for packed rows");
     const int64_t bound = (a.window > 0 ? a.n_tokens : 0) + a.n_seqs * packed_gap(a.window, a.n_first, all_rows);
     uint16_t *rows = reinterpret_cast<uint16_t *>(g.part_o);
-    if (a.q_start && !g.split && a.n_tokens >= kPackTokens && bound <= kPackRows && packed_map(&g.rows, rows, bound, a.kv.head_dim)) {
+    if (a.q_start && !g.split && a.n_tokens >= kPackTokens && bound <= kPackRows && packed_map(&g.rows, rows, bound, a.kv.head_dim, 64) &&
+        packed_map(&g.few, rows, bound, a.kv.head_dim, 16)) {
         g.fac = reinterpret_cast<const float *>(g.part_ml);
         g.odd = reinterpret_cast<const int *>(ws);
         attn_pack_kernel<NB><<<kPackCtas, kPackWarps * 32, 0, s>>>(a, bound, rows, reinterpret_cast<float *>(g.part_ml), reinterpret_cast<int *>(ws));
