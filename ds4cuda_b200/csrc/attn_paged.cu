@@ -42,9 +42,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 // loses nothing of bf16's 8 bits in f16.
 //
 // Work.  Where items are long and few the list of all tiles is cut into equal runs, one per CTA; an item that several CTAs share
-// leaves partial sums (f32 O^T, M and l) that attn_join_kernel adds in order.  Else each CTA takes whole items.  A chunk of
-// kPackTokens or more has its rows packed as f16 once (attn_pack_kernel); a tile is then eight TMA boxes, and the loaders
-// fetch query rows and drain O^T instead, beside the softmax of the next item.
+// leaves partial sums (f32 O^T, M and l) that attn_join_kernel adds in order.  Else each CTA takes whole items.  Of a chunk the rows
+// may be packed as f16 once (attn_pack_kernel); a tile is then eight TMA boxes, and the loaders fetch query rows and drain
+// O^T instead, beside the softmax of the next item.
 //
 // Bound.  Shared memory: a tile of 512 dims is 64 KiB written and, by the MMAs, 224 KiB read at 128 bytes a cycle (1792 cycles; an MMA
 // of M 64, N 64, K 16 reads 4 KiB in 32), which with the loads' own pass through L1, the weights and the query rows makes 2700 to
@@ -58,7 +58,6 @@ constexpr int kSoftWarps = 8, kLoadWarp0 = 8, kLoadWarps = 8, kMmaWarp = 16;
 constexpr int kThreads = 20 * 32;
 constexpr int kSplitItems = 4 * kCtas;      // more of them are not cut
 constexpr int kWholeTiles = 3;              // items of up to so many tiles are not cut
-constexpr int kPackTokens = 64;             // of a chunk whose rows are packed first
 constexpr int kMinTiles = 2;                // of a run: below, the join costs more than the run saves
 constexpr float kRescale = 8.0f;            // log2 units
 constexpr int kScaleSets = 4;
@@ -220,7 +219,7 @@ struct Segment {
     Item it;
     int t0, t1;
 };
-constexpr int kSegRing = 8;
+constexpr int kSegRing = 4;                 // with the query rows prefetched that far ahead: 8 items ahead 198 us for 4096 tokens, 16 206, 4 179
 constexpr int kTileRing = 8;                // tiles the finding warp may be ahead of the loaders
 constexpr int kHole = -2;                   // a row without a page
 constexpr int kSegReaders = kSoftWarps + 3;  // and the loaders with packed rows
@@ -734,7 +733,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const uint32_t who = __ballot_sync(0xffffffffu, spoilt >> j & 1);
-                    const bool is = (who & (kF32 ? 0xffffu << (16 * half) : 0x0f0f0f0fu << (4 * half))) != 0;
+                    const bool is = (who & (kF32 ? 0xffffu << (16 * half) : 0x0f0f0f0fu << (4 * half))) != 0;     // any lane of the row
                     if (l16 == 0 && (is || !odd)) {
                         const int k = rw + 2 * j;
                         row_fma[buf][2 * (k & ~1) + (k & 1)] = is ? __uint_as_float(0x7fffffffu) : 1.0f;
@@ -848,6 +847,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 const int i = seg & (kSegRing - 1);
                 tc::wait<300>(DS4B200_BAR(seg_free, i), (uint32_t)(((seg / kSegRing) & 1) ^ 1), abort_flag, status, tc::kWaitPolls + 16 * longest);
                 if (lane == 0) {
+                    if (kPre && !end) prefetch_l2(a.q + sg.it.row0 * D, sg.it.rows * D * 2);     // some items before they are wanted
                     seg_s[i] = sg;
                     tc::arrive(DS4B200_BAR(seg_full, i));
                 }
@@ -859,11 +859,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             Segment sg;
             int n = 0;
             while (next_segment(sg)) {
-                if (lane == 0) prefetch_l2(a.q + sg.it.row0 * D, sg.it.rows * D * 2);       // long before they are wanted
                 for (int t = sg.t0; t < sg.t1; ++t, ++n) {
                     const int buf = n & 1, ta = first_run_tiles(sg.it);
                     const int from = t < ta ? sg.it.at_a + 64 * t : sg.it.at_b + 64 * (t - ta);
-                    // up to 16 rows (the MMAs read no more of them either): a window of 128 and 4 first rows ...
+                    // up to 16 rows (the MMAs read no more of them either), e.g. the first rows beside a window of 128
                     const bool few = rows_in_tile(sg.it, t) <= 16;
 #pragma unroll
                     for (int part = 0; part < kParts; ++part) {
@@ -1400,7 +1399,10 @@ void launch_fmt(const AttnArgs &a, cudaStream_t s) {
     static_assert(kPackCtas * sizeof(int) <= kMetaBytes && kPackRows * sizeof(float) <= kMlBytes && kPackCtas <= kThreads, "room for packed rows");
     const int64_t bound = (a.window > 0 ? a.n_tokens : 0) + a.n_seqs * packed_gap(a.window, a.n_first, all_rows);
     uint16_t *rows = reinterpret_cast<uint16_t *>(g.part_o);
-    if (a.q_start && !g.split && a.n_tokens >= kPackTokens && bound <= kPackRows && packed_map(&g.rows, rows, bound, a.kv.head_dim, 64) &&
+    // Packing pays where a row is wanted by more than one item of a CTA, and where tokens share an item (masks straight from the cache
+    // cost more than the launch): 256 tokens of 64 heads 37 us straight, 27 packed, 128 tokens 20.4 and 22.5; of 8 heads, 32 tokens
+    // 27 and 20, 128 tokens 27 and 20.  (Window 128, 4 first rows.)
+    if (a.q_start && !g.split && (g.group > 1 || slots > kCtas) && bound <= kPackRows && packed_map(&g.rows, rows, bound, a.kv.head_dim, 64) &&
         packed_map(&g.few, rows, bound, a.kv.head_dim, 16)) {
         g.fac = reinterpret_cast<const float *>(g.part_ml);
         g.odd = reinterpret_cast<const int *>(ws);

@@ -533,10 +533,10 @@ def test_nan_in_packed_rows_reaches_only_the_tokens_that_see_it(ops):
 
 def test_packed_and_direct_chunks_agree(ops):
     """The same tokens in a call long enough to pack its rows and in calls that are not."""
-    c = Case(ops, "block", 64, 512, 64, [400], [128])
+    c = Case(ops, "block", 64, 512, 64, [400], [256])
     whole = ops.attn_window_paged(c.q, c.kv, c.table, c.kv_len, c.q_start, window=128, n_first=4)
-    for first in range(0, 128, 32):
-        part = ops.attn_window_paged(c.q[first:first + 32].contiguous(), c.kv, c.table, c.kv_len - (96 - first),
+    for first in range(0, 256, 32):
+        part = ops.attn_window_paged(c.q[first:first + 32].contiguous(), c.kv, c.table, c.kv_len - (224 - first),
                                      torch.tensor([0, 32], dtype=torch.int32, device="cuda"), window=128, n_first=4)
         d = (part.float() - whole[first:first + 32].float()).abs()
         assert bool((d <= 2.0 ** -7 * whole[first:first + 32].float().abs() + 2.0 ** -9).all())
@@ -544,11 +544,13 @@ def test_packed_and_direct_chunks_agree(ops):
 
 @pytest.mark.parametrize("fmt", FMTS)
 @pytest.mark.parametrize("spoil", ["first", "tail", "scale"])
-def test_rows_that_are_not_finite_reach_only_the_tokens_that_see_them(ops, fmt, spoil):
-    """Four tokens of 16 heads share the tiles of a chunk that is too short to be packed."""
+@pytest.mark.parametrize("window", [20, 0])              # packed rows, and tiles straight from the cache
+def test_rows_that_are_not_finite_reach_only_the_tokens_that_see_them(ops, fmt, spoil, window):
+    """Four tokens of 16 heads share their tiles."""
     c = Case(ops, fmt, 16, 512, 64, [200, 90], [30, 11])
-    call = lambda: ops.attn_window_paged(c.q, c.kv, c.table, c.kv_len, c.q_start, window=20, n_first=2)
+    call = lambda: ops.attn_window_paged(c.q, c.kv, c.table, c.kv_len, c.q_start, window=window, n_first=2)
     clean = call()
+    old = None if fmt == "f32" else c.st["scales"].view(c.st["scales"].shape[0], -1).clone()
     slots = c.slots[0][181], c.slots[1][70]                                 # tokens 11 .. 30 see the first; 30 .. 40 (rows 79 .. 89) the second
     for slot, value in zip(slots, (float("nan"), float("inf"))):
         if fmt == "f32":
@@ -561,10 +563,24 @@ def test_rows_that_are_not_finite_reach_only_the_tokens_that_see_them(ops, fmt, 
             c.st["codes"][slot, 447 if spoil == "tail" else 0] = 0x7f
     out = call()
     sees = torch.zeros(41, dtype=torch.bool)
-    sees[11:30] = True
+    sees[11:30] = True                                                      # (rows 181 .. 199, within 20 of the first)
     sees[30:41] = True
     assert torch.equal(out.isnan().flatten(1).any(1).cpu(), sees)
-    assert torch.equal(out[~sees.cuda()], clean[~sees.cuda()])
+    # The others: to the bits where rows keep no factor.  The eight rows that are loaded with one whose scale is not finite keep theirs, and
+    # weights times factors round elsewhere: within the bound of an output for either set of factors.
+    if spoil == "scale" and fmt != "f32":
+        keep = c.factors.clone()
+        for b, j in ((0, 181), (1, 70)):
+            for i in c.slots[b][j // 8 * 8:j // 8 * 8 + 8]:
+                top = torch.cat([old[i], c.st["tail"][i].abs() / 256 if fmt == "block" else old[i]]).max().double()
+                keep[i] = top if fmt == "row" else torch.exp2(torch.floor(torch.log2(top)))
+        bound = 0
+        for factors in (c.factors, keep):
+            want, _, ob, _ = model.attention(c.q, c.rows, c.slots_of, c.positions, window, 2, 512 ** -0.5, None, c.tail, factors)
+            bound = torch.maximum(ob, torch.as_tensor(bound, dtype=ob.dtype, device=ob.device))
+        assert bool(((out.double() - want).abs() <= bound)[~sees.cuda()].all())
+    else:
+        assert torch.equal(out[~sees.cuda()], clean[~sees.cuda()])
     assert ops.device_status() == 0
 
 
