@@ -49,9 +49,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Bound.  Shared memory: a tile of 512 dims is 64 KiB written and, by the MMAs, 224 KiB read at 128 bytes a cycle (1792 cycles; an MMA
 // of M 64, N 64, K 16 reads 4 KiB in 32), which with the loads' own pass through L1, the weights and the query rows makes 2700 to
 // 2900 cycles a tile; from HBM a tile of FP8 rows needs 1400, of f32 rows 5600.  Halves of that traffic would need the codes
-// themselves as operands, and the weights as two or three 8-bit pieces.  Measured (64 heads, 512 dims): one session of 131072
-// rows, codes with a tail, 62 us (77 MB: 1.25 TB/s, 15 us at 6566 GB/s); 64 sequences of 1 to 8192 FP8 rows 94 us (162 MB, 1.7 TB/s);
-// 96 sequences of 16 heads, window 128 + 64 first f32 rows 64 us (75 MB of distinct rows ...).
+// themselves as operands, and the weights as two or three 8-bit pieces.  Measured (512 dims): one session of 131072 rows, codes with
+// a tail, 64 heads: 64 us (96 MB, 1.5 TB/s); 64 sequences of up to 16384 FP8 rows: 94 us (162 MB, 1.7 TB/s; tensor pipe 33 %);
+// 96 sequences, 16 heads, f32 rows, window 1024: 66 us (158 MB, 2.4 TB/s); 4096 chunk tokens, window 128 + 4 first rows: 174 to
+// 180 us (538 MB, 3.0 TB/s; tensor pipe 31 %), a chain of S, softmax, product and drain per token.
 constexpr int kCtas = 148;
 constexpr int kRows = 64;                   // query rows of an item, cache rows of a tile
 constexpr int kSoftWarps = 8, kLoadWarp0 = 8, kLoadWarps = 8, kMmaWarp = 16;
