@@ -445,6 +445,10 @@ def _attn(q, kv, page_table, kv_len, q_start, window, n_first, scale, sink, work
     n_seqs, width = page_table.shape
     if q_start is None and n_seqs != T:
         raise ValueError("attn_decode_paged: one token per sequence")
+    if not (0 <= window < 1 << 31 and 0 <= n_first < 1 << 31):
+        raise ValueError("attention: window and n_first must be in [0, 2^31)")
+    if workspace is not None and workspace.device != dev:
+        raise ValueError("attention: the workspace must be on the cache's device")
     with torch.cuda.device(dev):
         out = torch.empty_like(q) if out is None else out
         lse = torch.empty((T, H), dtype=torch.float32, device=dev) if want_lse else None

@@ -638,3 +638,73 @@ def test_rows_of_zeros_and_tiny_rows_keep_their_weight(ops, fmt, toks):
     if toks == 70:
         c.factors = pack_factors(c)
     c.check(out, lse, 0, 0, None)
+
+
+@pytest.mark.parametrize("fmt", ["row", "f32"])
+def test_rows_behind_four_gigabytes(ops, fmt):
+    """Pages at the far end of a pool whose byte offsets need more than 32 bits, beside pages at its front."""
+    dim, page = 512, 64
+    n = (9 << 20) if fmt == "row" else (9 << 18)                            # 4.8 GB of rows
+    order = [n // page - 1, 0, n // page - 2, 1, n // page // 2]
+    g = torch.Generator(device="cuda").manual_seed(7)
+    some = model.make_rows(fmt, torch.randn((len(order) * page, dim), generator=g, device="cuda"))
+    slots = [p * page + r for p in order for r in range(page)]
+    big = {k: torch.empty((n, v.shape[1]), dtype=v.dtype, device="cuda") for k, v in some.items()}
+    for k, v in some.items():
+        big[k][torch.tensor(slots, device="cuda")] = v
+    kv = ops.PagedKv(kind(ops, fmt), page, 64, **big)
+    table = torch.tensor([order], dtype=torch.int32, device="cuda")
+    rows, factors = model.row_values(fmt, some), model.row_factors(fmt, some)
+    length = 5 * page - 3
+    for toks in (1, 150):
+        q = torch.randn((toks, 64, dim), generator=g, device="cuda").bfloat16()
+        kv_len = torch.tensor([length], dtype=torch.int32, device="cuda")
+        if toks == 1:
+            out = ops.attn_decode_paged(q, kv, table, kv_len)
+        else:
+            out = ops.attn_window_paged(q, kv, table, kv_len, torch.tensor([0, toks], dtype=torch.int32, device="cuda"), window=130, n_first=3)
+        want, _, bound, _ = model.attention(q, rows, [list(range(length))] * toks, list(range(length - toks, length)), 0 if toks == 1 else 130,
+                                            0 if toks == 1 else 3, dim ** -0.5, None, dim if fmt == "row" else 0, factors)
+        assert bool(((out.double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("heads", [64, 8])
+def test_captured_chunk_follows_the_cache_and_the_lengths(ops, heads):
+    """A graph of a chunk's call (rows packed in the workspace), replayed after rows, lengths and bounds have changed."""
+    c = Case(ops, "block", heads, 512, 64, [300, 200], [100, 80])
+    ws, out = ops.attn_workspace(heads, 512), torch.zeros_like(c.q)
+    call = lambda: ops.attn_window_paged(c.q, c.kv, c.table, c.kv_len, c.q_start, window=128, n_first=4, workspace=ws, out=out)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        call()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for change in (lambda: None, lambda: c.kv_len.sub_(31), lambda: c.st["scales"].mul_(2.0),
+                   lambda: c.q_start.copy_(torch.tensor([20, 90, 150], dtype=torch.int32, device="cuda"))):
+        change()
+        out.fill_(5.0)
+        want = call().clone()
+        out.fill_(5.0)
+        ws.fill_(0xff)
+        graph.replay()
+        assert torch.equal(out, want)
+    assert bool((out[:20] == 5).all()) and bool((out[150:] == 5).all())
+
+
+@pytest.mark.parametrize("window", [0, 7])
+def test_chunk_longer_than_its_sequence_with_tokens_that_share_tiles(ops, window):
+    c = Case(ops, "f32", 8, 128, 64, [10, 90], [10, 5])
+    q = torch.cat([c.q[:4], c.q])
+    out, lse = ops.attn_window_paged(q, c.kv, c.table, c.kv_len, torch.tensor([0, 14, 19], dtype=torch.int32, device="cuda"), window=window, want_lse=True)
+    assert not out[:4].any() and bool((lse[:4] == -float("inf")).all())
+    c.check(out[4:], lse[4:], window, 0, None)
+
+
+def test_attention_refuses_what_does_not_fit_its_arguments(ops):
+    c = Case(ops, "f32", 8, 128, 64, [10])
+    for bad in (dict(window=1 << 32), dict(n_first=1 << 32), dict(window=-1), dict(workspace=torch.empty(1 << 20, dtype=torch.uint8))):
+        with pytest.raises(ValueError):
+            ops.attn_decode_paged(c.q, c.kv, c.table, c.kv_len, **bad)
