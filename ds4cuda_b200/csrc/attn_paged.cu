@@ -1191,21 +1191,31 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     if (warp == kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem_s));
 }
 
-// Joins the parts of the items that a CTA began and did not finish, in order.  A unit is one query row and 128 dims of such an item, four
-// dims a lane.  An item of few parts takes a warp per unit; one of many (a session of 131072 rows leaves 148 parts of 128 KiB) a
-// CTA, whose eight warps take every eighth part, since the latency of the loads is what a unit costs.
+// Joins the parts of the items that a CTA began and did not finish, in order: with M the largest of the parts' maxima and the sink,
+// out = sum_k 2^(m_k - M) O_k / (sum_k 2^(m_k - M) l_k + 2^(sink - M)).  What a unit costs is the latency of its loads, so a unit
+// issues its first parts' sums ahead of the statistics that weigh them, and the items' descriptions are in shared memory.
+// Few parts: a warp per query row, two parts at a time.  Many (a session of 131072 rows leaves 148 of 128 KiB): a CTA per row and 128
+// dims, whose warps take every eighth part.  With a warp or CTA per 128 dims, and the statistics first, it took 11 to 17 us.
 constexpr int kJoinCtas = 4 * kCtas, kJoinWarps = 8, kJoinFew = 8;
+static_assert(kCtas <= kJoinWarps * 32, "a thread per part");
 
-__global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const AttnArgs a, const Meta *meta, const float2 *part_ml, const float *part_o) {
+__device__ __forceinline__ void add_scaled(float4 &o, float w, const float4 &x) {
+    o = make_float4(fmaf(w, x.x, o.x), fmaf(w, x.y, o.y), fmaf(w, x.z, o.z), fmaf(w, x.w, o.w));
+}
+
+__global__ void __launch_bounds__(kJoinWarps * 32, 4) attn_join_kernel(const AttnArgs a, const Meta *meta, const float2 *part_ml, const float *part_o) {
+    __shared__ Meta items[kCtas];
     __shared__ int begun[2][kCtas], n_begun[2];          // items of few and of many parts
-    __shared__ float weight[kJoinWarps][kCtas];
+    __shared__ float weight[kCtas], most_s[kJoinWarps], sum_s[kJoinWarps];
     __shared__ float4 sums[kJoinWarps][32];
     const int D = a.kv.head_dim, slices = D / 128, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     wait_dependency();
+    if (tid < kCtas) items[tid] = meta[tid];
+    __syncthreads();
     if (warp < 2) {
         int n = 0;
         for (int base = 0; base < kCtas; base += 32) {
-            const int c = base + lane, parts = c < kCtas ? meta[c].parts : 0;
+            const int c = base + lane, parts = c < kCtas ? items[c].parts : 0;
             const bool is = parts >= 2 && (parts > kJoinFew) == (warp == 1);
             const uint32_t all = __ballot_sync(0xffffffffu, is);
             if (is) begun[warp][n + __popc(all & ((1u << lane) - 1))] = c;
@@ -1214,56 +1224,96 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const AttnAr
         if (lane == 0) n_begun[warp] = n;
     }
     __syncthreads();
-    for (int many = 0; many < 2; ++many) {
-        const int units = n_begun[many] * kRows * slices;
-        const int lead = many ? warp : 0, step = many ? kJoinWarps : 1;     // this warp's first part and its stride
-        for (int u = many ? blockIdx.x : blockIdx.x * kJoinWarps + warp; u < units; u += many ? gridDim.x : gridDim.x * kJoinWarps) {
-            const int c = begun[many][u / (kRows * slices)], row = u / slices % kRows, slice = u % slices;
-            const Meta it = meta[c];
-            if (row >= it.rows) continue;
-            auto part_of = [&](int k) { return k == 0 ? 2 * c + 1 : 2 * (c + k); };
-            const float sink2 = a.sink ? __ldg(a.sink + it.h0 + row % a.n_heads) * kLog2e : -INFINITY;
-            const int d = slice * 128 + lane * 4;
-            float hi = sink2;
-            for (int k = lane; k < it.parts; k += 32) {
-                const float2 ml = part_ml[part_of(k) * kRows + row];
-                hi = fmaxf(hi, ml.y > 0.0f ? ml.x + __log2f(ml.y) : (ml.y == ml.y ? -INFINITY : ml.y));
+    auto part_of = [](int c, int k) { return k == 0 ? 2 * c + 1 : 2 * (c + k); };
+    auto sink_of = [&](const Meta &it, int row) { return a.sink ? __ldg(a.sink + it.h0 + row % a.n_heads) * kLog2e : -INFINITY; };
+
+    for (int u = blockIdx.x * kJoinWarps + warp; u < n_begun[0] * kRows; u += gridDim.x * kJoinWarps) {
+        const int c = begun[0][u / kRows], row = u % kRows;
+        const Meta it = items[c];
+        if (row >= it.rows) continue;
+        float2 ml = make_float2(-INFINITY, 0.0f);
+        if (lane < it.parts) ml = part_ml[part_of(c, lane) * kRows + row];
+        const float sink2 = sink_of(it, row);
+        float4 x[2][4], o[4];
+        auto load = [&](int k) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int s = 0; s < 4; ++s)
+                    x[j][s] = k + j < it.parts && s < slices
+                                  ? __ldg(reinterpret_cast<const float4 *>(part_o + ((int64_t)part_of(c, k + j) * kRows + row) * D + s * 128 + lane * 4))
+                                  : make_float4(0.f, 0.f, 0.f, 0.f);
+        };
+        load(0);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) o[s] = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float top = fmaxf(warp_max(ml.x), sink2);
+        const float w = ml.x == -INFINITY ? 0.0f : tc::exp2_approx(ml.x - top);
+        float l = warp_sum(w * ml.y);
+        if (sink2 > -INFINITY) l += tc::exp2_approx(sink2 - top);
+        for (int k = 0; k < it.parts; k += 2) {
+            if (k) load(k);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const float wk = __shfl_sync(0xffffffffu, w, k + j);       // 0 behind the last part
+#pragma unroll
+                for (int s = 0; s < 4; ++s) add_scaled(o[s], wk, x[j][s]);
             }
-            hi = warp_max(hi);
-            float sum = 0.0f;
-            for (int k = lane; k < it.parts; k += 32) {
-                const float2 ml = part_ml[part_of(k) * kRows + row];
-                const float v = ml.y > 0.0f ? ml.x + __log2f(ml.y) : (ml.y == ml.y ? -INFINITY : ml.y);
-                sum += hi == -INFINITY ? 0.0f : tc::exp2_approx(v - hi);
-                weight[warp][k] = ml.x;
-            }
-            sum = warp_sum(sum);
-            if (a.sink && hi > -INFINITY) sum += tc::exp2_approx(sink2 - hi);
-            const float lse2 = hi == -INFINITY ? hi : hi + __log2f(sum);
-            __syncwarp();
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-            for (int k = lead; k < it.parts; k += step) {
-                const float4 x = __ldg(reinterpret_cast<const float4 *>(part_o + ((int64_t)part_of(k) * kRows + row) * D + d));
-                const float m = weight[warp][k], w = m == -INFINITY ? 0.0f : tc::exp2_approx(m - lse2);
-                o = make_float4(fmaf(w, x.x, o.x), fmaf(w, x.y, o.y), fmaf(w, x.z, o.z), fmaf(w, x.w, o.w));
-            }
-            if (many) {
-                sums[warp][lane] = o;
-                __syncthreads();
-                o = sums[0][lane];
-                for (int k = 1; k < kJoinWarps; ++k) {
-                    const float4 x = sums[k][lane];
-                    o = make_float4(o.x + x.x, o.y + x.y, o.z + x.z, o.w + x.w);
-                }
-                __syncthreads();
-            }
-            if (lead == 0) {
-                st_bf16x4(a.out + (it.row0 + row) * D + d, o);
-                if (lane == 0 && slice == 0 && a.lse) a.lse[it.row0 + row] = lse2 * (1.0f / kLog2e);
-            }
-            __syncwarp();
         }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int s = 0; s < 4; ++s)
+            if (s < slices) st_bf16x4(a.out + (it.row0 + row) * D + s * 128 + lane * 4, make_float4(o[s].x * inv, o[s].y * inv, o[s].z * inv, o[s].w * inv));
+        if (lane == 0 && a.lse) a.lse[it.row0 + row] = (l == 0.0f ? -INFINITY : top + __log2f(l)) * (1.0f / kLog2e);
+    }
+
+    for (int u = blockIdx.x; u < n_begun[1] * kRows * slices; u += gridDim.x) {
+        const int c = begun[1][u / (kRows * slices)], row = u / slices % kRows, slice = u % slices;
+        const Meta it = items[c];
+        if (row >= it.rows) continue;
+        float2 ml = make_float2(-INFINITY, 0.0f);
+        if (tid < it.parts) ml = part_ml[part_of(c, tid) * kRows + row];
+        const float sink2 = sink_of(it, row);
+        constexpr int kBatch = 10;
+        float4 x[kBatch], o = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto load = [&](int k0) {
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const int k = k0 + i * kJoinWarps;
+                x[i] = k < it.parts ? __ldg(reinterpret_cast<const float4 *>(part_o + ((int64_t)part_of(c, k) * kRows + row) * D + slice * 128 + lane * 4))
+                                    : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+        };
+        load(warp);
+        const float warp_top = warp_max(ml.x);
+        if (lane == 0) most_s[warp] = warp_top;
+        __syncthreads();
+        float top = sink2;
+#pragma unroll
+        for (int i = 0; i < kJoinWarps; ++i) top = fmaxf(top, most_s[i]);
+        const float w = ml.x == -INFINITY ? 0.0f : tc::exp2_approx(ml.x - top), warp_l = warp_sum(w * ml.y);
+        if (tid < kCtas) weight[tid] = w;
+        if (lane == 0) sum_s[warp] = warp_l;
+        __syncthreads();
+        for (int k0 = warp; k0 < it.parts; k0 += kBatch * kJoinWarps) {
+            if (k0 != warp) load(k0);
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) add_scaled(o, k0 + i * kJoinWarps < it.parts ? weight[k0 + i * kJoinWarps] : 0.0f, x[i]);
+        }
+        sums[warp][lane] = o;
+        __syncthreads();
+        if (warp == 0) {
+            float l = sink2 > -INFINITY ? tc::exp2_approx(sink2 - top) : 0.0f;
+#pragma unroll
+            for (int i = 0; i < kJoinWarps; ++i) l += sum_s[i];
+            o = sums[0][lane];
+#pragma unroll
+            for (int i = 1; i < kJoinWarps; ++i) add_scaled(o, 1.0f, sums[i][lane]);
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            st_bf16x4(a.out + (it.row0 + row) * D + slice * 128 + lane * 4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
+            if (lane == 0 && slice == 0 && a.lse) a.lse[it.row0 + row] = (l == 0.0f ? -INFINITY : top + __log2f(l)) * (1.0f / kLog2e);
+        }
+        __syncthreads();                                 // sums and sum_s are read
     }
 }
 
