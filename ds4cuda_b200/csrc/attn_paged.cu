@@ -1203,7 +1203,7 @@ __device__ __forceinline__ void add_scaled(float4 &o, float w, const float4 &x) 
     o = make_float4(fmaf(w, x.x, o.x), fmaf(w, x.y, o.y), fmaf(w, x.z, o.z), fmaf(w, x.w, o.w));
 }
 
-__global__ void __launch_bounds__(kJoinWarps * 32, 4) attn_join_kernel(const AttnArgs a, const Meta *meta, const float2 *part_ml, const float *part_o) {
+__global__ void __launch_bounds__(kJoinWarps * 32, 3) attn_join_kernel(const AttnArgs a, const Meta *meta, const float2 *part_ml, const float *part_o) {
     __shared__ Meta items[kCtas];
     __shared__ int begun[2][kCtas], n_begun[2];          // items of few and of many parts
     __shared__ float weight[kCtas], most_s[kJoinWarps], sum_s[kJoinWarps];
@@ -1274,7 +1274,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 4) attn_join_kernel(const Att
         float2 ml = make_float2(-INFINITY, 0.0f);
         if (tid < it.parts) ml = part_ml[part_of(c, tid) * kRows + row];
         const float sink2 = sink_of(it, row);
-        constexpr int kBatch = 10;
+        constexpr int kBatch = 6;
         float4 x[kBatch], o = make_float4(0.f, 0.f, 0.f, 0.f);
         auto load = [&](int k0) {
 #pragma unroll
