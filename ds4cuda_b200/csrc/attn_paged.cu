@@ -50,9 +50,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 // of M 64, N 64, K 16 reads 4 KiB in 32), which with the loads' own pass through L1, the weights and the query rows makes 2700 to
 // 2900 cycles a tile; from HBM a tile of FP8 rows needs 1400, of f32 rows 5600.  Halves of that traffic would need the codes
 // themselves as operands, and the weights as two or three 8-bit pieces.  Measured (512 dims): one session of 131072 rows, codes with
-// a tail, 64 heads: 64 us (96 MB, 1.5 TB/s); 64 sequences of up to 16384 FP8 rows: 94 us (162 MB, 1.7 TB/s; tensor pipe 33 %);
-// 96 sequences, 16 heads, f32 rows, window 1024: 66 us (158 MB, 2.4 TB/s); 4096 chunk tokens, window 128 + 4 first rows: 174 to
-// 180 us (538 MB, 3.0 TB/s; tensor pipe 31 %), a chain of S, softmax, product and drain per token.
+// a tail, 64 heads: 55 us (96 MB, 1.7 TB/s); 64 sequences of up to 16384 FP8 rows: 90 us (162 MB, 1.8 TB/s; tensor pipe 33 %);
+// 96 sequences, 16 heads, f32 rows, window 1024: 60 us (158 MB, 2.6 TB/s); 4096 chunk tokens, window 128 + 4 first rows: 174 to
+// 186 us (538 MB, 2.9 to 3.1 TB/s; tensor pipe 31 %), a chain of S, softmax, product and drain per token.
 constexpr int kCtas = 148;
 constexpr int kRows = 64;                   // query rows of an item, cache rows of a tile
 constexpr int kSoftWarps = 8, kLoadWarp0 = 8, kLoadWarps = 8, kMmaWarp = 16;
@@ -1195,7 +1195,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 // out = sum_k 2^(m_k - M) O_k / (sum_k 2^(m_k - M) l_k + 2^(sink - M)).  What a unit costs is the latency of its loads, so a unit
 // issues its first parts' sums ahead of the statistics that weigh them, and the items' descriptions are in shared memory.
 // Few parts: a warp per query row, two parts at a time.  Many (a session of 131072 rows leaves 148 of 128 KiB): a CTA per row and 128
-// dims, whose warps take every eighth part.  With a warp or CTA per 128 dims, and the statistics first, it took 11 to 17 us.
+// dims, or per row where rows are many, whose warps take every eighth part.  Alone: 7.3 us (one session of 131072 rows), 8.4 (7 of up to 9001; 11.3 with slices), 8.0
+// (64 of up to 16384), 6.0 (96 of 16 heads); with the statistics ahead of the loads, and 64 registers, 11 to 17.
 constexpr int kJoinCtas = 4 * kCtas, kJoinWarps = 8, kJoinFew = 8;
 static_assert(kCtas <= kJoinWarps * 32, "a thread per part");
 
@@ -1207,7 +1208,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) attn_join_kernel(const Att
     __shared__ Meta items[kCtas];
     __shared__ int begun[2][kCtas], n_begun[2];          // items of few and of many parts
     __shared__ float weight[kCtas], most_s[kJoinWarps], sum_s[kJoinWarps];
-    __shared__ float4 sums[kJoinWarps][32];
+    __shared__ float4 sums[4][kJoinWarps][32];
     const int D = a.kv.head_dim, slices = D / 128, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     wait_dependency();
     if (tid < kCtas) items[tid] = meta[tid];
@@ -1267,54 +1268,70 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) attn_join_kernel(const Att
         if (lane == 0 && a.lse) a.lse[it.row0 + row] = (l == 0.0f ? -INFINITY : top + __log2f(l)) * (1.0f / kLog2e);
     }
 
-    for (int u = blockIdx.x; u < n_begun[1] * kRows * slices; u += gridDim.x) {
-        const int c = begun[1][u / (kRows * slices)], row = u / slices % kRows, slice = u % slices;
-        const Meta it = items[c];
-        if (row >= it.rows) continue;
-        float2 ml = make_float2(-INFINITY, 0.0f);
-        if (tid < it.parts) ml = part_ml[part_of(c, tid) * kRows + row];
-        const float sink2 = sink_of(it, row);
-        constexpr int kBatch = 6;
-        float4 x[kBatch], o = make_float4(0.f, 0.f, 0.f, 0.f);
-        auto load = [&](int k0) {
+    // SL slices of 128 dims in a CTA: all four where there are more rows than slices would leave CTAs for
+    auto many = [&](auto sl) {
+        constexpr int SL = decltype(sl)::value, kBatch = SL > 1 ? 2 : 6;
+        const int cuts = slices / SL;
+        for (int u = blockIdx.x; u < n_begun[1] * kRows * cuts; u += gridDim.x) {
+            const int c = begun[1][u / (kRows * cuts)], row = u / cuts % kRows, slice = u % cuts * SL;
+            const Meta &it = items[c];
+            const int parts = it.parts;
+            if (row >= it.rows) continue;
+            float2 ml = make_float2(-INFINITY, 0.0f);
+            if (tid < parts) ml = part_ml[part_of(c, tid) * kRows + row];
+            const float sink2 = sink_of(it, row);
+            float4 x[kBatch][SL], o[SL];
+            auto load = [&](int k0) {
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-                const int k = k0 + i * kJoinWarps;
-                x[i] = k < it.parts ? __ldg(reinterpret_cast<const float4 *>(part_o + ((int64_t)part_of(c, k) * kRows + row) * D + slice * 128 + lane * 4))
-                                    : make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int i = 0; i < kBatch; ++i) {
+                    const int k = k0 + i * kJoinWarps;
+                    const float4 *from = reinterpret_cast<const float4 *>(part_o + ((int64_t)part_of(c, k) * kRows + row) * D + slice * 128 + lane * 4);
+#pragma unroll
+                    for (int s = 0; s < SL; ++s) x[i][s] = k < parts ? __ldg(from + s * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+            };
+            load(warp);
+            const float warp_top = warp_max(ml.x);
+            if (lane == 0) most_s[warp] = warp_top;
+            __syncthreads();
+            float top = sink2;
+#pragma unroll
+            for (int i = 0; i < kJoinWarps; ++i) top = fmaxf(top, most_s[i]);
+            const float w = ml.x == -INFINITY ? 0.0f : tc::exp2_approx(ml.x - top), warp_l = warp_sum(w * ml.y);
+            if (tid < kCtas) weight[tid] = w;
+            if (lane == 0) sum_s[warp] = warp_l;
+            __syncthreads();
+#pragma unroll
+            for (int s = 0; s < SL; ++s) o[s] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+            for (int k0 = warp; k0 < parts; k0 += kBatch * kJoinWarps) {
+                if (k0 != warp) load(k0);
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    const float wk = k0 + i * kJoinWarps < parts ? weight[k0 + i * kJoinWarps] : 0.0f;
+#pragma unroll
+                    for (int s = 0; s < SL; ++s) add_scaled(o[s], wk, x[i][s]);
+                }
             }
-        };
-        load(warp);
-        const float warp_top = warp_max(ml.x);
-        if (lane == 0) most_s[warp] = warp_top;
-        __syncthreads();
-        float top = sink2;
 #pragma unroll
-        for (int i = 0; i < kJoinWarps; ++i) top = fmaxf(top, most_s[i]);
-        const float w = ml.x == -INFINITY ? 0.0f : tc::exp2_approx(ml.x - top), warp_l = warp_sum(w * ml.y);
-        if (tid < kCtas) weight[tid] = w;
-        if (lane == 0) sum_s[warp] = warp_l;
-        __syncthreads();
-        for (int k0 = warp; k0 < it.parts; k0 += kBatch * kJoinWarps) {
-            if (k0 != warp) load(k0);
+            for (int s = 0; s < SL; ++s) sums[s][warp][lane] = o[s];
+            __syncthreads();
+            if (warp < SL) {
+                float l = sink2 > -INFINITY ? tc::exp2_approx(sink2 - top) : 0.0f;
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) add_scaled(o, k0 + i * kJoinWarps < it.parts ? weight[k0 + i * kJoinWarps] : 0.0f, x[i]);
+                for (int i = 0; i < kJoinWarps; ++i) l += sum_s[i];
+                float4 y = sums[warp][0][lane];
+#pragma unroll
+                for (int i = 1; i < kJoinWarps; ++i) add_scaled(y, 1.0f, sums[warp][i][lane]);
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                st_bf16x4(a.out + (it.row0 + row) * D + (slice + warp) * 128 + lane * 4, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
+                if (lane == 0 && slice + warp == 0 && a.lse) a.lse[it.row0 + row] = (l == 0.0f ? -INFINITY : top + __log2f(l)) * (1.0f / kLog2e);
+            }
+            __syncthreads();                             // sums and sum_s are read
         }
-        sums[warp][lane] = o;
-        __syncthreads();
-        if (warp == 0) {
-            float l = sink2 > -INFINITY ? tc::exp2_approx(sink2 - top) : 0.0f;
-#pragma unroll
-            for (int i = 0; i < kJoinWarps; ++i) l += sum_s[i];
-            o = sums[0][lane];
-#pragma unroll
-            for (int i = 1; i < kJoinWarps; ++i) add_scaled(o, 1.0f, sums[i][lane]);
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            st_bf16x4(a.out + (it.row0 + row) * D + slice * 128 + lane * 4, make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv));
-            if (lane == 0 && slice == 0 && a.lse) a.lse[it.row0 + row] = (l == 0.0f ? -INFINITY : top + __log2f(l)) * (1.0f / kLog2e);
-        }
-        __syncthreads();                                 // sums and sum_s are read
-    }
+    };
+    if (slices == 4 && n_begun[1] * kRows * slices > (int)gridDim.x) many(std::integral_constant<int, 4>());
+    else many(std::integral_constant<int, 1>());
 }
 
 // The rows a chunk's tokens see, once each, as packed f16 rows: with a window of 128 rows every row is wanted by 128 tokens, and turning it into
