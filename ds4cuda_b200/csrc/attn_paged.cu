@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     __shared__ int abort_s, start_slot, start_tile;
     __shared__ long long scan_s[kThreads / 32];
     __shared__ __align__(16) float row_fma[2][2 * kRows], row_div[2][kRows];      // by pairs of rows: factor, factor, addend, addend
-    __shared__ __align__(16) int row_at[kPre ? 1 : 2 * kTileRing][kRows];       // a row's place in its sequence
+    __shared__ __align__(16) int row_at[kPre || !SHARED ? 1 : 2 * kTileRing][kRows];       // a row's place in its sequence
     __shared__ __align__(16) int slot_s[kPre ? 1 : kTileRing][kRows];          // a tile's rows in the pool (-1 past the rows, or kHole), see find_index()
     __shared__ int tile_rows[kTileRing];                            // query rows where a tile is its segment's first, else 0; -1 ends
     __shared__ int64_t tile_row0[kTileRing];                        // and the first of them
@@ -383,8 +383,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     if (warp >= kLoadWarp0 && warp < kLoadWarp0 + kLoadWarps) {
         // ------------------------------------------------------------------------------ loaders
         // A warp has eight rows of the tile.  Its loads cover two rows at a time, 256 contiguous bytes of each (16 lanes): whole lines,
-        // and stores of rows r and r + 1 with their 16-byte units XORed by the row fall on all banks.  Tails and the
-        // query rows go by four lanes per row.  A register is loaded again, with the next unit's bytes, as soon as
+        // and stores of rows r and r + 1 with their 16-byte units XORed by the row fall on all banks.  Tails go by
+        // four lanes per row.  A register is loaded again, with the next unit's bytes, as soon as
         // its value is converted, so loads run a tile ahead of the stores.  A unit is a tile, or 128 or 256 dims of one in f32.
         tc::set_max_registers_up<136>();
         constexpr bool kF32 = FMT == DS4B200_KV_F32, kBlock = FMT == DS4B200_KV_FP8_BLOCK64;
@@ -909,7 +909,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                             const int pg = g.page_shift >= 0 ? at >> g.page_shift : at / a.kv.page_rows;
                             in[h] = at - pg * a.kv.page_rows;
                             page[h] = k < sg.it.n ? max(__ldg(a.page_table + sg.it.b * a.table_width + pg), -1) : -2;
-                            row_at[kPre ? 0 : n & (2 * kTileRing - 1)][lane + 32 * h] = at;
+                            if (SHARED) row_at[kPre || !SHARED ? 0 : n & (2 * kTileRing - 1)][lane + 32 * h] = at;
                         }
 #pragma unroll
                         for (int h = 0; h < 2; ++h)
@@ -1038,7 +1038,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                             at.x = (t < first_run_tiles(it) ? it.lo + 64 * t : 64 * (t - first_run_tiles(it))) + 8 * i + 2 * (lane & 3);
                             at.y = at.x + 1;
                         } else {
-                            at = *reinterpret_cast<const int2 *>(&row_at[kPre ? 0 : n & (2 * kTileRing - 1)][8 * i + 2 * (lane & 3)]);
+                            at = *reinterpret_cast<const int2 *>(&row_at[kPre || !SHARED ? 0 : n & (2 * kTileRing - 1)][8 * i + 2 * (lane & 3)]);
                         }
                         if (at.x > p || (at.x <= from && at.x >= a.n_first)) v[i].x = -INFINITY;
                         if (at.y > p || (at.y <= from && at.y >= a.n_first)) v[i].y = -INFINITY;
