@@ -57,6 +57,9 @@ constexpr int kCtas = 148;
 constexpr int kRows = 64;                   // query rows of an item, cache rows of a tile
 constexpr int kSoftWarps = 8, kLoadWarp0 = 8, kLoadWarps = 8, kMmaWarp = 16;
 constexpr int kThreads = 20 * 32;
+// Registers a thread by role, out of what the block is launched with: a larger sum would wait for registers for ever.
+constexpr int kLaunchRegs = 96, kSoftRegs = 72, kLoadRegs = 136, kOtherRegs = 56;
+static_assert(kSoftWarps * kSoftRegs + kLoadWarps * kLoadRegs + (20 - kSoftWarps - kLoadWarps) * kOtherRegs <= 20 * kLaunchRegs, "register split");
 constexpr int kSplitItems = 4 * kCtas;      // more of them are not cut
 constexpr int kWholeTiles = 3;              // items of up to so many tiles are not cut
 constexpr int kMinTiles = 2;                // of a run: below, the join costs more than the run saves
@@ -386,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         // and stores of rows r and r + 1 with their 16-byte units XORed by the row fall on all banks.  Tails go by
         // four lanes per row.  A register is loaded again, with the next unit's bytes, as soon as
         // its value is converted, so loads run a tile ahead of the stores.  A unit is a tile, or 128 or 256 dims of one in f32.
-        tc::set_max_registers_up<136>();
+        tc::set_max_registers_up<kLoadRegs>();
         constexpr bool kF32 = FMT == DS4B200_KV_F32, kBlock = FMT == DS4B200_KV_FP8_BLOCK64;
         constexpr int kUnitChunks = !kF32 ? kChunks : (NB % 2 ? 2 : 4), kUnits = kChunks / kUnitChunks;
         constexpr int kSpan = kF32 ? 1 : 4;              // chunks a load of two rows covers (fewer with fewer dims)
@@ -750,7 +753,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         }
         }
     } else if (warp >= kMmaWarp) {
-        tc::set_max_registers_down<56>();
+        tc::set_max_registers_down<kOtherRegs>();
         const uint32_t one = tc::elect();
         const uint32_t k_desc = tc::desc_lo(smem_addr(k_s), 0);
         if (warp == kMmaWarp) {
@@ -941,7 +944,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         // ------------------------------------------------------------------------------ softmax and output
         // Eight warps, two per quarter of tensor memory's lanes: a quarter holds 16 rows of S (lanes 0-15), of which each warp takes
         // eight, four lanes and 16 columns each.
-        tc::set_max_registers_down<72>();
+        tc::set_max_registers_down<kSoftRegs>();
         const int quarter = warp & 3, group = warp >> 2;
         const int row = quarter * 16 + group * 8 + (lane >> 2);
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
@@ -1431,20 +1434,25 @@ constexpr int64_t kMetaBytes = (kCtas * (int64_t)sizeof(Meta) + 127) / 128 * 128
 constexpr int64_t kMlBytes = 2 * kCtas * kRows * (int64_t)sizeof(float2);
 
 template <int NB, int FMT, bool SHARED>
-void launch_tc(const TcArgs &g, cudaStream_t s) {
+bool launch_tc(const TcArgs &g, cudaStream_t s) {
     constexpr int kSmem = 3 * kRows * NB * 256 + (FMT == kPacked ? 3 : 2) * 8192;
     constexpr int kOneCta = 120 * 1024;               // one CTA per SM: each takes the whole tensor memory
     const int smem = kSmem > kOneCta ? kSmem : kOneCta;
     const auto kernel = attn_tc_kernel<NB, FMT, SHARED>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return;    // launched() reports it
+    static const bool enough = [&] {                 // a compiler that gives the kernel fewer registers than the roles' split needs
+        cudaFuncAttributes at;
+        return cudaFuncGetAttributes(&at, kernel) == cudaSuccess && at.numRegs >= kLaunchRegs;
+    }();
+    if (!enough || cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return false;
     const unsigned grid = (unsigned)(g.split || g.n_slots > kCtas ? kCtas : g.n_slots);
     if (FMT == kPacked) launch_behind(kernel, grid, kThreads, smem, s, g);
     else kernel<<<grid, kThreads, smem, s>>>(g);
     if (g.split) launch_behind(attn_join_kernel, kJoinCtas, kJoinWarps * 32, 0, s, g.a, (const Meta *)g.meta, (const float2 *)g.part_ml, (const float *)g.part_o);
+    return true;
 }
 
 template <int NB>
-void launch_fmt(const AttnArgs &a, cudaStream_t s) {
+bool launch_fmt(const AttnArgs &a, cudaStream_t s) {
     TcArgs g{};
     g.a = a;
     g.head_groups = (a.n_heads + kRows - 1) / kRows;
@@ -1475,13 +1483,12 @@ void launch_fmt(const AttnArgs &a, cudaStream_t s) {
         g.fac = reinterpret_cast<const float *>(g.part_ml);
         g.odd = reinterpret_cast<const int *>(ws);
         attn_pack_kernel<NB><<<kPackCtas, kPackWarps * 32, 0, s>>>(a, bound, rows, reinterpret_cast<float *>(g.part_ml), reinterpret_cast<int *>(ws));
-        launch_tc<NB, kPacked, true>(g, s);
-    } else if (a.kv.row_format == DS4B200_KV_F32) {
-        g.group > 1 ? launch_tc<NB, DS4B200_KV_F32, true>(g, s) : launch_tc<NB, DS4B200_KV_F32, false>(g, s);
-    } else if (a.kv.row_format == DS4B200_KV_FP8_ROW) {
-        g.group > 1 ? launch_tc<NB, DS4B200_KV_FP8_ROW, true>(g, s) : launch_tc<NB, DS4B200_KV_FP8_ROW, false>(g, s);
-    } else {
-        g.group > 1 ? launch_tc<NB, DS4B200_KV_FP8_BLOCK64, true>(g, s) : launch_tc<NB, DS4B200_KV_FP8_BLOCK64, false>(g, s);
+        return launch_tc<NB, kPacked, true>(g, s);
+    }
+    switch (a.kv.row_format) {
+        case DS4B200_KV_F32: return g.group > 1 ? launch_tc<NB, DS4B200_KV_F32, true>(g, s) : launch_tc<NB, DS4B200_KV_F32, false>(g, s);
+        case DS4B200_KV_FP8_ROW: return g.group > 1 ? launch_tc<NB, DS4B200_KV_FP8_ROW, true>(g, s) : launch_tc<NB, DS4B200_KV_FP8_ROW, false>(g, s);
+        default: return g.group > 1 ? launch_tc<NB, DS4B200_KV_FP8_BLOCK64, true>(g, s) : launch_tc<NB, DS4B200_KV_FP8_BLOCK64, false>(g, s);
     }
 }
 
@@ -1491,12 +1498,12 @@ int64_t attn_workspace_bytes(int n_heads, int head_dim) {
     return kMetaBytes + kMlBytes + 2 * kCtas * kRows * (int64_t)head_dim * 4;
 }
 
-void attn_paged(const AttnArgs &a, cudaStream_t s) {
+bool attn_paged(const AttnArgs &a, cudaStream_t s) {
     switch (a.kv.head_dim / 128) {
-        case 1: launch_fmt<1>(a, s); break;
-        case 2: launch_fmt<2>(a, s); break;
-        case 3: launch_fmt<3>(a, s); break;
-        default: launch_fmt<4>(a, s); break;
+        case 1: return launch_fmt<1>(a, s);
+        case 2: return launch_fmt<2>(a, s);
+        case 3: return launch_fmt<3>(a, s);
+        default: return launch_fmt<4>(a, s);
     }
 }
 

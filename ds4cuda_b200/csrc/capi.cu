@@ -661,8 +661,9 @@ int ds4b200_attn_decode_paged_bf16(const uint16_t *q, const ds4b200_paged_kv *ho
     if (rc) return rc;
     ds4b200::AttnArgs a{q, *host_kv, page_table, kv_len, nullptr, table_width, n_seqs, (int)n_seqs, n_heads, window, n_first,
                         scale, sink, out, lse, workspace};
-    ds4b200::attn_paged(a, STREAM(stream));
-    return launched("attn_decode_paged");
+    const bool can = ds4b200::attn_paged(a, STREAM(stream));
+    const int err = launched("attn_decode_paged");
+    return err || can ? err : fail(-EIO, "attn_decode_paged: the kernel was built with fewer registers than its roles need");
 }
 
 int ds4b200_attn_window_paged_bf16(const uint16_t *q, int64_t n_tokens, const ds4b200_paged_kv *host_kv,
@@ -679,8 +680,9 @@ int ds4b200_attn_window_paged_bf16(const uint16_t *q, int64_t n_tokens, const ds
     REQUIRE(n_tokens < ((int64_t)1 << 31) / n_heads, "attn_window_paged: n_tokens * n_heads must be below 2^31");
     ds4b200::AttnArgs a{q, *host_kv, page_table, kv_len, q_start, table_width, n_tokens, (int)n_seqs, n_heads, window, n_first,
                         scale, sink, out, lse, workspace};
-    ds4b200::attn_paged(a, STREAM(stream));
-    return launched("attn_window_paged");
+    const bool can = ds4b200::attn_paged(a, STREAM(stream));
+    const int err = launched("attn_window_paged");
+    return err || can ? err : fail(-EIO, "attn_window_paged: the kernel was built with fewer registers than its roles need");
 }
 
 int64_t ds4b200_pages_workspace_bytes(int64_t n_pages, int64_t n_seqs, int64_t n_list) {

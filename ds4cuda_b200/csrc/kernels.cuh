@@ -166,6 +166,6 @@ struct AttnArgs {
 constexpr int kMaxAttnHeads = 1024;
 constexpr int kMaxWindowSeqs = 4096;
 int64_t attn_workspace_bytes(int n_heads, int head_dim);
-void attn_paged(const AttnArgs &a, cudaStream_t s);
+bool attn_paged(const AttnArgs &a, cudaStream_t s);     // false: the kernel cannot be launched as it was built
 
 }  // namespace ds4b200
