@@ -1081,7 +1081,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     for (int i = 0; i < 8; ++i)
                         if (kPre) {
                             const float f0 = __ldg(fac + 8 * i + 2 * (lane & 3)), f1 = __ldg(fac + 8 * i + 2 * (lane & 3) + 1);
-                            v[i] = mul2(v[i], make_float2(f0 > 0.0f ? __fdividef(1.0f, f0) : 0.0f, f1 > 0.0f ? __fdividef(1.0f, f1) : 0.0f));
+                            // A column past the rows has the weight 0 and whatever its factor's place holds: only a factor that the
+                            // packing can have left (0, NaN, kLeast and above) has a reciprocal whose product with 0 is 0.
+                            v[i] = mul2(v[i], make_float2(f0 >= kLeast ? __fdividef(1.0f, f0) : 0.0f, f1 >= kLeast ? __fdividef(1.0f, f1) : 0.0f));
                         } else if (odd_w[buf][i] == n + 1) v[i] = mul2(v[i], *reinterpret_cast<const float2 *>(&row_div[buf][8 * i + 2 * (lane & 3)]));
                 }
                 l = add2(l, add2(add2(add2(v[0], v[1]), add2(v[2], v[3])), add2(add2(v[4], v[5]), add2(v[6], v[7]))));

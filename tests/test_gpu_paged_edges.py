@@ -1,0 +1,32 @@
+"""GPU tests of the paged cache at its edges: workspaces in any state, items of many tiles, sizes and values at a rule's border."""
+import pytest
+import torch
+
+import paged_model as model
+from test_gpu_paged import FMTS, Case, pack_factors
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("heads,lens,toks,window,first", [
+    (64, [200, 90], [200, 90], 100, 3),                  # last tiles of 36 rows that reach past the rows and the 16 zeros behind them
+    (16, [70, 300], [70, 20], 40, 0)])                   # four tokens share a tile's columns
+def test_small_integers_left_in_the_workspace_reach_no_result(ops, fmt, heads, lens, toks, window, first):
+    """As floats they are subnormal: the reciprocal of one is infinite.  Factors are looked at once one row of a call has a factor or
+    no page."""
+    c = Case(ops, fmt, heads, 512, 16, lens, toks, row_scale=lambda j: 1e-4 if j % 3 == 1 and fmt != "f32" else 1.0)
+    c.table[0, 1] = -1
+    for j in range(16, 32):
+        c.slots[0][j] = None
+    c.factors = pack_factors(c)
+    c.tail = 0 if fmt == "f32" else c.tail
+    ws = ops.attn_workspace(heads, 512)
+    ws.zero_()
+    clean = ops.attn_window_paged(c.q, c.kv, c.table, c.kv_len, c.q_start, window=window, n_first=first, workspace=ws)
+    for word in (1, 256, 1 << 20, 0x7f800000):
+        ws.view(torch.int32).fill_(word)
+        out, lse = ops.attn_window_paged(c.q, c.kv, c.table, c.kv_len, c.q_start, window=window, n_first=first, want_lse=True, workspace=ws)
+        c.check(out, lse, window, first, None)
+        assert torch.equal(out, clean)
+    assert ops.device_status() == 0
