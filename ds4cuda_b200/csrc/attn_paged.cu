@@ -271,7 +271,7 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 
 struct Bars {
-    uint64_t full[2][2], s_full[2], s_free[2], p_full[2], pv_done[2][2], scaled[2], q_full, q_free, o_ready[kScaleSets], o_half, o_free[2], quiet[2];
+    uint64_t full[2][2], s_full[2], s_free[2], p_full[2], pv_done[2][2], scaled[2], q_full, q_free, o_ready[kScaleSets], o_half, o_done[2], o_free[2], quiet[2];
     uint64_t seg_full[kSegRing], seg_free[kSegRing], tile_full[kTileRing], tile_free[kTileRing];
 };
 
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         start_tile = 0;
         for (int i = 0; i < 2; ++i) {
             grown_s[i] = odd_s[i] = 0;
-            mbar_init(&bars_s.quiet[i], 1); mbar_init(&bars_s.o_free[i], kLoadWarps);
+            mbar_init(&bars_s.quiet[i], 1); mbar_init(&bars_s.o_done[i], 1); mbar_init(&bars_s.o_free[i], kLoadWarps);
             for (int k = 0; k < kLoadWarps; ++k) odd_w[i][k] = 0;
             mbar_init(&bars_s.scaled[i], kSoftWarps);
             mbar_init(&bars_s.s_full[i], 1); mbar_init(&bars_s.s_free[i], kSoftWarps); mbar_init(&bars_s.p_full[i], kSoftWarps);
@@ -398,7 +398,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         const uint32_t row_off = (uint32_t)(r * 128), sw = (uint32_t)(r & 7);
         // of a load of two rows: which one, and the lane's 16 bytes of its 256; eight consecutive lanes (16 with the 8-byte stores
         // of f32 rows) have to fall on all banks
-        int drained = 0;                                 // tiles of the items whose accumulators are out (packed rows)
         const int half = kF32 ? lane >> 4 : (lane >> 2) & 1, l16 = kF32 ? lane & 15 : (lane & 3) | ((lane >> 3) << 2);
         const bool tail = kBlock && a.kv.n_rot != 0;
         const int n_scales = kBlock ? (D - a.kv.n_rot) / 64 : 1;
@@ -470,14 +469,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             const uint32_t lanes = (uint32_t)(quarter * 32 + which * 16) << 16;
             unsigned char *stage = p_s + 2 * 8192;                          // 32 rows of 128 dims
             auto sync_all = [&]() { asm volatile("bar.sync 4, 256;" ::: "memory"); };
-            struct Rows { int64_t row0; int rows, tiles; };
+            struct Rows { int64_t row0; int rows; };
             auto take = [&](Rows &it) -> bool {
                 Segment sg;
                 if (!next_segment(sg)) return false;
-                it = Rows{sg.it.row0, sg.it.rows, sg.t1 - sg.t0};
+                it = Rows{sg.it.row0, sg.it.rows};
                 return true;
             };
-            Rows cur{0, 0, 0}, next{0, 0, 0};
+            Rows cur{0, 0}, next{0, 0};
             int base = 0;
             bool more = take(next);
             for (int k = -1;; ++k) {
@@ -508,9 +507,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 }
                 if (k >= 0) {                                               // item k's accumulators
                     tc::wait(DS4B200_BAR(o_ready, k & (kScaleSets - 1)), (uint32_t)((k / kScaleSets) & 1), abort_flag, status);
-                    const int last = drained + cur.tiles - 1;               // its last tile
-                    drained = last + 1;
-                    tc::wait(DS4B200_BAR(pv_done, (last & 1) * 2 + kParts - 1), (uint32_t)((last >> 1) & 1), abort_flag, status);
+                    // Not the last tile's pv_done: with up to 384 dims the products of item k + 1 need nothing of this drain, and two tiles
+                    // of them would turn that barrier's parity back.  o_done[k & 1] waits for o_free of item k before its next turn.
+                    tc::wait(DS4B200_BAR(o_done, k & 1), (uint32_t)((k >> 1) & 1), abort_flag, status);
                     tc::fence_after();
                     // rolled up: with all blocks unrolled this loop alone was 30 KB, and the instruction fetches of all roles stalled for it
 #pragma unroll 1
@@ -824,6 +823,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     }
                     tc::commit(one, DS4B200_BAR(pv_done, (buf) * 2 + (kParts - 1)));
                 }
+                if (kPre) tc::commit(one, DS4B200_BAR(o_done, k & 1));
             }
             if (*abort_flag) { tc::commit(one, DS4B200_BAR(quiet, 1)); tc::settle(DS4B200_BAR(quiet, 1), 0); }
         } else if (warp == kMmaWarp + 2) {

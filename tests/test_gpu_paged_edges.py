@@ -30,3 +30,16 @@ def test_small_integers_left_in_the_workspace_reach_no_result(ops, fmt, heads, l
         c.check(out, lse, window, first, None)
         assert torch.equal(out, clean)
     assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("dim", [128, 256, 384])
+def test_packed_items_of_many_and_of_few_tiles_in_turn(ops, fmt, dim):
+    """With up to 384 dims nothing but a barrier of its own keeps the drain of an item's accumulators apart from the products of the next
+    one: long items ahead of short ones and the other way round, repeated."""
+    c = Case(ops, fmt, 64, dim, 64, [900, 40, 700, 30, 1], [120, 40, 60, 30, 1], seed=dim)
+    out, lse = ops.attn_window_paged(c.q, c.kv, c.table, c.kv_len, c.q_start, window=600, n_first=5, sink=c.sink, want_lse=True)
+    c.check(out, lse, 600, 5, c.sink)
+    for _ in range(20):
+        assert torch.equal(ops.attn_window_paged(c.q, c.kv, c.table, c.kv_len, c.q_start, window=600, n_first=5, sink=c.sink), out)
+    assert ops.device_status() == 0
