@@ -304,6 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     __shared__ __align__(16) float fac_s[2][kRows], inv_s[kScaleSets][kRows];
     __shared__ int odd_s[2], odd_w[2][kLoadWarps];  // 1 + the last tile with a row that is not a plain f16 row: of any loader, of each
     __shared__ int grown_s[2];                      // 1 + the last tile with a row that has grown
+    __shared__ int go_s[2][2];                      // see next_segment_together()
     volatile int *abort_flag = &abort_s;
     const uint32_t bars = tc::held(smem_addr(&bars_s));
 #define DS4B200_BAR(name, i) (bars + (uint32_t)offsetof(Bars, name) + 8u * (uint32_t)(i))
@@ -371,16 +372,36 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     }
     tc::fence_after();
 
+    // Whether a wait of this CTA has given up.  Asked behind a wait, with the answer of any lane for all: if it is no, the wait of every lane
+    // has found its phase, and what it waited for may be read.
+    auto gave_up = [&]() -> bool { return __any_sync(0xffffffffu, *abort_flag != 0); };
     // A role takes the segments in order from the ring; every warp of it calls this.
     int seg = 0;
-    auto next_segment = [&](Segment &sg) -> bool {
-        const int i = seg & (kSegRing - 1);
-        tc::wait(DS4B200_BAR(seg_full, i), (uint32_t)((seg / kSegRing) & 1), abort_flag, status);
+    auto take_segment = [&](Segment &sg, int i) -> bool {
         sg = seg_s[i];
         __syncwarp();
         if (lane == 0) tc::arrive(DS4B200_BAR(seg_free, i));
+        return sg.t1 >= 0;
+    };
+    auto next_segment = [&](Segment &sg) -> bool {
+        const int i = seg & (kSegRing - 1);
+        tc::wait(DS4B200_BAR(seg_full, i), (uint32_t)((seg / kSegRing) & 1), abort_flag, status);
         ++seg;
-        return sg.t1 >= 0 && !*abort_flag;
+        return !gave_up() && take_segment(sg, i);
+    };
+    // The same for the warps of a role that meet at named barriers, which have no limit: the first warp waits and says for all whether they go
+    // on, so that none stays behind at a barrier.  Two places in turn: a warp writes the next answer only when all have read the last but one.
+    auto next_segment_together = [&](Segment &sg, int role, bool first, auto &&sync) -> bool {
+        const int i = seg & (kSegRing - 1);
+        int *go = &go_s[role][seg & 1];
+        if (first) {
+            tc::wait(DS4B200_BAR(seg_full, i), (uint32_t)((seg / kSegRing) & 1), abort_flag, status);
+            const bool on = !gave_up();
+            if (lane == 0) *go = on;
+        }
+        sync();
+        ++seg;
+        return *(volatile int *)go != 0 && take_segment(sg, i);
     };
 
     if (warp >= kLoadWarp0 && warp < kLoadWarp0 + kLoadWarps) {
@@ -472,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             struct Rows { int64_t row0; int rows; };
             auto take = [&](Rows &it) -> bool {
                 Segment sg;
-                if (!next_segment(sg)) return false;
+                if (!next_segment_together(sg, 1, lw == 0, sync_all)) return false;
                 it = Rows{sg.it.row0, sg.it.rows};
                 return true;
             };
@@ -562,12 +583,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         uint4 v[kRegs];                                  // [step][row pair]
         float sc[kF32 ? 1 : kRegs];                      // the scale of each
         float4 tl[kBlock ? 4 : 1];
-        struct Slots { int pair[4], own; };              // of rows 2 j + half, and of row r
+        struct Slots { int pair[4], own, rows; };        // of rows 2 j + half, and of row r; tile_rows, -1 also where a wait has given up
         auto slots_of = [&](int n) -> Slots {
             const int i = n & (kTileRing - 1);
             tc::wait(DS4B200_BAR(tile_full, i), (uint32_t)((n / kTileRing) & 1), abort_flag, status);
+            if (gave_up()) return Slots{{-1, -1, -1, -1}, -1, -1};
             const int4 p = *reinterpret_cast<const int4 *>(&slot_s[kPre ? 0 : i][lw * 8 + half * 4]);
-            return Slots{{p.x, p.y, p.z, p.w}, kBlock && tail ? slot_s[kPre ? 0 : i][lw * 8 + ((lane >> 2) & 1) * 4 + (lane >> 3)] : 0};
+            return Slots{{p.x, p.y, p.z, p.w}, kBlock && tail ? slot_s[kPre ? 0 : i][lw * 8 + ((lane >> 2) & 1) * 4 + (lane >> 3)] : 0, tile_rows[i]};
         };
         auto load = [&](int my, bool all, int unit, int step, int j) {      // all: of the warp's rows exist
             const int k = step * 4 + j;
@@ -595,21 +617,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 }
         };
         Slots here = slots_of(0);
-        int rows = tile_rows[0];
-        if (rows >= 0) {
+        if (here.rows >= 0) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int step = 0; step < kSteps; ++step) load(here.pair[j], false, 0, step, j);
             load_tail(here.own);
         }
-        for (int n = 0, nq = 0; rows >= 0 && !*abort_flag; ++n) {
+        for (int n = 0, nq = 0; here.rows >= 0; ++n) {
             const int buf = n & 1, ring = n & (kTileRing - 1);
             const uint32_t use = (uint32_t)(((n >> 1) & 1) ^ 1);
             unsigned char *dst = k_s + buf * kTileBytes;
-            if (rows) load_query(tile_row0[ring], rows, nq++);              // a segment's query rows come ahead of its first tile
+            if (here.rows) load_query(tile_row0[ring], here.rows, nq++);    // a segment's query rows come ahead of its first tile
             const Slots next = slots_of(n + 1);          // the tile behind this one
-            const int next_rows = tile_rows[(n + 1) & (kTileRing - 1)];
             const bool all_here = kUnits > 1 && __all_sync(0xffffffffu, (here.pair[0] | here.pair[1] | here.pair[2] | here.pair[3]) >= 0);
             const bool all_next = __all_sync(0xffffffffu, (next.pair[0] | next.pair[1] | next.pair[2] | next.pair[3]) >= 0);
             // The MMA warp makes the stores visible to the async proxy: a proxy fence here would wait for the loads in flight.
@@ -708,7 +728,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                             }
                         }
                         if (unit + 1 < kUnits) load(here.pair[j], all_here, unit + 1, step, j);
-                        else if (next_rows >= 0) load(next.pair[j], all_next, 0, step, j);
+                        else if (next.rows >= 0) load(next.pair[j], all_next, 0, step, j);
                     }
                 }
             if (kBlock && tail) {
@@ -727,7 +747,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 unsigned char *to = dst + (kChunks - 1) * 8192 + row_off;
                 *reinterpret_cast<uint4 *>(to + (((uint32_t)(part * 2) ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
                 *reinterpret_cast<uint4 *>(to + (((uint32_t)(part * 2 + 1) ^ sw) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
-                if (next_rows >= 0) load_tail(next.own);
+                if (next.rows >= 0) load_tail(next.own);
             }
             // Several tokens share the tile, and 0 * NaN would reach the ones that do not see the row: it has zeros where it is not finite, and
             // the factor NaN for those that see it.
@@ -748,7 +768,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             hand_over(kParts - 1);
             if (lane == 0) tc::arrive(DS4B200_BAR(tile_free, ring));
             here = next;
-            rows = next_rows;
         }
         }
     } else if (warp >= kMmaWarp) {
@@ -786,7 +805,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 }
                 tc::commit(one, DS4B200_BAR(q_free, 0));
             }
-            if (*abort_flag) { tc::commit(one, DS4B200_BAR(quiet, 0)); tc::settle(DS4B200_BAR(quiet, 0), 0); }
+            if (gave_up()) { tc::commit(one, DS4B200_BAR(quiet, 0)); tc::settle(DS4B200_BAR(quiet, 0), 0); }
         } else if (warp == kMmaWarp + 1) {
             // -------------------------------------------------------------------------- O^T += V^T P^T
             const uint32_t v_desc = tc::desc_lo(smem_addr(k_s), 8192), p_desc = tc::desc_lo(smem_addr(p_s), 0);
@@ -825,7 +844,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 }
                 if (kPre) tc::commit(one, DS4B200_BAR(o_done, k & 1));
             }
-            if (*abort_flag) { tc::commit(one, DS4B200_BAR(quiet, 1)); tc::settle(DS4B200_BAR(quiet, 1), 0); }
+            if (gave_up()) { tc::commit(one, DS4B200_BAR(quiet, 1)); tc::settle(DS4B200_BAR(quiet, 1), 0); }
         } else if (warp == kMmaWarp + 2) {
             // -------------------------------------------------------------------------- schedule
             int slot = g.split ? start_slot : (int)blockIdx.x, tile = g.split ? start_tile : 0;
@@ -850,20 +869,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 }
                 const int i = seg & (kSegRing - 1);
                 tc::wait<300>(DS4B200_BAR(seg_free, i), (uint32_t)(((seg / kSegRing) & 1) ^ 1), abort_flag, status, tc::kWaitPolls + 16 * longest);
+                if (gave_up()) break;                    // the place may still be read
                 if (lane == 0) {
                     if (kPre && !end) prefetch_l2(a.q + sg.it.row0 * D, sg.it.rows * D * 2);     // some items before they are wanted
                     seg_s[i] = sg;
                     tc::arrive(DS4B200_BAR(seg_full, i));
                 }
                 __syncwarp();
-                if (*abort_flag) break;
             }
         } else if (kPre) {
             // -------------------------------------------------------------------------- copy packed rows
             Segment sg;
-            int n = 0;
-            while (next_segment(sg)) {
-                for (int t = sg.t0; t < sg.t1; ++t, ++n) {
+            int n = 0, sent = 0;                         // parts of tiles
+            bool stop = false;
+            while (!stop && next_segment(sg)) {
+                for (int t = sg.t0; t < sg.t1 && !stop; ++t, ++n) {
                     const int buf = n & 1, ta = first_run_tiles(sg.it);
                     const int from = t < ta ? sg.it.at_a + 64 * t : sg.it.at_b + 64 * (t - ta);
                     // up to 16 rows (the MMAs read no more of them either), e.g. the first rows beside a window of 128
@@ -871,6 +891,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 #pragma unroll
                     for (int part = 0; part < kParts; ++part) {
                         tc::wait<20>(DS4B200_BAR(pv_done, buf * 2 + part), (uint32_t)(((n >> 1) & 1) ^ 1), abort_flag, status);
+                        stop = stop || gave_up();
+                        if (stop) continue;              // the last copy to this place may be in flight
+                        ++sent;
                         if (lane == 0) {
                             constexpr int kFirst = kParts > 1 ? 2 * kPart0 : kChunks;
                             const int c0 = part * kFirst, c1 = part ? kChunks : kFirst;
@@ -882,9 +905,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     }
                 }
             }
-            if (*abort_flag)                             // no copy is in flight when the kernel ends
-                for (int k = max(n - 2, 0); k < n; ++k)
-                    for (int part = 0; part < kParts; ++part) tc::settle(DS4B200_BAR(full, (k & 1) * 2 + part), (uint32_t)((k >> 1) & 1));
+            if (gave_up())                               // no copy is in flight when the kernel ends
+                for (int q = max(sent - 2 * kParts, 0); q < sent; ++q) {
+                    const int k = q / kParts;
+                    tc::settle(DS4B200_BAR(full, (k & 1) * 2 + q % kParts), (uint32_t)((k >> 1) & 1));
+                }
         } else {
             // -------------------------------------------------------------------------- find
             // The pool rows of the tiles to come, two per lane, up to kTileRing tiles ahead of the loaders: a page-table entry, and the first
@@ -894,11 +919,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             Segment sg;
             int n = 0;
             for (bool more = true; more;) {
+                sg.t0 = 0;
                 more = next_segment(sg);
                 const int t1 = more ? sg.t1 : sg.t0 + 1;                    // one more entry says that it ends
                 for (int t = sg.t0; t < t1; ++t, ++n) {
                     const int i = n & (kTileRing - 1);
                     tc::wait<300>(DS4B200_BAR(tile_free, i), (uint32_t)(((n / kTileRing) & 1) ^ 1), abort_flag, status);
+                    if (gave_up()) { more = false; break; }                 // the place may still be read
                     if (lane == 0) {
                         tile_rows[i] = !more ? -1 : t == sg.t0 ? sg.it.rows : 0;
                         tile_row0[i] = sg.it.row0;
@@ -936,7 +963,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     if (more && t == sg.t0 && lane == 0) prefetch_l2(a.q + sg.it.row0 * D, sg.it.rows * D * 2);    // the segment's query rows
                     __syncwarp();
                     if (lane == 0) tc::arrive(DS4B200_BAR(tile_full, i));
-                    if (*abort_flag) more = false;
                 }
             }
         }
@@ -957,7 +983,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         int n = 0;
         long long done = 0;
         int base = 0;
-        for (int nq = 0; next_segment(sg); ++nq, base = next_base(base)) {
+        for (int nq = 0; next_segment_together(sg, 0, warp == 0, sync_all); ++nq, base = next_base(base)) {
             const Item &it = sg.it;
             float qk = 0.0f, m = -INFINITY;
             float2 l = make_float2(0.0f, 0.0f);
