@@ -1367,7 +1367,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) attn_join_kernel(const Att
 
 // The rows a chunk's tokens see, once each, as packed f16 rows: with a window of 128 rows every row is wanted by 128 tokens, and turning it into
 // f16 for each of them cost more than all the rest (4096 tokens: 294 us straight from the cache).  One warp per row.
-// A row whose largest value is outside [2^-9, 2^15] is scaled by a power of two, its factor; a hole has the factor 0, a row with a value
+// A row of codes whose largest value is outside [2^-9, 2^15] is scaled by a power of two, its factor; f32 rows become f16 numbers as they
+// do straight from the cache (beyond +-65504 that), so a token's rows do not depend on the path; a hole has the factor 0, a row with a value
 // that is not finite NaN, with zeros in place of such values, so that it reaches the tokens that see it and no others.
 template <int V>      // float4s of a row per lane: head_dim / 128
 __global__ void __launch_bounds__(kPackWarps * 32) attn_pack_kernel(const AttnArgs a, int64_t bound, uint16_t *rows, float *fac, int *odd) {
@@ -1421,13 +1422,13 @@ __global__ void __launch_bounds__(kPackWarps * 32) attn_pack_kernel(const AttnAr
             for (int j = 0; j < V; ++j) r[j] = make_float4(0.f, 0.f, 0.f, 0.f);
         } else {
             top = warp_max(top);
-            if (top != 0.0f && (top < 0x1p-9f || top > 0x1p15f)) pow2_parts(fmaxf(top, kLeast), f, down);
+            if (a.kv.row_format != DS4B200_KV_F32 && top != 0.0f && (top < 0x1p-9f || top > 0x1p15f)) pow2_parts(fmaxf(top, kLeast), f, down);
         }
         met = met || f != 1.0f;
         if (lane == 0) fac[row] = f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const uint2 u = make_uint2(h2_bits(__floats2half2_rn(r[j].x * down, r[j].y * down)), h2_bits(__floats2half2_rn(r[j].z * down, r[j].w * down)));
+            const uint2 u = make_uint2(sat_h2(r[j].x * down, r[j].y * down), sat_h2(r[j].z * down, r[j].w * down));
             *reinterpret_cast<uint2 *>(rows + row * dim + 4 * (lane + 32 * j)) = u;
         }
     }

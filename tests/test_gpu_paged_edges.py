@@ -43,3 +43,23 @@ def test_packed_items_of_many_and_of_few_tiles_in_turn(ops, fmt, dim):
     for _ in range(20):
         assert torch.equal(ops.attn_window_paged(c.q, c.kv, c.table, c.kv_len, c.q_start, window=600, n_first=5, sink=c.sink), out)
     assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("heads", [64, 16])
+def test_f32_rows_are_f16_numbers_on_every_path(ops, heads):
+    """Values beyond f16's range and below its normal numbers: 65504 and subnormals, whether the call packs its rows first or not."""
+    c = Case(ops, "f32", heads, 512, 64, [200, 120], [100, 100], row_scale=lambda j: 1e5 / 3 if j % 3 else 1.0)
+    c.st["raw"].nan_to_num_(nan=0.0, posinf=9e4, neginf=-9e4)
+    tiny = torch.tensor(c.slots[1], device="cuda")
+    c.st["raw"][tiny] = torch.randn((120, 512), generator=torch.Generator(device="cuda").manual_seed(3), device="cuda") * 2e-6
+    c.rows = c.st["raw"].clamp(-65504, 65504).half().double()
+    assert bool((c.st["raw"].abs() > 65504).any()) and bool((c.rows[tiny] != c.st["raw"][tiny].double()).any())
+    scale = 1e-5
+    long = ops.attn_window_paged(c.q, c.kv, c.table, c.kv_len, c.q_start, window=64, scale=scale)
+    c.check(long, None, 64, 0, None, scale=scale)
+    # the same tokens as sequences of their own, straight from the cache
+    table = c.table.repeat_interleave(100, 0).contiguous()
+    lens = torch.tensor([p + 1 for p in c.positions], dtype=torch.int32, device="cuda")
+    short = ops.attn_decode_paged(c.q, c.kv, table, lens, window=64, scale=scale)
+    c.check(short, None, 64, 0, None, scale=scale)
+    assert heads < 64 or torch.equal(short, long)        # at 64 heads the same tiles in the same order
