@@ -153,11 +153,12 @@ __global__ void __launch_bounds__(kPlanThreads) plan_fork_kernel(Tables t, const
 __global__ void __launch_bounds__(kPlanThreads) plan_reserve_kernel(Tables t, const int *new_lens, Work w, int *status) {
     __shared__ int scratch[33];
     __shared__ int bad;
+    __shared__ unsigned long long asked;
     launch_dependents();
     const int tid = threadIdx.x;
-    if (tid == 0) bad = 0;
+    if (tid == 0) { bad = 0; asked = 0; }
     __syncthreads();
-    int64_t need = 0;
+    int64_t need = 0, mine = 0;                     // pages: before this round of sequences, cut at the pool's size; of this thread's, all
     const int64_t most = t.width * t.page_rows;
     for (int64_t base = 0; base < t.n_seqs; base += kPlanThreads) {
         const int64_t b = base + tid;
@@ -165,7 +166,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_reserve_kernel(Tables t, co
         if (b < t.n_seqs) {
             const int64_t len = t.lens_in[b], want = max(len, (int64_t)new_lens[b]);
             if (len < 0 || want > most) bad = 1;
-            else k = (int)min(pages_of(want, t.page_rows) - pages_of(len, t.page_rows), t.n_pages + 1);
+            else {
+                const int64_t more = pages_of(want, t.page_rows) - pages_of(len, t.page_rows);
+                k = (int)min(more, t.n_pages + 1);
+                mine += more;
+            }
             if (!bad) w.mark[b] = (int)pages_of(len, t.page_rows);
         }
         int total;
@@ -174,11 +179,12 @@ __global__ void __launch_bounds__(kPlanThreads) plan_reserve_kernel(Tables t, co
         if (b < t.n_seqs) w.first[b] = (int)min(need + r, t.n_pages);
         need += total;
     }
+    atomicAdd(&asked, (unsigned long long)mine);
     __syncthreads();
     const int ask = (int)min(need, t.n_pages);
     const int found = bad ? 0 : collect_free(t, ask, w.fresh, scratch);
     __syncthreads();
-    const int st = bad ? -1 : (int)min(need - found, (int64_t)0x7fffffff);
+    const int st = bad ? -1 : (int)min((int64_t)asked - found, (int64_t)0x7fffffff);
     copy_refs(t);
     __syncthreads();
     if (st == 0)

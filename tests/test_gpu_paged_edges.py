@@ -63,3 +63,19 @@ def test_f32_rows_are_f16_numbers_on_every_path(ops, heads):
     short = ops.attn_decode_paged(c.q, c.kv, table, lens, window=64, scale=scale)
     c.check(short, None, 64, 0, None, scale=scale)
     assert heads < 64 or torch.equal(short, long)        # at 64 heads the same tiles in the same order
+
+
+@pytest.mark.parametrize("n_pages,page,width,used,want", [
+    (4, 4, 10, 0, [40, 0]),                              # one sequence that asks for more than the pool has
+    (4, 4, 10, 3, [9, 40]), (1, 1, 7, 1, [7] * 2500), (50, 2, 40, 20, [80, 80])])
+def test_reserve_counts_every_missing_page(ops, n_pages, page, width, used, want):
+    t = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    n = len(want)
+    m = model.Pages([1] * used + [0] * (n_pages - used), [[-1] * width] * n, [0] * n, page)
+    m.reserve(want)
+    assert m.status > 0
+    pool = ops.PagePool([], page, n, width, n_pages=n_pages)
+    refs, table, lens = t(m.refs), t(m.table), t(m.lens)
+    out = ops.pages_reserve(pool, refs, table, lens, t(want))
+    assert out[3].item() == m.status
+    assert out[0].tolist() == m.refs and out[1].tolist() == m.table and out[2].tolist() == m.lens
