@@ -689,6 +689,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 }
                 if (kBlock) down = 1.0f / mine;
             }
+            // A scale of a whole row is any number, and below 2^-14 f16 would keep too few of its bits (2^-8 of it at 2^-17): such a row's codes take
+            // 2^8 times it, and 2^-8 behind that, which costs at most half of f16's smallest step.
+            bool fine = false;
+            if (FMT == DS4B200_KV_FP8_ROW) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) fine = fine || sc[kF32 ? 0 : j] < 0x1p-14f;
+                fine = __any_sync(0xffffffffu, fine) && !odd;
+            }
             uint32_t spoilt = 0;                         // bit j: row 2 j + half has a value that is not finite
             const int rw = lw * 8 + half;
 #pragma unroll
@@ -712,13 +720,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                                 make_uint2(o[0], o[1]);
                         } else {
                             const int c = c0 + (l16 >> 2);
-                            const __half2 f = __float2half2_rn(sc[kF32 ? 0 : step * 4 + j]);
+                            const float scale = sc[kF32 ? 0 : step * 4 + j];
+                            const bool up = fine && scale < 0x1p-14f;
+                            const __half2 f = __float2half2_rn(up ? scale * 0x1p8f : scale);
                             uint32_t o[8];
                             const uint32_t y[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                             for (int k = 0; k < 4; ++k) e4m3x4(y[k], o[2 * k], o[2 * k + 1]);
 #pragma unroll
                             for (int k = 0; k < 8; ++k) o[k] = h2_bits(__hmul2(*reinterpret_cast<__half2 *>(&o[k]), f));
+                            if (FMT == DS4B200_KV_FP8_ROW && fine) {
+                                const __half2 back = __float2half2_rn(up ? 0x1p-8f : 1.0f);
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) o[k] = h2_bits(__hmul2(*reinterpret_cast<__half2 *>(&o[k]), back));
+                            }
                             if (c < kChunks && !(tail && c == kChunks - 1)) {
                                 if (SHARED && several) spoilt |= (uint32_t)drop_nonfinite(o) << j;
                                 unsigned char *to = dst + c * 8192 + (rw + 2 * j) * 128;

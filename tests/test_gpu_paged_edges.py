@@ -79,3 +79,24 @@ def test_reserve_counts_every_missing_page(ops, n_pages, page, width, used, want
     out = ops.pages_reserve(pool, refs, table, lens, t(want))
     assert out[3].item() == m.status
     assert out[0].tolist() == m.refs and out[1].tolist() == m.table and out[2].tolist() == m.lens
+
+
+@pytest.mark.parametrize("toks", [None, [3, 2, 1] * 8])
+def test_row_scales_below_f16s_normal_numbers_keep_their_bits(ops, toks):
+    """Scales of 2^-17 to 2^-13 (rows of up to 2^-8 to 2^-4) and, beside them in a tile, larger ones; queries along a row, so that a
+    scale that is off moves every score the same way."""
+    lens = [1, 20, 3] * 8 if toks is None else [9, 20, 70] * 8
+    c = Case(ops, "row", 16, 128, 4, lens, toks)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    for slots in c.slots:
+        at = torch.tensor(slots, device="cuda")
+        c.st["scales"][at] = torch.exp2(torch.rand((len(slots), 1), generator=g, device="cuda") * 4 - 17)
+        c.st["scales"][at[-1]] = 2.0 ** -17 * (1 + 2.0 ** -8)          # half a step off in f16
+    c.rows = model.row_values("row", c.st)
+    for t, slots in enumerate(c.slots_of):
+        c.q[t] = torch.sign(c.rows[slots[-1]])[None].bfloat16()
+    scale = 30.0 / max(c.rows[s[-1]].abs().sum().item() for s in c.slots)
+    call = ops.attn_decode_paged if toks is None else ops.attn_window_paged
+    args = (c.q, c.kv, c.table, c.kv_len) + (() if toks is None else (c.q_start,))
+    out, lse = call(*args, scale=scale, want_lse=True)
+    c.check(out, lse, 0, 0, None, scale=scale)
