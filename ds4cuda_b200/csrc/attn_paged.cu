@@ -218,6 +218,13 @@ __device__ __forceinline__ void pow2_parts(float x, float &up, float &down) {
     down = __uint_as_float((uint32_t)(127 - e) << 23);
 }
 
+// A sink in log2 units, held within f32: beyond that it is heavier, or lighter, than every row all the same.  NaN stays.
+__device__ __forceinline__ float sink_log2(float sink) {
+    constexpr float most = 3.402823466e38f;
+    const float x = sink * kLog2e;
+    return x == x ? fminf(fmaxf(x, -most), most) : x;
+}
+
 // What the scheduling warp hands to the others: an item and the tiles [t0, t1) of it that this CTA takes; t1 < 0 ends.
 struct Segment {
     Item it;
@@ -1140,18 +1147,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
             const bool whole = sg.t0 == 0 && sg.t1 == it.tiles;
             const int part = 2 * (int)blockIdx.x + (sg.t0 == 0 ? 1 : 0);
-            float inv = 1.0f, lse2 = 0.0f;
+            float inv = 1.0f, lse = 0.0f;
             if (whole) {
-                lse2 = sum > 0.0f ? m + __log2f(sum) : (sum == sum ? -INFINITY : sum);
+                float lse2 = sum > 0.0f ? m + __log2f(sum) : (sum == sum ? -INFINITY : sum);
+                lse = lse2 * (1.0f / kLog2e);
                 if (a.sink && row < it.rows) {
-                    const float own = lse2, s2 = __ldg(a.sink + it.h0 + (several ? row % a.n_heads : row)) * kLog2e, hi = fmaxf(own, s2);
-                    if (hi > -INFINITY) lse2 = hi + __log2f(tc::exp2_approx(own - hi) + tc::exp2_approx(s2 - hi));
+                    const float own = lse2, sink = __ldg(a.sink + it.h0 + (several ? row % a.n_heads : row)), s2 = sink_log2(sink);
+                    const bool heavy = s2 >= own;        // then the sum is the sink and a little
+                    const float hi = heavy ? s2 : own, more = __log2f(1.0f + tc::exp2_approx((heavy ? own : s2) - hi));
+                    lse2 = hi + more;
+                    lse = heavy ? sink + more * (1.0f / kLog2e) : lse2 * (1.0f / kLog2e);
                 }
                 inv = m == -INFINITY ? 0.0f : tc::exp2_approx(m - lse2);
             }
             if (kPre) {                                  // the loaders drain the accumulators
                 if ((lane & 3) == 0) {
-                    if (a.lse && row < it.rows) a.lse[it.row0 + row] = lse2 * (1.0f / kLog2e);
+                    if (a.lse && row < it.rows) a.lse[it.row0 + row] = lse;
                     inv_s[nq & (kScaleSets - 1)][row] = inv;
                 }
                 __syncwarp();
@@ -1163,7 +1174,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
             tc::fence_after();
             if ((lane & 3) == 0) {
                 if (!whole) g.part_ml[part * kRows + row] = make_float2(m, sum);
-                else if (a.lse && row < it.rows) a.lse[it.row0 + row] = lse2 * (1.0f / kLog2e);
+                else if (a.lse && row < it.rows) a.lse[it.row0 + row] = lse;
                 inv_s[0][row] = inv;
             }
             sync_all();
@@ -1272,7 +1283,11 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) attn_join_kernel(const Att
     }
     __syncthreads();
     auto part_of = [](int c, int k) { return k == 0 ? 2 * c + 1 : 2 * (c + k); };
-    auto sink_of = [&](const Meta &it, int row) { return a.sink ? __ldg(a.sink + it.h0 + row % a.n_heads) * kLog2e : -INFINITY; };
+    auto sink_of = [&](const Meta &it, int row) { return a.sink ? __ldg(a.sink + it.h0 + row % a.n_heads) : -INFINITY; };
+    // of a sum l relative to 2^top
+    auto lse_of = [](float l, float top, float sink, float sink2) {
+        return l == 0.0f ? -INFINITY : sink2 == top ? sink + __log2f(l) * (1.0f / kLog2e) : (top + __log2f(l)) * (1.0f / kLog2e);
+    };
 
     for (int u = blockIdx.x * kJoinWarps + warp; u < n_begun[0] * kRows; u += gridDim.x * kJoinWarps) {
         const int c = begun[0][u / kRows], row = u % kRows;
@@ -1280,7 +1295,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) attn_join_kernel(const Att
         if (row >= it.rows) continue;
         float2 ml = make_float2(-INFINITY, 0.0f);
         if (lane < it.parts) ml = part_ml[part_of(c, lane) * kRows + row];
-        const float sink2 = sink_of(it, row);
+        const float sink = sink_of(it, row), sink2 = a.sink ? sink_log2(sink) : -INFINITY;
         float4 x[2][4], o[4];
         auto load = [&](int k) {
 #pragma unroll
@@ -1297,7 +1312,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) attn_join_kernel(const Att
         const float top = fmaxf(warp_max(ml.x), sink2);
         const float w = ml.x == -INFINITY ? 0.0f : tc::exp2_approx(ml.x - top);
         float l = warp_sum(w * ml.y);
-        if (sink2 > -INFINITY) l += tc::exp2_approx(sink2 - top);
+        if (a.sink) l += tc::exp2_approx(sink2 - top);
         for (int k = 0; k < it.parts; k += 2) {
             if (k) load(k);
 #pragma unroll
@@ -1311,7 +1326,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) attn_join_kernel(const Att
 #pragma unroll
         for (int s = 0; s < 4; ++s)
             if (s < slices) st_bf16x4(a.out + (it.row0 + row) * D + s * 128 + lane * 4, make_float4(o[s].x * inv, o[s].y * inv, o[s].z * inv, o[s].w * inv));
-        if (lane == 0 && a.lse) a.lse[it.row0 + row] = (l == 0.0f ? -INFINITY : top + __log2f(l)) * (1.0f / kLog2e);
+        if (lane == 0 && a.lse) a.lse[it.row0 + row] = lse_of(l, top, sink, sink2);
     }
 
     // SL slices of 128 dims in a CTA: all four where there are more rows than slices would leave CTAs for
@@ -1325,7 +1340,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) attn_join_kernel(const Att
             if (row >= it.rows) continue;
             float2 ml = make_float2(-INFINITY, 0.0f);
             if (tid < parts) ml = part_ml[part_of(c, tid) * kRows + row];
-            const float sink2 = sink_of(it, row);
+            const float sink = sink_of(it, row), sink2 = a.sink ? sink_log2(sink) : -INFINITY;
             float4 x[kBatch][SL], o[SL];
             auto load = [&](int k0) {
 #pragma unroll
@@ -1363,7 +1378,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) attn_join_kernel(const Att
             for (int s = 0; s < SL; ++s) sums[s][warp][lane] = o[s];
             __syncthreads();
             if (warp < SL) {
-                float l = sink2 > -INFINITY ? tc::exp2_approx(sink2 - top) : 0.0f;
+                float l = a.sink ? tc::exp2_approx(sink2 - top) : 0.0f;
 #pragma unroll
                 for (int i = 0; i < kJoinWarps; ++i) l += sum_s[i];
                 float4 y = sums[warp][0][lane];
@@ -1371,7 +1386,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) attn_join_kernel(const Att
                 for (int i = 1; i < kJoinWarps; ++i) add_scaled(y, 1.0f, sums[warp][i][lane]);
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                 st_bf16x4(a.out + (it.row0 + row) * D + (slice + warp) * 128 + lane * 4, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
-                if (lane == 0 && slice + warp == 0 && a.lse) a.lse[it.row0 + row] = (l == 0.0f ? -INFINITY : top + __log2f(l)) * (1.0f / kLog2e);
+                if (lane == 0 && slice + warp == 0 && a.lse) a.lse[it.row0 + row] = lse_of(l, top, sink, sink2);
             }
             __syncthreads();                             // sums and sum_s are read
         }

@@ -100,3 +100,37 @@ def test_row_scales_below_f16s_normal_numbers_keep_their_bits(ops, toks):
     args = (c.q, c.kv, c.table, c.kv_len) + (() if toks is None else (c.q_start,))
     out, lse = call(*args, scale=scale, want_lse=True)
     c.check(out, lse, 0, 0, None, scale=scale)
+
+
+@pytest.mark.parametrize("how", ["whole", "cut, few parts", "cut, many parts", "packed", "no rows"])
+def test_sinks_of_every_size(ops, how):
+    """The largest and lowest f32 values and infinities count as what they are: a sink that outweighs all rows leaves an output of 0 and
+    is the log-sum, a lowest one leaves the rows as they are, and without rows the log-sum is the sink to the bit."""
+    top, inf = torch.finfo(torch.float32).max, float("inf")
+    lens = {"whole": [100, 3], "cut, few parts": [1000] * 50, "cut, many parts": [20000, 5], "packed": [90, 90], "no rows": [0, 0]}[how]
+    c = Case(ops, "f32", 16, 128, 64, lens, [80, 80] if how == "packed" else None, width=None if lens[0] else 8)
+    sink = torch.tensor([-top, top, inf, -inf, -1e38, 1e38, -1e30, 1e30, 0.0, 3.0, -90.0, 90.0, 1e-45, -0.0, 2.5e38, -2.5e38], device="cuda")
+    args = (c.q, c.kv, c.table, c.kv_len)
+    call = lambda **kw: ops.attn_window_paged(*args, c.q_start, want_lse=True, **kw) if how == "packed" else ops.attn_decode_paged(*args, want_lse=True, **kw)
+    out, lse = call(sink=sink)
+    if how == "no rows":
+        assert not out.any() and torch.equal(lse, sink.expand_as(lse))
+        return
+    bare, bare_lse = call()
+    heavy, light = [1, 2, 5, 7, 14], [0, 3, 4, 6, 15]
+    assert not out[:, heavy].any() and torch.equal(lse[:, heavy], sink[heavy].expand(len(c.q), 5))
+    assert torch.equal(out[:, light], bare[:, light])
+    assert torch.allclose(lse[:, light], bare_lse[:, light], rtol=0, atol=1e-5)
+    rest = [8, 9, 10, 11, 12, 13]
+    c.q, small = c.q[:, rest].contiguous(), sink[rest]
+    c.check(out[:, rest], lse[:, rest], 0, 0, small)
+
+
+@pytest.mark.parametrize("lens", [[100, 3], [20000, 5]])
+def test_a_sink_that_is_not_a_number_spoils_its_head_only(ops, lens):
+    c = Case(ops, "f32", 16, 128, 64, lens)
+    c.sink[5] = float("nan")
+    out, lse = ops.attn_decode_paged(c.q, c.kv, c.table, c.kv_len, sink=c.sink, want_lse=True)
+    others = [h for h in range(16) if h != 5]
+    assert bool(out[:, 5].isnan().all()) and bool(lse[:, 5].isnan().all())
+    assert not out[:, others].isnan().any() and not lse[:, others].isnan().any()
