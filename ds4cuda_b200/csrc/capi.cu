@@ -623,7 +623,7 @@ int64_t ds4b200_attn_workspace_bytes(int n_heads, int head_dim) {
 
 static int check_attn(const char *what, const ds4b200_paged_kv *kv, const void *q, const void *out, const void *page_table,
                       int64_t table_width, const void *kv_len, int64_t n_seqs, int n_heads, float scale, int window,
-                      int n_first, const void *workspace, int64_t workspace_bytes) {
+                      int n_first, const void *sink, const void *lse, const void *workspace, int64_t workspace_bytes) {
     REQUIRE(kv && q && out && page_table && kv_len && workspace, "%s: null pointer", what);
     REQUIRE(kv->row_format == DS4B200_KV_FP8_BLOCK64 || kv->row_format == DS4B200_KV_FP8_ROW || kv->row_format == DS4B200_KV_F32,
             "%s: unknown row format", what);
@@ -641,6 +641,7 @@ static int check_attn(const char *what, const ds4b200_paged_kv *kv, const void *
         }
     }
     REQUIRE(a16(q) && a16(out) && a16(workspace), "%s: q, out and workspace need 16-byte alignment", what);
+    REQUIRE(a4(page_table) && a4(kv_len) && a4(sink) && a4(lse), "%s: page_table, kv_len, sink and lse need 4-byte alignment", what);
     REQUIRE(table_width >= 1 && table_width <= (INT32_MAX - 64) / kv->page_rows, "%s: table_width * page_rows must be in [1, 2^31 - 64)", what);
     REQUIRE(n_seqs <= ds4b200::kMaxWindowSeqs, "%s: at most 4096 sequences per call", what);
     REQUIRE(n_heads >= 1 && n_heads <= ds4b200::kMaxAttnHeads, "%s: n_heads must be in [1, 1024]", what);
@@ -657,7 +658,7 @@ int ds4b200_attn_decode_paged_bf16(const uint16_t *q, const ds4b200_paged_kv *ho
     REQUIRE(n_seqs >= 0, "attn_decode_paged: n_seqs < 0");
     if (n_seqs == 0) return 0;
     const int rc = check_attn("attn_decode_paged", host_kv, q, out, page_table, table_width, kv_len, n_seqs, n_heads, scale,
-                              window, n_first, workspace, workspace_bytes);
+                              window, n_first, sink, lse, workspace, workspace_bytes);
     if (rc) return rc;
     ds4b200::AttnArgs a{q, *host_kv, page_table, kv_len, nullptr, table_width, n_seqs, (int)n_seqs, n_heads, window, n_first,
                         scale, sink, out, lse, workspace};
@@ -674,9 +675,9 @@ int ds4b200_attn_window_paged_bf16(const uint16_t *q, int64_t n_tokens, const ds
     REQUIRE(n_seqs >= 0 && n_tokens >= 0, "attn_window_paged: negative size");
     if (n_seqs == 0 || n_tokens == 0) return 0;
     const int rc = check_attn("attn_window_paged", host_kv, q, out, page_table, table_width, kv_len, n_seqs, n_heads, scale,
-                              window, n_first, workspace, workspace_bytes);
+                              window, n_first, sink, lse, workspace, workspace_bytes);
     if (rc) return rc;
-    REQUIRE(q_start, "attn_window_paged: null pointer");
+    REQUIRE(q_start && a4(q_start), "attn_window_paged: q_start missing or not 4-byte aligned");
     REQUIRE(n_tokens < ((int64_t)1 << 31) / n_heads, "attn_window_paged: n_tokens * n_heads must be below 2^31");
     ds4b200::AttnArgs a{q, *host_kv, page_table, kv_len, q_start, table_width, n_tokens, (int)n_seqs, n_heads, window, n_first,
                         scale, sink, out, lse, workspace};
@@ -705,6 +706,8 @@ static int check_tables(const char *what, const ds4b200::PageTables &t, bool len
     REQUIRE(t.width >= 1 && t.width < ((int64_t)1 << 31) / t.page_rows, "%s: table_width * page_rows must be in [1, 2^31)", what);
     REQUIRE(t.n_pages == 0 || (t.refs_in && t.refs_out), "%s: null pointer", what);
     REQUIRE(t.n_seqs == 0 || (t.table_in && t.table_out && (!lens || (t.lens_in && t.lens_out))), "%s: null pointer", what);
+    REQUIRE(a4(t.refs_in) && a4(t.refs_out) && a4(t.table_in) && a4(t.table_out) && a4(t.lens_in) && a4(t.lens_out),
+            "%s: refs, table and lens need 4-byte alignment", what);
     return 0;
 }
 static int check_arrays(const char *what, const ds4b200_page_array *host_arrays, int n_arrays) {
@@ -752,7 +755,7 @@ int ds4b200_pages_reserve(int64_t n_pages, int page_rows, const int32_t *refs_in
     const ds4b200::PageTables t{refs_in, refs_out, table_in, table_out, lens_in, lens_out, n_pages, n_seqs, table_width, page_rows};
     CHECKED(check_pages("pages_reserve", n_pages, n_seqs, 0, status, workspace, workspace_bytes));
     CHECKED(check_tables("pages_reserve", t, true));
-    REQUIRE(n_seqs == 0 || new_lens, "pages_reserve: null pointer");
+    REQUIRE(n_seqs == 0 || (new_lens && a4(new_lens)), "pages_reserve: new_lens missing or not 4-byte aligned");
     ds4b200::pages_reserve(t, new_lens, status, workspace, STREAM(stream));
     return launched("pages_reserve");
 }
@@ -764,7 +767,7 @@ int ds4b200_pages_free(int64_t n_pages, int page_rows, const int32_t *refs_in, i
     const ds4b200::PageTables t{refs_in, refs_out, table_in, table_out, lens_in, lens_out, n_pages, n_seqs, table_width, page_rows};
     CHECKED(check_pages("pages_free", n_pages, n_seqs, n_list, status, workspace, workspace_bytes));
     CHECKED(check_tables("pages_free", t, true));
-    REQUIRE(n_list == 0 || seqs, "pages_free: null pointer");
+    REQUIRE(n_list == 0 || (seqs && a4(seqs)), "pages_free: seqs missing or not 4-byte aligned");
     ds4b200::pages_free(t, seqs, n_list, status, workspace, STREAM(stream));
     return launched("pages_free");
 }

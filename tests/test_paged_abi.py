@@ -108,3 +108,27 @@ def test_list_model_of_the_pages():
     m.free([3])
     m.moves = []
     assert m.compact() == 5 and m.moves == [(5, 0)] and m.table[0] == [3, 4, 0]
+
+
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_arrays_of_words_off_their_four_bytes_are_refused(lib, off):
+    """Tables, lengths, lists, sinks and log-sums are read as words: an odd address is an error here, and no fault on the device."""
+    bad = PTR + off
+    dec = lambda **k: lib.ds4b200_attn_decode_paged_bf16(PTR, C.byref(kv()), k.get("table", PTR), 4, k.get("lens", PTR), 2, 64, 1.0, k.get("sink"), 0, 0,
+                                                         PTR, k.get("lse"), PTR, 1 << 40, None)
+    win = lambda **k: lib.ds4b200_attn_window_paged_bf16(PTR, 5, C.byref(kv()), k.get("table", PTR), 4, k.get("lens", PTR), k.get("start", PTR), 2, 64, 1.0,
+                                                         k.get("sink"), 128, 0, PTR, k.get("lse"), PTR, 1 << 40, None)
+    for k in ("table", "lens", "sink", "lse"):
+        assert dec(**{k: bad}) == EINVAL and win(**{k: bad}) == EINVAL, k
+        assert b"align" in lib.ds4b200_last_error()
+    assert win(start=bad) == EINVAL
+    for i in range(6):
+        p = [PTR] * 6
+        p[i] = bad
+        assert lib.ds4b200_pages_fork(None, 0, 10, 4, *p, 3, 4, PTR, 2, PTR, PTR, 1 << 40, None) == EINVAL, i
+        assert lib.ds4b200_pages_reserve(10, 4, *p, PTR, 3, 4, PTR, PTR, 1 << 40, None) == EINVAL, i
+        assert lib.ds4b200_pages_free(10, 4, *p, 3, 4, PTR, 2, PTR, PTR, 1 << 40, None) == EINVAL, i
+        if i < 4:
+            assert lib.ds4b200_pages_compact(None, 0, 10, *p[:4], 3, 4, PTR, PTR, 1 << 40, None) == EINVAL, i
+    assert lib.ds4b200_pages_reserve(10, 4, *[PTR] * 6, bad, 3, 4, PTR, PTR, 1 << 40, None) == EINVAL
+    assert lib.ds4b200_pages_free(10, 4, *[PTR] * 6, 3, 4, bad, 2, PTR, PTR, 1 << 40, None) == EINVAL
