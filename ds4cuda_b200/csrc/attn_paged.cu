@@ -31,14 +31,14 @@ constexpr float kLog2e = 1.4426950408889634f;
 //     rows, 512 columns) would leave no room for S.  S of tile n + 1 is issued ahead of O^T of tile n, so the tensor
 //     cores work while the softmax of a tile runs;
 //   * eight take S from tensor memory, keep the running maximum and sum of the softmax in f32, and leave the weights as f16 (half a
-//     step: 2^-12 of each) in shared memory.  The accumulators are rescaled only when a row's maximum has grown by more
+//     step: 2^-11 of each) in shared memory.  The accumulators are rescaled only when a row's maximum has grown by more
 //     than 2^8 since its last reference, which later tiles rarely bring;
 //   * one hands out the items, one looks the tiles' rows up in the page table and touches them ahead of the loads.
 //
 // Scales.  A cache row is a row factor times f16 numbers.  Rows of ordinary size have the factor 1: codes times a scale that is
 // a power of two are exact in f16, codes times another scale are rounded (2^-11), as f32 rows are.  A row whose
 // scale or tail is far from one keeps a factor r_j, which enters the scores, and as log2 r_j the exponent of the weights,
-// so that P holds r_j exp(s_j - M) <= 1 and the sum takes P / r_j back.  A query row is scaled by a power of two, which
+// so that P holds r_j exp(s_j - M) <= 2^15 (see kLift) and the sum takes P / r_j back.  A query row is scaled by a power of two, which
 // loses nothing of bf16's 8 bits in f16.
 //
 // Work.  Where items are long and few the list of all tiles is cut into equal runs, one per CTA; an item that several CTAs share
@@ -64,8 +64,9 @@ constexpr int kSplitItems = 4 * kCtas;      // more of them are not cut
 constexpr int kWholeTiles = 3;              // items of up to so many tiles are not cut
 constexpr int kMinTiles = 2;                // of a run: below, the join costs more than the run saves
 constexpr float kRescale = 8.0f;            // log2 units
+constexpr float kLift = 7.0f;               // and with it a weight is below 2^15
 constexpr int kScaleSets = 4;
-constexpr float kLeast = 0x1p-100f;         // of a row's factor
+constexpr float kLeast = 0x1p-93f;          // of a row's factor
 constexpr uint32_t kTmem = 0;               // all 512 columns are allocated, so they begin at column 0
 
 struct Meta { int64_t row0; int rows, h0, parts, pad; };
@@ -1099,12 +1100,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 #pragma unroll
                 for (int i = 0; i < 4; ++i) w[i] = fmaxf(fmaxf(v[i].x, v[i].y), fmaxf(v[i + 4].x, v[i + 4].y));
                 float top = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])), f = 1.0f;
-                // A row keeps the reference its maximum had until one of its values lies kRescale above it.  Then it takes a
-                // new one, and every row's factor for the accumulators (a column of O^T) is left for follow(), which the
+                // A row's reference lies kLift below its maximum, so that weights down to 2^-21 of the largest are normal f16 numbers and smaller
+                // ones off by 2^-32 of it (without the lift 2^-25, which 131072 rows can add up to 2^-8).  A row keeps its reference
+                // until one of its values lies kRescale above the maximum it had then.  Then it takes a new one, and every row's factor for the accumulators (a column of O^T) is left for follow(), which the
                 // warps run together, at the next tile.
-                if (__any_sync(0xffffffffu, !(top <= m + kRescale))) {
+                if (__any_sync(0xffffffffu, !(top <= m + (kRescale + kLift)))) {
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    top -= kLift;
                     if (m > -INFINITY && top > m + kRescale) {
                         f = tc::exp2_approx(m - top);
                         m = top;

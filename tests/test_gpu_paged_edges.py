@@ -134,3 +134,28 @@ def test_a_sink_that_is_not_a_number_spoils_its_head_only(ops, lens):
     others = [h for h in range(16) if h != 5]
     assert bool(out[:, 5].isnan().all()) and bool(lse[:, 5].isnan().all())
     assert not out[:, others].isnan().any() and not lse[:, others].isnan().any()
+
+
+@pytest.mark.parametrize("heads,n_seqs", [(1024, 40), (64, 2)])          # whole items (more of them than are cut), and cut ones
+def test_many_small_weights_add_up(ops, heads, n_seqs):
+    """One row with a weight near 1 and 40000 of 2^-25.5 of it, which together are a thousandth.  A weight is held in f16 as 2^7 times what it
+    is relative to its reference, so it is off by at most 2^-32 where it is small; the sum of 40000 by 1e-5."""
+    n, dim, page = 40000, 128, 64
+    g = torch.zeros((n // page * page, dim), device="cuda")
+    g[:, 1] = 1.0
+    g[0] = 0.0
+    g[0, 0] = 1.0
+    kv = ops.PagedKv(ops.KV_F32, page, raw=g)
+    table = torch.arange(n // page, dtype=torch.int32, device="cuda").repeat(n_seqs, 1)
+    q = torch.zeros((n_seqs, heads, dim), device="cuda", dtype=torch.bfloat16)
+    q[:, :, 0] = 1.0
+    for length in (n, n - 777):
+        kv_len = torch.full((n_seqs,), length, dtype=torch.int32, device="cuda")
+        out, lse = ops.attn_decode_paged(q, kv, table, kv_len, scale=25.5 * 0.6931471805599453, want_lse=True)
+        rest = (length - 1) * 2.0 ** -25.5
+        want = rest / (1 + rest)
+        # bf16's half step, the weights', and 2^-10 of it for the exponents' f32 roundings (25.5 is held to 2^-20) and the sums
+        assert bool(((out[:, :, 1].double() - want).abs() <= want * (2.0 ** -8 + 2.0 ** -10) + length * 2.0 ** -32).all())
+        assert bool(((out[:, :, 0].double() - 1 / (1 + rest)).abs() <= 2.0 ** -8 + 2.0 ** -10).all())
+        assert not out[:, :, 2:].any()
+    assert ops.device_status() == 0
