@@ -38,7 +38,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Scales.  A cache row is a row factor times f16 numbers.  Rows of ordinary size have the factor 1: codes times a scale that is
 // a power of two are exact in f16, codes times another scale are rounded (2^-11), as f32 rows are.  A row whose
 // scale or tail is far from one keeps a factor r_j, which enters the scores, and as log2 r_j the exponent of the weights,
-// so that P holds r_j exp(s_j - M) <= 2^15 (see kLift) and the sum takes P / r_j back.  A query row is scaled by a power of two, which
+// so that P holds r_j exp(s_j - M) (times kLift, and below 2^15) and the sum takes P / r_j back.  A query row is scaled by a power of two, which
 // loses nothing of bf16's 8 bits in f16.
 //
 // Work.  Where items are long and few the list of all tiles is cut into equal runs, one per CTA; an item that several CTAs share
@@ -64,9 +64,9 @@ constexpr int kSplitItems = 4 * kCtas;      // more of them are not cut
 constexpr int kWholeTiles = 3;              // items of up to so many tiles are not cut
 constexpr int kMinTiles = 2;                // of a run: below, the join costs more than the run saves
 constexpr float kRescale = 8.0f;            // log2 units
-constexpr float kLift = 7.0f;               // and with it a weight is below 2^15
+constexpr float kLift = 0x1p7f;              // of the weights as stored, and so of the accumulators
 constexpr int kScaleSets = 4;
-constexpr float kLeast = 0x1p-93f;          // of a row's factor
+constexpr float kLeast = 0x1p-100f;         // of a row's factor
 constexpr uint32_t kTmem = 0;               // all 512 columns are allocated, so they begin at column 0
 
 struct Meta { int64_t row0; int rows, h0, parts, pad; };
@@ -1100,14 +1100,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 #pragma unroll
                 for (int i = 0; i < 4; ++i) w[i] = fmaxf(fmaxf(v[i].x, v[i].y), fmaxf(v[i + 4].x, v[i + 4].y));
                 float top = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])), f = 1.0f;
-                // A row's reference lies kLift below its maximum, so that weights down to 2^-21 of the largest are normal f16 numbers and smaller
-                // ones off by 2^-32 of it (without the lift 2^-25, which 131072 rows can add up to 2^-8).  A row keeps its reference
-                // until one of its values lies kRescale above the maximum it had then.  Then it takes a new one, and every row's factor for the accumulators (a column of O^T) is left for follow(), which the
+                // A row keeps the reference its maximum had until one of its values lies kRescale above it.  Then it takes a new one, and every row's factor for the accumulators (a column of O^T) is left for follow(), which the
                 // warps run together, at the next tile.
-                if (__any_sync(0xffffffffu, !(top <= m + (kRescale + kLift)))) {
+                if (__any_sync(0xffffffffu, !(top <= m + kRescale))) {
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    top -= kLift;
                     if (m > -INFINITY && top > m + kRescale) {
                         f = tc::exp2_approx(m - top);
                         m = top;
@@ -1118,14 +1115,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 }
                 if ((lane & 3) == 0) fac_s[buf][row] = f;
                 const float ref = m == -INFINITY ? 0.0f : -m;
-                const float2 ref2 = make_float2(ref, ref);
+                const float2 ref2 = make_float2(ref, ref), lift2 = make_float2(kLift, kLift);
+                // Weights are stored as kLift times what they are relative to the reference: down to 2^-21 of it they are normal f16 numbers, smaller
+                // ones are off by 2^-32 of it (without the lift 2^-25, which 131072 rows can add up to 2^-8).
                 unsigned char *dst = p_s + buf * 8192 + row * 128 + (lane & 3) * 4;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     v[i] = add2(v[i], ref2);
                     v[i].x = tc::exp2_approx(v[i].x);
                     v[i].y = tc::exp2_approx(v[i].y);
-                    *reinterpret_cast<uint32_t *>(dst + (((uint32_t)i ^ (uint32_t)(row & 7)) << 4)) = h2_bits(__floats2half2_rn(v[i].x, v[i].y));
+                    const float2 y = mul2(v[i], lift2);
+                    *reinterpret_cast<uint32_t *>(dst + (((uint32_t)i ^ (uint32_t)(row & 7)) << 4)) = h2_bits(__floats2half2_rn(y.x, y.y));
                 }
                 if (odd) {
 #pragma unroll
@@ -1161,7 +1161,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     lse2 = hi + more;
                     lse = heavy ? sink + more * (1.0f / kLog2e) : lse2 * (1.0f / kLog2e);
                 }
-                inv = m == -INFINITY ? 0.0f : tc::exp2_approx(m - lse2);
+                inv = m == -INFINITY ? 0.0f : tc::exp2_approx(m - lse2) * (1.0f / kLift);
             }
             if (kPre) {                                  // the loaders drain the accumulators
                 if ((lane & 3) == 0) {
@@ -1325,7 +1325,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) attn_join_kernel(const Att
                 for (int s = 0; s < 4; ++s) add_scaled(o[s], wk, x[j][s]);
             }
         }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const float inv = l == 0.0f ? 0.0f : (1.0f / kLift) / l;
 #pragma unroll
         for (int s = 0; s < 4; ++s)
             if (s < slices) st_bf16x4(a.out + (it.row0 + row) * D + s * 128 + lane * 4, make_float4(o[s].x * inv, o[s].y * inv, o[s].z * inv, o[s].w * inv));
@@ -1387,7 +1387,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) attn_join_kernel(const Att
                 float4 y = sums[warp][0][lane];
 #pragma unroll
                 for (int i = 1; i < kJoinWarps; ++i) add_scaled(y, 1.0f, sums[warp][i][lane]);
-                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                const float inv = l == 0.0f ? 0.0f : (1.0f / kLift) / l;
                 st_bf16x4(a.out + (it.row0 + row) * D + (slice + warp) * 128 + lane * 4, make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv));
                 if (lane == 0 && slice + warp == 0 && a.lse) a.lse[it.row0 + row] = lse_of(l, top, sink, sink2);
             }

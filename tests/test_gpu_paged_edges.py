@@ -159,3 +159,22 @@ def test_many_small_weights_add_up(ops, heads, n_seqs):
         assert bool(((out[:, :, 0].double() - 1 / (1 + rest)).abs() <= 2.0 ** -8 + 2.0 ** -10).all())
         assert not out[:, :, 2:].any()
     assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("toks,heads,window", [(36000, 128, 1), (70000, 64, 1)])      # packed first, and straight from the cache
+def test_queries_and_outputs_behind_four_gigabytes(ops, toks, heads, window):
+    """With a window of one row a token's output is its own row, to bf16's bits."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    page, dim = 64, 512
+    n = -(-toks // page) * page
+    raw = torch.randn((n, dim), generator=g, device="cuda").half().float()
+    order = torch.randperm(n // page, generator=g, device="cuda").int()
+    kv = ops.PagedKv(ops.KV_F32, page, raw=raw)
+    q = torch.empty((toks, heads, dim), dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    assert q.numel() * 2 > 1 << 32
+    out = ops.attn_window_paged(q, kv, order[None].contiguous(), torch.tensor([toks], dtype=torch.int32, device="cuda"),
+                                torch.tensor([0, toks], dtype=torch.int32, device="cuda"), window=window)
+    want = raw.view(n // page, page, dim)[order.long()].view(n, dim)[:toks].bfloat16()
+    for at in range(0, toks, 5000):
+        assert torch.equal(out[at:at + 5000], want[at:at + 5000, None].expand(-1, heads, -1))
+    assert ops.device_status() == 0
