@@ -1065,7 +1065,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {                          // column block i is loader i's
                         if (kPre) {
-                            const float f0 = __ldg(fac + 8 * i + 2 * (lane & 3)), f1 = __ldg(fac + 8 * i + 2 * (lane & 3) + 1);
+                            const float f0 = fac[8 * i + 2 * (lane & 3)], f1 = fac[8 * i + 2 * (lane & 3) + 1];
                             v[i] = fma2(v[i], make_float2(f0, f1), make_float2(__log2f(f0), __log2f(f1)));
                             continue;
                         }
@@ -1131,7 +1131,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
                         if (kPre) {
-                            const float f0 = __ldg(fac + 8 * i + 2 * (lane & 3)), f1 = __ldg(fac + 8 * i + 2 * (lane & 3) + 1);
+                            const float f0 = fac[8 * i + 2 * (lane & 3)], f1 = fac[8 * i + 2 * (lane & 3) + 1];
                             // A column past the rows has the weight 0 and whatever its factor's place holds: only a factor that the
                             // packing can have left (0, NaN, kLeast and above) has a reciprocal whose product with 0 is 0.
                             v[i] = mul2(v[i], make_float2(f0 >= kLeast ? __fdividef(1.0f, f0) : 0.0f, f1 >= kLeast ? __fdividef(1.0f, f1) : 0.0f));
@@ -1270,6 +1270,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) attn_join_kernel(const Att
     __shared__ float weight[kCtas], most_s[kJoinWarps], sum_s[kJoinWarps];
     __shared__ float4 sums[4][kJoinWarps][32];
     const int D = a.kv.head_dim, slices = D / 128, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // What the kernel before writes while this one is resident already may not go through the read-only path, so no __ldg() of it.
     wait_dependency();
     if (tid < kCtas) items[tid] = meta[tid];
     __syncthreads();
@@ -1306,7 +1307,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) attn_join_kernel(const Att
 #pragma unroll
                 for (int s = 0; s < 4; ++s)
                     x[j][s] = k + j < it.parts && s < slices
-                                  ? __ldg(reinterpret_cast<const float4 *>(part_o + ((int64_t)part_of(c, k + j) * kRows + row) * D + s * 128 + lane * 4))
+                                  ? *reinterpret_cast<const float4 *>(part_o + ((int64_t)part_of(c, k + j) * kRows + row) * D + s * 128 + lane * 4)
                                   : make_float4(0.f, 0.f, 0.f, 0.f);
         };
         load(0);
@@ -1351,7 +1352,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) attn_join_kernel(const Att
                     const int k = k0 + i * kJoinWarps;
                     const float4 *from = reinterpret_cast<const float4 *>(part_o + ((int64_t)part_of(c, k) * kRows + row) * D + slice * 128 + lane * 4);
 #pragma unroll
-                    for (int s = 0; s < SL; ++s) x[i][s] = k < parts ? __ldg(from + s * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int s = 0; s < SL; ++s) x[i][s] = k < parts ? from[s * 32] : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
             };
             load(warp);
