@@ -1,9 +1,12 @@
 """GPU tests of the paged cache at its edges: workspaces in any state, items of many tiles, sizes and values at a rule's border."""
+import random
+
 import pytest
 import torch
 
 import paged_model as model
-from test_gpu_paged import FMTS, Case, pack_factors
+from ds4cuda_b200 import _lib
+from test_gpu_paged import FMTS, Case, pack_factors, pool_state, same
 
 pytestmark = pytest.mark.gpu
 
@@ -161,6 +164,122 @@ def test_many_small_weights_add_up(ops, heads, n_seqs):
     assert ops.device_status() == 0
 
 
+# ------------------------------------------------------------------------------------- the caches that the store ops fill
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("toks", [1, 40])
+def test_attention_over_rows_the_store_ops_left(ops, fmt, toks):
+    """kv rows -> norm, RoPE and quantiser of the framework -> attention; the rows are what the framework's own load op reads back."""
+    D, H, page, n = 512, 16, 16, 90
+    g = torch.Generator(device="cuda").manual_seed(5)
+    order = torch.randperm(8, generator=g, device="cuda").int()
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    slots = (order[(pos // page).long()] * page + pos % page).int()
+    params, kv_rows = ops.rope_params_for_layer(3), torch.randn((n, D), generator=g, device="cuda") * 3
+    w = 1 + 0.1 * torch.randn((D,), generator=g, device="cuda")
+    slots_n, rows = 8 * page, torch.full((8 * page, D), float("nan"), dtype=torch.float64, device="cuda")
+    if fmt == "f32":
+        st = dict(raw=torch.full((slots_n, D), float("nan"), device="cuda"))
+        ops.kv_rows_to_raw(kv_rows, pos, params, st["raw"], slots=slots, norm_w=w)
+        rows[slots.long()] = st["raw"][slots.long()].double()
+        kv = ops.PagedKv(ops.KV_F32, page, **st)
+    else:
+        mode = ops.FP8_ROW_AMAX if fmt == "row" else ops.FP8_BLOCK64_POW2
+        st = dict(codes=torch.full((slots_n, D), 0x7f, dtype=torch.uint8, device="cuda"),
+                  scales=torch.full((slots_n, 1 if fmt == "row" else 7), float("nan"), device="cuda"))
+        if fmt == "block":
+            st["tail"] = torch.full((slots_n, 64), float("nan"), device="cuda")
+        ops.rope_fp8_store_rows(kv_rows, pos, params, 64, mode, st["codes"], st["scales"], slots=slots, norm_w=w, tail_out=st.get("tail"))
+        rows[slots.long()] = ops.fp8_cache_load_rows(st["codes"], st["scales"], slots, 64, mode, tail=st.get("tail")).double()
+        kv = ops.PagedKv(ops.KV_FP8_ROW if fmt == "row" else ops.KV_FP8_BLOCK64, page, 64, **st)
+    assert not rows[slots.long()].isnan().any()
+    q = torch.randn((toks, H, D), generator=g, device="cuda").bfloat16()
+    table, kv_len = order[None].contiguous(), torch.tensor([n], dtype=torch.int32, device="cuda")
+    sink = torch.randn((H,), generator=g, device="cuda")
+    if toks == 1:
+        out = ops.attn_decode_paged(q, kv, table, kv_len, window=50, n_first=3, sink=sink)
+    else:
+        out = ops.attn_window_paged(q, kv, table, kv_len, torch.tensor([0, toks], dtype=torch.int32, device="cuda"), window=50, n_first=3, sink=sink)
+    want, _, bound, _ = model.attention(q, rows, [slots.tolist()] * toks, list(range(n - toks, n)), 50, 3, D ** -0.5, sink,
+                                        {"f32": 0, "row": D, "block": 64}[fmt], model.row_factors(fmt, st))
+    assert bool(((out.double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_single_rows_by_pages_of_one(ops, fmt):
+    """A page of one row makes the table a list of rows: any order, the same row twice, rows of other sequences."""
+    c = Case(ops, fmt, 64, 512, 1, [150, 70])
+    picks = [c.slots[0][::-1] + c.slots[0][:30] + [c.slots[1][5]] * 40, c.slots[1][3:4], c.slots[1] + c.slots[0][10:90:2]]
+    table = torch.full((3, max(map(len, picks))), -1, dtype=torch.int32)
+    for b, p in enumerate(picks):
+        table[b, :len(p)] = torch.tensor(p)
+    c.table, c.kv_len = table.cuda(), torch.tensor([len(p) for p in picks], dtype=torch.int32, device="cuda")
+    c.q = torch.cat([c.q, c.q[:1]])
+    c.slots_of, c.positions = picks, [len(p) - 1 for p in picks]
+    out, lse = ops.attn_decode_paged(c.q, c.kv, c.table, c.kv_len, sink=c.sink, want_lse=True)
+    c.check(out, lse, 0, 0, c.sink)
+
+
+# ------------------------------------------------------------------------------------------------- work and its division
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_short_sequences_under_a_wide_table(ops, fmt):
+    """A table as wide as the longest sequence may ever get: tiles are cut into runs by the room, lengths and first rows by what is there."""
+    c = Case(ops, fmt, 64, 512, 16, [130, 1, 0, 64, 300, 5], width=1000)
+    out, lse = ops.attn_decode_paged(c.q, c.kv, c.table, c.kv_len, sink=c.sink, want_lse=True)
+    c.check(out, lse, 0, 0, c.sink)
+    w = Case(ops, fmt, 16, 512, 16, [130, 40, 64], [33, 40, 1], width=1000)
+    out, lse = ops.attn_window_paged(w.q, w.kv, w.table, w.kv_len, w.q_start, sink=w.sink, want_lse=True)
+    w.check(out, lse, 0, 0, w.sink)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_more_items_than_are_cut(ops, fmt):
+    c = Case(ops, fmt, 128, 128, 64, [1 + (37 * i) % 400 for i in range(300)])
+    out, lse = ops.attn_decode_paged(c.q, c.kv, c.table, c.kv_len, sink=c.sink, want_lse=True)
+    c.check(out, lse, 0, 0, c.sink)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_the_most_sequences_a_call_takes(ops, fmt):
+    c = Case(ops, fmt, 3, 128, 64, [1 + i % 70 for i in range(64)])
+    which = torch.arange(4096) % 64
+    table, lens, q = c.table[which].contiguous(), c.kv_len[which].contiguous(), c.q[which].contiguous()
+    one = ops.attn_decode_paged(c.q, c.kv, c.table, c.kv_len)
+    c.check(one, None, 0, 0, None)
+    out = ops.attn_decode_paged(q, c.kv, table, lens)
+    assert torch.equal(out.view(64, 64, 3, 128), one.expand(64, 64, 3, 128))
+    start = torch.arange(4097, dtype=torch.int32, device="cuda")
+    chunk = ops.attn_window_paged(q, c.kv, table, lens, start)
+    assert torch.equal(chunk.view(64, 64, 3, 128), chunk[:64].expand(64, 64, 3, 128))
+    c.check(chunk[:64], None, 0, 0, None)
+    with pytest.raises(_lib.Ds4Error):
+        ops.attn_decode_paged(torch.cat([q, q[:1]]), c.kv, torch.cat([table, table[:1]]), torch.cat([lens, lens[:1]]))
+
+
+def test_a_token_gives_the_same_bits_in_a_chunk_cut_elsewhere(ops):
+    """One token per item, whole items, straight from the cache in each of these calls: the same order of the same sums."""
+    c = Case(ops, "block", 64, 512, 64, [300], [60])
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    call = lambda rows, length: ops.attn_window_paged(c.q[rows].contiguous(), c.kv, c.table, i32(length), i32(0, rows.stop - rows.start), window=128, n_first=4)
+    whole = call(slice(0, 60), 300)
+    for cut in (1, 23, 59):
+        assert torch.equal(torch.cat([call(slice(0, cut), 240 + cut), call(slice(cut, 60), 300)]), whole)
+    one = ops.attn_decode_paged(c.q[-1:].contiguous(), c.kv, c.table, c.kv_len, window=128, n_first=4)
+    assert torch.equal(one, whole[-1:])
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("heads,dim", [(64, 512), (64, 128), (8, 256)])
+@pytest.mark.parametrize("scale", [lambda j: 1.0 + j / 40.0, lambda j: 30.0 if j % 90 == 80 else 0.01])
+def test_packed_maxima_that_grow_along_the_rows(ops, fmt, heads, dim, scale):
+    """The accumulators are rescaled between the tiles of packed items, and behind their last one."""
+    c = Case(ops, fmt, heads, dim, 64, [400, 333], [180, 20], row_scale=scale, q_scale=2.0)
+    out, lse = ops.attn_window_paged(c.q, c.kv, c.table, c.kv_len, c.q_start, window=300, n_first=2, sink=c.sink, want_lse=True)
+    c.factors = pack_factors(c) if fmt != "f32" else c.factors
+    c.check(out, lse, 300, 2, c.sink)
+
+
 @pytest.mark.parametrize("toks,heads,window", [(36000, 128, 1), (70000, 64, 1)])      # packed first, and straight from the cache
 def test_queries_and_outputs_behind_four_gigabytes(ops, toks, heads, window):
     """With a window of one row a token's output is its own row, to bf16's bits."""
@@ -178,3 +297,83 @@ def test_queries_and_outputs_behind_four_gigabytes(ops, toks, heads, window):
     for at in range(0, toks, 5000):
         assert torch.equal(out[at:at + 5000], want[at:at + 5000, None].expand(-1, heads, -1))
     assert ops.device_status() == 0
+
+
+# ------------------------------------------------------------------------------------------- streams, graphs, workspaces
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_decode_does_not_look_at_what_a_workspace_holds(ops, fmt):
+    c = Case(ops, fmt, 64, 512, 64, [3000, 17, 0, 900])
+    ws = ops.attn_workspace(64, 512)
+    ws.zero_()
+    clean, clean_lse = ops.attn_decode_paged(c.q, c.kv, c.table, c.kv_len, want_lse=True, workspace=ws)
+    c.check(clean, clean_lse, 0, 0, None)
+    for word in (1, 256, 0x7f800000, -1, 148):
+        ws.view(torch.int32).fill_(word)
+        out, lse = ops.attn_decode_paged(c.q, c.kv, c.table, c.kv_len, want_lse=True, workspace=ws)
+        assert torch.equal(out, clean) and torch.equal(lse, clean_lse)
+
+
+def test_captured_page_operators_follow_their_inputs(ops):
+    """fork, reserve, free and compact in one graph, in place, replayed over two states of the pool, and with workspaces in any state."""
+    rng = random.Random(4)
+    pool, refs, table, lens, _ = pool_state(ops, rng, 32, 8, 6, 4)
+    start = [t.clone() for t in (refs, table, lens, *pool.arrays)]
+    t = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    pairs, new, gone = t([0, 6], [1, 7]), t(0, 0, 0, 0, 9, 0, 0, 24), t(2, 6)
+    status = [t(5) for _ in range(3)]
+    live = t(5)
+
+    def chain():
+        ops.pages_fork(pool, refs, table, lens, pairs, status=status[0])
+        ops.pages_reserve(pool, refs, table, lens, new, status=status[1])
+        ops.pages_free(pool, refs, table, lens, gone, status=status[2])
+        ops.pages_compact(pool, refs, table, n_live=live)
+
+    def reset():
+        for a, b in zip((refs, table, lens, *pool.arrays), start):
+            a.copy_(b)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        chain()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        chain()
+    changes = [lambda: None, lambda: new.fill_(24), lambda: pairs.copy_(t([0, 6], [0, 6])), lambda: start[2].clamp_(max=1)]
+    seen = set()
+    for change in changes:                               # (more pages than there are, a list that is refused, other lengths)
+        change()
+        results = []
+        for run in (chain, graph.replay):
+            reset()
+            pool.workspace.fill_(0x41)
+            run()
+            results.append([x.clone() for x in (refs, table, lens, live, *status, *pool.arrays)])
+        for a, b in zip(*results):
+            assert torch.equal(a, b)
+        seen.add(tuple(s.item() for s in status))
+    assert len(seen) >= 3
+
+
+def test_two_pools_on_two_streams(ops):
+    t = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    made = []
+    for seed in (1, 2):
+        pool, refs, table, lens, m = pool_state(ops, random.Random(seed), 400, 40, 9, 16)
+        empty = [s for s in range(40) if m.lens[s] == 0]
+        held = [s for s in range(40) if m.lens[s]]
+        pairs = [(held[i % len(held)], b) for i, b in enumerate(empty[:15])]
+        before = [a.clone() for a in pool.arrays]
+        m.fork(pairs)
+        made.append((pool, refs, table, lens, t(pairs), m, before, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    got = []
+    for pool, refs, table, lens, pairs, m, before, stream in made:
+        with torch.cuda.stream(stream):
+            got.append(ops.pages_fork(pool, refs, table, lens, pairs))
+    torch.cuda.synchronize()
+    for (pool, *_, m, before, _), (refs, table, lens, st) in zip(made, got):
+        same(m, before, pool, refs, table, lens, st)
