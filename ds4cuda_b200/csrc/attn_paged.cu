@@ -31,28 +31,32 @@ constexpr float kLog2e = 1.4426950408889634f;
 //     rows, 512 columns) would leave no room for S.  S of tile n + 1 is issued ahead of O^T of tile n, so the tensor
 //     cores work while the softmax of a tile runs;
 //   * eight take S from tensor memory, keep the running maximum and sum of the softmax in f32, and leave the weights as f16 (half a
-//     step: 2^-11 of each) in shared memory.  The accumulators are rescaled only when a row's maximum has grown by more
+//     step: 2^-11 of each; see kLift) in shared memory.  The accumulators are rescaled only when a row's maximum has grown by more
 //     than 2^8 since its last reference, which later tiles rarely bring;
 //   * one hands out the items, one looks the tiles' rows up in the page table and touches them ahead of the loads.
 //
-// Scales.  A cache row is a row factor times f16 numbers.  Rows of ordinary size have the factor 1: codes times a scale that is
-// a power of two are exact in f16, codes times another scale are rounded (2^-11), as f32 rows are.  A row whose
-// scale or tail is far from one keeps a factor r_j, which enters the scores, and as log2 r_j the exponent of the weights,
-// so that P holds r_j exp(s_j - M) (times kLift, and below 2^15) and the sum takes P / r_j back.  A query row is scaled by a power of two, which
-// loses nothing of bf16's 8 bits in f16.
+// Scales.  A cache row is a row factor times f16 numbers.  Rows of ordinary size have the factor 1: codes times a scale that is a power
+// of two are exact in f16 where the product is a multiple of 2^-24 (a scale of 2^-15 and above; below, and in blocks far smaller than their
+// row's largest, a value is off by up to 2^-25 of the factor), codes times another scale are rounded (scale and product, 2^-11 each), as
+// f32 rows and tails are (2^-11).  A row whose scale or tail is far from one keeps a factor r_j, which enters the scores, and as log2 r_j the exponent of the weights,
+// so that P holds r_j exp(s_j - M) (times kLift, and below 2^15) and the sum takes P / r_j back.  A query row whose
+// largest value is outside [2^-4, 2^15] is scaled by a power of two: bf16's 8 bits fit f16, but for values below
+// 2^-17, which are off by up to 2^-25.
 //
 // Work.  Where items are long and few the list of all tiles is cut into equal runs, one per CTA; an item that several CTAs share
 // leaves partial sums (f32 O^T, M and l) that attn_join_kernel adds in order.  Else each CTA takes whole items.  Of a chunk the rows
 // may be packed as f16 once (attn_pack_kernel); a tile is then eight TMA boxes, and the loaders fetch query rows and drain
 // O^T instead, beside the softmax of the next item.
 //
-// Bound.  Shared memory: a tile of 512 dims is 64 KiB written and, by the MMAs, 224 KiB read at 128 bytes a cycle (1792 cycles; an MMA
-// of M 64, N 64, K 16 reads 4 KiB in 32), which with the loads' own pass through L1, the weights and the query rows makes 2700 to
-// 2900 cycles a tile; from HBM a tile of FP8 rows needs 1400, of f32 rows 5600.  Halves of that traffic would need the codes
-// themselves as operands, and the weights as two or three 8-bit pieces.  Measured (512 dims): one session of 131072 rows, codes with
-// a tail, 64 heads: 55 us (96 MB, 1.7 TB/s); 64 sequences of up to 16384 FP8 rows: 90 us (162 MB, 1.8 TB/s; tensor pipe 33 %);
-// 96 sequences, 16 heads, f32 rows, window 1024: 60 us (158 MB, 2.6 TB/s); 4096 chunk tokens, window 128 + 4 first rows: 174 to
-// 186 us (538 MB, 2.9 to 3.1 TB/s; tensor pipe 31 %), a chain of S, softmax, product and drain per token.
+// Bound.  Shared memory: a tile of 512 dims is 64 KiB written and, by the MMAs, 224 KiB read at 128 bytes a cycle, 2300 cycles with nothing
+// else on the port (an MMA of M 64, N 64, K 16 reads 4 KiB in 32); the loads' own pass through L1, the weights and the query rows come on
+// top.  Measured, as the slope over 8 to 48 tiles a CTA of one session (64 heads): 1.7 us a tile of FP8 rows (3400 cycles at 1965 MHz),
+// 2.2 of codes with a tail, 4.2 of f32 rows; start, partial sums and join take 18 to 21 us besides.  From HBM a tile of FP8 rows
+// needs 1400 cycles, of f32 rows 5600.  Halves of the MMAs' traffic would need the codes themselves as operands, and the weights as two
+// or three 8-bit pieces.  Whole calls: one session of 131072 rows, codes with a tail: 55 us (96 MB, 1.7 TB/s); 64 sequences of up to 16384
+// FP8 rows: 90 us (162 MB, 1.8 TB/s; tensor pipe 33 %); 96 sequences, 16 heads, f32 rows, window 1024: 61 us (158 MB, 2.6 TB/s); 4096
+// chunk tokens, window 128 + 4 first rows: 176 to 187 us (538 MB, 2.9 to 3.1 TB/s; tensor pipe 31 %), a chain of S, softmax, product and
+// drain per token.
 constexpr int kCtas = 148;
 constexpr int kRows = 64;                   // query rows of an item, cache rows of a tile
 constexpr int kSoftWarps = 8, kLoadWarp0 = 8, kLoadWarps = 8, kMmaWarp = 16;
@@ -60,7 +64,7 @@ constexpr int kThreads = 20 * 32;
 // Registers a thread by role, out of what the block is launched with: a larger sum would wait for registers for ever.
 constexpr int kLaunchRegs = 96, kSoftRegs = 72, kLoadRegs = 136, kOtherRegs = 56;
 static_assert(kSoftWarps * kSoftRegs + kLoadWarps * kLoadRegs + (20 - kSoftWarps - kLoadWarps) * kOtherRegs <= 20 * kLaunchRegs, "register split");
-constexpr int kSplitItems = 4 * kCtas;      // more of them are not cut
+constexpr int kSplitItems = 4 * kCtas;      // more of them are not cut, see launch_fmt()
 constexpr int kWholeTiles = 3;              // items of up to so many tiles are not cut
 constexpr int kMinTiles = 2;                // of a run: below, the join costs more than the run saves
 constexpr float kRescale = 8.0f;            // log2 units
@@ -1522,9 +1526,13 @@ bool launch_fmt(const AttnArgs &a, cudaStream_t s) {
     g.group = a.q_start && g.head_groups == 1 ? kRows / a.n_heads : 1;
     const int64_t slots = (a.q_start ? a.n_tokens / g.group + a.n_seqs + 1 : a.n_seqs) * g.head_groups;
     g.n_slots = (int)slots;
-    // Equal runs of tiles pay where items are long and few: a run's two ends cost 128 KiB of partial sums each and the join
-    // another launch.  512 prompt tokens of 3 tiles took 91 us cut into runs and 49 us as whole items; one session of 131072 rows
-    // takes one CTA as a whole item.
+    // Equal runs of tiles pay where items are long and few: a run's two ends cost 128 KiB of partial sums each and the join another launch.
+    // The host knows the table's width and not the lengths, so the width stands for them: 592 sequences of 120 rows take 46 us under a table
+    // of two pages and 50, cut, under one of 1000.  Tiles: 512 prompt tokens of 3 tiles take 30 us as whole items and 79 cut (512 dims, replayed).
+    // Items: a chunk's are many and alike, and cutting them costs (1000 tokens of 128 dims, window 512: 42 us whole, 110 cut; nine prompts
+    // of 1531 tokens 76 and 182).  A decode's gain little from it where they are alike (592 sequences of 2000 rows 255 us whole, 259 cut; 1200 of
+    // 1000 rows 296 and 314) and much where they are not (592 of up to 8000 rows 771 and 491; 591 of 1000 rows beside one of 65536
+    // 1834 and 190), also beyond kSplitItems, where they are whole all the same (600 of up to 8000 rows: 771, cut they would take 494).
     const int64_t all_rows = a.table_width * a.kv.page_rows;
     const int64_t seen = a.window > 0 ? std::min<int64_t>(all_rows, (int64_t)a.window + a.n_first + g.group - 1) : all_rows;
     g.split = seen > kWholeTiles * kRows && slots <= kSplitItems;

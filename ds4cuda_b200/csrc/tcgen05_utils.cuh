@@ -1,5 +1,5 @@
 // tcgen05_utils.cuh — wrappers of the tensor-memory and mbarrier instructions the attention kernels use, and waits
-// that give up after about a second.
+// that give up after a second or so.
 #pragma once
 
 #include "device_utils.cuh"
@@ -7,7 +7,7 @@
 namespace ds4b200 {
 namespace tc {
 
-constexpr int kWaitPolls = 1 << 22;               // of about 0.1 us each: about half a second
+constexpr int kWaitPolls = 1 << 22;               // with a sleep of 20 to 300 ns (NS) ahead of each: a tenth of a second to one or two
 
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }

@@ -471,7 +471,7 @@ def attn_decode_paged(q, kv, page_table, kv_len, window=0, n_first=0, scale=None
     """Attention of one new token per sequence.  q bf16 [n_seqs, n_heads, head_dim], kv a PagedKv, page_table int32
     [n_seqs, width], kv_len int32 [n_seqs] (rows in the cache, the token's own among them).  The token sees the
     last `window` rows (0: all) and the `n_first` first ones.  scale: 1/sqrt(head_dim) by default; sink f32
-    [n_heads]: a logit without a row.  Returns out bf16 like q, with want_lse (out, lse f32 [n_seqs, n_heads])."""
+    [n_heads]: a logit without a row.  At most 4096 sequences; `out` overlaps none of the inputs.  Returns out bf16 like q, with want_lse (out, lse f32 [n_seqs, n_heads])."""
     return _attn(q, kv, page_table, kv_len, None, window, n_first, scale, sink, workspace, out, want_lse)
 
 

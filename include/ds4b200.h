@@ -473,11 +473,16 @@ typedef struct ds4b200_paged_kv {
  * sink (f32 [n_heads], nullable) is the reference's per-head logit without a row (cuda/flash_attn.cu:148).
  * lse is nullable.  A token that sees no row gets out = 0 and lse = sink[h] or -inf.  kv_len is clamped to
  * [0, table_width * page_rows], which must be below 2^31 - 64.  A row with a value that is not finite reaches the tokens that
- * see it, as NaN, and no others.
- * The products run in f16 with f32 accumulation: q exactly (scaled by a power of two where its range asks for it), cache rows
- * as f16 numbers, as the reference's attention reads its cache (cuda/flash_attn.cu:113-115): exact for
- * FP8_BLOCK64 codes and for the f16-rounded rows of ds4b200_kv_rows_to_raw_f32, else rounded (FP8 rows outside
- * [2^-9, 2^14] keep a factor beside them; F32 values beyond +-65504 become that); softmax weights rounded to f16.
+ * see it, as NaN, and no others.  out overlaps none of the inputs.  n_seqs <= 4096.
+ * The products run in f16 with f32 accumulation, cache rows as f16 numbers, as the reference's attention reads its cache
+ * (cuda/flash_attn.cu:113-115).  f16 holds 11 bits of a value and no step below 2^-24, so:
+ *   - q is exact (a row whose largest value is outside [2^-4, 2^15] is scaled by a power of two), but for values that lie below 2^-17
+ *     then, which are off by up to 2^-25;
+ *   - FP8 rows outside [2^-9, 2^14] or so keep a factor of at least 2^-100 beside them, their unit; the unit of others is 1;
+ *   - FP8_BLOCK64 codes are exact where their scale is at least 2^-15 units, else off by up to 2^-25 units; tails are rounded (2^-11);
+ *   - FP8_ROW rows are rounded, scale and product (2^-11 each);
+ *   - F32 rows are rounded, and exact as ds4b200_kv_rows_to_raw_f32 leaves them; values beyond +-65504 become that;
+ *   - softmax weights are rounded (2^-11 of each, and 2^-32 of a row's largest).
  * workspace: ds4b200_attn_workspace_bytes(n_heads, head_dim) bytes of device memory, 16-byte aligned, not shared by calls that may
  * overlap.  n_heads <= 1024.  Results do not depend on the contents of the workspace, and a call repeats its bits; the
  * lengths of all sequences decide where a long one is split, so the last bits of a sequence's result depend on them. */
@@ -491,7 +496,7 @@ int ds4b200_attn_decode_paged_bf16(const uint16_t *q, const ds4b200_paged_kv *ho
  * [n_tokens][n_heads][head_dim]; tokens q_start[b] .. q_start[b+1] - 1 (device int32 [n_seqs + 1], ascending from
  * q_start[0] >= 0, clamped to [0, n_tokens]) are the last rows of sequence b, so token i of its n stands at row kv_len[b] - n + i and
  * sees rows up to its own, with window and n_first as above.  Tokens outside [q_start[0], q_start[n_seqs])
- * keep what out (and lse [n_tokens][n_heads]) held.  n_seqs <= 4096. */
+ * keep what out (and lse [n_tokens][n_heads]) held. */
 int ds4b200_attn_window_paged_bf16(const uint16_t *q, int64_t n_tokens, const ds4b200_paged_kv *host_kv,
                                    const int32_t *page_table, int64_t table_width, const int32_t *kv_len,
                                    const int32_t *q_start, int64_t n_seqs, int n_heads, float scale,
