@@ -13,6 +13,14 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA device (run with -m gpu on a B200)")
 
 
+def pytest_collection_modifyitems(items):
+    """Where the reference's rebuilt library is missing, the tests that need it fail (see `ref`).  They come last then, so that a run which
+    stops at its first failure has run every other test."""
+    import ref_lib
+    if not ref_lib.available():
+        items.sort(key=lambda item: "ref" in getattr(item, "fixturenames", ()))
+
+
 @pytest.fixture(scope="session")
 def oracle():
     import oracle_lib
