@@ -377,3 +377,135 @@ def test_two_pools_on_two_streams(ops):
     torch.cuda.synchronize()
     for (pool, *_, m, before, _), (refs, table, lens, st) in zip(made, got):
         same(m, before, pool, refs, table, lens, st)
+
+
+# ---------------------------------------------------------------------------------------- arguments the headers allow
+
+@pytest.mark.parametrize("toks", [None, [40, 7], [150, 30]])             # decode; a chunk straight from the cache or packed, by its heads
+@pytest.mark.parametrize("heads,dim", [(64, 128), (16, 384), (64, 512)])
+def test_queries_of_any_size_and_scales_of_any_sign(ops, toks, heads, dim):
+    """A power of two moved from the query to the scale changes no bit; negative and zero scales are scales."""
+    c = Case(ops, "block", heads, dim, 64, [200, 70], toks)
+    call = ops.attn_decode_paged if toks is None else ops.attn_window_paged
+    args = (c.kv, c.table, c.kv_len) + (() if toks is None else (c.q_start,))
+    c.q[0, 0] = 0.0
+    want, want_lse = call(c.q, *args, scale=-0.04, window=90, sink=c.sink, want_lse=True)
+    c.check(want, want_lse, 90, 0, c.sink, scale=-0.04)
+    for e in (-40, -9, 9, 40):
+        out, lse = call((c.q.float() * 2.0 ** e).bfloat16(), *args, scale=-0.04 * 2.0 ** -e, window=90, sink=c.sink, want_lse=True)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    out, lse = call(c.q, *args, scale=0.0, window=90, want_lse=True)
+    c.check(out, lse, 90, 0, None, scale=0.0)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("toks,heads", [(None, 64), ([40, 7], 64), ([150, 30], 64), ([40, 7], 5)])
+def test_a_query_that_is_not_finite_spoils_its_head_only(ops, fmt, toks, heads):
+    c = Case(ops, fmt, heads, 256, 64, [200, 70], toks)
+    call = ops.attn_decode_paged if toks is None else ops.attn_window_paged
+    args = (c.kv, c.table, c.kv_len) + (() if toks is None else (c.q_start,))
+    clean, clean_lse = call(c.q, *args, window=90, want_lse=True)
+    q = c.q.clone()
+    q[0, 3, 200], q[-1, 2, 0] = float("nan"), float("inf")
+    out, lse = call(q, *args, window=90, want_lse=True)
+    bad = torch.zeros(q.shape[:2], dtype=torch.bool, device="cuda")
+    bad[0, 3] = bad[-1, 2] = True
+    assert bool(out[bad].isnan().any(-1).all())
+    assert torch.equal(out[~bad], clean[~bad]) and torch.equal(lse[~bad], clean_lse[~bad])
+
+
+@pytest.mark.parametrize("mag", [1e-6, 1e-3, 30.0, 1e4])
+@pytest.mark.parametrize("fmt", ["row", "block"])
+@pytest.mark.parametrize("heads,n_rot", [(64, 64), (8, 0)])
+def test_packed_rows_far_from_one(ops, mag, fmt, heads, n_rot):
+    c = Case(ops, fmt, heads, 256, 16, [200, 70], [150, 60], n_rot=n_rot, row_scale=lambda j: mag)
+    c.factors = pack_factors(c)
+    if fmt == "block":
+        c.tail = n_rot
+    scale = 1.0 / mag / 16
+    out, lse = ops.attn_window_paged(c.q, c.kv, c.table, c.kv_len, c.q_start, window=100, n_first=3, scale=scale, want_lse=True)
+    c.check(out, lse, 100, 3, None, scale=scale)
+
+
+def test_one_workspace_for_calls_one_behind_the_other(ops):
+    """Cut, whole and packed calls of several shapes on one stream, each right behind the other."""
+    cases = [Case(ops, "block", 64, 512, 64, [5000, 40]), Case(ops, "f32", 16, 128, 16, [100, 30], [90, 30]), Case(ops, "row", 64, 512, 64, [300], [200]),
+             Case(ops, "f32", 64, 512, 64, [9000])]
+    ws = ops.attn_workspace(64, 512)
+
+    def call(c, **kw):
+        if len(c.q) == len(c.kv_len):
+            return ops.attn_decode_paged(c.q, c.kv, c.table, c.kv_len, sink=c.sink, **kw)
+        return ops.attn_window_paged(c.q, c.kv, c.table, c.kv_len, c.q_start, window=70, sink=c.sink, **kw)
+
+    want = [call(c) for c in cases]
+    torch.cuda.synchronize()
+    got = [[call(c, workspace=ws) for c in cases] for _ in range(8)]
+    for outs in got:
+        for a, b in zip(outs, want):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("fmt", FMTS)
+def test_lengths_of_a_chunk_beyond_its_table_and_below_zero(ops, fmt):
+    c = Case(ops, fmt, 16, 128, 16, [64, 48], [9, 5])
+    args = (c.q, c.kv, c.table)
+    for window in (0, 20):
+        want = ops.attn_window_paged(*args, c.kv_len, c.q_start, window=window)
+        c.check(want, None, window, 0, None)
+        got = ops.attn_window_paged(*args, torch.tensor([2 ** 31 - 1, 48], dtype=torch.int32, device="cuda"), c.q_start, window=window)
+        assert torch.equal(got, want)
+        got = ops.attn_window_paged(*args, torch.tensor([-2 ** 31, 48], dtype=torch.int32, device="cuda"), c.q_start, window=window)
+        assert not got[:9].any() and torch.equal(got[9:], want[9:])
+    # the largest window and number of first rows are every row
+    # (not to the bits of window=0: the room for packed rows goes by the window)
+    c.check(ops.attn_window_paged(*args, c.kv_len, c.q_start, window=2 ** 31 - 1), None, 0, 0, None)
+    c.check(ops.attn_window_paged(*args, c.kv_len, c.q_start, window=1, n_first=2 ** 31 - 1), None, 0, 0, None)
+
+
+@pytest.mark.parametrize("n_pages,n_seqs,width,page", [(1, 2, 1, 1), (9, 5, 3, 2), (70000, 30000, 2, 3), (40, 6, 5, 1000)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_page_lists_that_are_empty_and_pools_that_are_full_or_free(ops, n_pages, n_seqs, width, page, in_place):
+    t = lambda v, *shape: torch.tensor(v, dtype=torch.int32, device="cuda").view(*(shape or (-1,)))
+    words = torch.randint(-2 ** 31, 2 ** 31 - 1, (n_pages, 5), device="cuda", dtype=torch.int32)
+    pool = ops.PagePool([words], page, n_seqs, width)
+    refs, table, lens = [0] * n_pages, [[-1] * width for _ in range(n_seqs)], [0] * n_seqs
+    m = model.Pages(refs, table, lens, page)
+    state = [t(refs), t(table, n_seqs, width), t(lens)]
+
+    def step(call, *lists):
+        before, m.moves, m.status = words.clone(), [], 0
+        outs = {} if in_place else dict(refs_out=torch.full_like(state[0], 99), table_out=torch.full_like(state[1], 99))
+        if not in_place and call is not ops.pages_compact:
+            outs["lens_out"] = torch.full_like(state[2], 99)
+        got = call(pool, *state[:2], **outs) if call is ops.pages_compact else call(pool, *state, *lists, **outs)
+        state[:2] = got[:2]
+        if call is not ops.pages_compact:
+            state[2] = got[2]
+        return before, got
+
+    def check(before, got, status=True):
+        same(m, [before], pool, *state, got[3] if status else None)
+
+    nothing = t([]).reshape(0, 2)
+    for fill in (False, True):
+        if fill:                                         # every page taken, from the first sequence on
+            want = [min(width, max(0, n_pages - width * b)) * page for b in range(n_seqs)]
+            done = step(ops.pages_reserve, t(want))
+            m.reserve(want)
+            check(*done)
+        done = step(ops.pages_fork, nothing)
+        m.fork([])
+        check(*done)
+        done = step(ops.pages_free, t([]))
+        m.free([])
+        check(*done)
+        done = step(ops.pages_compact)
+        assert done[1][2].item() == m.compact() and not m.moves
+        check(*done, status=False)
+    done = step(ops.pages_reserve, t([width * page] * n_seqs))
+    m.reserve([width * page] * n_seqs)
+    check(*done)
+    done = step(ops.pages_free, t(list(range(n_seqs))[::-1] * 1))
+    m.free(list(range(n_seqs)))
+    check(*done)
