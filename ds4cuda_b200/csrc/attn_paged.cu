@@ -384,9 +384,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     }
     tc::fence_after();
 
-    // Whether a wait of this CTA has given up.  Asked behind a wait, with the answer of any lane for all: if it is no, the wait of every lane
-    // has found its phase, and what it waited for may be read.
-    auto gave_up = [&]() -> bool { return __any_sync(0xffffffffu, *abort_flag != 0); };
+    // A wait whose answer is the same for all lanes: whether each has found the phase, so that what it waited for may be used.
+    auto found = [&](bool mine) -> bool { return __all_sync(0xffffffffu, mine); };
+    auto gave_up = [&]() -> bool { return __any_sync(0xffffffffu, *abort_flag != 0); };     // whether a wait of this CTA has
     // A role takes the segments in order from the ring; every warp of it calls this.
     int seg = 0;
     auto take_segment = [&](Segment &sg, int i) -> bool {
@@ -397,9 +397,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
     };
     auto next_segment = [&](Segment &sg) -> bool {
         const int i = seg & (kSegRing - 1);
-        tc::wait(DS4B200_BAR(seg_full, i), (uint32_t)((seg / kSegRing) & 1), abort_flag, status);
+        const bool on = found(tc::wait(DS4B200_BAR(seg_full, i), (uint32_t)((seg / kSegRing) & 1), abort_flag, status));
         ++seg;
-        return !gave_up() && take_segment(sg, i);
+        return on && take_segment(sg, i);
     };
     // The same for the warps of a role that meet at named barriers, which have no limit: the first warp waits and says for all whether they go
     // on, so that none stays behind at a barrier.  Two places in turn: a warp writes the next answer only when all have read the last but one.
@@ -407,8 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         const int i = seg & (kSegRing - 1);
         int *go = &go_s[role][seg & 1];
         if (first) {
-            tc::wait(DS4B200_BAR(seg_full, i), (uint32_t)((seg / kSegRing) & 1), abort_flag, status);
-            const bool on = !gave_up();
+            const bool on = found(tc::wait(DS4B200_BAR(seg_full, i), (uint32_t)((seg / kSegRing) & 1), abort_flag, status));
             if (lane == 0) *go = on;
         }
         sync();
@@ -598,8 +597,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
         struct Slots { int pair[4], own, rows; };        // of rows 2 j + half, and of row r; tile_rows, -1 also where a wait has given up
         auto slots_of = [&](int n) -> Slots {
             const int i = n & (kTileRing - 1);
-            tc::wait(DS4B200_BAR(tile_full, i), (uint32_t)((n / kTileRing) & 1), abort_flag, status);
-            if (gave_up()) return Slots{{-1, -1, -1, -1}, -1, -1};
+            if (!found(tc::wait(DS4B200_BAR(tile_full, i), (uint32_t)((n / kTileRing) & 1), abort_flag, status))) return Slots{{-1, -1, -1, -1}, -1, -1};
             const int4 p = *reinterpret_cast<const int4 *>(&slot_s[kPre ? 0 : i][lw * 8 + half * 4]);
             return Slots{{p.x, p.y, p.z, p.w}, kBlock && tail ? slot_s[kPre ? 0 : i][lw * 8 + ((lane >> 2) & 1) * 4 + (lane >> 3)] : 0, tile_rows[i]};
         };
@@ -895,8 +893,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     break;
                 }
                 const int i = seg & (kSegRing - 1);
-                tc::wait<300>(DS4B200_BAR(seg_free, i), (uint32_t)(((seg / kSegRing) & 1) ^ 1), abort_flag, status, tc::kWaitPolls + 16 * longest);
-                if (gave_up()) break;                    // the place may still be read
+                // (without the phase the place may still be read)
+                if (!found(tc::wait<300>(DS4B200_BAR(seg_free, i), (uint32_t)(((seg / kSegRing) & 1) ^ 1), abort_flag, status, tc::kWaitPolls + 16 * longest)) ||
+                    gave_up()) break;
                 if (lane == 0) {
                     if (kPre && !end) prefetch_l2(a.q + sg.it.row0 * D, sg.it.rows * D * 2);     // some items before they are wanted
                     seg_s[i] = sg;
@@ -917,8 +916,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                     const bool few = rows_in_tile(sg.it, t) <= 16;
 #pragma unroll
                     for (int part = 0; part < kParts; ++part) {
-                        tc::wait<20>(DS4B200_BAR(pv_done, buf * 2 + part), (uint32_t)(((n >> 1) & 1) ^ 1), abort_flag, status);
-                        stop = stop || gave_up();
+                        stop = !found(tc::wait<20>(DS4B200_BAR(pv_done, buf * 2 + part), (uint32_t)(((n >> 1) & 1) ^ 1), abort_flag, status)) || stop;
                         if (stop) continue;              // the last copy to this place may be in flight
                         ++sent;
                         if (lane == 0) {
@@ -951,8 +949,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
                 const int t1 = more ? sg.t1 : sg.t0 + 1;                    // one more entry says that it ends
                 for (int t = sg.t0; t < t1; ++t, ++n) {
                     const int i = n & (kTileRing - 1);
-                    tc::wait<300>(DS4B200_BAR(tile_free, i), (uint32_t)(((n / kTileRing) & 1) ^ 1), abort_flag, status);
-                    if (gave_up()) { more = false; break; }                 // the place may still be read
+                    // without the phase the place may still be read
+                    if (!found(tc::wait<300>(DS4B200_BAR(tile_free, i), (uint32_t)(((n / kTileRing) & 1) ^ 1), abort_flag, status))) { more = false; break; }
                     if (lane == 0) {
                         tile_rows[i] = !more ? -1 : t == sg.t0 ? sg.it.rows : 0;
                         tile_row0[i] = sg.it.row0;
@@ -1264,6 +1262,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 constexpr int kJoinCtas = 4 * kCtas, kJoinWarps = 8, kJoinFew = 8;
 static_assert(kCtas <= kJoinWarps * 32, "a thread per part");
 
+// Four partial sums, read once: no place in L1 (up to 0.7 us of a join), and not through the read-only path, since the kernel that writes them has
+// not ended when the join becomes resident.
+__device__ __forceinline__ float4 ld_part(const float *p) {
+    float4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+    return v;
+}
 __device__ __forceinline__ void add_scaled(float4 &o, float w, const float4 &x) {
     o = make_float4(fmaf(w, x.x, o.x), fmaf(w, x.y, o.y), fmaf(w, x.z, o.z), fmaf(w, x.w, o.w));
 }
@@ -1274,7 +1279,6 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) attn_join_kernel(const Att
     __shared__ float weight[kCtas], most_s[kJoinWarps], sum_s[kJoinWarps];
     __shared__ float4 sums[4][kJoinWarps][32];
     const int D = a.kv.head_dim, slices = D / 128, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    // What the kernel before writes while this one is resident already may not go through the read-only path, so no __ldg() of it.
     wait_dependency();
     if (tid < kCtas) items[tid] = meta[tid];
     __syncthreads();
@@ -1311,7 +1315,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) attn_join_kernel(const Att
 #pragma unroll
                 for (int s = 0; s < 4; ++s)
                     x[j][s] = k + j < it.parts && s < slices
-                                  ? *reinterpret_cast<const float4 *>(part_o + ((int64_t)part_of(c, k + j) * kRows + row) * D + s * 128 + lane * 4)
+                                  ? ld_part(part_o + ((int64_t)part_of(c, k + j) * kRows + row) * D + s * 128 + lane * 4)
                                   : make_float4(0.f, 0.f, 0.f, 0.f);
         };
         load(0);
@@ -1356,7 +1360,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32, 3) attn_join_kernel(const Att
                     const int k = k0 + i * kJoinWarps;
                     const float4 *from = reinterpret_cast<const float4 *>(part_o + ((int64_t)part_of(c, k) * kRows + row) * D + slice * 128 + lane * 4);
 #pragma unroll
-                    for (int s = 0; s < SL; ++s) x[i][s] = k < parts ? from[s * 32] : make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int s = 0; s < SL; ++s) x[i][s] = k < parts ? ld_part(reinterpret_cast<const float *>(from + s * 32)) : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
             };
             load(warp);

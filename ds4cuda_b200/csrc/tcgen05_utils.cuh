@@ -104,20 +104,22 @@ __device__ __forceinline__ void load_box(uint32_t dst, const void *map, int x, i
                  ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar) : "memory");
 }
 // A wait on an mbarrier phase.  It polls at most kWaitPolls times; the first that runs out raises the status bit and a
-// CTA-wide flag with which every later wait returns soon, so the kernel always ends (its results are invalid then).  A poll takes
+// CTA-wide flag with which every later wait returns soon, so the kernel always ends (its results are invalid then).  Returns whether the
+// phase was found: if not, what the wait was for may not be used.  A poll takes
 // issue slots and shared-memory bandwidth from the warps that work: with polls every 40 ns the waiting warps issued a third of
 // all instructions.
 template <int NS = 100>
-__device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status, int polls = kWaitPolls) {
-    if (try_phase(bar, parity)) return;
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int *status, int polls = kWaitPolls) {
+    if (try_phase(bar, parity)) return true;
 #pragma unroll 1
     for (int i = 1; i <= polls; ++i) {
         __nanosleep(NS);
-        if (try_phase(bar, parity)) return;
-        if ((i & 63) == 0 && *abort_flag) return;
+        if (try_phase(bar, parity)) return true;
+        if ((i & 63) == 0 && *abort_flag) return false;
     }
     *abort_flag = 1;
     atomicOr(status, kStatusBulkCopyTimeout);
+    return false;
 }
 
 // For what is still in flight when a kernel gives up.
