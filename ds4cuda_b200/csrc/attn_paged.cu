@@ -38,8 +38,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Scales.  A cache row is a row factor times f16 numbers.  Rows of ordinary size have the factor 1: codes times a scale that is a power
 // of two are exact in f16 where the product is a multiple of 2^-24 (a scale of 2^-15 and above; below, and in blocks far smaller than their
 // row's largest, a value is off by up to 2^-25 of the factor), codes times another scale are rounded (scale and product, 2^-11 each), as
-// f32 rows and tails are (2^-11).  A row whose scale or tail is far from one keeps a factor r_j, which enters the scores, and as log2 r_j the exponent of the weights,
-// so that P holds r_j exp(s_j - M) (times kLift, and below 2^15) and the sum takes P / r_j back.  A query row whose
+// f32 rows and tails are (2^-11).  A row whose scale or tail is far from one keeps a factor r_j, which enters the scores, and as
+// log2 r_j the exponent of the weights, so that P holds r_j exp(s_j - M) (times kLift, and below 2^15) and the sum takes P / r_j back.  A query row whose
 // largest value is outside [2^-4, 2^15] is scaled by a power of two: bf16's 8 bits fit f16, but for values below
 // 2^-17, which are off by up to 2^-25.
 //
@@ -1102,7 +1102,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const __grid_const
 #pragma unroll
                 for (int i = 0; i < 4; ++i) w[i] = fmaxf(fmaxf(v[i].x, v[i].y), fmaxf(v[i + 4].x, v[i + 4].y));
                 float top = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3])), f = 1.0f;
-                // A row keeps the reference its maximum had until one of its values lies kRescale above it.  Then it takes a new one, and every row's factor for the accumulators (a column of O^T) is left for follow(), which the
+                // A row keeps the reference its maximum had until one of its values lies kRescale above it.  Then it takes a
+                // new one, and every row's factor for the accumulators (a column of O^T) is left for follow(), which the
                 // warps run together, at the next tile.
                 if (__any_sync(0xffffffffu, !(top <= m + kRescale))) {
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));

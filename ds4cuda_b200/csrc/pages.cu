@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_reserve_kernel(Tables t, co
     const int tid = threadIdx.x;
     if (tid == 0) { bad = 0; asked = 0; }
     __syncthreads();
-    int64_t need = 0, mine = 0;                     // pages: before this round of sequences, cut at the pool's size; of this thread's, all
+    int64_t need = 0, mine = 0;                     // pages: of the sequences before these, cut at the pool's size; of this thread's, all
     const int64_t most = t.width * t.page_rows;
     for (int64_t base = 0; base < t.n_seqs; base += kPlanThreads) {
         const int64_t b = base + tid;

@@ -118,7 +118,7 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int
         if ((i & 63) == 0 && *abort_flag) return false;
     }
     *abort_flag = 1;
-    atomicOr(status, kStatusBulkCopyTimeout);
+    if (status) atomicOr(status, kStatusBulkCopyTimeout);
     return false;
 }
 
